@@ -46,6 +46,7 @@ typedef int32_t shp_status_t;
 /* ggml_type values (upstream enum ggml_type). */
 #define SHP_TYPE_F32  0
 #define SHP_TYPE_F16  1
+#define SHP_TYPE_Q4_0 2 /* the KV cache's entry points only (shp_kv_store, shp_kv_load, shp_attn_kv) */
 #define SHP_TYPE_Q8_0 8
 #define SHP_TYPE_Q5_K 13
 #define SHP_TYPE_I32  26
@@ -687,6 +688,98 @@ shp_status_t shp_diag_mask_inf(const shp_tensor * x, int32_t n_past, shp_tensor 
  */
 shp_status_t shp_soft_max_causal(const shp_tensor * a, int32_t n_past, float scale, shp_tensor * y,
                                  shp_stream_t stream);
+
+/*
+ * The KV cache in fewer bits, and the attention over it.
+ *
+ * A cache is a pair of tensors [head_dim, kv_heads, capacity, N] of one type:
+ * F32, F16, BF16, or, with head_dim a multiple of 32, blocks of 32 values
+ * along head_dim in ggml's formats: Q8_0 {f16 d; int8 q[32]}, a value q*d, and
+ * Q4_0 {f16 d; uint8 q[16]}, the low nibbles values 0..15 and the high nibbles
+ * values 16..31, a value (nibble - 8)*d. N sequences each have capacity rows;
+ * rows, heads and sequences may sit at any strides that are multiples of the
+ * element's size (2 bytes for the block types). Per-sequence numbers are I32
+ * tensors [N] in device memory, read when the kernel runs, so one captured
+ * graph serves every step of a decoding loop.
+ *
+ * shp_kv_store writes new rows: for t < count[n] (T without a count) row t of
+ * k and v, F32 [head_dim, kv_heads, T, N], becomes cache row slot[n] + t.
+ *   F32 copied; F16, BF16 rounded to nearest even;
+ *   Q8_0 d = amax/127, q = x*(1/d) rounded half away from zero;
+ *   Q4_0 d = m/-8 with m the block's value of largest magnitude (the first of
+ *        equals), nibble = min(15, trunc(x*(1/d) + 8.5));
+ *   each product, sum and quotient rounded in f32, 1/d taken as 0 where |d| is
+ *   below 2^-126, and d then rounded to f16. A block that holds an infinity or
+ *   NaN reads back as 32 NaNs.
+ * A sequence whose rows do not fit (count[n] outside [0, T], or count[n] > 0
+ * and slot[n] < 0 or slot[n] + count[n] > capacity) is not written at all, and
+ * *status (I32, one element, or NULL) is then set to 1; the library never
+ * clears it. Every other cache row is left as it was. The ggml node run of
+ * src/arch/qwen3-tts/operations.cpp:109-116 with a quantised cache.
+ *
+ * shp_kv_load reads rows back, exactly the values the attention sees (one f32
+ * product each): row t of k and v = cache row slot[n] + t for t < count[n]
+ * (clamped to [0, T]), NaN where that row is outside the cache; rows t >=
+ * count[n] are left as they were.
+ *
+ * head_dim 1..256. No tensor that is written may overlap another of the call,
+ * nor its own rows each other (SHP_ERR_UNSUPPORTED).
+ */
+shp_status_t shp_kv_store(const shp_tensor * k,
+                          const shp_tensor * v,
+                          const shp_tensor * slot,
+                          const shp_tensor * count,
+                          shp_tensor *       k_cache,
+                          shp_tensor *       v_cache,
+                          shp_tensor *       status,
+                          shp_stream_t       stream);
+shp_status_t shp_kv_load(const shp_tensor * k_cache,
+                         const shp_tensor * v_cache,
+                         const shp_tensor * slot,
+                         const shp_tensor * count,
+                         shp_tensor *       k,
+                         shp_tensor *       v,
+                         shp_stream_t       stream);
+
+/*
+ * Causal attention of the newest positions over a cache, each query over the
+ * whole cache before it or over a sliding window and the first rows: the run
+ * of src/arch/qwen3-tts/operations.cpp:123-140 (two matrix products around the
+ * softmax) without its score matrix. q, y F32 [head_dim, heads, T, N], heads a
+ * multiple of kv_heads; query head h reads kv head h / (heads/kv_heads).
+ * length[n] (capacity without a length; clamped to [0, capacity]) counts the
+ * filled rows, those of the call's own positions among them; query t < count[n]
+ * (T without a count; clamped to [0, T]) stands at row p = length[n] - count[n]
+ * + t and sees row j when 0 <= j <= p and (window == 0 or j > p - window or
+ * j < sinks):
+ *   y = sum_j softmax_j(scale * q.k_j) v_j over the rows it sees; 0 where p < 0.
+ * Queries t >= count[n] are left as they were. Rows that no query of a
+ * sequence sees are never used, whatever they hold. head_dim 1..256; y and work
+ * overlap nothing else of the call.
+ * Products are formed to f32's precision and summed in f32.
+ *
+ * work: F32, contiguous, at least the number of floats that
+ * shp_attn_kv_work gives for the same q, k_cache, window and sinks (partial
+ * results where the rows of a sequence are split over workgroups); NULL where
+ * that is 0. Its contents need not be set, and do not matter after the call;
+ * calls that may run at the same time need a workspace each.
+ */
+shp_status_t shp_attn_kv_work(const shp_tensor * q,
+                              const shp_tensor * k_cache,
+                              int32_t            window,
+                              int32_t            sinks,
+                              int64_t *          floats);
+shp_status_t shp_attn_kv(const shp_tensor * q,
+                         const shp_tensor * k_cache,
+                         const shp_tensor * v_cache,
+                         const shp_tensor * length,
+                         const shp_tensor * count,
+                         float              scale,
+                         int32_t            window,
+                         int32_t            sinks,
+                         shp_tensor *       work,
+                         shp_tensor *       y,
+                         shp_stream_t       stream);
 
 /*
  * ggml_exp: y = expf(x) per element, F32 of one shape

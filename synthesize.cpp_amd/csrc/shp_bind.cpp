@@ -377,6 +377,25 @@ PyObject * run_layer(void * fn, PyObject * const * args, Py_ssize_t n) {
     return PyLong_FromLong(st);
 }
 
+// The workspace of shp_attn_kv: q, k_cache, window and sinks to its floats, or
+// to minus the status.
+PyObject * run_attn_work(void * fn, PyObject * const * args, Py_ssize_t n) {
+    if (!counted(n, 4)) {
+        return nullptr;
+    }
+    Slot               s[4];
+    const shp_tensor * q      = nullptr;
+    const shp_tensor * k      = nullptr;
+    int32_t            window = 0, sinks = 0;
+    int64_t            floats = 0;
+    if (!Arg<const shp_tensor *>::get(args[0], s[0], q) || !Arg<const shp_tensor *>::get(args[1], s[1], k) ||
+        !Arg<int32_t>::get(args[2], s[2], window) || !Arg<int32_t>::get(args[3], s[3], sinks)) {
+        return nullptr;
+    }
+    const shp_status_t st = reinterpret_cast<decltype(&shp_attn_kv_work)>(fn)(q, k, window, sinks, &floats);
+    return PyLong_FromLongLong(st == SHP_OK ? floats : -static_cast<int64_t>(st));
+}
+
 using Runner = PyObject * (*) (void *, PyObject * const *, Py_ssize_t);
 
 struct Entry {
@@ -401,6 +420,7 @@ const Entry kEntries[] = {
     SHP_ENTRY(shp_acc), SHP_ENTRY_FIRST(shp_im2col, kShape), SHP_ENTRY(shp_cont_add_leaky_relu), SHP_ENTRY(shp_soft_max_ext),
     SHP_ENTRY(shp_diag_mask_inf), SHP_ENTRY(shp_soft_max_causal), SHP_ENTRY(shp_exp), SHP_ENTRY(shp_scale_bias),
     SHP_ENTRY_FIRST(shp_sum_scale_leaky_relu, kArray), { "shp_layer_nongemm_step", &run_layer },
+    SHP_ENTRY(shp_kv_store), SHP_ENTRY(shp_kv_load), SHP_ENTRY(shp_attn_kv), { "shp_attn_kv_work", &run_attn_work },
 };
 
 struct Bound {

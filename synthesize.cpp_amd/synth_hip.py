@@ -24,10 +24,11 @@ LIB_PATH = os.environ.get("SHP_LIB") or os.path.join(HERE, "libsynth_hip.so")
 BIND_PATH = os.path.join(HERE, "shp_bind.so")
 
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_BACKEND = 0, 1, 2, 17
-TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q5_K, TYPE_I32, TYPE_BF16 = 0, 1, 8, 13, 26, 30
+TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q5_K, TYPE_I32, TYPE_BF16 = 0, 1, 2, 8, 13, 26, 30
 ROPE_TYPE_NEOX = 2
 Q8_0_BLOCK_BYTES, Q8_0_BLOCK_ELEMS = 34, 32
 Q5_K_BLOCK_BYTES, Q5_K_BLOCK_ELEMS = 176, 256
+Q4_0_BLOCK_BYTES, Q4_0_BLOCK_ELEMS = 18, 32
 
 
 class ShpTensor(ctypes.Structure):
@@ -123,6 +124,10 @@ def load(path=None):
         "shp_gelu_erf": [_PT, _PT, vp],
         "shp_clamp": [_PT, f, f, _PT, vp],
         "shp_norm": [_PT, f, _PT, vp],
+        "shp_kv_store": [_PT, _PT, _PT, _PT, _PT, _PT, _PT, vp],
+        "shp_kv_load": [_PT, _PT, _PT, _PT, _PT, _PT, vp],
+        "shp_attn_kv": [_PT, _PT, _PT, _PT, _PT, f, i32, i32, _PT, _PT, vp],
+        "shp_attn_kv_work": [_PT, _PT, i32, i32, ctypes.POINTER(i64)],
         "shp_graph_compute": [ctypes.POINTER(ShpNode), i32, vp],
         "shp_graph_plan": [ctypes.POINTER(ShpNode), i32, ctypes.POINTER(ShpGraphRun), i32, ctypes.POINTER(i32)],
     }
@@ -195,6 +200,11 @@ class Q8Tensor(BlockTensor):
 class Q5KTensor(BlockTensor):
     """Q5_K: 256-element super-blocks of 176 bytes."""
     TYPE, ELEMS, BYTES = TYPE_Q5_K, Q5_K_BLOCK_ELEMS, Q5_K_BLOCK_BYTES
+
+
+class Q4Tensor(BlockTensor):
+    """Q4_0: 32-element blocks {f16 d; uint8 qs[16]}; a KV cache (kv_store, kv_load, attn_kv)."""
+    TYPE, ELEMS, BYTES = TYPE_Q4_0, Q4_0_BLOCK_ELEMS, Q4_0_BLOCK_BYTES
 
 
 _bind = None
@@ -384,6 +394,54 @@ def soft_max_ext(a, mask, scale, max_bias=0.0, out=None):
     out = a.new_empty(a.shape) if out is None else out
     _check(_fn("shp_soft_max_ext")(a, mask, float(scale), float(max_bias), out,
                                    _stream()), "soft_max_ext")
+    return out
+
+
+def kv_store(k, v, k_cache, v_cache, slot, count=None, status=None):
+    """New rows into a KV cache: k, v (N, T, kv_heads, head_dim) F32; the caches
+    (N, capacity, kv_heads, head_dim) F32, F16, BF16, Q8Tensor or Q4Tensor; row
+    t < count[n] (all T without count) of sequence n becomes cache row slot[n] + t.
+    slot and count are int32 (N,); a sequence whose rows do not fit is not
+    written, and `status` (int32, one element) is then set to 1."""
+    _check(_fn("shp_kv_store")(k, v, slot, count, k_cache, v_cache, status, _stream()), "kv_store")
+
+
+def kv_load(k_cache, v_cache, slot, t, count=None, k_out=None, v_out=None):
+    """Rows [slot[n], slot[n] + t) of a KV cache as F32: (k, v), each (N, t,
+    kv_heads, head_dim); rows past count[n] are not written."""
+    raw = k_cache.data if isinstance(k_cache, BlockTensor) else k_cache
+    ne0 = k_cache.ne0 if isinstance(k_cache, BlockTensor) else k_cache.shape[-1]
+    shape = tuple(raw.shape[:-3]) + (int(t), raw.shape[-2], ne0)
+    k_out = _empty_like_f32(shape, raw.device) if k_out is None else k_out
+    v_out = _empty_like_f32(shape, raw.device) if v_out is None else v_out
+    _check(_fn("shp_kv_load")(k_cache, v_cache, slot, count, k_out, v_out, _stream()), "kv_load")
+    return k_out, v_out
+
+
+def attn_kv_work(q, k_cache, window=0, sinks=0):
+    """The floats of workspace that attn_kv needs for these shapes (0: none)."""
+    n = _fn("shp_attn_kv_work")(q, k_cache, int(window), int(sinks))
+    if n < 0:
+        raise ShpError(-n, "attn_kv_work")
+    return n
+
+
+def attn_kv(q, k_cache, v_cache, length=None, count=None, scale=None, window=0, sinks=0, out=None, work=None):
+    """Causal attention of the newest positions over a KV cache: q (N, T, heads,
+    head_dim) F32, caches as in kv_store. length (int32 (N,); the capacity
+    without one) counts a sequence's filled rows, these positions among them;
+    query t < count[n] stands at row length[n] - count[n] + t and sees the rows up to
+    its own, with a window only the last `window` of them and the first `sinks`.
+    scale: head_dim ** -0.5 unless given. work: F32 of attn_kv_work()'s floats,
+    allocated here unless given. Returns (N, T, heads, head_dim); a query that
+    sees no row gives zeros, and rows past count[n] are not written."""
+    out = q.new_empty(q.shape) if out is None else out
+    if work is None:
+        n = attn_kv_work(q, k_cache, window, sinks)
+        work = q.new_empty(n) if n else None
+    _check(_fn("shp_attn_kv")(q, k_cache, v_cache, length, count,
+                              float(q.shape[-1] ** -0.5 if scale is None else scale), int(window), int(sinks), work,
+                              out, _stream()), "attn_kv")
     return out
 
 
