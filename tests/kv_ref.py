@@ -68,7 +68,10 @@ def attend(q, k, v, length, count, scale, window=0, sinks=0):
     sum of n terms adds n more half steps, with 32 for the weights' own roundings
     and the joins of parts. Where f32 ends: a weight e^(s - max) below 2^-126 may
     become 0, which moves a result by at most 2^-126 |v| (the weights' sum is at
-    least 1), and a result below 2^-126 may become 0 itself."""
+    least 1), and a result below 2^-126 may become 0 itself. Where weights go
+    through the matrix units as two F16 pieces, 2^15 e^(s - max) = hi + lo, the
+    pieces' smallest step is 2^-24: half of it, 2^-25 / 2^15 = 2^-40, is how far a
+    weight may be off however small it is, which moves a result by 2^-40 |v|."""
     n, t, heads, hd = q.shape
     group = heads // k.shape[2]
     q = q.double()
@@ -89,5 +92,5 @@ def attend(q, k, v, length, count, scale, window=0, sinks=0):
                 w = torch.softmax(s, 0)
                 y[b, i, h] = w @ vh
                 e = (hd + 16) * EPS * float((kh.abs() @ q[b, i, h].abs()).max()) * abs(scale)
-                bound[b, i, h] = (np.expm1(2 * e) + (len(seen) + 32) * EPS) * (w @ vh.abs()) + 2.0 ** -126 * (1 + vh.abs().sum(0))
+                bound[b, i, h] = (np.expm1(2 * e) + (len(seen) + 32) * EPS) * (w @ vh.abs()) + 2.0 ** -40 * vh.abs().sum(0) + 2.0 ** -126
     return y, bound
