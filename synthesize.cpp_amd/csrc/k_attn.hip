@@ -25,7 +25,7 @@ struct AttnArgs {
     char *          y;
     const int32_t * length;  // or null: cap
     const int32_t * count;   // or null: T
-    float *         work;    // partials of nsplit > 1: [rows][nsplit][hd], then m and l [rows][nsplit][2]
+    float *         work;    // partials of nsplit > 1: [rows][nsplit][hd4], then m and l [rows][nsplit][2]
     int64_t         qh, qt, qn, kh, kt, kn, vh, vt, vn, yh, yt, yn;
     float           scale;  // times log2 e
     int32_t         window;  // 0: none
@@ -35,6 +35,7 @@ struct AttnArgs {
     int32_t         KV;
     int32_t         N;
     int32_t         hd;
+    int32_t         hd4;  // hd up to a multiple of 4: a partial row's length
     int32_t         cap;
     int32_t         nsplit;
     int32_t         tiles;  // of rows
@@ -97,23 +98,48 @@ __device__ __forceinline__ SeqLens seq_lens(const AttnArgs & a, int n) {
 }
 
 __device__ __forceinline__ float * partial_o(const AttnArgs & a, int64_t row, int split) {
-    return a.work + (row * a.nsplit + split) * a.hd;
+    return a.work + (row * a.nsplit + split) * a.hd4;
 }
 
 __device__ __forceinline__ float * partial_ml(const AttnArgs & a, int64_t row, int split) {
     const int64_t rows = static_cast<int64_t>(a.N) * a.KV * a.T * a.G;
-    return a.work + rows * a.nsplit * a.hd + (row * a.nsplit + split) * 2;
+    return a.work + rows * a.nsplit * a.hd4 + (row * a.nsplit + split) * 2;
 }
 
-// The maximum, or the sum, over the four lanes c, c+16, c+32, c+48.
+// The maximum, or the sum, over the four lanes c, c+16, c+32, c+48, in each of
+// them: lanes change places with those 16, then 32 away, without LDS.
+struct Pair {
+    float a, b;
+};
+
+__device__ __forceinline__ Pair swap16(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return Pair{ __uint_as_float(r[0]), __uint_as_float(r[1]) };
+#else
+    return Pair{ v, v };
+#endif
+}
+
+__device__ __forceinline__ Pair swap32(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return Pair{ __uint_as_float(r[0]), __uint_as_float(r[1]) };
+#else
+    return Pair{ v, v };
+#endif
+}
+
 __device__ __forceinline__ float max_quarters(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    const Pair p = swap16(v);
+    const Pair q = swap32(fmaxf(p.a, p.b));
+    return fmaxf(q.a, q.b);
 }
 
 __device__ __forceinline__ float sum_quarters(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    const Pair p = swap16(v);
+    const Pair q = swap32(p.a + p.b);
+    return q.a + q.b;
 }
 
 // What a row's softmax comes to: 1/l, or 0 where the row sees nothing. A row
@@ -272,7 +298,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int   kChunk   = 32;     // cache rows of a chunk
 constexpr float kPShift  = 15.0f;  // P times 2^15, at most half of F16's range
-constexpr int   kMaxWaves = 4;     // of a workgroup
 
 __device__ __forceinline__ f16x2 as_f16x2(uint32_t v) {
     return __builtin_bit_cast(f16x2, v);
@@ -293,39 +318,55 @@ __device__ __forceinline__ void split2(float a, float b, f16x2 & hi, f16x2 & lo)
     lo = __builtin_convertvector((f32x2{ a - static_cast<float>(hi[0]), b - static_cast<float>(hi[1]) }), f16x2);
 }
 
+// Exponents that turn an integer in a mantissa's low bits into an F16. Held in
+// vector registers once a kernel, behind the compiler's back: (w & mask) | bits
+// is then one v_and_or_b32, which takes at most one scalar or literal operand.
+struct Magic {
+    uint32_t e1024;  // 0x6400 | n is 1024 + n
+    uint32_t e64;    // 0x5400 | n << 4 is 64 + n
+
+    __device__ Magic() : e1024(0x64006400u), e64(0x54005400u) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        asm("" : "+v"(e1024), "+v"(e64));
+#endif
+    }
+};
+
 // How a cache type's bytes become matrix operands.
 //   kWords   dwords of codes in 32 values
 //   kTiles   values of a dword: each is the row of another 16-row tile of V^T
-//   element  value index within 32 of operand element e of quarter g
-//   k_codes  operand of the 32 values at `block`, quarter g
+//   quarter g's eight operand elements are the values kFirst g + order(0..3)
+//   and kSecond more
+//   kStep    dwords of codes in a quarter's operand
+//   k_codes  that operand
 //   v_codes  from a dword of two keys: their values u as F16, without d
 //   v_index  value index within 32 of value u of dword w
 template <int KIND> struct Codes;
 
 template <> struct Codes<kKvQ4> {
     static constexpr int kWords = 4;
+    static constexpr int kStep  = 1;
     static constexpr int kTiles = 8;
 
-    __device__ static constexpr int element(int g, int e) {
-        return 4 * g + (e >= 4 ? 16 : 0) + (e & 1) * 2 + ((e >> 1) & 1);
-    }
+    static constexpr int kFirst  = 4;
+    static constexpr int kSecond = 16;
 
-    // n in a mantissa's low bits: 0x6400 | n is 1024 + n, 0x5400 | n << 4 is 64 + n
-    __device__ static f16x2 low(uint32_t w) { return as_f16x2((w & 0x000f000fu) | 0x64006400u) - splat2(1032.0f); }
+    __device__ static constexpr int order(int e) { return (e & 1) * 2 + (e >> 1); }
 
-    __device__ static f16x2 high(uint32_t w) { return as_f16x2((w & 0x00f000f0u) | 0x54005400u) - splat2(72.0f); }
+    __device__ static f16x2 low(const Magic & m, uint32_t w) { return as_f16x2((w & 0x000f000fu) | m.e1024) - splat2(1032.0f); }
 
-    __device__ static f16x8 k_codes(const char * block, int g) {
-        const uint32_t w = *reinterpret_cast<const u32_at2 *>(block + 2 + 4 * g);
-        return join8(low(w), low(w >> 8), high(w), high(w >> 8));
+    __device__ static f16x2 high(const Magic & m, uint32_t w) { return as_f16x2((w & 0x00f000f0u) | m.e64) - splat2(72.0f); }
+
+    __device__ static f16x8 k_codes(const Magic & m, const uint32_t (&w)[1]) {
+        return join8(low(m, w[0]), low(m, w[0] >> 8), high(m, w[0]), high(m, w[0] >> 8));
     }
 
     __device__ static int word_offset(int w) { return (w >> 2) * 18 + 2 + 4 * (w & 3); }
 
-    template <int U> __device__ static f16x2 v_codes(uint32_t w0, uint32_t w1) {
+    template <int U> __device__ static f16x2 v_codes(const Magic & m, uint32_t w0, uint32_t w1) {
         constexpr uint32_t kSel = 0x0c040c00u + (U >> 1) * 0x00010001u;  // byte U/2 of w0 and of w1
         const uint32_t     x    = __builtin_amdgcn_perm(w1, w0, kSel);
-        return U & 1 ? high(x) : low(x);
+        return U & 1 ? high(m, x) : low(m, x);
     }
 
     __device__ static int v_index(int w, int u) { return 32 * (w >> 2) + 4 * (w & 3) + (u >> 1) + 16 * (u & 1); }
@@ -333,27 +374,56 @@ template <> struct Codes<kKvQ4> {
 
 template <> struct Codes<kKvQ8> {
     static constexpr int kWords = 8;
+    static constexpr int kStep  = 2;
     static constexpr int kTiles = 4;
 
-    __device__ static constexpr int element(int g, int e) { return 8 * g + e; }
+    static constexpr int kFirst  = 8;
+    static constexpr int kSecond = 4;
 
-    // q + 128 in a mantissa's low bits
-    __device__ static f16x2 biased(uint32_t x) { return as_f16x2(x | 0x64006400u) - splat2(1152.0f); }
+    __device__ static constexpr int order(int e) { return e; }
 
-    __device__ static f16x8 k_codes(const char * block, int g) {
-        const uint32_t w0 = *reinterpret_cast<const u32_at2 *>(block + 2 + 8 * g) ^ 0x80808080u;
-        const uint32_t w1 = *reinterpret_cast<const u32_at2 *>(block + 6 + 8 * g) ^ 0x80808080u;
-        return join8(biased(__builtin_amdgcn_perm(0, w0, 0x0c010c00u)), biased(__builtin_amdgcn_perm(0, w0, 0x0c030c02u)),
-                     biased(__builtin_amdgcn_perm(0, w1, 0x0c010c00u)), biased(__builtin_amdgcn_perm(0, w1, 0x0c030c02u)));
+    // from q + 128
+    __device__ static f16x2 biased(const Magic & m, uint32_t x) { return as_f16x2(x | m.e1024) - splat2(1152.0f); }
+
+    __device__ static f16x8 k_codes(const Magic & m, const uint32_t (&w)[2]) {
+        const uint32_t a = w[0] ^ 0x80808080u;
+        const uint32_t b = w[1] ^ 0x80808080u;
+        return join8(biased(m, __builtin_amdgcn_perm(0, a, 0x0c010c00u)), biased(m, __builtin_amdgcn_perm(0, a, 0x0c030c02u)),
+                     biased(m, __builtin_amdgcn_perm(0, b, 0x0c010c00u)), biased(m, __builtin_amdgcn_perm(0, b, 0x0c030c02u)));
     }
 
     __device__ static int word_offset(int w) { return (w >> 3) * 34 + 2 + 4 * (w & 7); }
 
-    template <int U> __device__ static f16x2 v_codes(uint32_t w0, uint32_t w1) {
-        return biased(__builtin_amdgcn_perm(w1 ^ 0x80808080u, w0 ^ 0x80808080u, 0x0c040c00u + U * 0x00010001u));
+    template <int U> __device__ static f16x2 v_codes(const Magic & m, uint32_t w0, uint32_t w1) {
+        return biased(m, __builtin_amdgcn_perm(w1 ^ 0x80808080u, w0 ^ 0x80808080u, 0x0c040c00u + U * 0x00010001u));
     }
 
     __device__ static int v_index(int w, int u) { return 4 * w + u; }
+};
+
+// Dwords at two-byte boundaries of LDS. A wave's read of them as they are takes
+// 65 cycles of the LDS unit on this chip, an aligned one 3.2, so each is put
+// together from the two aligned dwords that it lies in. `lo` and `hi` are the
+// same address a dword apart, kept from being joined into one 8-byte read (35
+// to 65 cycles at a 4-byte boundary).
+struct LdsWords {
+    const char * lo;
+    const char * hi;
+    uint32_t     shift;  // 0 or 2 bytes
+
+    __device__ explicit LdsWords(const char * base, int at) {
+        lo    = base + (at & ~3);
+        int d = 4;
+        asm("" : "+v"(d));
+        hi    = lo + d;
+        shift = static_cast<uint32_t>(at) & 2u;
+    }
+
+    // The dword `off` bytes on, a multiple of 4.
+    __device__ uint32_t at(int off) const {
+        return __builtin_amdgcn_alignbyte(*reinterpret_cast<const uint32_t *>(hi + off),
+                                          *reinterpret_cast<const uint32_t *>(lo + off), shift);
+    }
 };
 
 struct FewArgs {
@@ -366,71 +436,168 @@ struct FewArgs {
     FastDiv  frun;
     FastDiv  fcols;
     int32_t  wave_lds;
+    int32_t  groups;   // of HG heads
+    int32_t  wgs;      // workgroups that share the work
+    FastDiv  fwgs;
+    int32_t  per;      // chunks of a unit
+    FastDiv  fper;
 };
+
+// How the work is dealt out. A sequence's chunks make units of one chunk or a
+// few for each of a workgroup's waves; sequence after sequence, head group after head
+// group, the units of the call stand in one line, of which every workgroup
+// takes an equal stretch. So lengths may differ as they like (64 streams of 512
+// to 8192 rows, MI355X: XX us, YY with an equal number of workgroups for each
+// sequence). A stretch that ends inside a group leaves a partial result; a
+// workgroup has two at most, of the group that it begins in and did not begin
+// (0), and of the one that it began and did not end (1).
+constexpr int kCols = 16;
+
+__device__ __forceinline__ float * few_o(const FewArgs & f, int wg, int which, int col) {
+    return f.a.work + (static_cast<int64_t>(wg * 2 + which) * kCols + col) * f.a.hd4;
+}
+
+__device__ __forceinline__ float * few_ml(const FewArgs & f, int wg, int which, int col) {
+    return f.a.work + static_cast<int64_t>(f.wgs) * 2 * kCols * f.a.hd4 + ((wg * 2 + which) * kCols + col) * 2;
+}
+
+// A sequence's key chunks; `len` as seq_lens gives it.
+__device__ __forceinline__ KeyTiles few_tiles(const FewArgs & f, const SeqLens & len) {
+    const AttnArgs & a     = f.a;
+    const int        shift = 5 - f.hgs;
+    const int32_t    base  = len.length - len.count;
+    const int32_t    p1    = len.length - 1;
+    KeyTiles         kt{ 0, 0, 0 };
+    if (p1 >= 0) {
+        if (a.window > 0) {
+            kt.second = max(base - a.window + 1, 0) >> shift;
+            kt.first  = min((min(a.sinks, p1 + 1) + (1 << shift) - 1) >> shift, kt.second);
+        }
+        kt.n = kt.first + (p1 >> shift) - kt.second + 1;
+    }
+    return kt;
+}
+
+// Units of sequence n and head group: at least one where it has a query, which
+// then writes its zeros.
+__device__ __forceinline__ int few_units(const FewArgs & f, int n) {
+    const SeqLens len = seq_lens(f.a, n);
+    return len.count == 0 ? 0 : max(static_cast<int>(fastdiv(static_cast<uint32_t>(few_tiles(f, len).n + f.per - 1), f.fper)), 1);
+}
+
+// The line's length, and the place of sequence n in it (units of one head
+// group), for a whole wave: 64 sequences at a time, a sum over lanes.
+struct Line {
+    int32_t before;
+    int32_t total;
+};
+
+__device__ __forceinline__ Line few_line(const FewArgs & f, int n, int lane) {
+    if (f.a.N == 1) {
+        return Line{ 0, few_units(f, 0) };
+    }
+    Line s{ 0, 0 };
+    for (int first = 0; first < f.a.N; first += kWave) {
+        const int i     = first + lane;
+        int       units = i < f.a.N ? few_units(f, i) : 0;
+        int       below = i < n ? units : 0;
+#pragma unroll
+        for (int off = 1; off < kWave; off *= 2) {
+            units += __shfl_xor(units, off);
+            below += __shfl_xor(below, off);
+        }
+        s.total += __builtin_amdgcn_readfirstlane(units);
+        s.before += __builtin_amdgcn_readfirstlane(below);
+    }
+    return s;
+}
+
+// The sequence that unit u of the line falls in.
+struct Place {
+    int32_t n;
+    int32_t units;   // of one head group of it
+    int32_t before;  // of all head groups of the sequences before it
+};
+
+__device__ __forceinline__ Place few_find(const FewArgs & f, int32_t u, int lane) {
+    if (f.a.N == 1) {
+        return Place{ 0, few_units(f, 0), 0 };
+    }
+    int32_t before = 0;
+    for (int first = 0; first < f.a.N; first += kWave) {
+        const int i     = first + lane;
+        const int units = i < f.a.N ? few_units(f, i) : 0;
+        int       sum   = units;
+#pragma unroll
+        for (int off = 1; off < kWave; off *= 2) {
+            const int v = __shfl_up(sum, off);
+            sum += lane >= off ? v : 0;
+        }
+        const uint64_t past = __ballot(before + sum * f.groups > u);
+        if (past != 0) {
+            const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            const int k = __builtin_amdgcn_readlane(units, l);
+            return Place{ first + l, k, before + (__builtin_amdgcn_readlane(sum, l) - k) * f.groups };
+        }
+        before += __builtin_amdgcn_readlane(sum, kWave - 1) * f.groups;
+    }
+    return Place{ 0, 1, u };  // (u lies in the line)
+}
+
+// Where workgroup wg's stretch of `total` units begins, and whose unit u is.
+__device__ __forceinline__ int32_t few_start(const FewArgs & f, int32_t total, int32_t wg) {
+    const int32_t each = static_cast<int32_t>(fastdiv(static_cast<uint32_t>(total), f.fwgs));
+    return each * wg + min(wg, total - each * f.wgs);
+}
+
+__device__ __forceinline__ int32_t few_owner(const FewArgs & f, int32_t total, int32_t u) {
+    const int32_t each = static_cast<int32_t>(fastdiv(static_cast<uint32_t>(total), f.fwgs));
+    const int32_t more = total - each * f.wgs;  // workgroups with one more
+    return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each;
+}
 
 template <class Go, int... U> __device__ __forceinline__ void for_each(std::integer_sequence<int, U...>, const Go & go) {
     (go(std::integral_constant<int, U>{}), ...);
 }
 
-// A piece of 16 or 4 bytes of a chunk as one load.
-template <int BYTES> struct PieceOf {
-    typedef u32x4 T;
-};
+// One cache's chunk on its way to LDS: a lane's pieces of 16 or 4 bytes, read
+// through a buffer descriptor that ends with the cache's rows, so that what is
+// behind them reads as zero without a test in the kernel.
+typedef __amdgpu_buffer_rsrc_t Rsrc;
 
-template <> struct PieceOf<4> {
-    typedef uint32_t T;
-};
-
-// One cache's chunk on its way to LDS: P pieces a lane.
-template <int BYTES, int P> struct Staged {
-    typename PieceOf<BYTES>::T piece[P];
-};
-
-// The pieces of the chunk at key j0, as this lane takes them. Where the chunk
-// goes past the cache's end the bytes there are zero, and the piece that the
-// end falls in is read in two-byte steps.
-template <int BYTES, int P>
-__device__ __forceinline__ void fetch(const FewArgs & f, const char * base, int64_t kt, const int32_t (&rel)[P], int lane,
-                                      int32_t j0, int32_t keys, int row_bytes, Staged<BYTES, P> & s) {
-    typedef typename PieceOf<BYTES>::T T;
-    const char * at   = base + static_cast<int64_t>(j0) * kt;
-    const int    left = f.a.cap - j0;
-    if (left >= keys) {
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            if (lane + i * kWave < f.pieces) {
-                s.piece[i] = *to_global(reinterpret_cast<const T *>(at + rel[i]));
-            }
-        }
-        return;
-    }
-    const int bytes = (left << f.hgs) * row_bytes;  // of one run
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-        const int p = lane + i * kWave;
-        if (p < f.pieces) {
-            const char * src  = at + rel[i];
-            const int    have = f.run > 0 ? (static_cast<int>(fastdiv(static_cast<uint32_t>(p), f.frun)) < left ? BYTES : 0)
-                                          : min(max(bytes - BYTES * p, 0), BYTES);
-            if (have == BYTES) {
-                s.piece[i] = *to_global(reinterpret_cast<const T *>(src));
-            } else {
-                uint32_t v[BYTES / 4] = {};
-#pragma unroll
-                for (int h = 0; h < BYTES / 2; ++h) {
-                    if (2 * h < have) {
-                        v[h / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(src)[h]) << (16 * (h & 1));
-                    }
-                }
-                s.piece[i] = __builtin_bit_cast(T, v);
-            }
-        }
-    }
+__device__ __forceinline__ Rsrc rows_from(const char * at, int64_t bytes) {
+    constexpr int kRaw32 = 0x00027000;  // 32-bit data, no swizzle
+    const int64_t most   = int64_t{ 1 } << 30;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at), 0, static_cast<int>(bytes < most ? bytes : most), kRaw32);
 }
 
-// KIND Q4 or Q8, at most NB blocks a row, read in pieces of BYTES.
-template <int KIND, int NB, int BYTES, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_attn_few(const FewArgs f) {
+template <int BYTES, int P> struct Staged;
+
+template <int P> struct Staged<16, P> {
+    u32x4 piece[P];
+
+    __device__ void load(int i, const Rsrc & r, int off) { piece[i] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
+
+    __device__ void keep(int i, char * lds, int at) const { reinterpret_cast<u32x4 *>(lds)[at] = piece[i]; }
+};
+
+template <int P> struct Staged<4, P> {
+    uint32_t piece[P];
+
+    __device__ void load(int i, const Rsrc & r, int off) { piece[i] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0); }
+
+    __device__ void keep(int i, char * lds, int at) const { reinterpret_cast<uint32_t *>(lds)[at] = piece[i]; }
+};
+
+// LDS of a workgroup ahead of its waves' parts: the queries' operands and maxima.
+__host__ __device__ constexpr int few_shared(int nb, int waves) {
+    return 2 * nb * kWave * 16 + waves * kWave * 4;
+}
+
+// KIND Q4 or Q8, NB blocks a row (NB 8: at most 8), read in pieces of BYTES;
+// RUNS: a key's rows are apart from the next key's.
+template <int KIND, int NB, int BYTES, bool RUNS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, NB <= 4 ? 2 : 1) void k_attn_few(const FewArgs f) {
     using C                 = Codes<KIND>;
     constexpr int    UNIT   = kv_unit_bytes(KIND);
     constexpr int    SLOTS  = (NB * C::kWords + 15) / 16;
@@ -442,83 +609,81 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_few(const FewArgs f) {
     const int        lane = threadIdx.x % kWave;
     const int        c    = lane & 15;
     const int        g    = lane >> 4;
-    const int        split = blockIdx.x;
-    const int        h0    = static_cast<int>(blockIdx.y) << f.hgs;
-    const int        n     = blockIdx.z;
-    const SeqLens    len   = seq_lens(a, n);
-    if (len.count == 0) {
-        return;
+    const int        wg   = blockIdx.x;
+    const int        keys = kChunk >> f.hgs;
+    const int        mask = (1 << f.hgs) - 1;
+    const int        nb   = NB <= 4 ? NB : f.nb;
+    const int        rb   = nb * UNIT;
+    const int32_t    total = few_line(f, 0, lane).total * f.groups;
+    const int32_t    last  = few_start(f, total, wg + 1);
+    int32_t          unit  = few_start(f, total, wg);
+
+    const Magic      magic;
+
+    // this lane's query, the same in every group
+    const int hc = static_cast<int>(fastdiv(static_cast<uint32_t>(c), f.fcols));
+    const int r  = c - hc * f.cols;
+    const int t  = static_cast<int>(fastdiv(static_cast<uint32_t>(r), a.fG));
+    // the least upper bound of a score of row 4 g + e (and 16 more): none where
+    // the row is of this query's head
+    float own[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        own[e] = ((4 * g + e) & mask) == hc ? INFINITY : -INFINITY;
     }
-    const int     keys = kChunk >> f.hgs;
-    const int     mask = (1 << f.hgs) - 1;
-    const int     rb   = f.nb * UNIT;
-    const int32_t base = len.length - len.count;
-    const int32_t p1   = len.length - 1;
-
-    // this lane's query
-    const int  hc   = static_cast<int>(fastdiv(static_cast<uint32_t>(c), f.fcols));
-    const int  r    = c - hc * f.cols;
-    const int  t    = static_cast<int>(fastdiv(static_cast<uint32_t>(r), a.fG));
-    const int  head = (h0 + hc) * a.G + r - t * a.G;
-    const bool live = hc <= mask && t < len.count;
-    const int32_t p = live ? base + t : -1;
-
-    f16x8 qh[NB], ql[NB];
-    float qscale;
-    {
-        const float * qr  = reinterpret_cast<const float *>(a.q + n * a.qn + t * a.qt + head * a.qh);
-        float         q[NB][8];
-        float         top = 0.0f;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                q[b][e] = live && b < f.nb ? qr[32 * b + C::element(g, e)] * a.scale : 0.0f;
-                top     = fmaxf(top, fabsf(q[b][e]));
-            }
-        }
-        top = max_quarters(top);
-        // the largest of the row in [2^13, 2^14)
-        const int ex    = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 127) - 13;
-        const float to  = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-        qscale          = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            f16x2 h[4], l[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                split2(q[b][2 * e] * to, q[b][2 * e + 1] * to, h[e], l[e]);
-            }
-            qh[b] = join8(h[0], h[1], h[2], h[3]);
-            ql[b] = join8(l[0], l[1], l[2], l[3]);
-        }
-    }
-
-    char *     kl = lds + wave * f.wave_lds;
+    f16x8 *    qop  = reinterpret_cast<f16x8 *>(lds);
+    float *    qmax = reinterpret_cast<float *>(qop + 2 * NB * kWave);
+    char *     kl   = lds + few_shared(NB, WAVES) + wave * f.wave_lds;
     char *     vl = kl + kChunk * rb;
     float *    kd = reinterpret_cast<float *>(vl + kChunk * rb);
     _Float16 * vd = reinterpret_cast<_Float16 *>(kd + NB * kChunk);
 
-    int32_t krel[P], vrel[P];
+    // where this lane's pieces lie, from a chunk's first byte: one run, or runs a key apart
+    int32_t krel[RUNS ? P : 1], vrel[RUNS ? P : 1];
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
+    for (int i = 0; i < (RUNS ? P : 1); ++i) {
         const int pc  = lane + i * kWave;
-        const int key = f.run > 0 ? static_cast<int>(fastdiv(static_cast<uint32_t>(pc), f.frun)) : 0;
+        const int key = RUNS ? static_cast<int>(fastdiv(static_cast<uint32_t>(pc), f.frun)) : 0;
         const int off = BYTES * (pc - key * f.run);
-        krel[i]       = key * static_cast<int32_t>(f.run > 0 ? a.kt : 0) + off;
-        vrel[i]       = key * static_cast<int32_t>(f.run > 0 ? a.vt : 0) + off;
+        krel[i]       = key * static_cast<int32_t>(RUNS ? a.kt : 0) + off;
+        vrel[i]       = key * static_cast<int32_t>(RUNS ? a.vt : 0) + off;
     }
-    const char * kb = a.k + n * a.kn + h0 * a.kh;
-    const char * vb = a.v + n * a.vn + h0 * a.vh;
-
-    // this lane's V words: word c + 16 s of each row
-    int vword[SLOTS], vblock[SLOTS];
+    // This lane's K words, those of its quarter in row c, and V words, word
+    // c + 16 s of the rows 4 g and on; a second start, two bytes on, for the
+    // blocks and rows that are an odd multiple of two bytes further.
+    const LdsWords k0(kl, c * rb + 2 + 4 * C::kStep * g);
+    const LdsWords k1(kl, c * rb + 4 + 4 * C::kStep * g);
+    int            vblock[SLOTS];
+    int            vword[SLOTS];
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-        const int w = min(c + 16 * s, f.nb * C::kWords - 1);
-        vword[s]    = C::word_offset(w);
+        const int w = min(c + 16 * s, nb * C::kWords - 1);
+        vword[s]    = 4 * g * rb + C::word_offset(w);
         vblock[s]   = w / C::kWords;
     }
+
+
+    if (unit >= last) {
+        return;
+    }
+    Place   at    = few_find(f, unit, lane);
+    int     n     = at.n;
+    int     hg    = f.groups == 1 ? 0 : (unit - at.before) / at.units;
+    int32_t begin = at.before + hg * at.units;  // the group's first unit
+    for (;;) {
+    const int     u0     = unit - begin;
+    const int     u1     = min(last - begin, at.units);
+    const int     h0     = hg << f.hgs;
+    const SeqLens  len   = seq_lens(a, n);
+    const KeyTiles kt    = few_tiles(f, len);
+    const int32_t base   = len.length - len.count;
+    const int32_t p1     = len.length - 1;
+    const int     head   = (h0 + hc) * a.G + r - t * a.G;
+    const bool    live   = hc <= mask && t < len.count;
+    const int32_t p      = live ? base + t : -1;
+
+    const char * kb = a.k + n * a.kn + h0 * a.kh;
+    const char * vb = a.v + n * a.vn + h0 * a.vh;
 
     f32x4 o[TILES];
 #pragma unroll
@@ -528,26 +693,71 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_few(const FewArgs f) {
     float m = -INFINITY;
     float l = 0.0f;
 
-    // the chunks of this split, every WAVES-th from `wave` on
-    KeyTiles kt{ 0, 0, 0 };
-    if (p1 >= 0) {
-        const int32_t last = p1 >> (5 - f.hgs);
-        if (a.window > 0) {
-            kt.second = max(base - a.window + 1, 0) >> (5 - f.hgs);
-            kt.first  = min((min(a.sinks, p1 + 1) + keys - 1) >> (5 - f.hgs), kt.second);
-        }
-        kt.n = kt.first + last - kt.second + 1;
-    }
-    const int per = (kt.n + a.nsplit - 1) / a.nsplit;
-    const int end = min(kt.n, (split + 1) * per);
-    int       i   = split * per + wave;
+    // the chunks of these units, one a wave
+    const int end = min(kt.n, u1 * f.per);
+    int       i   = u0 * f.per + wave;
 
     Staged<BYTES, P> ks, vs;
+    auto             fetch = [&](int32_t tile) {
+        const int32_t j0 = key_tile(kt, tile) << (5 - f.hgs);
+        const Rsrc    kr = rows_from(kb + static_cast<int64_t>(j0) * a.kt, static_cast<int64_t>(a.cap - j0 - 1) * a.kt + (rb << f.hgs));
+        const Rsrc    vr = rows_from(vb + static_cast<int64_t>(j0) * a.vt, static_cast<int64_t>(a.cap - j0 - 1) * a.vt + (rb << f.hgs));
+#pragma unroll
+        for (int x = 0; x < P; ++x) {
+            ks.load(x, kr, RUNS ? krel[x] : krel[0] + x * kWave * BYTES);
+            vs.load(x, vr, RUNS ? vrel[x] : krel[0] + x * kWave * BYTES);
+        }
+    };
     if (i < end) {
-        const int32_t j0 = key_tile(kt, i) << (5 - f.hgs);
-        fetch<BYTES, P>(f, kb, a.kt, krel, lane, j0, keys, rb, ks);
-        fetch<BYTES, P>(f, vb, a.vt, vrel, lane, j0, keys, rb, vs);
+        fetch(i);
     }
+    // The queries' operands, the same for every wave: in LDS, each wave's blocks
+    // formed by it. A query is scaled by a power of two that brings its largest
+    // value to [2^13, 2^14), so that both pieces of all that counts are normal.
+    float qscale;
+    {
+        constexpr int MINE = (NB + WAVES - 1) / WAVES;
+        const float * qr   = reinterpret_cast<const float *>(a.q + n * a.qn + t * a.qt + head * a.qh);
+        float         q[MINE][8];
+        float         top = 0.0f;
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) {
+            const int   b   = wave + k * WAVES;
+            const bool  has = live && b < nb;
+            const f32x4 x0  = has ? ld4u(qr + 32 * b + C::kFirst * g) : splat4(0.0f);
+            const f32x4 x1  = has ? ld4u(qr + 32 * b + C::kFirst * g + C::kSecond) : splat4(0.0f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                q[k][e] = (e < 4 ? x0[C::order(e)] : x1[C::order(e - 4)]) * a.scale;
+                top     = fmaxf(top, fabsf(q[k][e]));
+            }
+        }
+        qmax[wave * kWave + lane] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            top = fmaxf(top, qmax[w * kWave + lane]);
+        }
+        top = max_quarters(top);
+        const int ex   = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 127) - 13;
+        const float to = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+        qscale         = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) {
+            const int b = wave + k * WAVES;
+            f16x2     h[4], l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                split2(q[k][2 * e] * to, q[k][2 * e + 1] * to, h[e], l[e]);
+            }
+            if (b < nb) {
+                qop[(2 * b) * kWave + lane]     = join8(h[0], h[1], h[2], h[3]);
+                qop[(2 * b + 1) * kWave + lane] = join8(l[0], l[1], l[2], l[3]);
+            }
+        }
+        __syncthreads();
+    }
+
     for (; i < end; i += WAVES) {
         const int32_t j0 = key_tile(kt, i) << (5 - f.hgs);
         __builtin_amdgcn_wave_barrier();
@@ -555,14 +765,12 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_few(const FewArgs f) {
         for (int x = 0; x < P; ++x) {
             const int pc = lane + x * kWave;
             if (pc < f.pieces) {
-                reinterpret_cast<typename PieceOf<BYTES>::T *>(kl)[pc] = ks.piece[x];
-                reinterpret_cast<typename PieceOf<BYTES>::T *>(vl)[pc] = vs.piece[x];
+                ks.keep(x, kl, pc);
+                vs.keep(x, vl, pc);
             }
         }
         if (i + WAVES < end) {
-            const int32_t jn = key_tile(kt, i + WAVES) << (5 - f.hgs);
-            fetch<BYTES, P>(f, kb, a.kt, krel, lane, jn, keys, rb, ks);
-            fetch<BYTES, P>(f, vb, a.vt, vrel, lane, jn, keys, rb, vs);
+            fetch(i + WAVES);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -575,7 +783,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_few(const FewArgs f) {
             const bool         keep = isk || seen_by(a, base, p1, j0 + (row >> f.hgs));
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                if (b < f.nb) {
+                if (b < nb) {
                     const uint16_t d = *reinterpret_cast<const uint16_t *>(from + b * UNIT);
                     if (isk) {
                         kd[b * kChunk + row] = f16_bits_to_f32(d);
@@ -589,16 +797,23 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_few(const FewArgs f) {
         __builtin_amdgcn_wave_barrier();
 
         // scores: rows 16 mt + 4 g + e of the chunk against query c
-        f32x4 sc[2];
+        f32x4 sc[2] = { splat4(0.0f), splat4(0.0f) };
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-            sc[mt] = splat4(0.0f);
+        for (int b = 0; b < NB; ++b) {
+            if (b < nb) {
+                const f16x8 qh = qop[(2 * b) * kWave + lane];
+                const f16x8 ql = qop[(2 * b + 1) * kWave + lane];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                if (b < f.nb) {
-                    const f16x8 k = C::k_codes(kl + (16 * mt + c) * rb + b * UNIT, g);
-                    f32x4       x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[b], splat4(0.0f), 0, 0, 0);
-                    x             = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[b], x, 0, 0, 0);
+                for (int mt = 0; mt < 2; ++mt) {
+                    uint32_t w[C::kStep];
+#pragma unroll
+                    for (int i = 0; i < C::kStep; ++i) {
+                        const int off = 16 * mt * rb + b * UNIT + 4 * i;
+                        w[i]          = b % 2 == 0 ? k0.at(off) : k1.at(off - 2);
+                    }
+                    const f16x8 k = C::k_codes(magic, w);
+                    f32x4       x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh, splat4(0.0f), 0, 0, 0);
+                    x             = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql, x, 0, 0, 0);
                     const f32x4 d = *reinterpret_cast<const f32x4 *>(kd + b * kChunk + 16 * mt + 4 * g);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -607,15 +822,32 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_few(const FewArgs f) {
                 }
             }
         }
-        float top = m;
+        const bool all = j0 + keys - 1 <= base && (a.window == 0 || j0 > p1 - a.window || j0 + keys <= a.sinks);
+        float      top = m;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int  row = 16 * mt + 4 * g + e;
-                const bool see = (row & mask) == hc && sees(a, p, j0 + (row >> f.hgs));
-                sc[mt][e]      = see ? sc[mt][e] * qscale : -INFINITY;
-                top            = fmaxf(top, sc[mt][e]);
+                // (a NaN of its own head becomes +infinity, and the weights NaN)
+                sc[mt][e] = fminf(sc[mt][e] * qscale, own[e]);
+            }
+        }
+        if (!all) {  // keys that some queries do not see
+            int g4 = 4 * g;
+            asm volatile("" : "+v"(g4));  // (the rows' keys are not to wait in registers for this)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[mt][e] = sees(a, p, j0 + ((16 * mt + g4 + e) >> f.hgs)) ? sc[mt][e] : -INFINITY;
+                }
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                top = fmaxf(top, sc[mt][e]);
             }
         }
         top             = max_quarters(top);
@@ -653,17 +885,19 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_few(const FewArgs f) {
             const f16x4 d1 = *reinterpret_cast<const f16x4 *>(vd + vblock[s] * kChunk + 16 + 4 * g);
             d[0] = f16x2{ d0[0], d0[1] }, d[1] = f16x2{ d0[2], d0[3] };
             d[2] = f16x2{ d1[0], d1[1] }, d[3] = f16x2{ d1[2], d1[3] };
+            const LdsWords v0(vl, vword[s]);
+            const LdsWords v1(vl, vword[s] + 2);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int row = (e < 4 ? 0 : 12) + 4 * g + e;
-                w[e]          = *reinterpret_cast<const u32_at2 *>(vl + row * rb + vword[s]);
+                const int off = ((e < 4 ? 0 : 12) + e) * rb;
+                w[e]          = nb % 2 == 0 || e % 2 == 0 ? v0.at(off) : v1.at(off - 2);
             }
             auto tile = [&](auto uc) {
                 constexpr int U = decltype(uc)::value;
                 f16x2         hi[4], lo[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const f16x2 code = C::template v_codes<U>(w[2 * e], w[2 * e + 1]);
+                    const f16x2 code = C::template v_codes<U>(magic, w[2 * e], w[2 * e + 1]);
                     hi[e]            = code * d[e];
                     lo[e]            = __builtin_elementwise_fma(code, d[e], -hi[e]);
                 }
@@ -708,19 +942,17 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_few(const FewArgs f) {
         part[w] = __builtin_amdgcn_exp2f(ml[(w * 16 + c) * 2] - ref);
         l += part[w] * ml[(w * 16 + c) * 2 + 1];
     }
-    if (!live) {
-        return;
-    }
-    const int64_t row = ((static_cast<int64_t>(n) * a.KV + h0 + hc) * a.T + t) * a.G + r - t * a.G;
-    float *       out;
-    float         by = 1.0f;
-    if (a.nsplit == 1) {
+    if (live) {
+    float * out;
+    float   by = 1.0f;
+    if (u0 == 0 && u1 == at.units) {
         out = reinterpret_cast<float *>(a.y + n * a.yn + t * a.yt + head * a.yh);
         by  = over(l, p >= 0);
     } else {
-        out = partial_o(a, row, split);
+        const int which = u0 == 0 ? 1 : 0;
+        out             = few_o(f, wg, which, c);
         if (wave == 0 && g == 0) {
-            float * pml = partial_ml(a, row, split);
+            float * pml = few_ml(f, wg, which, c);
             pml[0]      = top;
             pml[1]      = l;
         }
@@ -734,37 +966,44 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_few(const FewArgs f) {
                 v += part[w] * of[((w * TILES + u) * 4 + e) * kWave + lane];
             }
             const int word = 16 * (u / C::kTiles) + 4 * g + e;
-            if (word < f.nb * C::kWords) {
+            if (word < nb * C::kWords) {
                 out[C::v_index(word, u % C::kTiles)] = v * by;
             }
         }
     }
+    }
+    unit = begin + u1;
+    if (unit >= last) {
+        return;
+    }
+    __syncthreads();  // the next group's chunks go where the results were
+    begin = unit;
+    if (++hg == f.groups) {
+        hg = 0;
+        do {
+            at.units = few_units(f, ++n);
+        } while (at.units == 0);
+    }
+    }
 }
 
-// The splits of a row joined: a workgroup a row, whose threads take HD values
-// of 256/HD of the splits each.
+// The parts of a row joined: a workgroup a row, whose threads take four values
+// of every 1024/HD-th part each.
 constexpr int kJoinThreads = 256;
 constexpr int kMaxSplits   = 512;
 
-template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join(const AttnArgs a, int64_t row0) {
-    constexpr int GROUPS = kJoinThreads / HD;
+// `parts` partial results of a row into out: ml(s) points to part s's m and l,
+// o(s) to its values. Left alone where the row has fewer than two parts.
+template <int HD, class ML, class O>
+__device__ __forceinline__ void join_parts(int parts, int hd, const ML & ml, const O & o, float * out, bool sees_any) {
+    constexpr int    GROUPS = kJoinThreads * 4 / HD;
     __shared__ float weight[kMaxSplits];
     __shared__ float lane_max[kJoinThreads / kWave], lane_sum[kJoinThreads / kWave];
-    __shared__ float sums[kJoinThreads];
-    const int64_t row = row0 + blockIdx.x;
-    const int     tid = threadIdx.x;
-    const int64_t gq  = row % a.G;
-    const int64_t t   = row / a.G % a.T;
-    const int64_t h   = row / a.G / a.T % a.KV;
-    const int     n   = static_cast<int>(row / a.G / a.T / a.KV);
-    const SeqLens len = seq_lens(a, n);
-    if (t >= len.count) {
-        return;
-    }
-    const float * ml  = partial_ml(a, row, 0);
-    float         top = -INFINITY;
-    for (int s = tid; s < a.nsplit; s += kJoinThreads) {
-        top = fmaxf(top, ml[2 * s]);
+    __shared__ f32x4 sums[kJoinThreads];
+    const int        tid = threadIdx.x;
+    float            top = -INFINITY;
+    for (int s = tid; s < parts; s += kJoinThreads) {
+        top = fmaxf(top, ml(s)[0]);
     }
     top = wave_max(top);
     if (tid % kWave == 0) {
@@ -777,10 +1016,10 @@ template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join(co
     }
     const float ref = top == -INFINITY ? 0.0f : top;
     float       l   = 0.0f;
-    for (int s = tid; s < a.nsplit; s += kJoinThreads) {
-        const float w = ml[2 * s + 1] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[2 * s] - ref);
+    for (int s = tid; s < parts; s += kJoinThreads) {
+        const float w = ml(s)[1] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml(s)[0] - ref);
         weight[s]     = w;
-        l += w * ml[2 * s + 1];
+        l += w * ml(s)[1];
     }
 #pragma unroll
     for (int off = 1; off < kWave; off *= 2) {
@@ -795,27 +1034,83 @@ template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join(co
     for (int w = 0; w < kJoinThreads / kWave; ++w) {
         l += lane_sum[w];
     }
-    const int     dim   = tid % HD;
-    const int     group = tid / HD;
-    const float * o     = partial_o(a, row, 0) + dim;
-    float         v     = 0.0f;
-    if (dim < a.hd) {
+    const int dim   = tid % (HD / 4) * 4;
+    const int group = tid / (HD / 4);
+    f32x4     v     = splat4(0.0f);
+    if (dim < hd) {
 #pragma unroll 8
-        for (int s = group; s < a.nsplit; s += GROUPS) {
-            const float w = weight[s];  // 0: no key, and nothing that counts in o
-            v += w != 0.0f ? o[static_cast<int64_t>(s) * a.hd] * w : 0.0f;
+        for (int s = group; s < parts; s += GROUPS) {
+            // weight 0: no key, and nothing that counts in o
+            const float w = weight[s];
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(o(s) + dim);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] += w != 0.0f ? x[e] * w : 0.0f;
+            }
         }
     }
     sums[tid] = v;
     __syncthreads();
-    if (group == 0 && dim < a.hd) {
-#pragma unroll
+    if (group == 0) {
         for (int k = 1; k < GROUPS; ++k) {
-            v += sums[k * HD + dim];
+            v += sums[k * (HD / 4) + tid];
         }
-        float * out = reinterpret_cast<float *>(a.y + n * a.yn + t * a.yt + (h * a.G + gq) * a.yh);
-        out[dim]    = v * over(l, len.length - len.count + t >= 0);
+        const float by = over(l, sees_any);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (dim + e < hd) {
+                out[dim + e] = v[e] * by;
+            }
+        }
     }
+}
+
+// A row of a call: sequence, kv head, position and query head of it.
+struct RowOf {
+    int32_t n, h, t, gq;
+};
+
+__device__ __forceinline__ RowOf row_of(const AttnArgs & a, int64_t row) {
+    const int64_t rt = row / a.G;
+    const int64_t rh = rt / a.T;
+    return RowOf{ static_cast<int32_t>(rh / a.KV), static_cast<int32_t>(rh % a.KV), static_cast<int32_t>(rt % a.T),
+                  static_cast<int32_t>(row % a.G) };
+}
+
+__device__ __forceinline__ float * out_of(const AttnArgs & a, const RowOf & r) {
+    return reinterpret_cast<float *>(a.y + r.n * a.yn + r.t * a.yt + (static_cast<int64_t>(r.h) * a.G + r.gq) * a.yh);
+}
+
+template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join(const AttnArgs a, int64_t row0) {
+    const int64_t row = row0 + blockIdx.x;
+    const RowOf   r   = row_of(a, row);
+    const SeqLens len = seq_lens(a, r.n);
+    if (r.t >= len.count) {
+        return;
+    }
+    join_parts<HD>(a.nsplit, a.hd, [&](int s) { return partial_ml(a, row, s); }, [&](int s) { return partial_o(a, row, s); },
+                   out_of(a, r), len.length - len.count + r.t >= 0);
+}
+
+template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join_few(const FewArgs f, int64_t row0) {
+    const AttnArgs & a   = f.a;
+    const RowOf      r   = row_of(a, row0 + blockIdx.x);
+    const SeqLens    len = seq_lens(a, r.n);
+    if (r.t >= len.count) {
+        return;
+    }
+    const Line    line  = few_line(f, r.n, threadIdx.x % kWave);
+    const int32_t total = line.total * f.groups;
+    const int32_t units = few_units(f, r.n);
+    const int32_t begin = line.before * f.groups + (r.h >> f.hgs) * units;
+    const int32_t w0    = few_owner(f, total, begin);
+    const int32_t w1    = few_owner(f, total, begin + units - 1);
+    if (w0 == w1) {
+        return;  // whole already
+    }
+    const int col = (r.h & ((1 << f.hgs) - 1)) * f.cols + r.t * a.G + r.gq;
+    join_parts<HD>(w1 - w0 + 1, a.hd, [&](int s) { return few_ml(f, w0 + s, s == 0, col); },
+                   [&](int s) { return few_o(f, w0 + s, s == 0, col); }, out_of(a, r), len.length - len.count + r.t >= 0);
 }
 
 // ---------------------------------------------------------------------------
@@ -836,11 +1131,21 @@ constexpr int64_t kAttnMaxKeys = int64_t{ 1 } << 30;
 struct AttnPlan {
     bool    few;
     int32_t hgs;
+    int32_t wgs;
+    int32_t per;
+    bool    parts;
     int32_t window;
     int32_t sinks;
     int32_t tiles;
     int32_t nsplit;
 };
+
+constexpr int64_t kWhole = 4;
+
+// Waves of a workgroup of k_attn_few: two where a row is long.
+constexpr int few_waves(int64_t hd) {
+    return hd <= 4 * kKvBlock ? 4 : 2;
+}
 
 shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t window, int32_t sinks, AttnPlan & p) {
     if (!well_formed(q) || !kv_well_formed(k_cache) || q->ne[0] != k_cache->ne[0] || q->ne[1] % k_cache->ne[1] != 0 ||
@@ -870,16 +1175,32 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
                k_cache->nb[1] == kv_bytes_of_row(*k_cache)) {
             ++p.hgs;
         }
-        const int64_t chunks = ((keys << p.hgs) + kChunk - 1) / kChunk;
-        p.nsplit             = plan_splits((kv >> p.hgs) * q->ne[3], (chunks + kMaxWaves - 1) / kMaxWaves, 1024);
-    } else {
+        const int     waves  = few_waves(k_cache->ne[0]);
+        const int64_t groups = (kv >> p.hgs) * q->ne[3];
+        const int64_t chunks = ((keys << p.hgs) + kChunk - 1) / kChunk + (p.window > 0 ? 2 : 0);
+        // up to kWhole chunks a wave a group is not split: that many take less than a second launch
+        const int64_t deep  = chunks <= kWhole * waves ? (chunks + waves - 1) / waves : 1;
+        const int64_t units = (chunks + waves * deep - 1) / (waves * deep) * groups;
+        p.per               = static_cast<int32_t>(waves * deep);
+        p.few               = units < INT32_MAX;
+        p.wgs               = static_cast<int32_t>(units < kMaxSplits ? units : kMaxSplits);
+        p.parts             = units > groups && p.wgs > 1;
+        // where the caches' strides are not that kernel's: as many splits as its workspace holds
+        const int64_t most = p.wgs * 2 * kCols / (q->ne[1] * q->ne[2] * q->ne[3]);
+        p.nsplit           = p.parts ? plan_splits(p.tiles * kv * q->ne[3], most, 2048) : 1;
+    }
+    if (!p.few) {
         p.nsplit = plan_splits(p.tiles * kv * q->ne[3], (keys + 63) / 64, 2048);
     }
     return SHP_OK;
 }
 
 int64_t plan_floats(const AttnPlan & p, const shp_tensor & q) {
-    return p.nsplit == 1 ? 0 : q.ne[1] * q.ne[2] * q.ne[3] * p.nsplit * (q.ne[0] + 2);
+    const int64_t row = (q.ne[0] + 3) / 4 * 4 + 2;
+    if (p.few) {
+        return !p.parts ? 0 : static_cast<int64_t>(p.wgs) * 2 * kCols * row;
+    }
+    return p.nsplit == 1 ? 0 : q.ne[1] * q.ne[2] * q.ne[3] * p.nsplit * row;
 }
 
 template <int KIND> shp_status_t launch_any(const AttnArgs & a, hipStream_t stream) {
@@ -916,7 +1237,8 @@ bool few_layout(const shp_tensor & c, int hgs, int piece, bool & together) {
         return false;
     }
     together = c.ne[2] == 1 || c.nb[2] == run;
-    return true;
+    // a descriptor's last bytes are read by the dword
+    return (run + (together ? static_cast<size_t>(c.ne[2] - 1) * run : size_t{ 0 })) % 4 == 0;
 }
 
 bool few_runs(const shp_tensor & c, int hgs, int piece) {
@@ -934,7 +1256,7 @@ int few_piece(const shp_tensor & k, const shp_tensor & v, int hgs, int32_t & run
         if (!few_layout(k, hgs, piece, kt) || !few_layout(v, hgs, piece, vt)) {
             continue;
         }
-        if (kt && vt) {
+        if (kt && vt && piece == 16) {
             run = 0;
             return piece;
         }
@@ -946,32 +1268,63 @@ int few_piece(const shp_tensor & k, const shp_tensor & v, int hgs, int32_t & run
     return 0;
 }
 
-template <int KIND, int NB, int BYTES, int WAVES> shp_status_t launch_few_as(FewArgs & f, hipStream_t stream) {
+template <int KIND, int NB, int BYTES, bool RUNS, int WAVES> shp_status_t launch_few_as(FewArgs & f, hipStream_t stream) {
     using C             = Codes<KIND>;
     constexpr int TILES = (NB * C::kWords + 15) / 16 * C::kTiles;
     const int     rb    = f.nb * kv_unit_bytes(KIND);
     f.wave_lds          = 2 * kChunk * rb + NB * kChunk * 6;
     const int join      = WAVES * (TILES * 4 * kWave + 32) * 4;
-    const int lds       = f.wave_lds * WAVES > join ? f.wave_lds * WAVES : join;
-    const dim3 grid(static_cast<unsigned>(f.a.nsplit), static_cast<unsigned>(f.a.KV >> f.hgs), static_cast<unsigned>(f.a.N));
-    hipLaunchKernelGGL((k_attn_few<KIND, NB, BYTES, WAVES>), grid, dim3(64 * WAVES), lds, stream, f);
-    return launch_status();
+    const int stage     = few_shared(NB, WAVES) + f.wave_lds * WAVES;
+    const int lds       = stage > join ? stage : join;
+    hipLaunchKernelGGL((k_attn_few<KIND, NB, BYTES, RUNS, WAVES>), dim3(static_cast<unsigned>(f.wgs)), dim3(64 * WAVES), lds, stream, f);
+    const shp_status_t st = launch_status();
+    if (st != SHP_OK || f.a.work == nullptr) {
+        return st;  // no group was split
+    }
+    constexpr int HD   = NB <= 2 ? 64 : NB <= 4 ? 128 : 256;
+    const int64_t rows = static_cast<int64_t>(f.a.N) * f.a.KV * f.a.T * f.a.G;
+    return in_launches(rows, kJoinThreads, [&](int64_t first, dim3 grid) {
+        hipLaunchKernelGGL((k_attn_join_few<HD>), grid, dim3(kJoinThreads), 0, stream, f, first);
+    });
 }
 
-template <int KIND> shp_status_t launch_few(const AttnArgs & a, int hgs, int piece, int32_t run, hipStream_t stream) {
+template <int KIND> shp_status_t launch_few(const AttnArgs & a, const AttnPlan & p, int piece, int32_t run, hipStream_t stream) {
     FewArgs f{};
     f.a      = a;
-    f.hgs    = hgs;
+    f.hgs    = p.hgs;
+    f.groups = a.KV >> p.hgs;
+    f.wgs    = p.wgs;
+    f.fwgs   = make_fastdiv(static_cast<uint32_t>(p.wgs));
+    f.per    = p.per;
+    f.fper   = make_fastdiv(static_cast<uint32_t>(p.per));
     f.cols   = a.T * a.G;
     f.nb     = a.hd / kKvBlock;
     f.pieces = kChunk * f.nb * kv_unit_bytes(KIND) / piece;
     f.run    = run;
     f.frun   = make_fastdiv(static_cast<uint32_t>(run > 0 ? run : 1));
     f.fcols  = make_fastdiv(static_cast<uint32_t>(f.cols));
-    if (f.nb <= 4) {
-        return piece == 16 ? launch_few_as<KIND, 4, 16, 4>(f, stream) : launch_few_as<KIND, 4, 4, 4>(f, stream);
+    auto go = [&](auto nb, auto waves) {
+        constexpr int NB = decltype(nb)::value, WAVES = decltype(waves)::value;
+        if constexpr (NB <= 4) {
+            if (piece == 4) {
+                return launch_few_as<KIND, NB, 4, true, WAVES>(f, stream);
+            }
+        }
+        return run > 0 ? launch_few_as<KIND, NB, 16, true, WAVES>(f, stream) : launch_few_as<KIND, NB, 16, false, WAVES>(f, stream);
+    };
+    using Four = std::integral_constant<int, 4>;
+    switch (f.nb) {
+        case 1:
+            return go(std::integral_constant<int, 1>{}, Four{});
+        case 2:
+            return go(std::integral_constant<int, 2>{}, Four{});
+        case 3:
+            return go(std::integral_constant<int, 3>{}, Four{});
+        case 4:
+            return go(Four{}, Four{});
+        default:
+            return go(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
     }
-    return launch_few_as<KIND, 8, 16, 2>(f, stream);
 }
 
 }  // namespace
@@ -1057,6 +1410,7 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
     a.G      = static_cast<int32_t>(q->ne[1] / k_cache->ne[1]);
     a.N      = static_cast<int32_t>(q->ne[3]);
     a.hd     = static_cast<int32_t>(q->ne[0]);
+    a.hd4    = (a.hd + 3) / 4 * 4;
     a.cap    = static_cast<int32_t>(k_cache->ne[2]);
     a.nsplit = p.nsplit;
     a.tiles  = p.tiles;
@@ -1067,8 +1421,7 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
     int32_t           run   = 0;
     const int         piece = p.few ? few_piece(*k_cache, *v_cache, p.hgs, run) : 0;
     if (piece > 0) {
-        st = kind == kKvQ4 ? launch_few<kKvQ4>(a, p.hgs, piece, run, s) : launch_few<kKvQ8>(a, p.hgs, piece, run, s);
-        return st == SHP_OK && a.nsplit > 1 ? launch_join(a, s) : st;
+        return kind == kKvQ4 ? launch_few<kKvQ4>(a, p, piece, run, s) : launch_few<kKvQ8>(a, p, piece, run, s);
     }
     switch (kind) {
         case kKvF32:
