@@ -41,6 +41,7 @@ struct AttnArgs {
     int32_t         tiles;  // of rows
     FastDiv         fG;
     FastDiv         fsplit;
+    FastDiv         fKV;
 };
 
 // The key tiles, KT rows each, that a tile of queries at positions p0..p1
@@ -987,6 +988,394 @@ __global__ __launch_bounds__(64 * WAVES, NB <= 4 ? 2 : 1) void k_attn_few(const 
     }
 }
 
+// ---------------------------------------------------------------------------
+// Many queries (prompts): a workgroup takes 128 rows, 32 a wave, and 64 keys at
+// a time, whose K and V it brings into LDS once, as matrix operands: K by row,
+// V by column with the keys in the order in which the scores stand in
+// registers. A block's code * d is exact as two F16 pieces; q and P are two
+// pieces as well, and each product is hi hi + hi lo + lo hi (a 16-bit cache has
+// no second piece). Matrix instructions 32x32x16: S^T = K Q^T has a query in
+// each lane, O^T = V^T P^T too.
+// ---------------------------------------------------------------------------
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kTileKeys  = 64;
+constexpr int kWideRows  = 128;
+constexpr int kWideBlock = 256;
+constexpr int kVStride   = kTileKeys * 2 + 16;  // bytes of a column of V in LDS, off the banks' period
+
+// A thread's part of a tile on its way to LDS: 32 values of a row of K, and of
+// V the four values u = 0..3 of each of eight keys, those that lie next to each
+// other in an operand: 16 s + 4 h + 0..3 and 8 more, group 2 s + h.
+template <int KIND> struct Part;
+
+template <> struct Part<kKvQ4> {
+    static constexpr bool kTwo = true;
+    uint32_t              k[4];
+    uint32_t              v[8];
+    uint16_t              kd;
+    uint16_t              vd[8];
+
+    __device__ void load_k(const char * block) {
+        kd = *reinterpret_cast<const uint16_t *>(block);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            k[i] = *reinterpret_cast<const u32_at2 *>(block + 2 + 4 * i);
+        }
+    }
+
+    // item: word `item % words` and half item / words of its nibbles
+    __device__ void load_v(int e, const char * row, int item, int words) {
+        const char * block = row + ((item % words) >> 2) * 18;
+        v[e]               = *reinterpret_cast<const u32_at2 *>(block + 2 + 4 * (item & 3));
+        vd[e]              = *reinterpret_cast<const uint16_t *>(block);
+    }
+
+    __device__ static int items(int nb) { return 8 * nb; }
+
+    __device__ static int words(int nb) { return 4 * nb; }
+
+    // value u of `item`
+    __device__ static int index(int item, int words, int u) {
+        const int w = item % words;
+        return 32 * (w >> 2) + 4 * (w & 3) + u + (item >= words ? 16 : 0);
+    }
+
+    __device__ f16x8 k_codes(const Magic & m, int j) const {
+        const uint32_t w[1] = { k[j] };
+        return Codes<kKvQ4>::k_codes(m, w);
+    }
+
+    template <int U> __device__ f16x2 v_codes(const Magic & m, int e, int item, int words) const {
+        const uint32_t shift = item >= words ? 4u : 0u;
+        return Codes<kKvQ4>::v_codes<2 * U>(m, v[e] >> shift, v[e + 1] >> shift);
+    }
+};
+
+template <> struct Part<kKvQ8> {
+    static constexpr bool kTwo = true;
+    uint32_t              k[8];
+    uint32_t              v[8];
+    uint16_t              kd;
+    uint16_t              vd[8];
+
+    __device__ void load_k(const char * block) {
+        kd = *reinterpret_cast<const uint16_t *>(block);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            k[i] = *reinterpret_cast<const u32_at2 *>(block + 2 + 4 * i);
+        }
+    }
+
+    __device__ void load_v(int e, const char * row, int item, int) {
+        const char * block = row + (item >> 3) * 34;
+        v[e]               = *reinterpret_cast<const u32_at2 *>(block + 2 + 4 * (item & 7));
+        vd[e]              = *reinterpret_cast<const uint16_t *>(block);
+    }
+
+    __device__ static int items(int nb) { return 8 * nb; }
+
+    __device__ static int words(int nb) { return 8 * nb; }
+
+    __device__ static int index(int item, int, int u) { return 4 * item + u; }
+
+    __device__ f16x8 k_codes(const Magic & m, int j) const {
+        const uint32_t w[2] = { k[2 * j], k[2 * j + 1] };
+        return Codes<kKvQ8>::k_codes(m, w);
+    }
+
+    template <int U> __device__ f16x2 v_codes(const Magic & m, int e, int, int) const {
+        return Codes<kKvQ8>::v_codes<U>(m, v[e], v[e + 1]);
+    }
+};
+
+template <int KIND, int NB> constexpr int wide_lds() {
+    constexpr int HD = NB * kKvBlock;
+    return (kTileKeys * (HD * 2 + 16) + HD * kVStride) * (Part<KIND>::kTwo ? 2 : 1);
+}
+
+template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_attn_wide(const AttnArgs a) {
+    using PartT             = Part<KIND>;
+    using C                 = Codes<KIND>;
+    constexpr int  HD       = NB * kKvBlock;
+    constexpr int  UNIT     = kv_unit_bytes(KIND);
+    constexpr int  KSTRIDE  = HD * 2 + 16;
+    constexpr bool TWO      = PartT::kTwo;
+    extern __shared__ char lds[];
+    char * const   kh   = lds;
+    char * const   kl   = kh + kTileKeys * KSTRIDE;  // (of two pieces)
+    char * const   vh   = kl + (TWO ? kTileKeys * KSTRIDE : 0);
+    char * const   vl   = vh + HD * kVStride;
+
+    const int     tid   = threadIdx.x;
+    const int     wave  = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int     lane  = tid % kWave;
+    const int     c     = lane & 31;
+    const int     g     = lane >> 5;
+    // a kv head's workgroups share an XCD where there are eight heads; the longest rows first
+    const int     part0 = static_cast<int>(fastdiv(blockIdx.x, a.fKV));
+    const int     h     = static_cast<int>(blockIdx.x) - part0 * a.KV;
+    const int     back  = static_cast<int>(fastdiv(static_cast<uint32_t>(part0), a.fsplit));
+    const int     tile  = a.tiles - 1 - back;
+    const int     split = part0 - back * a.nsplit;
+    const int     n     = blockIdx.y;
+    const SeqLens len   = seq_lens(a, n);
+    auto          t_of  = [&](int r) { return static_cast<int>(fastdiv(static_cast<uint32_t>(r), a.fG)); };
+    const int     t0    = t_of(tile * kWideRows);
+    if (t0 >= len.count) {
+        return;
+    }
+    const Magic   magic;
+    const int32_t base = len.length - len.count;
+    const int32_t p0   = base + t0;
+    const int32_t p1   = base + min(t_of(tile * kWideRows + kWideRows - 1), len.count - 1);
+    // this wave's positions, and this lane's query
+    const int     r0   = tile * kWideRows + wave * 32;
+    const int32_t w0   = base + t_of(r0);
+    const int32_t w1   = base + min(t_of(r0 + 31), len.count - 1);
+    const int     r    = r0 + c;
+    const int     t    = t_of(r);
+    const int     gq   = r - t * a.G;
+    const bool    live = t < len.count;
+    const int32_t p    = live ? base + t : -1;
+    const int     head = h * a.G + gq;
+
+    const KeyTiles kt  = key_tiles<kTileKeys>(a, p0, p1);
+    const int      per = static_cast<int>(fastdiv(static_cast<uint32_t>(kt.n + a.nsplit - 1), a.fsplit));
+    const int      end = min(kt.n, (split + 1) * per);
+    const int      beg = split * per;
+
+    // K: row tid / NB, block tid % NB; V: item tid % items of group tid / items
+    const int    items  = PartT::items(NB);
+    const int    words  = PartT::words(NB);
+    const bool   mine   = tid < kTileKeys * NB;
+    const int    krow   = tid / NB;
+    const int    kblk   = tid % NB;
+    const int    vgroup = tid / items;
+    const int    vitem  = tid % items;
+    const int    vkey   = 16 * (vgroup >> 1) + 4 * (vgroup & 1);
+    const char * kb     = a.k + n * a.kn + h * a.kh + kblk * UNIT;
+    const char * vb     = a.v + n * a.vn + h * a.vh;
+    PartT        part;
+    auto         fetch = [&](int i) {
+        const int32_t j0 = key_tile(kt, i) * kTileKeys;
+        if (mine) {
+            part.load_k(kb + static_cast<int64_t>(min(j0 + krow, p1)) * a.kt);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int32_t j = j0 + vkey + (e < 4 ? e : e + 4);
+                part.load_v(e, vb + static_cast<int64_t>(min(j, p1)) * a.vt, vitem, words);
+            }
+        }
+    };
+    if (beg < end) {
+        fetch(beg);
+    }
+
+    // the query's operands; the largest of its values scaled to [2^13, 2^14)
+    f16x8 qh[2 * NB], ql[2 * NB];
+    float qscale;
+    {
+        const float * qr = reinterpret_cast<const float *>(a.q + n * a.qn + t * a.qt + head * a.qh);
+        float         q[2 * NB][8];
+        float         top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 2 * NB; ++s) {
+            const float * at = qr + 32 * (s / 2) + C::kFirst * (2 * (s % 2) + g);
+            const f32x4   x0 = live ? ld4u(at) : splat4(0.0f);
+            const f32x4   x1 = live ? ld4u(at + C::kSecond) : splat4(0.0f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                q[s][e] = (e < 4 ? x0[C::order(e)] : x1[C::order(e - 4)]) * a.scale;
+                top     = fmaxf(top, fabsf(q[s][e]));
+            }
+        }
+        const Pair both = swap32(top);
+        top             = fmaxf(both.a, both.b);
+        const int ex    = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 127) - 13;
+        const float to  = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+        qscale          = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+#pragma unroll
+        for (int s = 0; s < 2 * NB; ++s) {
+            f16x2 hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                split2(q[s][2 * e] * to, q[s][2 * e + 1] * to, hi[e], lo[e]);
+            }
+            qh[s] = join8(hi[0], hi[1], hi[2], hi[3]);
+            ql[s] = join8(lo[0], lo[1], lo[2], lo[3]);
+        }
+    }
+
+    f32x16 o[NB];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+        o[u] = f32x16{};
+    }
+    float m = -INFINITY;
+    float l = 0.0f;
+
+    for (int i = beg; i < end; ++i) {
+        const int32_t j0 = key_tile(kt, i) * kTileKeys;
+        __syncthreads();  // the tile before is used up
+        if (mine) {
+            const bool  edge = j0 + kTileKeys - 1 > p0 || (a.window > 0 && j0 <= p1 - a.window && j0 + kTileKeys > a.sinks);
+            const f16x2 dk   = as_f16x2(part.kd * 0x10001u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f16x8 code = part.k_codes(magic, j);
+                f16x2       hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f16x2 x = { code[2 * e], code[2 * e + 1] };
+                    hi[e]         = x * dk;
+                    lo[e]         = __builtin_elementwise_fma(x, dk, -hi[e]);
+                }
+                const int at                            = krow * KSTRIDE + kblk * 64 + 16 * j;
+                *reinterpret_cast<f16x8 *>(kh + at) = join8(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<f16x8 *>(kl + at) = join8(lo[0], lo[1], lo[2], lo[3]);
+            }
+            f16x2 dv[4];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                uint32_t d = part.vd[e] | static_cast<uint32_t>(part.vd[e + 1]) << 16;
+                if (edge) {  // rows that no query of the tile sees count for nothing, whatever they hold
+                    const int32_t j = j0 + vkey + (e < 4 ? e : e + 4);
+                    d &= (seen_by(a, p0, p1, j) ? 0x0000ffffu : 0u) | (seen_by(a, p0, p1, j + 1) ? 0xffff0000u : 0u);
+                }
+                dv[e / 2] = as_f16x2(d);
+            }
+            auto column = [&](auto uc) {
+                constexpr int U = decltype(uc)::value;
+                f16x2         hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f16x2 x = part.template v_codes<U>(magic, 2 * e, vitem, words);
+                    hi[e]         = x * dv[e];
+                    lo[e]         = __builtin_elementwise_fma(x, dv[e], -hi[e]);
+                }
+                const int at                            = PartT::index(vitem, words, U) * kVStride + vgroup * 16;
+                *reinterpret_cast<f16x8 *>(vh + at) = join8(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<f16x8 *>(vl + at) = join8(lo[0], lo[1], lo[2], lo[3]);
+            };
+            for_each(std::make_integer_sequence<int, 4>{}, column);
+        }
+        if (i + 1 < end) {
+            fetch(i + 1);
+        }
+        __syncthreads();
+        if (j0 > w1) {
+            continue;  // none of it is seen by this wave's queries
+        }
+
+        // scores of key 32 x + 8 (i / 4) + 4 g + i % 4
+        f32x16 sc[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            sc[x] = f32x16{};
+#pragma unroll
+            for (int s = 0; s < 2 * NB; ++s) {
+                const int   at = (32 * x + c) * KSTRIDE + 32 * s + 16 * g;
+                const f16x8 hi = *reinterpret_cast<const f16x8 *>(kh + at);
+                sc[x]          = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qh[s], sc[x], 0, 0, 0);
+                sc[x]          = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, ql[s], sc[x], 0, 0, 0);
+                if constexpr (TWO) {
+                    const f16x8 lo = *reinterpret_cast<const f16x8 *>(kl + at);
+                    sc[x]          = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, qh[s], sc[x], 0, 0, 0);
+                }
+            }
+        }
+        const bool all = j0 + kTileKeys - 1 <= w0 && (a.window == 0 || j0 > w1 - a.window || j0 + kTileKeys <= a.sinks);
+        if (!all) {
+            int g4 = 4 * g;
+            asm volatile("" : "+v"(g4));
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    sc[x][e] = sees(a, p, j0 + 32 * x + 8 * (e / 4) + e % 4 + g4) ? sc[x][e] : -INFINITY;
+                }
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                top = fmaxf(top, sc[x][e]);
+            }
+        }
+        const Pair both = swap32(top);
+        top             = fmaxf(m, fmaxf(both.a, both.b) * qscale);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        if (__any(top > m)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - ref);
+            l *= alpha;
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+                o[u] *= alpha;
+            }
+        }
+        m = top;
+        const float less = kPShift - ref;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                f16x2 hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][8 * s + 2 * e], qscale, less));
+                    const float a1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][8 * s + 2 * e + 1], qscale, less));
+                    l += a0 + a1;
+                    split2(a0, a1, hi[e], lo[e]);
+                }
+                const f16x8 ph = join8(hi[0], hi[1], hi[2], hi[3]);
+                const f16x8 pl = join8(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+                for (int u = 0; u < NB; ++u) {
+                    const int   at = (32 * u + c) * kVStride + 64 * x + 32 * s + 16 * g;
+                    const f16x8 vv = *reinterpret_cast<const f16x8 *>(vh + at);
+                    o[u]           = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, ph, o[u], 0, 0, 0);
+                    o[u]           = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, pl, o[u], 0, 0, 0);
+                    if constexpr (TWO) {
+                        const f16x8 vw = *reinterpret_cast<const f16x8 *>(vl + at);
+                        o[u]           = __builtin_amdgcn_mfma_f32_32x32x16_f16(vw, ph, o[u], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+    const Pair sum = swap32(l);
+    l              = sum.a + sum.b;
+    if (!live) {
+        return;
+    }
+    const int64_t row = ((static_cast<int64_t>(n) * a.KV + h) * a.T + t) * a.G + gq;
+    float *       out;
+    float         by = 1.0f;
+    if (a.nsplit == 1) {
+        out = reinterpret_cast<float *>(a.y + n * a.yn + t * a.yt + head * a.yh);
+        by  = over(l, p >= 0);
+    } else {
+        out = partial_o(a, row, split);
+        if (g == 0) {
+            float * ml = partial_ml(a, row, split);
+            ml[0]      = m;
+            ml[1]      = l;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const f32x4 v                                            = { o[u][e] * by, o[u][e + 1] * by, o[u][e + 2] * by, o[u][e + 3] * by };
+            *reinterpret_cast<f32x4u *>(out + 32 * u + 2 * e + 4 * g) = v;
+        }
+    }
+}
+
 // The parts of a row joined: a workgroup a row, whose threads take four values
 // of every 1024/HD-th part each.
 constexpr int kJoinThreads = 256;
@@ -1130,6 +1519,7 @@ constexpr int64_t kAttnMaxKeys = int64_t{ 1 } << 30;
 
 struct AttnPlan {
     bool    few;
+    bool    wide;
     int32_t hgs;
     int32_t wgs;
     int32_t per;
@@ -1189,7 +1579,11 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
         const int64_t most = p.wgs * 2 * kCols / (q->ne[1] * q->ne[2] * q->ne[3]);
         p.nsplit           = p.parts ? plan_splits(p.tiles * kv * q->ne[3], most, 2048) : 1;
     }
-    if (!p.few) {
+    p.wide = !p.few && rows > 16 && kv_blocks(kv_kind(k_cache->type)) && k_cache->ne[0] <= 4 * kKvBlock;
+    if (p.wide) {
+        p.tiles  = static_cast<int32_t>((rows + kWideRows - 1) / kWideRows);
+        p.nsplit = plan_splits(p.tiles * kv * q->ne[3], (keys + 4 * kTileKeys - 1) / (4 * kTileKeys), 512);
+    } else if (!p.few) {
         p.nsplit = plan_splits(p.tiles * kv * q->ne[3], (keys + 63) / 64, 2048);
     }
     return SHP_OK;
@@ -1214,6 +1608,26 @@ template <int KIND> shp_status_t launch_any(const AttnArgs & a, hipStream_t stre
         hipLaunchKernelGGL((k_attn_any<KIND, 256>), grid, dim3(64), 0, stream, a);
     }
     return launch_status();
+}
+
+template <int KIND, int NB> shp_status_t launch_wide_as(const AttnArgs & a, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(a.KV) * static_cast<unsigned>(a.tiles) * static_cast<unsigned>(a.nsplit),
+                    static_cast<unsigned>(a.N));
+    hipLaunchKernelGGL((k_attn_wide<KIND, NB>), grid, dim3(kWideBlock), (wide_lds<KIND, NB>()), stream, a);
+    return launch_status();
+}
+
+template <int KIND> shp_status_t launch_wide(const AttnArgs & a, hipStream_t stream) {
+    switch ((a.hd + kKvBlock - 1) / kKvBlock) {
+        case 1:
+            return launch_wide_as<KIND, 1>(a, stream);
+        case 2:
+            return launch_wide_as<KIND, 2>(a, stream);
+        case 3:
+            return launch_wide_as<KIND, 3>(a, stream);
+        default:
+            return launch_wide_as<KIND, 4>(a, stream);
+    }
 }
 
 shp_status_t launch_join(const AttnArgs & a, hipStream_t stream) {
@@ -1416,12 +1830,17 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
     a.tiles  = p.tiles;
     a.fG     = make_fastdiv(static_cast<uint32_t>(a.G));
     a.fsplit = make_fastdiv(static_cast<uint32_t>(a.nsplit));
+    a.fKV    = make_fastdiv(static_cast<uint32_t>(a.KV));
     const hipStream_t s     = as_stream(stream);
     const int         kind  = kv_kind(k_cache->type);
     int32_t           run   = 0;
     const int         piece = p.few ? few_piece(*k_cache, *v_cache, p.hgs, run) : 0;
     if (piece > 0) {
         return kind == kKvQ4 ? launch_few<kKvQ4>(a, p, piece, run, s) : launch_few<kKvQ8>(a, p, piece, run, s);
+    }
+    if (p.wide) {
+        st = kind == kKvQ4 ? launch_wide<kKvQ4>(a, s) : launch_wide<kKvQ8>(a, s);
+        return st == SHP_OK && a.nsplit > 1 ? launch_join(a, s) : st;
     }
     switch (kind) {
         case kKvF32:
