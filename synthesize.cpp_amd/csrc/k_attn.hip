@@ -1007,11 +1007,15 @@ constexpr int kVStride   = kTileKeys * 2 + 16;  // bytes of a column of V in LDS
 
 // A thread's part of a tile on its way to LDS: 32 values of a row of K, and of
 // V the four values u = 0..3 of each of eight keys, those that lie next to each
-// other in an operand: 16 s + 4 h + 0..3 and 8 more, group 2 s + h.
+// other in an operand: 16 s + 4 h + 0..3 and 8 more, group 2 s + h. In column
+// `dim` of V the groups stand in the order group ^ (dim >> kTurn & 3): sixteen
+// lanes that write a group of sixteen columns then meet every bank once (four
+// times four without it: a third of the LDS unit's time).
 template <int KIND> struct Part;
 
 template <> struct Part<kKvQ4> {
-    static constexpr bool kTwo = true;
+    static constexpr bool kTwo  = true;
+    static constexpr int  kTurn = 5;
     uint32_t              k[4];
     uint32_t              v[8];
     uint16_t              kd;
@@ -1054,7 +1058,8 @@ template <> struct Part<kKvQ4> {
 };
 
 template <> struct Part<kKvQ8> {
-    static constexpr bool kTwo = true;
+    static constexpr bool kTwo  = true;
+    static constexpr int  kTurn = 4;
     uint32_t              k[8];
     uint32_t              v[8];
     uint16_t              kd;
@@ -1208,6 +1213,11 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
         }
     }
 
+    // group `even` + g of column 32 u + c
+    auto vat = [&](int u, int even) {
+        const int turn = (32 * u >> PartT::kTurn & 3) ^ (PartT::kTurn == 4 ? c >> 4 : 0);
+        return (32 * u + c) * kVStride + ((even + g) ^ turn) * 16;
+    };
     f32x16 o[NB];
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
@@ -1232,7 +1242,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
                     hi[e]         = x * dk;
                     lo[e]         = __builtin_elementwise_fma(x, dk, -hi[e]);
                 }
-                const int at                            = krow * KSTRIDE + kblk * 64 + 16 * j;
+                const int at = krow * KSTRIDE + kblk * 64 + 16 * j;
                 *reinterpret_cast<f16x8 *>(kh + at) = join8(hi[0], hi[1], hi[2], hi[3]);
                 *reinterpret_cast<f16x8 *>(kl + at) = join8(lo[0], lo[1], lo[2], lo[3]);
             }
@@ -1255,7 +1265,8 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
                     hi[e]         = x * dv[e];
                     lo[e]         = __builtin_elementwise_fma(x, dv[e], -hi[e]);
                 }
-                const int at                            = PartT::index(vitem, words, U) * kVStride + vgroup * 16;
+                const int dim = PartT::index(vitem, words, U);
+                const int at  = dim * kVStride + (vgroup ^ (dim >> PartT::kTurn & 3)) * 16;
                 *reinterpret_cast<f16x8 *>(vh + at) = join8(hi[0], hi[1], hi[2], hi[3]);
                 *reinterpret_cast<f16x8 *>(vl + at) = join8(lo[0], lo[1], lo[2], lo[3]);
             };
@@ -1270,19 +1281,30 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
         }
 
         // scores of key 32 x + 8 (i / 4) + 4 g + i % 4
-        f32x16 sc[2];
+        f32x16 sc[2] = { f32x16{}, f32x16{} };
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            sc[x] = f32x16{};
+        for (int s = 0; s < 2 * NB; ++s) {
+            f16x8 hi[2], lo[2];
 #pragma unroll
-            for (int s = 0; s < 2 * NB; ++s) {
-                const int   at = (32 * x + c) * KSTRIDE + 32 * s + 16 * g;
-                const f16x8 hi = *reinterpret_cast<const f16x8 *>(kh + at);
-                sc[x]          = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qh[s], sc[x], 0, 0, 0);
-                sc[x]          = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, ql[s], sc[x], 0, 0, 0);
+            for (int x = 0; x < 2; ++x) {
+                const int at = (32 * x + c) * KSTRIDE + 32 * s + 16 * g;
+                hi[x]        = *reinterpret_cast<const f16x8 *>(kh + at);
                 if constexpr (TWO) {
-                    const f16x8 lo = *reinterpret_cast<const f16x8 *>(kl + at);
-                    sc[x]          = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, qh[s], sc[x], 0, 0, 0);
+                    lo[x] = *reinterpret_cast<const f16x8 *>(kl + at);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[x], qh[s], sc[x], 0, 0, 0);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[x], ql[s], sc[x], 0, 0, 0);
+            }
+            if constexpr (TWO) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo[x], qh[s], sc[x], 0, 0, 0);
                 }
             }
         }
@@ -1333,15 +1355,27 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
                 }
                 const f16x8 ph = join8(hi[0], hi[1], hi[2], hi[3]);
                 const f16x8 pl = join8(lo[0], lo[1], lo[2], lo[3]);
+                f16x8 vv[NB];
 #pragma unroll
                 for (int u = 0; u < NB; ++u) {
-                    const int   at = (32 * u + c) * kVStride + 64 * x + 32 * s + 16 * g;
-                    const f16x8 vv = *reinterpret_cast<const f16x8 *>(vh + at);
-                    o[u]           = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, ph, o[u], 0, 0, 0);
-                    o[u]           = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv, pl, o[u], 0, 0, 0);
-                    if constexpr (TWO) {
-                        const f16x8 vw = *reinterpret_cast<const f16x8 *>(vl + at);
-                        o[u]           = __builtin_amdgcn_mfma_f32_32x32x16_f16(vw, ph, o[u], 0, 0, 0);
+                    vv[u] = *reinterpret_cast<const f16x8 *>(vh + vat(u, 4 * x + 2 * s));
+                }
+#pragma unroll
+                for (int u = 0; u < NB; ++u) {
+                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u], ph, o[u], 0, 0, 0);
+                }
+#pragma unroll
+                for (int u = 0; u < NB; ++u) {
+                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u], pl, o[u], 0, 0, 0);
+                }
+                if constexpr (TWO) {
+#pragma unroll
+                    for (int u = 0; u < NB; ++u) {
+                        vv[u] = *reinterpret_cast<const f16x8 *>(vl + vat(u, 4 * x + 2 * s));
+                    }
+#pragma unroll
+                    for (int u = 0; u < NB; ++u) {
+                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u], ph, o[u], 0, 0, 0);
                     }
                 }
             }
