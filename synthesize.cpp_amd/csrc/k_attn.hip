@@ -1021,20 +1021,25 @@ template <> struct Part<kKvQ4> {
     uint16_t              kd;
     uint16_t              vd[8];
 
-    __device__ void load_k(const char * block) {
-        kd = *reinterpret_cast<const uint16_t *>(block);
+    // the block `at` bytes into the tile
+    __device__ void load_k(const Rsrc & r, int at) {
+        kd = __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            k[i] = *reinterpret_cast<const u32_at2 *>(block + 2 + 4 * i);
+            k[i] = __builtin_amdgcn_raw_buffer_load_b32(r, at + 2 + 4 * i, 0, 0);
         }
     }
 
-    // item: word `item % words` and half item / words of its nibbles
-    __device__ void load_v(int e, const char * row, int item, int words) {
-        const char * block = row + ((item % words) >> 2) * 18;
-        v[e]               = *reinterpret_cast<const u32_at2 *>(block + 2 + 4 * (item & 3));
-        vd[e]              = *reinterpret_cast<const uint16_t *>(block);
+    // key e's word, `at` bytes into its row that is `row` bytes into the tile, and its d at `block`
+    __device__ void load_v(int e, const Rsrc & r, int at, int block, int row) {
+        v[e]  = __builtin_amdgcn_raw_buffer_load_b32(r, at, row, 0);
+        vd[e] = __builtin_amdgcn_raw_buffer_load_b16(r, block, row, 0);
     }
+
+    // item: word `item % words` and half item / words of its nibbles
+    __device__ static int block_at(int item, int words) { return ((item % words) >> 2) * 18; }
+
+    __device__ static int word_at(int item, int words) { return block_at(item, words) + 2 + 4 * (item & 3); }
 
     __device__ static int items(int nb) { return 8 * nb; }
 
@@ -1065,19 +1070,22 @@ template <> struct Part<kKvQ8> {
     uint16_t              kd;
     uint16_t              vd[8];
 
-    __device__ void load_k(const char * block) {
-        kd = *reinterpret_cast<const uint16_t *>(block);
+    __device__ void load_k(const Rsrc & r, int at) {
+        kd = __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            k[i] = *reinterpret_cast<const u32_at2 *>(block + 2 + 4 * i);
+            k[i] = __builtin_amdgcn_raw_buffer_load_b32(r, at + 2 + 4 * i, 0, 0);
         }
     }
 
-    __device__ void load_v(int e, const char * row, int item, int) {
-        const char * block = row + (item >> 3) * 34;
-        v[e]               = *reinterpret_cast<const u32_at2 *>(block + 2 + 4 * (item & 7));
-        vd[e]              = *reinterpret_cast<const uint16_t *>(block);
+    __device__ void load_v(int e, const Rsrc & r, int at, int block, int row) {
+        v[e]  = __builtin_amdgcn_raw_buffer_load_b32(r, at, row, 0);
+        vd[e] = __builtin_amdgcn_raw_buffer_load_b16(r, block, row, 0);
     }
+
+    __device__ static int block_at(int item, int) { return (item >> 3) * 34; }
+
+    __device__ static int word_at(int item, int) { return block_at(item, 0) + 2 + 4 * (item & 7); }
 
     __device__ static int items(int nb) { return 8 * nb; }
 
@@ -1160,17 +1168,24 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
     const int    vgroup = tid / items;
     const int    vitem  = tid % items;
     const int    vkey   = 16 * (vgroup >> 1) + 4 * (vgroup & 1);
-    const char * kb     = a.k + n * a.kn + h * a.kh + kblk * UNIT;
+    const char * kb     = a.k + n * a.kn + h * a.kh;
     const char * vb     = a.v + n * a.vn + h * a.vh;
+    const int    kstep  = static_cast<int>(a.kt);
+    const int    vstep  = static_cast<int>(a.vt);
+    const int    kat    = krow * kstep + kblk * UNIT;
+    const int    vat0   = vkey * vstep + PartT::word_at(vitem, words);
+    const int    vat1   = vkey * vstep + PartT::block_at(vitem, words);
     PartT        part;
-    auto         fetch = [&](int i) {
+    // (rows past the last that a query sees read as zero)
+    auto fetch = [&](int i) {
         const int32_t j0 = key_tile(kt, i) * kTileKeys;
+        const Rsrc    kr = rows_from(kb + j0 * a.kt, (p1 - j0) * a.kt + UNIT * NB);
+        const Rsrc    vr = rows_from(vb + j0 * a.vt, (p1 - j0) * a.vt + UNIT * NB);
         if (mine) {
-            part.load_k(kb + static_cast<int64_t>(min(j0 + krow, p1)) * a.kt);
+            part.load_k(kr, kat);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int32_t j = j0 + vkey + (e < 4 ? e : e + 4);
-                part.load_v(e, vb + static_cast<int64_t>(min(j, p1)) * a.vt, vitem, words);
+                part.load_v(e, vr, vat0, vat1, (e < 4 ? e : e + 4) * vstep);
             }
         }
     };
@@ -1281,6 +1296,9 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
         }
 
         // scores of key 32 x + 8 (i / 4) + 4 g + i % 4
+        // (ahead of the waves that are at their exponentials: 8192 positions 860
+        // to 790 us)
+        __builtin_amdgcn_s_setprio(1);
         f32x16 sc[2] = { f32x16{}, f32x16{} };
 #pragma unroll
         for (int s = 0; s < 2 * NB; ++s) {
@@ -1308,6 +1326,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
                 }
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         const bool all = j0 + kTileKeys - 1 <= w0 && (a.window == 0 || j0 > w1 - a.window || j0 + kTileKeys <= a.sinks);
         if (!all) {
             int g4 = 4 * g;
@@ -1551,6 +1570,9 @@ int32_t plan_splits(int64_t tiles, int64_t units, int64_t want) {
 // Positions and windows are int32, and so are their sums and differences.
 constexpr int64_t kAttnMaxKeys = int64_t{ 1 } << 30;
 
+// 64 rows at 32-bit offsets.
+constexpr size_t kWideStride = size_t{ 1 } << 24;
+
 struct AttnPlan {
     bool    few;
     bool    wide;
@@ -1613,7 +1635,7 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
         const int64_t most = p.wgs * 2 * kCols / (q->ne[1] * q->ne[2] * q->ne[3]);
         p.nsplit           = p.parts ? plan_splits(p.tiles * kv * q->ne[3], most, 2048) : 1;
     }
-    p.wide = !p.few && rows > 16 && kv_blocks(kv_kind(k_cache->type)) && k_cache->ne[0] <= 4 * kKvBlock;
+    p.wide = !p.few && rows > 16 && k_cache->nb[2] < kWideStride && kv_blocks(kv_kind(k_cache->type)) && k_cache->ne[0] <= 4 * kKvBlock;
     if (p.wide) {
         p.tiles  = static_cast<int32_t>((rows + kWideRows - 1) / kWideRows);
         p.nsplit = plan_splits(p.tiles * kv * q->ne[3], (keys + 4 * kTileKeys - 1) / (4 * kTileKeys), 512);
@@ -1871,6 +1893,10 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
     const int         piece = p.few ? few_piece(*k_cache, *v_cache, p.hgs, run) : 0;
     if (piece > 0) {
         return kind == kKvQ4 ? launch_few<kKvQ4>(a, p, piece, run, s) : launch_few<kKvQ8>(a, p, piece, run, s);
+    }
+    if (p.wide && v_cache->nb[2] >= kWideStride) {
+        p.wide  = false;  // the splits stay as the workspace has them
+        a.tiles = static_cast<int32_t>((static_cast<int64_t>(a.T) * a.G + 15) / 16);
     }
     if (p.wide) {
         st = kind == kKvQ4 ? launch_wide<kKvQ4>(a, s) : launch_wide<kKvQ8>(a, s);
