@@ -1,0 +1,742 @@
+// shp_attn_kv for many queries (prompts).
+#include "shp_attn.hpp"
+
+namespace shp {
+namespace {
+
+// ---------------------------------------------------------------------------
+// Many queries (prompts): a workgroup takes 128 rows, 32 a wave, and 64 keys at
+// a time, whose K and V it brings into LDS once, as matrix operands: K by row,
+// V by column with the keys in the order in which the scores stand in
+// registers. A block's code * d is exact as two F16 pieces; q and P are two
+// pieces as well, and each product is hi hi + hi lo + lo hi (a 16-bit cache has
+// no second piece). Matrix instructions 32x32x16: S^T = K Q^T has a query in
+// each lane, O^T = V^T P^T too.
+// ---------------------------------------------------------------------------
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kWideBlock = 256;
+constexpr int kVStride   = kTileKeys * 2 + 16;  // bytes of a column of V in LDS, off the banks' period
+
+// A thread's part of a tile on its way to LDS: 32 values of a row of K, and of
+// V the four values u = 0..3 of each of eight keys, those that lie next to each
+// other in an operand: 16 s + 4 h + 0..3 and 8 more, group 2 s + h. In column
+// `dim` of V the groups stand in the order group ^ (dim >> kTurn & 3): sixteen
+// lanes that write a group of sixteen columns then meet every bank once (four
+// times four without it: a third of the LDS unit's time).
+// The pieces are of the values times 2^-shift, where a tile's values are out of
+// F16's range or, F32 and BF16, always: their largest comes to [2^13, 2^14).
+//   load_k, load_v  from the cache, through descriptors of the tile
+//   keep_k, keep_v  or zeros in place of K's row, of V's of key e
+//   top_k, top_v    something that bounds the values' magnitudes (kScaled)
+//   k_pieces        operand j of the row's four, times `by`
+//   v_pieces        value U of the eight keys
+template <int KIND> struct Part;
+
+// Codes and d: exact products; a scale goes to d.
+template <int KIND, int WORDS> struct BlockPart {
+    static constexpr bool kTwo    = true;
+    static constexpr bool kScaled = true;
+    uint32_t              k[WORDS];
+    uint32_t              v[8];
+    uint16_t              kd;
+    uint16_t              vd[8];
+
+    // the block `at` bytes into the tile
+    __device__ void load_k(const Rsrc & r, int at) {
+        kd = __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0);
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            k[i] = __builtin_amdgcn_raw_buffer_load_b32(r, at + 2 + 4 * i, 0, 0);
+        }
+    }
+
+    // key e's word `at` bytes into its row, which is `row` bytes into the tile, and its d at `block`
+    __device__ void load_v(int e, const Rsrc & r, int at, int block, int row) {
+        v[e]  = __builtin_amdgcn_raw_buffer_load_b32(r, at, row, 0);
+        vd[e] = __builtin_amdgcn_raw_buffer_load_b16(r, block, row, 0);
+    }
+
+    __device__ void keep_k(bool yes) { kd = yes ? kd : 0; }
+
+    __device__ void keep_v(int e, bool yes) { vd[e] = yes ? vd[e] : 0; }
+
+    // d of at most 256 needs no scale: |code| <= 128
+    __device__ float top_k() const { return f16_bits_to_f32(kd & 0x7fffu); }
+
+    __device__ float top_v() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            m = max(m, vd[e] & 0x7fffu);
+        }
+        return f16_bits_to_f32(m);
+    }
+
+    static constexpr float kLeave = 256.0f;
+
+    __device__ static void exact(f16x2 code, f16x2 d, f16x2 & hi, f16x2 & lo) {
+        hi = code * d;
+        lo = __builtin_elementwise_fma(code, d, -hi);
+    }
+
+    __device__ void k_pieces(const Magic & m, float by, int j, f16x8 & hi, f16x8 & lo) const {
+        constexpr int STEP = WORDS / 4;
+        uint32_t      w[STEP];
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) {
+            w[i] = k[STEP * j + i];
+        }
+        const f16x8 code = Codes<KIND>::k_codes(m, w);
+        const f16x2 d    = as_f16x2(kd * 0x10001u) * splat2(by);
+        f16x2       h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            exact(f16x2{ code[2 * e], code[2 * e + 1] }, d, h[e], l[e]);
+        }
+        hi = join8(h[0], h[1], h[2], h[3]);
+        lo = join8(l[0], l[1], l[2], l[3]);
+    }
+
+    template <int U> __device__ void v_pieces(const Magic & m, float by, int shift, f16x8 & hi, f16x8 & lo) const {
+        f16x2 h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const f16x2 d = as_f16x2(vd[2 * e] | static_cast<uint32_t>(vd[2 * e + 1]) << 16) * splat2(by);
+            exact(Codes<KIND>::template v_codes<U>(m, v[2 * e] >> shift, v[2 * e + 1] >> shift), d, h[e], l[e]);
+        }
+        hi = join8(h[0], h[1], h[2], h[3]);
+        lo = join8(l[0], l[1], l[2], l[3]);
+    }
+};
+
+// V's items are a dword's four low or four high nibbles: item `words` + w.
+template <> struct Part<kKvQ4> : BlockPart<kKvQ4, 4> {
+    static constexpr int kTurn = 5;
+
+    __device__ static int words(int nb) { return 4 * nb; }
+
+    __device__ static int block_at(int item, int words) { return ((item % words) >> 2) * 18; }
+
+    __device__ static int word_at(int item, int words) { return block_at(item, words) + 2 + 4 * (item & 3); }
+
+    __device__ static int index(int item, int words, int u) {
+        const int w = item % words;
+        return 32 * (w >> 2) + 4 * (w & 3) + u + (item >= words ? 16 : 0);
+    }
+
+    template <int U> __device__ void v_column(const Magic & m, float by, int item, int words, f16x8 & hi, f16x8 & lo) const {
+        v_pieces<2 * U>(m, by, item >= words ? 4 : 0, hi, lo);
+    }
+};
+
+template <> struct Part<kKvQ8> : BlockPart<kKvQ8, 8> {
+    static constexpr int kTurn = 4;
+
+    __device__ static int words(int nb) { return 8 * nb; }
+
+    __device__ static int block_at(int item, int) { return (item >> 3) * 34; }
+
+    __device__ static int word_at(int item, int) { return block_at(item, 0) + 2 + 4 * (item & 7); }
+
+    __device__ static int index(int item, int, int u) { return 4 * item + u; }
+
+    template <int U> __device__ void v_column(const Magic & m, float by, int, int, f16x8 & hi, f16x8 & lo) const {
+        v_pieces<U>(m, by, 0, hi, lo);
+    }
+};
+
+// Plain values, four next to each other a key of V.
+template <int KIND> struct PlainPart {
+    static constexpr bool  kTwo    = KIND == kKvF32;
+    static constexpr bool  kScaled = KIND != kKvF16;
+    static constexpr int   kTurn   = 4;
+    static constexpr float kLeave  = 0.0f;
+    static constexpr int   kSize   = kv_unit_bytes(KIND);
+    static constexpr int   kFour   = kSize;  // dwords of four values
+    uint32_t               k[8 * kFour];
+    uint32_t               v[8][kFour];
+
+    __device__ void load_k(const Rsrc & r, int at) {
+#pragma unroll
+        for (int i = 0; i < 2 * kFour; ++i) {
+            const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, at + 16 * i, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                k[4 * i + e] = x[e];
+            }
+        }
+    }
+
+    // What a row has only `ks` values of K's 32 and `vs` of V's four (what was
+    // read behind them is the next row's, or zero).
+    __device__ void cut(int ks, int vs) {
+#pragma unroll
+        for (int i = 0; i < 8 * kFour; ++i) {
+            k[i] = within(k[i], i, ks);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+#pragma unroll
+            for (int i = 0; i < kFour; ++i) {
+                v[e][i] = within(v[e][i], i, vs);
+            }
+        }
+    }
+
+    __device__ static uint32_t within(uint32_t w, int i, int values) {
+        if constexpr (kSize == 4) {
+            return i < values ? w : 0;
+        } else {
+            return 2 * i + 1 < values ? w : 2 * i < values ? w & 0xffffu : 0;
+        }
+    }
+
+    __device__ void load_v(int e, const Rsrc & r, int at, int, int row) {
+        if constexpr (kFour == 4) {
+            const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, at, row, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[e][i] = x[i];
+            }
+        } else {
+            const auto x = __builtin_amdgcn_raw_buffer_load_b64(r, at, row, 0);
+            v[e][0]      = x[0];
+            v[e][1]      = x[1];
+        }
+    }
+
+    __device__ void keep_k(bool yes) {
+#pragma unroll
+        for (int i = 0; i < 8 * kFour; ++i) {
+            k[i] = yes ? k[i] : 0;
+        }
+    }
+
+    __device__ void keep_v(int e, bool yes) {
+#pragma unroll
+        for (int i = 0; i < kFour; ++i) {
+            v[e][i] = yes ? v[e][i] : 0;
+        }
+    }
+
+    __device__ static float value(const uint32_t * w, int i) {
+        if constexpr (KIND == kKvF32) {
+            return __uint_as_float(w[i]);
+        } else {
+            return i % 2 == 0 ? __uint_as_float(w[i / 2] << 16) : __uint_as_float(w[i / 2] & 0xffff0000u);
+        }
+    }
+
+    __device__ float top_k() const {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            m = fmaxf(m, fabsf(value(k, i)));
+        }
+        return m;
+    }
+
+    __device__ float top_v() const {
+        float m = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                m = fmaxf(m, fabsf(value(v[e], i)));
+            }
+        }
+        return m;
+    }
+
+    __device__ static int words(int nb) { return 8 * nb; }
+
+    __device__ static int block_at(int, int) { return 0; }
+
+    __device__ static int word_at(int item, int) { return item * 4 * kSize; }
+
+    __device__ static int index(int item, int, int u) { return 4 * item + u; }
+
+    __device__ static void pieces(float a, float b, float by, f16x2 & hi, f16x2 & lo) {
+        if constexpr (kTwo) {
+            split2(a * by, b * by, hi, lo);
+        } else {
+            hi = f16x2{ static_cast<_Float16>(a * by), static_cast<_Float16>(b * by) };
+        }
+    }
+
+    __device__ void k_pieces(const Magic &, float by, int j, f16x8 & hi, f16x8 & lo) const {
+        f16x2 h[4], l[4] = {};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (KIND == kKvF16) {
+                h[e] = as_f16x2(k[4 * j + e]);
+            } else {
+                pieces(value(k, 8 * j + 2 * e), value(k, 8 * j + 2 * e + 1), by, h[e], l[e]);
+            }
+        }
+        hi = join8(h[0], h[1], h[2], h[3]);
+        lo = join8(l[0], l[1], l[2], l[3]);
+    }
+
+    template <int U> __device__ void v_column(const Magic &, float by, int, int, f16x8 & hi, f16x8 & lo) const {
+        f16x2 h[4], l[4] = {};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (KIND == kKvF16) {
+                constexpr uint32_t kSel = U % 2 == 0 ? 0x05040100u : 0x07060302u;
+                h[e]                    = as_f16x2(__builtin_amdgcn_perm(v[2 * e + 1][U / 2], v[2 * e][U / 2], kSel));
+            } else {
+                pieces(value(v[2 * e], U), value(v[2 * e + 1], U), by, h[e], l[e]);
+            }
+        }
+        hi = join8(h[0], h[1], h[2], h[3]);
+        lo = join8(l[0], l[1], l[2], l[3]);
+    }
+};
+
+template <> struct Part<kKvF16> : PlainPart<kKvF16> {};
+
+template <> struct Part<kKvBF16> : PlainPart<kKvBF16> {};
+
+template <> struct Part<kKvF32> : PlainPart<kKvF32> {};
+
+// Bytes of 32 values of a row, and the order of K's in an operand of eight:
+// kFirst g + order(0..3), then kSecond more.
+template <int KIND> struct KOrder {
+    static constexpr int kFirst = 8, kSecond = 4;
+
+    __device__ static constexpr int order(int e) { return e; }
+};
+
+template <> struct KOrder<kKvQ4> : Codes<kKvQ4> {};
+
+// 2^e, e in [-126, 127].
+__device__ __forceinline__ float pow2(int e) {
+    return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
+// The shift that brings values bounded by `top` to [2^13, 2^14), if they need one.
+template <int KIND> __device__ __forceinline__ int shift_of(float top) {
+    if (!Part<KIND>::kScaled || (kv_blocks(KIND) && top <= Part<KIND>::kLeave)) {
+        return 0;
+    }
+    const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 127) - 13;
+    return kv_blocks(KIND) ? e + 8 : e;  // of d: codes are up to 2^7
+}
+
+template <int KIND, int NB> constexpr int wide_lds() {
+    constexpr int HD = NB * kKvBlock;
+    return (kTileKeys * (HD * 2 + 16) + HD * kVStride) * (Part<KIND>::kTwo ? 2 : 1) + (Part<KIND>::kScaled ? 32 : 0);
+}
+
+template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_attn_wide(const AttnArgs a) {
+    using PartT             = Part<KIND>;
+    using C                 = KOrder<KIND>;
+    constexpr int  HD       = NB * kKvBlock;
+    constexpr int  UNIT     = kv_unit_bytes(KIND) * (kv_blocks(KIND) ? 1 : kKvBlock);
+    constexpr int  KSTRIDE  = HD * 2 + 16;
+    constexpr bool TWO      = PartT::kTwo;
+    extern __shared__ char lds[];
+    char * const   kh   = lds;
+    char * const   kl   = kh + kTileKeys * KSTRIDE;  // (of two pieces)
+    char * const   vh   = kl + (TWO ? kTileKeys * KSTRIDE : 0);
+    char * const   vl   = vh + HD * kVStride;
+    float * const  tops = reinterpret_cast<float *>(vl + (TWO ? HD * kVStride : 0));  // of each wave's K and V
+
+    const int     tid   = threadIdx.x;
+    const int     wave  = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int     lane  = tid % kWave;
+    const int     c     = lane & 31;
+    const int     g     = lane >> 5;
+    // a kv head's workgroups share an XCD where there are eight heads; the longest rows first
+    const int     part0 = static_cast<int>(fastdiv(blockIdx.x, a.fKV));
+    const int     h     = static_cast<int>(blockIdx.x) - part0 * a.KV;
+    const int     back  = static_cast<int>(fastdiv(static_cast<uint32_t>(part0), a.fsplit));
+    const int     tile  = a.tiles - 1 - back;
+    const int     split = part0 - back * a.nsplit;
+    const int     n     = blockIdx.y;
+    const SeqLens len   = seq_lens(a, n);
+    auto          t_of  = [&](int r) { return static_cast<int>(fastdiv(static_cast<uint32_t>(r), a.fG)); };
+    const int     t0    = t_of(tile * kWideRows);
+    if (t0 >= len.count) {
+        return;
+    }
+    const Magic   magic;
+    const int32_t base = len.length - len.count;
+    const int32_t p0   = base + t0;
+    const int32_t p1   = base + min(t_of(tile * kWideRows + kWideRows - 1), len.count - 1);
+    // this wave's positions, and this lane's query
+    const int     r0   = tile * kWideRows + wave * 32;
+    const int32_t w0   = base + t_of(r0);
+    const int32_t w1   = t_of(r0) < len.count ? base + min(t_of(r0 + 31), len.count - 1) : -1;
+    const int     r    = r0 + c;
+    const int     t    = t_of(r);
+    const int     gq   = r - t * a.G;
+    const bool    live = t < len.count;
+    const int32_t p    = live ? base + t : -1;
+    const int     head = h * a.G + gq;
+
+    const KeyTiles kt  = key_tiles<kTileKeys>(a, p0, p1);
+    const int      per = static_cast<int>(fastdiv(static_cast<uint32_t>(kt.n + a.nsplit - 1), a.fsplit));
+    const int      end = min(kt.n, (split + 1) * per);
+    const int      beg = split * per;
+
+    // K: row tid / NB, block tid % NB; V: item tid % items of group tid / items
+    const int    items  = 8 * NB;
+    const int    words  = PartT::words(NB);
+    const bool   mine   = tid < kTileKeys * NB;
+    const int    krow   = tid / NB;
+    const int    kblk   = tid % NB;
+    const int    vgroup = tid / items;
+    const int    vitem  = tid % items;
+    const int    vkey   = 16 * (vgroup >> 1) + 4 * (vgroup & 1);
+    const char * kb     = a.k + n * a.kn + h * a.kh;
+    const char * vb     = a.v + n * a.vn + h * a.vh;
+    const int    kstep  = static_cast<int>(a.kt);
+    const int    vstep  = static_cast<int>(a.vt);
+    const int    kat    = krow * kstep + kblk * UNIT;
+    const int    vat0   = vkey * vstep + PartT::word_at(vitem, words);
+    const int    vat1   = vkey * vstep + PartT::block_at(vitem, words);
+    const int    rb     = static_cast<int>(kv_row_bytes(KIND, a.hd));
+    PartT        part;
+    // (rows past the last that a query sees read as zero)
+    auto fetch = [&](int i) {
+        const int32_t j0 = key_tile(kt, i) * kTileKeys;
+        const Rsrc    kr = rows_from(kb + j0 * a.kt, (p1 - j0) * a.kt + rb);
+        const Rsrc    vr = rows_from(vb + j0 * a.vt, (p1 - j0) * a.vt + rb);
+        if (mine) {
+            part.load_k(kr, kat);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                part.load_v(e, vr, vat0, vat1, (e < 4 ? e : e + 4) * vstep);
+            }
+        }
+    };
+    if (beg < end) {
+        fetch(beg);
+    }
+
+    auto values = [&](const float * row, int at, bool has) {
+        f32x4 x = splat4(0.0f);
+        if (has && (kv_blocks(KIND) || at + 4 <= a.hd)) {
+            x = ld4u(row + at);
+        } else if (has) {
+            for (int e = 0; at + e < a.hd; ++e) {
+                x[e] = row[at + e];
+            }
+        }
+        return x;
+    };
+    // the query's operands; the largest of its values scaled to [2^13, 2^14)
+    f16x8 qh[2 * NB], ql[2 * NB];
+    float qscale;
+    {
+        const float * qr = reinterpret_cast<const float *>(a.q + n * a.qn + t * a.qt + head * a.qh);
+        float         q[2 * NB][8];
+        float         top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 2 * NB; ++s) {
+            const int     at = 32 * (s / 2) + C::kFirst * (2 * (s % 2) + g);
+            const f32x4   x0 = values(qr, at, live);
+            const f32x4   x1 = values(qr, at + C::kSecond, live);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                q[s][e] = (e < 4 ? x0[C::order(e)] : x1[C::order(e - 4)]) * a.scale;
+                top     = fmaxf(top, fabsf(q[s][e]));
+            }
+        }
+        const Pair both = swap32(top);
+        top             = fmaxf(both.a, both.b);
+        const int ex    = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 127) - 13;
+        const float to  = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+        qscale          = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+#pragma unroll
+        for (int s = 0; s < 2 * NB; ++s) {
+            f16x2 hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                split2(q[s][2 * e] * to, q[s][2 * e + 1] * to, hi[e], lo[e]);
+            }
+            qh[s] = join8(hi[0], hi[1], hi[2], hi[3]);
+            ql[s] = join8(lo[0], lo[1], lo[2], lo[3]);
+        }
+    }
+
+    // group `even` + g of column 32 u + c
+    auto vat = [&](int u, int even) {
+        const int turn = (32 * u >> PartT::kTurn & 3) ^ (PartT::kTurn == 4 ? c >> 4 : 0);
+        return (32 * u + c) * kVStride + ((even + g) ^ turn) * 16;
+    };
+    f32x16 o[NB];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+        o[u] = f32x16{};
+    }
+    float m    = -INFINITY;
+    float l    = 0.0f;
+    int   vexp = shift_of<KIND>(0.0f);  // V in LDS is times 2^-vexp, o times 2^-oexp
+    int   oexp = vexp;
+
+    for (int i = beg; i < end; ++i) {
+        const int32_t j0 = key_tile(kt, i) * kTileKeys;
+        float kby = 1.0f, vby = 1.0f;
+        int   kexp = 0;
+        if (mine) {
+            const bool edge = j0 + kTileKeys - 1 > p0 || (a.window > 0 && j0 <= p1 - a.window && j0 + kTileKeys > a.sinks);
+            if (edge) {  // rows that no query of the tile sees count for nothing, whatever they hold
+                part.keep_k(seen_by(a, p0, p1, j0 + krow));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    part.keep_v(e, seen_by(a, p0, p1, j0 + vkey + (e < 4 ? e : e + 4)));
+                }
+            }
+            if constexpr (!kv_blocks(KIND)) {
+                if (a.hd < HD) {
+                    part.cut(a.hd - kKvBlock * kblk, a.hd - 4 * vitem);
+                }
+            }
+        }
+        if constexpr (PartT::kScaled) {
+            const float tk = wave_max(mine ? part.top_k() : 0.0f);
+            const float tv = wave_max(mine ? part.top_v() : 0.0f);
+            if (lane == 0) {
+                tops[2 * wave]     = tk;
+                tops[2 * wave + 1] = tv;
+            }
+        }
+        __syncthreads();  // the tile before is used up
+        if constexpr (PartT::kScaled) {
+            float tk = 0.0f, tv = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWideBlock / kWave; ++w) {
+                tk = fmaxf(tk, tops[2 * w]);
+                tv = fmaxf(tv, tops[2 * w + 1]);
+            }
+            // K by tile; V never less than for the tiles before, which o holds
+            kexp = shift_of<KIND>(tk);
+            vexp = max(vexp, shift_of<KIND>(tv));
+            kby  = pow2(-kexp);
+            vby  = pow2(-vexp);
+        }
+        if (mine) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f16x8 hi, lo;
+                part.k_pieces(magic, kby, j, hi, lo);
+                const int at = krow * KSTRIDE + kblk * 64 + 16 * j;
+                *reinterpret_cast<f16x8 *>(kh + at) = hi;
+                if constexpr (TWO) {
+                    *reinterpret_cast<f16x8 *>(kl + at) = lo;
+                }
+            }
+            auto column = [&](auto uc) {
+                constexpr int U = decltype(uc)::value;
+                f16x8         hi, lo;
+                part.template v_column<U>(magic, vby, vitem, words, hi, lo);
+                const int dim = PartT::index(vitem, words, U);
+                const int at  = dim * kVStride + (vgroup ^ (dim >> PartT::kTurn & 3)) * 16;
+                *reinterpret_cast<f16x8 *>(vh + at) = hi;
+                if constexpr (TWO) {
+                    *reinterpret_cast<f16x8 *>(vl + at) = lo;
+                }
+            };
+            for_each(std::make_integer_sequence<int, 4>{}, column);
+        }
+        if (i + 1 < end) {
+            fetch(i + 1);
+        }
+        __syncthreads();
+        if (j0 > w1) {
+            continue;  // none of it is seen by this wave's queries
+        }
+        const float qs = qscale * pow2(kexp);
+        if (PartT::kScaled && vexp != oexp) {
+            const float by = pow2(max(oexp - vexp, -126));
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+                o[u] *= by;
+            }
+            oexp = vexp;
+        }
+
+        // scores of key 32 x + 8 (i / 4) + 4 g + i % 4
+        // (ahead of the waves that are at their exponentials: 8192 positions 860
+        // to 790 us)
+        __builtin_amdgcn_s_setprio(1);
+        f32x16 sc[2] = { f32x16{}, f32x16{} };
+#pragma unroll
+        for (int s = 0; s < 2 * NB; ++s) {
+            f16x8 hi[2], lo[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int at = (32 * x + c) * KSTRIDE + 32 * s + 16 * g;
+                hi[x]        = *reinterpret_cast<const f16x8 *>(kh + at);
+                if constexpr (TWO) {
+                    lo[x] = *reinterpret_cast<const f16x8 *>(kl + at);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[x], qh[s], sc[x], 0, 0, 0);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[x], ql[s], sc[x], 0, 0, 0);
+            }
+            if constexpr (TWO) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo[x], qh[s], sc[x], 0, 0, 0);
+                }
+            }
+        }
+        __builtin_amdgcn_s_setprio(0);
+        const bool all = j0 + kTileKeys - 1 <= w0 && (a.window == 0 || j0 > w1 - a.window || j0 + kTileKeys <= a.sinks);
+        if (!all) {
+            int g4 = 4 * g;
+            asm volatile("" : "+v"(g4));
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    sc[x][e] = sees(a, p, j0 + 32 * x + 8 * (e / 4) + e % 4 + g4) ? sc[x][e] : -INFINITY;
+                }
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                top = fmaxf(top, sc[x][e]);
+            }
+        }
+        const Pair both = swap32(top);
+        top             = fmaxf(m, fmaxf(both.a, both.b) * qs);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        if (__any(top > m)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - ref);
+            l *= alpha;
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+                o[u] *= alpha;
+            }
+        }
+        m = top;
+        const float less = kPShift - ref;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                f16x2 hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][8 * s + 2 * e], qs, less));
+                    const float a1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][8 * s + 2 * e + 1], qs, less));
+                    l += a0 + a1;
+                    split2(a0, a1, hi[e], lo[e]);
+                }
+                const f16x8 ph = join8(hi[0], hi[1], hi[2], hi[3]);
+                const f16x8 pl = join8(lo[0], lo[1], lo[2], lo[3]);
+                f16x8 vv[NB];
+#pragma unroll
+                for (int u = 0; u < NB; ++u) {
+                    vv[u] = *reinterpret_cast<const f16x8 *>(vh + vat(u, 4 * x + 2 * s));
+                }
+#pragma unroll
+                for (int u = 0; u < NB; ++u) {
+                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u], ph, o[u], 0, 0, 0);
+                }
+#pragma unroll
+                for (int u = 0; u < NB; ++u) {
+                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u], pl, o[u], 0, 0, 0);
+                }
+                if constexpr (TWO) {
+#pragma unroll
+                    for (int u = 0; u < NB; ++u) {
+                        vv[u] = *reinterpret_cast<const f16x8 *>(vl + vat(u, 4 * x + 2 * s));
+                    }
+#pragma unroll
+                    for (int u = 0; u < NB; ++u) {
+                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u], ph, o[u], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+    const Pair sum = swap32(l);
+    l              = sum.a + sum.b;
+    if (!live) {
+        return;
+    }
+    const int64_t row = ((static_cast<int64_t>(n) * a.KV + h) * a.T + t) * a.G + gq;
+    float *       out;
+    float         by = pow2(oexp);
+    if (a.nsplit == 1) {
+        out = reinterpret_cast<float *>(a.y + n * a.yn + t * a.yt + head * a.yh);
+        by *= over(l, p >= 0);
+    } else {
+        out = partial_o(a, row, split);
+        if (g == 0) {
+            float * ml = partial_ml(a, row, split);
+            ml[0]      = m;
+            ml[1]      = l;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int   dim = 32 * u + 2 * e + 4 * g;
+            const f32x4 v   = { o[u][e] * by, o[u][e + 1] * by, o[u][e + 2] * by, o[u][e + 3] * by };
+            if (kv_blocks(KIND) || dim + 4 <= a.hd) {
+                *reinterpret_cast<f32x4u *>(out + dim) = v;
+            } else {
+                for (int k = 0; dim + k < a.hd; ++k) {
+                    out[dim + k] = v[k];
+                }
+            }
+        }
+    }
+}
+
+template <int KIND, int NB> shp_status_t launch_wide_as(const AttnArgs & a, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(a.KV) * static_cast<unsigned>(a.tiles) * static_cast<unsigned>(a.nsplit),
+                    static_cast<unsigned>(a.N));
+    hipLaunchKernelGGL((k_attn_wide<KIND, NB>), grid, dim3(kWideBlock), (wide_lds<KIND, NB>()), stream, a);
+    return launch_status();
+}
+
+template <int KIND> shp_status_t launch_wide(const AttnArgs & a, hipStream_t stream) {
+    switch ((a.hd + kKvBlock - 1) / kKvBlock) {
+        case 1:
+            return launch_wide_as<KIND, 1>(a, stream);
+        case 2:
+            return launch_wide_as<KIND, 2>(a, stream);
+        case 3:
+            return launch_wide_as<KIND, 3>(a, stream);
+        default:
+            return launch_wide_as<KIND, 4>(a, stream);
+    }
+}
+
+}  // namespace
+
+shp_status_t launch_attn_wide(int kind, const AttnArgs & a, hipStream_t stream) {
+    switch (kind) {
+        case kKvF32:
+            return launch_wide<kKvF32>(a, stream);
+        case kKvF16:
+            return launch_wide<kKvF16>(a, stream);
+        case kKvBF16:
+            return launch_wide<kKvBF16>(a, stream);
+        case kKvQ8:
+            return launch_wide<kKvQ8>(a, stream);
+        default:
+            return launch_wide<kKvQ4>(a, stream);
+    }
+}
+
+}  // namespace shp
