@@ -150,6 +150,55 @@ template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join(co
                    out_of(a, r), len.length - len.count + r.t >= 0);
 }
 
+// Many rows of a few parts: HD/4 lanes a row, each the row's weights for itself
+// (16336 rows of four parts, MI355X: 9.7 us, 26 a workgroup a row).
+constexpr int kFewParts = 8;
+
+template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join_rows(const AttnArgs a, int64_t row0) {
+    constexpr int ROWS = kJoinThreads * 4 / HD;
+    const int64_t row  = row0 + static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / (HD / 4);
+    const int     dim  = threadIdx.x % (HD / 4) * 4;
+    if (row >= static_cast<int64_t>(a.N) * a.KV * a.T * a.G || dim >= a.hd) {
+        return;
+    }
+    const RowOf   r   = row_of(a, row);
+    const SeqLens len = seq_lens(a, r.n);
+    if (r.t >= len.count) {
+        return;
+    }
+    float m[kFewParts], l[kFewParts];
+    f32x4 o[kFewParts];
+    float top = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < kFewParts; ++s) {
+        const int     p  = min(s, a.nsplit - 1);
+        const float * ml = partial_ml(a, row, p);
+        m[s]             = ml[0];
+        l[s]             = s < a.nsplit ? ml[1] : 0.0f;
+        o[s]             = s < a.nsplit ? *reinterpret_cast<const f32x4 *>(partial_o(a, row, p) + dim) : splat4(0.0f);
+        top              = fmaxf(top, m[s]);
+    }
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float       sum = 0.0f;
+    f32x4       v   = splat4(0.0f);
+#pragma unroll
+    for (int s = 0; s < kFewParts; ++s) {
+        if (l[s] != 0.0f) {  // (no key, and nothing that counts in o)
+            const float w = __builtin_amdgcn_exp2f(m[s] - ref);
+            sum += w * l[s];
+            v += o[s] * w;
+        }
+    }
+    const float by  = over(sum, len.length - len.count + r.t >= 0);
+    float *     out = out_of(a, r) + dim;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (dim + e < a.hd) {
+            out[e] = v[e] * by;
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -173,12 +222,8 @@ bool wide_takes(const shp_tensor & c) {
            (kv_blocks(kv_kind(c.type)) || kv_bytes_of_row(c) % 4 == 0);
 }
 
-constexpr int64_t kWhole = 4;
-
-// Waves of a workgroup of k_attn_few: two where a row is long.
-constexpr int few_waves(int64_t hd) {
-    return hd <= 4 * kKvBlock ? 4 : 2;
-}
+constexpr int64_t kWhole       = 4;
+constexpr int64_t kShortGroups = 256;
 
 shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t window, int32_t sinks, AttnPlan & p) {
     if (!well_formed(q) || !kv_well_formed(k_cache) || q->ne[0] != k_cache->ne[0] || q->ne[1] % k_cache->ne[1] != 0 ||
@@ -208,19 +253,30 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
                k_cache->nb[1] == kv_bytes_of_row(*k_cache)) {
             ++p.hgs;
         }
-        const int     waves  = few_waves(k_cache->ne[0]);
-        const int64_t groups = (kv >> p.hgs) * q->ne[3];
-        const int64_t chunks = ((keys << p.hgs) + kChunk - 1) / kChunk + (p.window > 0 ? 2 : 0);
+        const int waves  = few_waves(k_cache->ne[0]);
+        auto      groups = [&] { return (kv >> p.hgs) * q->ne[3]; };
+        auto      chunks = [&] { return ((keys << p.hgs) + kChunk - 1) / kChunk + (p.window > 0 ? 2 : 0); };
+        // A short cache is shared out by heads, so that no group has more than a
+        // chunk for each wave, rather than by keys (38 rows of 8 heads, MI355X:
+        // 11.3 to 7.1 us a call).
+        while (p.hgs > 0 && chunks() > waves && groups() * 2 <= kShortGroups && chunks() <= kWhole * waves << p.hgs &&
+               (kv_bytes_of_row(*k_cache) << (p.hgs - 1)) % 16 == 0) {
+            --p.hgs;
+        }
         // up to kWhole chunks a wave a group is not split: that many take less than a second launch
-        const int64_t deep  = chunks <= kWhole * waves ? (chunks + waves - 1) / waves : 1;
-        const int64_t units = (chunks + waves * deep - 1) / (waves * deep) * groups;
+        const int64_t deep  = chunks() <= kWhole * waves ? (chunks() + waves - 1) / waves : 1;
+        const int64_t units = (chunks() + waves * deep - 1) / (waves * deep) * groups();
         p.per               = static_cast<int32_t>(waves * deep);
         p.few               = units < INT32_MAX;
-        p.wgs               = static_cast<int32_t>(units < kMaxSplits ? units : kMaxSplits);
-        p.parts             = units > groups && p.wgs > 1;
+        p.parts             = units > groups();
+        // a group that is split: two chunks a wave at least (one stream of 8191
+        // rows: 20 us with the join, 24 with one chunk, 22 with four)
+        const int64_t want = p.parts ? (units + 1) / 2 : units;
+        const int64_t most = few_resident(kv_kind(k_cache->type), k_cache->ne[0]);
+        p.wgs              = static_cast<int32_t>(want < most ? want : most);
         // where the caches' strides are not that kernel's: as many splits as its workspace holds
-        const int64_t most = p.wgs * 2 * kCols / (q->ne[1] * q->ne[2] * q->ne[3]);
-        p.nsplit           = p.parts ? plan_splits(tiles16 * kv * q->ne[3], most, 2048) : 1;
+        const int64_t fit = p.wgs * 2 * kCols / (q->ne[1] * q->ne[2] * q->ne[3]);
+        p.nsplit          = p.parts ? plan_splits(tiles16 * kv * q->ne[3], fit, 2048) : 1;
     }
     p.wide = !p.few && wide_takes(*k_cache);
     if (p.wide) {
@@ -260,6 +316,16 @@ shp_status_t launch_join(const AttnArgs & a, hipStream_t stream) {
             hipLaunchKernelGGL(kernel, grid, dim3(kJoinThreads), 0, stream, a, first);
         });
     };
+    if (a.nsplit <= kFewParts) {
+        auto rows_a_block = [&](auto kernel, int each) {
+            return in_launches((rows + each - 1) / each, kJoinThreads, [&](int64_t first, dim3 grid) {
+                hipLaunchKernelGGL(kernel, grid, dim3(kJoinThreads), 0, stream, a, first * each);
+            });
+        };
+        return a.hd <= 64  ? rows_a_block(k_attn_join_rows<64>, 16) :
+               a.hd <= 128 ? rows_a_block(k_attn_join_rows<128>, 8) :
+                             rows_a_block(k_attn_join_rows<256>, 4);
+    }
     return a.hd <= 64 ? go(k_attn_join<64>) : a.hd <= 128 ? go(k_attn_join<128>) : go(k_attn_join<256>);
 }
 

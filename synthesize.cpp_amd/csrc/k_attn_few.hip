@@ -202,7 +202,7 @@ __host__ __device__ constexpr int few_shared(int nb, int waves) {
 // KIND Q4 or Q8, NB blocks a row (NB 8: at most 8), read in pieces of BYTES;
 // RUNS: a key's rows are apart from the next key's.
 template <int KIND, int NB, int BYTES, bool RUNS, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, NB <= 4 ? 2 : 1) void k_attn_few(const FewArgs f) {
+__global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) void k_attn_few(const FewArgs f) {
     using C                 = Codes<KIND>;
     constexpr int    UNIT   = kv_unit_bytes(KIND);
     constexpr int    SLOTS  = (NB * C::kWords + 15) / 16;
@@ -295,8 +295,9 @@ __global__ __launch_bounds__(64 * WAVES, NB <= 4 ? 2 : 1) void k_attn_few(const 
     for (int u = 0; u < TILES; ++u) {
         o[u] = splat4(0.0f);
     }
-    float m = -INFINITY;
-    float l = 0.0f;
+    float m    = -INFINITY;
+    float l    = 0.0f;
+    int   vexp = 0;  // V's d is times 2^-vexp, and o
 
     // the chunks of these units, one a wave
     const int end = min(kt.n, u1 * f.per);
@@ -344,9 +345,9 @@ __global__ __launch_bounds__(64 * WAVES, NB <= 4 ? 2 : 1) void k_attn_few(const 
             top = fmaxf(top, qmax[w * kWave + lane]);
         }
         top = max_quarters(top);
-        const int ex   = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 127) - 13;
-        const float to = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-        qscale         = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+        const int ex   = exponent_of(top) - 13;
+        const float to = pow2(-ex);
+        qscale         = pow2(ex);
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
             const int b = wave + k * WAVES;
@@ -382,18 +383,35 @@ __global__ __launch_bounds__(64 * WAVES, NB <= 4 ? 2 : 1) void k_attn_few(const 
         // d of the 32 rows: K's as F32, V's as they are; a V row that no query
         // of the call sees has d = 0
         {
-            const int          row  = lane & 31;
-            const bool         isk  = lane < 32;
-            const char *       from = (isk ? kl : vl) + row * rb;
-            const bool         keep = isk || seen_by(a, base, p1, j0 + (row >> f.hgs));
+            const int    row  = lane & 31;
+            const bool   isk  = lane < 32;
+            const char * from = (isk ? kl : vl) + row * rb;
+            const bool   keep = isk || seen_by(a, base, p1, j0 + (row >> f.hgs));
+            uint16_t     d[NB];
+            uint32_t     most = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                d[b] = b < nb && keep ? *reinterpret_cast<const uint16_t *>(from + b * UNIT) : 0;
+                most = max(most, d[b] & 0x7fffu);
+            }
+            if (__any(!isk && most > kBigD)) {  // V's code * d may be out of F16's range: 2^vexp out of it
+                const int shift = shift_of_d(wave_max(isk ? 0.0f : f16_bits_to_f32(most)));
+                if (shift > vexp) {
+#pragma unroll
+                    for (int u = 0; u < TILES; ++u) {
+                        o[u] *= pow2(vexp - shift);
+                    }
+                    vexp = shift;
+                }
+            }
+            const _Float16 by = static_cast<_Float16>(pow2(-vexp));
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (b < nb) {
-                    const uint16_t d = *reinterpret_cast<const uint16_t *>(from + b * UNIT);
                     if (isk) {
-                        kd[b * kChunk + row] = f16_bits_to_f32(d);
+                        kd[b * kChunk + row] = f16_bits_to_f32(d[b]);
                     } else {
-                        vd[b * kChunk + row] = __builtin_bit_cast(_Float16, static_cast<uint16_t>(keep ? d : 0));
+                        vd[b * kChunk + row] = __builtin_bit_cast(_Float16, d[b]) * by;
                     }
                 }
             }
@@ -526,7 +544,7 @@ __global__ __launch_bounds__(64 * WAVES, NB <= 4 ? 2 : 1) void k_attn_few(const 
     for (int u = 0; u < TILES; ++u) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            of[((wave * TILES + u) * 4 + e) * kWave + lane] = o[u][e];
+            of[((wave * TILES + u) * 4 + e) * kWave + lane] = o[u][e] * pow2(vexp);
         }
     }
     if (g == 0) {

@@ -62,7 +62,6 @@ template <int KIND, int WORDS> struct BlockPart {
 
     __device__ void keep_v(int e, bool yes) { vd[e] = yes ? vd[e] : 0; }
 
-    // d of at most 256 needs no scale: |code| <= 128
     __device__ float top_k() const { return f16_bits_to_f32(kd & 0x7fffu); }
 
     __device__ float top_v() const {
@@ -74,7 +73,7 @@ template <int KIND, int WORDS> struct BlockPart {
         return f16_bits_to_f32(m);
     }
 
-    static constexpr float kLeave = 256.0f;
+    static constexpr float kLeave = 256.0f;  // kBigD
 
     __device__ static void exact(f16x2 code, f16x2 d, f16x2 & hi, f16x2 & lo) {
         hi = code * d;
@@ -312,18 +311,9 @@ template <int KIND> struct KOrder {
 
 template <> struct KOrder<kKvQ4> : Codes<kKvQ4> {};
 
-// 2^e, e in [-126, 127].
-__device__ __forceinline__ float pow2(int e) {
-    return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-}
-
 // The shift that brings values bounded by `top` to [2^13, 2^14), if they need one.
 template <int KIND> __device__ __forceinline__ int shift_of(float top) {
-    if (!Part<KIND>::kScaled || (kv_blocks(KIND) && top <= Part<KIND>::kLeave)) {
-        return 0;
-    }
-    const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 127) - 13;
-    return kv_blocks(KIND) ? e + 8 : e;  // of d: codes are up to 2^7
+    return kv_blocks(KIND) ? shift_of_d(top) : Part<KIND>::kScaled ? exponent_of(top) - 13 : 0;
 }
 
 template <int KIND, int NB> constexpr int wide_lds() {
@@ -449,9 +439,9 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
         }
         const Pair both = swap32(top);
         top             = fmaxf(both.a, both.b);
-        const int ex    = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 127) - 13;
-        const float to  = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-        qscale          = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+        const int ex    = exponent_of(top) - 13;
+        const float to  = pow2(-ex);
+        qscale          = pow2(ex);
 #pragma unroll
         for (int s = 0; s < 2 * NB; ++s) {
             f16x2 hi[4], lo[4];
@@ -499,24 +489,26 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
             }
         }
         if constexpr (PartT::kScaled) {
-            const float tk = wave_max(mine ? part.top_k() : 0.0f);
-            const float tv = wave_max(mine ? part.top_v() : 0.0f);
+            float tk = mine ? part.top_k() : 0.0f;
+            float tv = mine ? part.top_v() : 0.0f;
+            if (!kv_blocks(KIND) || __any(fmaxf(tk, tv) > PartT::kLeave)) {  // (blocks: hardly ever)
+                tk = wave_max(tk);
+                tv = wave_max(tv);
+            }
             if (lane == 0) {
-                tops[2 * wave]     = tk;
-                tops[2 * wave + 1] = tv;
+                tops[wave]                      = tk;
+                tops[kWideBlock / kWave + wave] = tv;
             }
         }
         __syncthreads();  // the tile before is used up
         if constexpr (PartT::kScaled) {
-            float tk = 0.0f, tv = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWideBlock / kWave; ++w) {
-                tk = fmaxf(tk, tops[2 * w]);
-                tv = fmaxf(tv, tops[2 * w + 1]);
-            }
+            auto most = [&](int at) {
+                const f32x4 t = *reinterpret_cast<const f32x4 *>(tops + at);
+                return __builtin_amdgcn_readfirstlane(shift_of<KIND>(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]))));
+            };
             // K by tile; V never less than for the tiles before, which o holds
-            kexp = shift_of<KIND>(tk);
-            vexp = max(vexp, shift_of<KIND>(tv));
+            kexp = most(0);
+            vexp = max(vexp, most(4));
             kby  = pow2(-kexp);
             vby  = pow2(-vexp);
         }

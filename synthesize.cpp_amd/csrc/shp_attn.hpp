@@ -173,6 +173,25 @@ __device__ __forceinline__ void split2(float a, float b, f16x2 & hi, f16x2 & lo)
     lo = __builtin_convertvector((f32x2{ a - static_cast<float>(hi[0]), b - static_cast<float>(hi[1]) }), f16x2);
 }
 
+// 2^e, e in [-126, 127].
+__device__ __forceinline__ float pow2(int e) {
+    return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
+// The exponent of a magnitude, within what pow2() can undo.
+__device__ __forceinline__ int exponent_of(float top) {
+    return min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 127);
+}
+
+// A block's code * d, |code| <= 128, is within F16's range for d up to 256;
+// where a larger one is about, d is divided by 2^shift, which brings it below
+// 2^6 (what that takes from the small ones is below 2^-24 of the large).
+constexpr uint32_t kBigD = 0x5c00;
+
+__device__ __forceinline__ int shift_of_d(float top) {
+    return top > 256.0f ? exponent_of(top) - 5 : 0;
+}
+
 // Exponents that turn an integer in a mantissa's low bits into an F16. Held in
 // vector registers once a kernel, behind the compiler's back: (w & mask) | bits
 // is then one v_and_or_b32, which takes at most one scalar or literal operand.
@@ -273,7 +292,7 @@ __device__ __forceinline__ Rsrc rows_from(const char * at, int64_t bytes) {
 // The parts of a row joined: a workgroup a row, whose threads take four values
 // of every 1024/HD-th part each.
 constexpr int kJoinThreads = 256;
-constexpr int kMaxSplits   = 512;
+constexpr int kMaxSplits   = 768;
 
 // `parts` partial results of a row into out: ml(s) points to part s's m and l,
 // o(s) to its values. Left alone where the row has fewer than two parts.
@@ -379,6 +398,21 @@ struct AttnPlan {
     int32_t sinks;
     int32_t nsplit;
 };
+
+// Waves of a workgroup of k_attn_few: two where a row is long; those that each
+// of a CU's four SIMDs holds, by the registers they take; and the workgroups
+// that the chip's 256 CUs hold.
+constexpr int few_waves(int64_t hd) {
+    return hd <= 4 * kKvBlock ? 4 : 2;
+}
+
+constexpr int few_occupancy(int kind, int64_t hd) {
+    return hd > 4 * kKvBlock ? 1 : kind == kKvQ4 || hd <= 2 * kKvBlock ? 3 : 2;
+}
+
+constexpr int few_resident(int kind, int64_t hd) {
+    return 256 * 4 * few_occupancy(kind, hd) / few_waves(hd);
+}
 
 // k_attn_few.hip: block caches and at most 16 queries of a kv head. The piece
 // size in which it can read both caches, or 0; and its launches, join included.

