@@ -269,6 +269,7 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
         p.per               = static_cast<int32_t>(waves * deep);
         p.few               = units < INT32_MAX;
         p.parts             = units > groups();
+        p.groups            = static_cast<int32_t>(groups());
         // a group that is split: two chunks a wave at least (one stream of 8191
         // rows: 20 us with the join, 24 with one chunk, 22 with four)
         const int64_t want = p.parts ? (units + 1) / 2 : units;
@@ -291,7 +292,7 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
 int64_t plan_floats(const AttnPlan & p, const shp_tensor & q) {
     const int64_t row = (q.ne[0] + 3) / 4 * 4 + 2;
     if (p.few) {
-        return !p.parts ? 0 : static_cast<int64_t>(p.wgs) * 2 * kCols * row;
+        return !p.parts ? 0 : static_cast<int64_t>(p.wgs) * 2 * kCols * row + 2 * static_cast<int64_t>(p.groups);
     }
     return p.nsplit == 1 ? 0 : q.ne[1] * q.ne[2] * q.ne[3] * p.nsplit * row;
 }

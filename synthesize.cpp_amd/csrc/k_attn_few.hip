@@ -80,6 +80,11 @@ __device__ __forceinline__ float * few_ml(const FewArgs & f, int wg, int which, 
     return f.a.work + static_cast<int64_t>(f.wgs) * 2 * kCols * f.a.hd4 + ((wg * 2 + which) * kCols + col) * 2;
 }
 
+// The first and last workgroup of a head group.
+__device__ __forceinline__ int32_t * few_span(const FewArgs & f, int64_t group) {
+    return reinterpret_cast<int32_t *>(few_ml(f, f.wgs, 0, 0)) + 2 * group;
+}
+
 // A sequence's key chunks; `len` as seq_lens gives it.
 __device__ __forceinline__ KeyTiles few_tiles(const FewArgs & f, const SeqLens & len) {
     const AttnArgs & a     = f.a;
@@ -104,63 +109,74 @@ __device__ __forceinline__ int few_units(const FewArgs & f, int n) {
     return len.count == 0 ? 0 : max(static_cast<int>(fastdiv(static_cast<uint32_t>(few_tiles(f, len).n + f.per - 1), f.fper)), 1);
 }
 
-// The line's length, and the place of sequence n in it (units of one head
-// group), for a whole wave: 64 sequences at a time, a sum over lanes.
-struct Line {
-    int32_t before;
-    int32_t total;
-};
-
-__device__ __forceinline__ Line few_line(const FewArgs & f, int n, int lane) {
-    if (f.a.N == 1) {
-        return Line{ 0, few_units(f, 0) };
-    }
-    Line s{ 0, 0 };
-    for (int first = 0; first < f.a.N; first += kWave) {
-        const int i     = first + lane;
-        int       units = i < f.a.N ? few_units(f, i) : 0;
-        int       below = i < n ? units : 0;
-#pragma unroll
-        for (int off = 1; off < kWave; off *= 2) {
-            units += __shfl_xor(units, off);
-            below += __shfl_xor(below, off);
-        }
-        s.total += __builtin_amdgcn_readfirstlane(units);
-        s.before += __builtin_amdgcn_readfirstlane(below);
-    }
-    return s;
+// The sum of a wave's lanes up to and with this one.
+__device__ __forceinline__ int32_t sum_up_to(int32_t v) {
+    auto below = [](int32_t x, auto ctrl, auto rows) {
+        return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+    };
+    using All = std::integral_constant<int, 0xF>;
+    v += below(v, std::integral_constant<int, 0x111>{}, All{});  // row_shr:1, 2, 4, 8
+    v += below(v, std::integral_constant<int, 0x112>{}, All{});
+    v += below(v, std::integral_constant<int, 0x114>{}, All{});
+    v += below(v, std::integral_constant<int, 0x118>{}, All{});
+    v += below(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15
+    v += below(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31
+    return v;
 }
 
-// The sequence that unit u of the line falls in.
+// The sequence that a unit of the line falls in.
 struct Place {
     int32_t n;
     int32_t units;   // of one head group of it
     int32_t before;  // of all head groups of the sequences before it
 };
 
-__device__ __forceinline__ Place few_find(const FewArgs & f, int32_t u, int lane) {
+// The line's units of all head groups, and where workgroup wg's stretch begins
+// in it, for a whole wave: 64 sequences at a time, a sum over lanes.
+struct Line {
+    int32_t total;
+    int32_t begin;
+    int32_t end;
+    Place   at;  // of begin, if the stretch is not empty
+};
+
+__device__ __forceinline__ int32_t few_start(const FewArgs & f, int32_t total, int32_t wg);
+
+__device__ __forceinline__ Line few_line(const FewArgs & f, int wg, int lane) {
+    Line s{};
     if (f.a.N == 1) {
-        return Place{ 0, few_units(f, 0), 0 };
-    }
-    int32_t before = 0;
-    for (int first = 0; first < f.a.N; first += kWave) {
-        const int i     = first + lane;
-        const int units = i < f.a.N ? few_units(f, i) : 0;
-        int       sum   = units;
-#pragma unroll
-        for (int off = 1; off < kWave; off *= 2) {
-            const int v = __shfl_up(sum, off);
-            sum += lane >= off ? v : 0;
+        const int units = few_units(f, 0);
+        s.total         = units * f.groups;
+        s.at            = Place{ 0, units, 0 };
+    } else {
+        auto units_of = [&](int first) { return first + lane < f.a.N ? few_units(f, first + lane) : 0; };
+        int  units    = units_of(0);
+        int  sum      = sum_up_to(units);
+        s.total       = __builtin_amdgcn_readlane(sum, kWave - 1);
+        for (int first = kWave; first < f.a.N; first += kWave) {
+            s.total += __builtin_amdgcn_readlane(sum_up_to(units_of(first)), kWave - 1);
         }
-        const uint64_t past = __ballot(before + sum * f.groups > u);
-        if (past != 0) {
-            const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            const int k = __builtin_amdgcn_readlane(units, l);
-            return Place{ first + l, k, before + (__builtin_amdgcn_readlane(sum, l) - k) * f.groups };
+        s.total *= f.groups;
+        const int32_t unit   = few_start(f, s.total, wg);
+        int32_t       before = 0;
+        for (int first = 0; first < f.a.N; first += kWave) {
+            if (first > 0) {
+                units = units_of(first);
+                sum   = sum_up_to(units);
+            }
+            const uint64_t past = __ballot(before + sum * f.groups > unit);
+            if (past != 0) {
+                const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+                const int k = __builtin_amdgcn_readlane(units, l);
+                s.at        = Place{ first + l, k, before + (__builtin_amdgcn_readlane(sum, l) - k) * f.groups };
+                break;
+            }
+            before += __builtin_amdgcn_readlane(sum, kWave - 1) * f.groups;
         }
-        before += __builtin_amdgcn_readlane(sum, kWave - 1) * f.groups;
     }
-    return Place{ 0, 1, u };  // (u lies in the line)
+    s.begin = few_start(f, s.total, wg);
+    s.end   = few_start(f, s.total, wg + 1);
+    return s;
 }
 
 // Where workgroup wg's stretch of `total` units begins, and whose unit u is.
@@ -219,9 +235,9 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
     const int        mask = (1 << f.hgs) - 1;
     const int        nb   = NB <= 4 ? NB : f.nb;
     const int        rb   = nb * UNIT;
-    const int32_t    total = few_line(f, 0, lane).total * f.groups;
-    const int32_t    last  = few_start(f, total, wg + 1);
-    int32_t          unit  = few_start(f, total, wg);
+    const Line       line = few_line(f, wg, lane);
+    const int32_t    last = line.end;
+    int32_t          unit = line.begin;
 
     const Magic      magic;
 
@@ -271,7 +287,7 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
     if (unit >= last) {
         return;
     }
-    Place   at    = few_find(f, unit, lane);
+    Place   at    = line.at;
     int     n     = at.n;
     int     hg    = f.groups == 1 ? 0 : (unit - at.before) / at.units;
     int32_t begin = at.before + hg * at.units;  // the group's first unit
@@ -280,6 +296,10 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
     const int     u1     = min(last - begin, at.units);
     const int     h0     = hg << f.hgs;
     const SeqLens  len   = seq_lens(a, n);
+    if (a.work != nullptr && u0 == 0 && threadIdx.x == 0) {
+        few_span(f, n * f.groups + hg)[0] = wg;
+        few_span(f, n * f.groups + hg)[1] = few_owner(f, line.total, begin + at.units - 1);
+    }
     const KeyTiles kt    = few_tiles(f, len);
     const int32_t base   = len.length - len.count;
     const int32_t p1     = len.length - 1;
@@ -580,19 +600,18 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
             pml[1]      = l;
         }
     }
-    for (int u = wave; u < TILES; u += WAVES) {
+    // four values of a column a thread, so that a row is written in runs of 64 bytes
+    for (int dim = threadIdx.x / 16 * 4; dim < a.hd; dim += 16 * WAVES) {
+        f32x4 v = splat4(0.0f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float v = 0.0f;
+        for (int k = 0; k < 4; ++k) {
+            const int at = C::v_place(dim + k);
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                v += part[w] * of[((w * TILES + u) * 4 + e) * kWave + lane];
-            }
-            const int word = 16 * (u / C::kTiles) + 4 * g + e;
-            if (word < nb * C::kWords) {
-                out[C::v_index(word, u % C::kTiles)] = v * by;
+                v[k] += part[w] * of[w * TILES * 4 * kWave + at + c];
             }
         }
+        *reinterpret_cast<f32x4u *>(out + dim) = v * by;
     }
     }
     unit = begin + u1;
@@ -617,12 +636,9 @@ template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join_fe
     if (r.t >= len.count) {
         return;
     }
-    const Line    line  = few_line(f, r.n, threadIdx.x % kWave);
-    const int32_t total = line.total * f.groups;
-    const int32_t units = few_units(f, r.n);
-    const int32_t begin = line.before * f.groups + (r.h >> f.hgs) * units;
-    const int32_t w0    = few_owner(f, total, begin);
-    const int32_t w1    = few_owner(f, total, begin + units - 1);
+    const int32_t * span = few_span(f, static_cast<int64_t>(r.n) * f.groups + (r.h >> f.hgs));
+    const int32_t   w0   = span[0];
+    const int32_t   w1   = span[1];
     if (w0 == w1) {
         return;  // whole already
     }

@@ -214,7 +214,7 @@ struct Magic {
 //   kStep    dwords of codes in a quarter's operand
 //   k_codes  that operand
 //   v_codes  from a dword of two keys: their values u as F16, without d
-//   v_index  value index within 32 of value u of dword w
+//   v_place  where value `dim` of O^T is found
 template <int KIND> struct Codes;
 
 template <> struct Codes<kKvQ4> {
@@ -243,7 +243,13 @@ template <> struct Codes<kKvQ4> {
         return U & 1 ? high(m, x) : low(m, x);
     }
 
-    __device__ static int v_index(int w, int u) { return 32 * (w >> 2) + 4 * (w & 3) + (u >> 1) + 16 * (u & 1); }
+    // Where value `dim` stands among a wave's results [tile][element][lane]: in
+    // tile 16-word slot * kTiles + u, row w % 16 = 4 g + e, lanes 16 g and on.
+    __device__ static int v_place(int dim) {
+        const int w = 4 * (dim >> 5) + ((dim & 15) >> 2);
+        const int u = 2 * (dim & 3) + ((dim >> 4) & 1);
+        return (((w >> 4) * kTiles + u) * 4 + (w & 3)) * kWave + 16 * ((w >> 2) & 3);
+    }
 };
 
 template <> struct Codes<kKvQ8> {
@@ -272,7 +278,10 @@ template <> struct Codes<kKvQ8> {
         return biased(m, __builtin_amdgcn_perm(w1 ^ 0x80808080u, w0 ^ 0x80808080u, 0x0c040c00u + U * 0x00010001u));
     }
 
-    __device__ static int v_index(int w, int u) { return 4 * w + u; }
+    __device__ static int v_place(int dim) {
+        const int w = dim >> 2;
+        return (((w >> 4) * kTiles + (dim & 3)) * 4 + (w & 3)) * kWave + 16 * ((w >> 2) & 3);
+    }
 };
 
 template <class Go, int... U> __device__ __forceinline__ void for_each(std::integer_sequence<int, U...>, const Go & go) {
@@ -302,8 +311,17 @@ __device__ __forceinline__ void join_parts(int parts, int hd, const ML & ml, con
     __shared__ float weight[kMaxSplits];
     __shared__ float lane_max[kJoinThreads / kWave], lane_sum[kJoinThreads / kWave];
     __shared__ f32x4 sums[kJoinThreads];
-    const int        tid = threadIdx.x;
-    float            top = -INFINITY;
+    const int        tid   = threadIdx.x;
+    const int        dim   = tid % (HD / 4) * 4;
+    const int        group = tid / (HD / 4);
+    // this thread's first two values on their way while the weights are formed
+    f32x4 first[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int s = group + k * GROUPS;
+        first[k]    = dim < hd && s < parts ? *reinterpret_cast<const f32x4 *>(o(s) + dim) : splat4(0.0f);
+    }
+    float top = -INFINITY;
     for (int s = tid; s < parts; s += kJoinThreads) {
         top = fmaxf(top, ml(s)[0]);
     }
@@ -336,19 +354,24 @@ __device__ __forceinline__ void join_parts(int parts, int hd, const ML & ml, con
     for (int w = 0; w < kJoinThreads / kWave; ++w) {
         l += lane_sum[w];
     }
-    const int dim   = tid % (HD / 4) * 4;
-    const int group = tid / (HD / 4);
-    f32x4     v     = splat4(0.0f);
-    if (dim < hd) {
-#pragma unroll 8
-        for (int s = group; s < parts; s += GROUPS) {
-            // weight 0: no key, and nothing that counts in o
-            const float w = weight[s];
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(o(s) + dim);
+    f32x4 v   = splat4(0.0f);
+    auto  add = [&](int s, const f32x4 & x) {
+        const float w = weight[s];  // 0: no key, and nothing that counts in o
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] += w != 0.0f ? x[e] * w : 0.0f;
+        for (int e = 0; e < 4; ++e) {
+            v[e] += w != 0.0f ? x[e] * w : 0.0f;
+        }
+    };
+    if (dim < hd) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (group + k * GROUPS < parts) {
+                add(group + k * GROUPS, first[k]);
             }
+        }
+#pragma unroll 8
+        for (int s = group + 2 * GROUPS; s < parts; s += GROUPS) {
+            add(s, *reinterpret_cast<const f32x4 *>(o(s) + dim));
         }
     }
     sums[tid] = v;
@@ -391,6 +414,7 @@ struct AttnPlan {
     bool    few;
     bool    wide;
     int32_t hgs;
+    int32_t groups;  // of heads, all sequences'
     int32_t wgs;
     int32_t per;
     bool    parts;
