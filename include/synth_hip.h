@@ -722,7 +722,8 @@ shp_status_t shp_soft_max_causal(const shp_tensor * a, int32_t n_past, float sca
  * (clamped to [0, T]), NaN where that row is outside the cache; rows t >=
  * count[n] are left as they were.
  *
- * head_dim 1..256. No tensor that is written may overlap another of the call,
+ * head_dim 1..256, and up to 2^28 blocks of 32 values a sequence in a call
+ * (else SHP_ERR_UNSUPPORTED). No tensor that is written may overlap another of the call,
  * nor its own rows each other (SHP_ERR_UNSUPPORTED).
  */
 shp_status_t shp_kv_store(const shp_tensor * k,
@@ -753,10 +754,13 @@ shp_status_t shp_kv_load(const shp_tensor * k_cache,
  * + t and sees row j when 0 <= j <= p and (window == 0 or j > p - window or
  * j < sinks):
  *   y = sum_j softmax_j(scale * q.k_j) v_j over the rows it sees; 0 where p < 0.
- * Queries t >= count[n] are left as they were. Rows that no query of a
- * sequence sees are never used, whatever they hold. head_dim 1..256; y and work
- * overlap nothing else of the call.
- * Products are formed to f32's precision and summed in f32.
+ * Queries t >= count[n] are left as they were. A row that a query does not see
+ * has no part in its result, whatever it holds; an infinity or NaN in a row of V
+ * that it sees (or in its q, or through K in its scores) makes the result NaN.
+ * head_dim 1..256; y and work overlap nothing else of the call. Products are
+ * formed to f32's precision and summed in f32; a weight is held to 2^-40 of the
+ * row's largest. SHP_ERR_UNSUPPORTED past 2^28 query rows or 2^30 cache rows a
+ * sequence, and past 65535 heads or sequences.
  *
  * work: F32, contiguous, at least the number of floats that
  * shp_attn_kv_work gives for the same q, k_cache, window and sinks (partial

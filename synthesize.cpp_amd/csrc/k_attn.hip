@@ -102,8 +102,18 @@ template <int KIND, int HD> __global__ __launch_bounds__(64) void k_attn_any(con
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     const int32_t j = j0 + 4 * g + s;
-                    const float   x = dim < a.hd && seen_by(a, p0, p1, j) ?
+                    float         x = dim < a.hd && seen_by(a, p0, p1, j) ?
                                           kv_value<KIND>(vb + static_cast<int64_t>(j) * a.vt, dim) : 0.0f;
+                    const uint64_t bad = __ballot(!(fabsf(x) < INFINITY));
+                    if (bad != 0) {  // NaN for the queries that see it, and no others
+                        x = fabsf(x) < INFINITY ? x : 0.0f;
+#pragma unroll
+                        for (int quarter = 0; quarter < 4; ++quarter) {
+                            if ((bad >> (16 * quarter) & 0xffffu) != 0 && sees(a, p, j0 + 4 * quarter + s)) {
+                                l = NAN;
+                            }
+                        }
+                    }
                     o[u]            = __builtin_amdgcn_mfma_f32_16x16x4f32(x, acc[s], o[u], 0, 0, 0);
                 }
             }

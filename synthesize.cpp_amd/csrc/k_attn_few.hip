@@ -414,6 +414,24 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
                 d[b] = b < nb && keep ? *reinterpret_cast<const uint16_t *>(from + b * UNIT) : 0;
                 most = max(most, d[b] & 0x7fffu);
             }
+            // a row of V that holds an infinity or NaN counts for nothing in the products ...
+            if (__any(!isk && most >= kInfD)) {
+                uint32_t bad = static_cast<uint32_t>(__ballot(!isk && most >= kInfD) >> 32);
+                if (!isk && most >= kInfD) {
+                    most = 0;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        d[b] = 0;
+                    }
+                }
+                // ... make the result of a query that sees one NaN, and no other's
+                for (; bad != 0; bad &= bad - 1) {
+                    const int x = __ffs(static_cast<int>(bad)) - 1;
+                    if ((x & mask) == hc && sees(a, p, j0 + (x >> f.hgs))) {
+                        l = NAN;
+                    }
+                }
+            }
             if (__any(!isk && most > kBigD)) {  // V's code * d may be out of F16's range: 2^vexp out of it
                 const int shift = shift_of_d(wave_max(isk ? 0.0f : f16_bits_to_f32(most)));
                 if (shift > vexp) {
@@ -664,7 +682,7 @@ bool few_layout(const shp_tensor & c, int hgs, int piece, bool & together) {
 
 bool few_runs(const shp_tensor & c, int hgs, int piece) {
     const size_t p = static_cast<size_t>(piece);
-    return (kv_bytes_of_row(c) << hgs) % p == 0 && c.nb[2] % p == 0 && c.nb[2] < (size_t{ 1 } << 26);
+    return (kv_bytes_of_row(c) << hgs) % p == 0 && c.nb[2] % p == 0 && c.nb[2] < (size_t{ 1 } << 25);  // 32 keys within a descriptor's 2^30 bytes
 }
 
 template <int KIND, int NB, int BYTES, bool RUNS, int WAVES> shp_status_t launch_few_as(FewArgs & f, hipStream_t stream) {

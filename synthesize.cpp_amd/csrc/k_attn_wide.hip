@@ -17,6 +17,7 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWideBlock = 256;
+constexpr int kWaves     = kWideBlock / kWave;
 constexpr int kVStride   = kTileKeys * 2 + 16;  // bytes of a column of V in LDS, off the banks' period
 
 // A thread's part of a tile on its way to LDS: 32 values of a row of K, and of
@@ -29,7 +30,9 @@ constexpr int kVStride   = kTileKeys * 2 + 16;  // bytes of a column of V in LDS
 // F16's range or, F32 and BF16, always: their largest comes to [2^13, 2^14).
 //   load_k, load_v  from the cache, through descriptors of the tile
 //   keep_k, keep_v  or zeros in place of K's row, of V's of key e
-//   top_k, top_v    something that bounds the values' magnitudes (kScaled)
+//   top_k, top_v    bits that bound the magnitudes, kInf and more where one is
+//                   infinite or NaN; finite_k without those; no scale is needed
+//                   up to kLeave
 //   k_pieces        operand j of the row's four, times `by`
 //   v_pieces        value U of the eight keys
 template <int KIND> struct Part;
@@ -62,18 +65,16 @@ template <int KIND, int WORDS> struct BlockPart {
 
     __device__ void keep_v(int e, bool yes) { vd[e] = yes ? vd[e] : 0; }
 
-    __device__ float top_k() const { return f16_bits_to_f32(kd & 0x7fffu); }
+    static constexpr uint32_t kInf   = kInfD;
+    static constexpr uint32_t kLeave = kBigD;
 
-    __device__ float top_v() const {
-        uint32_t m = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            m = max(m, vd[e] & 0x7fffu);
-        }
-        return f16_bits_to_f32(m);
-    }
+    __device__ uint32_t top_k() const { return kd & 0x7fffu; }
 
-    static constexpr float kLeave = 256.0f;  // kBigD
+    __device__ uint32_t top_v(int e) const { return vd[e] & 0x7fffu; }
+
+    __device__ uint32_t finite_k() const { return 0; }
+
+    __device__ static float magnitude(uint32_t bits) { return f16_bits_to_f32(bits); }
 
     __device__ static void exact(f16x2 code, f16x2 d, f16x2 & hi, f16x2 & lo) {
         hi = code * d;
@@ -151,7 +152,7 @@ template <int KIND> struct PlainPart {
     static constexpr bool  kTwo    = KIND == kKvF32;
     static constexpr bool  kScaled = KIND != kKvF16;
     static constexpr int   kTurn   = 4;
-    static constexpr float kLeave  = 0.0f;
+    static constexpr uint32_t kLeave = 0;
     static constexpr int   kSize   = kv_unit_bytes(KIND);
     static constexpr int   kFour   = kSize;  // dwords of four values
     uint32_t               k[8 * kFour];
@@ -228,25 +229,54 @@ template <int KIND> struct PlainPart {
         }
     }
 
-    __device__ float top_k() const {
-        float m = 0.0f;
+    // Magnitudes as their bits, in whose order a NaN is the largest.
+    static constexpr uint32_t kInf = KIND == kKvF32 ? 0x7f800000u : KIND == kKvF16 ? 0x7c00u : 0x7f80u;
+
+    __device__ static uint32_t top_of(uint32_t m, uint32_t w) {
+        if constexpr (kSize == 4) {
+            return max(m, w & 0x7fffffffu);
+        } else {
+            return max(m, max(w & 0x7fffu, w >> 16 & 0x7fffu));
+        }
+    }
+
+    __device__ uint32_t top_k() const {
+        uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            m = fmaxf(m, fabsf(value(k, i)));
+        for (int i = 0; i < 8 * kFour; ++i) {
+            m = top_of(m, k[i]);
         }
         return m;
     }
 
-    __device__ float top_v() const {
-        float m = 0.0f;
+    // ... of K's finite ones: an infinity or NaN is its own row's alone
+    __device__ uint32_t finite_k() const {
+        uint32_t m = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                m = fmaxf(m, fabsf(value(v[e], i)));
+        for (int i = 0; i < 8 * kFour; ++i) {
+            if constexpr (kSize == 4) {
+                const uint32_t x = k[i] & 0x7fffffffu;
+                m                = x < kInf ? max(m, x) : m;
+            } else {
+                const uint32_t x = k[i] & 0x7fffu, y = k[i] >> 16 & 0x7fffu;
+                m                = x < kInf ? max(m, x) : m;
+                m                = y < kInf ? max(m, y) : m;
             }
         }
         return m;
+    }
+
+    __device__ uint32_t top_v(int e) const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < kFour; ++i) {
+            m = top_of(m, v[e][i]);
+        }
+        return m;
+    }
+
+    __device__ static float magnitude(uint32_t bits) {
+        return KIND == kKvF32 ? __uint_as_float(bits) : KIND == kKvF16 ? f16_bits_to_f32(bits) : bf16_bits_to_f32(bits);
     }
 
     __device__ static int words(int nb) { return 8 * nb; }
@@ -318,7 +348,7 @@ template <int KIND> __device__ __forceinline__ int shift_of(float top) {
 
 template <int KIND, int NB> constexpr int wide_lds() {
     constexpr int HD = NB * kKvBlock;
-    return (kTileKeys * (HD * 2 + 16) + HD * kVStride) * (Part<KIND>::kTwo ? 2 : 1) + (Part<KIND>::kScaled ? 32 : 0);
+    return (kTileKeys * (HD * 2 + 16) + HD * kVStride) * (Part<KIND>::kTwo ? 2 : 1) + 16 * kWaves;
 }
 
 template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_attn_wide(const AttnArgs a) {
@@ -334,6 +364,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
     char * const   vh   = kl + (TWO ? kTileKeys * KSTRIDE : 0);
     char * const   vl   = vh + HD * kVStride;
     float * const  tops = reinterpret_cast<float *>(vl + (TWO ? HD * kVStride : 0));  // of each wave's K and V
+    uint64_t *     bads = reinterpret_cast<uint64_t *>(tops + 2 * kWaves);            // a wave's keys that are not finite in V
 
     const int     tid   = threadIdx.x;
     const int     wave  = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -488,19 +519,54 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
                 }
             }
         }
-        if constexpr (PartT::kScaled) {
-            float tk = mine ? part.top_k() : 0.0f;
-            float tv = mine ? part.top_v() : 0.0f;
-            if (!kv_blocks(KIND) || __any(fmaxf(tk, tv) > PartT::kLeave)) {  // (blocks: hardly ever)
-                tk = wave_max(tk);
-                tv = wave_max(tv);
+        {
+            uint32_t tk = 0, tv = 0;
+            uint64_t bad = 0;  // keys
+            if (mine) {
+                tk = part.top_k();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    tv = max(tv, part.top_v(e));
+                }
+            }
+            if (__any(max(tk, tv) >= PartT::kInf)) {
+                // what is not finite in K is its key's alone; a key whose V has
+                // such a value counts for nothing in the products
+                if (mine) {
+                    tk = tk >= PartT::kInf ? part.finite_k() : tk;
+                    tv = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const bool is = part.top_v(e) >= PartT::kInf;
+                        bad |= static_cast<uint64_t>(is) << (vkey + (e < 4 ? e : e + 4));
+                        part.keep_v(e, !is);
+                        tv = max(tv, part.top_v(e));
+                    }
+                }
+#pragma unroll
+                for (int off = 1; off < kWave; off *= 2) {
+                    bad |= __shfl_xor(static_cast<unsigned long long>(bad), off);
+                }
+            }
+            if (PartT::kScaled && (!kv_blocks(KIND) || __any(max(tk, tv) > PartT::kLeave))) {  // (blocks: hardly ever)
+                const float fk = wave_max(PartT::magnitude(tk));
+                const float fv = wave_max(PartT::magnitude(tv));
+                if (lane == 0) {
+                    tops[wave]         = fk;
+                    tops[kWaves + wave] = fv;
+                }
+            } else if (lane == 0) {
+                tops[wave]         = 0.0f;
+                tops[kWaves + wave] = 0.0f;
             }
             if (lane == 0) {
-                tops[wave]                      = tk;
-                tops[kWideBlock / kWave + wave] = tv;
+                bads[wave] = bad;
             }
         }
         __syncthreads();  // the tile before is used up
+        const uint64_t every = bads[0] | bads[1] | bads[2] | bads[3];
+        uint64_t       none  = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(every >> 32)));
+        none                 = none << 32 | static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(every)));
         if constexpr (PartT::kScaled) {
             auto most = [&](int at) {
                 const f32x4 t = *reinterpret_cast<const f32x4 *>(tops + at);
@@ -542,6 +608,13 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
         __syncthreads();
         if (j0 > w1) {
             continue;  // none of it is seen by this wave's queries
+        }
+        if (none != 0) {  // ... but it makes the result of a query that sees it NaN, and no other's
+            for (; none != 0; none &= none - 1) {
+                if (sees(a, p, j0 + __ffsll(static_cast<unsigned long long>(none)) - 1)) {
+                    l = NAN;
+                }
+            }
         }
         const float qs = qscale * pow2(kexp);
         if (PartT::kScaled && vexp != oexp) {

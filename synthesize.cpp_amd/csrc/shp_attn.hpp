@@ -187,6 +187,7 @@ __device__ __forceinline__ int exponent_of(float top) {
 // where a larger one is about, d is divided by 2^shift, which brings it below
 // 2^6 (what that takes from the small ones is below 2^-24 of the large).
 constexpr uint32_t kBigD = 0x5c00;
+constexpr uint32_t kInfD = 0x7c00;
 
 __device__ __forceinline__ int shift_of_d(float top) {
     return top > 256.0f ? exponent_of(top) - 5 : 0;

@@ -408,12 +408,14 @@ def kv_store(k, v, k_cache, v_cache, slot, count=None, status=None):
 
 def kv_load(k_cache, v_cache, slot, t, count=None, k_out=None, v_out=None):
     """Rows [slot[n], slot[n] + t) of a KV cache as F32: (k, v), each (N, t,
-    kv_heads, head_dim); rows past count[n] are not written."""
-    raw = k_cache.data if isinstance(k_cache, BlockTensor) else k_cache
-    ne0 = k_cache.ne0 if isinstance(k_cache, BlockTensor) else k_cache.shape[-1]
-    shape = tuple(raw.shape[:-3]) + (int(t), raw.shape[-2], ne0)
-    k_out = _empty_like_f32(shape, raw.device) if k_out is None else k_out
-    v_out = _empty_like_f32(shape, raw.device) if v_out is None else v_out
+    kv_heads, head_dim), or k_out and v_out, whose positions count; rows past
+    count[n] are not written, rows outside the cache are NaN."""
+    if k_out is None or v_out is None:
+        raw = k_cache.data if isinstance(k_cache, BlockTensor) else k_cache
+        ne0 = k_cache.ne0 if isinstance(k_cache, BlockTensor) else k_cache.shape[-1]
+        shape = tuple(raw.shape[:-3]) + (int(t), raw.shape[-2], ne0)
+        k_out = _empty_like_f32(shape, raw.device) if k_out is None else k_out
+        v_out = _empty_like_f32(shape, raw.device) if v_out is None else v_out
     _check(_fn("shp_kv_load")(k_cache, v_cache, slot, count, k_out, v_out, _stream()), "kv_load")
     return k_out, v_out
 

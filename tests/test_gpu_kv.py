@@ -403,3 +403,54 @@ def test_head_layouts(gpu, kind, hd, t, kv, g):
     """Groups of heads that do and do not fill the matrix unit's columns."""
     q, k, v = rand(2, t, kv * g, kv, hd, 85, 15)
     check(gpu, kind, q, k, v, [85, 40])
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("t,hd", [(1, 64), (3, 64), (40, 64), (6, 160)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_what_is_not_finite_is_its_own_rows_queries_alone(gpu, kind, t, hd, bad):
+    """An infinity or NaN in k of one head and v of another, at rows that some of
+    the queries see, and in one query: NaN there, every other result as ever."""
+    n, kv, g, cap = 1, 4, 2, 100
+    q, k, v = rand(n, t, kv * g, kv, hd, cap, 16)
+    row, late = cap - t // 2 - 1, cap - 1
+    caches = [R.pack(x, kind) for x in (k, v)]
+    y, bound = R.attend(q, R.values(caches[0], kind), R.values(caches[1], kind), [cap], [t], hd ** -0.5, window=60, sinks=2)
+    k, v = k.clone(), v.clone()
+    k[0, row, 0, 5] = float("nan")
+    v[0, row, 1, 7] = bad
+    v[0, late, 3, hd - 1] = bad
+    v[0, 30, 2] = bad                     # behind the window of all queries, or of the later ones
+    k[0, 30, 2] = bad
+    q = q.clone()
+    q[0, 0, 4] = float("nan")             # the first query of kv head 2's first head
+    nan = torch.zeros(t, kv * g, dtype=torch.bool)
+    p = torch.arange(cap - t, cap)
+    nan[p >= row, 0:4] = True
+    nan[p >= late, 6:8] = True
+    nan[30 > p - 60, 4:6] = True
+    nan[0, 4] = True
+    c = [R.handle(gpu, R.pack(x, kind).cuda(), kind, hd) for x in (k, v)]
+    got = gpu.attn_kv(q.cuda(), c[0], c[1], ints(cap), window=60, sinks=2).cpu().double()
+    assert torch.isnan(got[0][nan]).any(-1).all()
+    assert ((got - y).abs()[0][~nan] <= bound[0][~nan]).all()
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q8_0", "f16"])
+@pytest.mark.parametrize("t,row", [(1, 12 << 20), (1, 20 << 20), (1, 40 << 20), (40, 12 << 20), (40, 20 << 20)])
+def test_rows_megabytes_apart(gpu, kind, t, row):
+    """Row strides on either side of what the kernels take at 32-bit offsets."""
+    kv, hd, cap = 2, 64, 70
+    q, k, v = rand(1, t, 4, kv, hd, cap, 17)
+    width = hd if kind in R.FLOAT else hd // 32 * R.UNIT[kind]
+    size = R.pack(k, kind).element_size()
+    pool = torch.empty((cap * row + (1 << 20)) // size, dtype=R.pack(k, kind).dtype, device="cuda")
+    make = [0]
+
+    def far(c):
+        s = pool.as_strided((1, cap, kv, width), (0, row // size, width, 1), 4096 * make[0])
+        make[0] += 1
+        s.copy_(c)
+        return s
+
+    check(gpu, kind, q, k, v, [cap], make=far)
