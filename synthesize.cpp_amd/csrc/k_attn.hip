@@ -149,6 +149,11 @@ template <int KIND, int HD> __global__ __launch_bounds__(64) void k_attn_any(con
     }
 }
 
+// Parts of a row's result; one has been written to y.
+__device__ __forceinline__ int parts_of(const AttnArgs & a, const SeqLens & len, const RowOf & r) {
+    return a.per == 0 ? a.nsplit : wide_parts(a, len.length, len.count, (r.t * a.G + r.gq) / kWideRows);
+}
+
 template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join(const AttnArgs a, int64_t row0) {
     const int64_t row = row0 + blockIdx.x;
     const RowOf   r   = row_of(a, row);
@@ -156,7 +161,11 @@ template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join(co
     if (r.t >= len.count) {
         return;
     }
-    join_parts<HD>(a.nsplit, a.hd, [&](int s) { return partial_ml(a, row, s); }, [&](int s) { return partial_o(a, row, s); },
+    const int parts = parts_of(a, len, r);
+    if (parts <= 1) {
+        return;
+    }
+    join_parts<HD>(parts, a.hd, [&](int s) { return partial_ml(a, row, s); }, [&](int s) { return partial_o(a, row, s); },
                    out_of(a, r), len.length - len.count + r.t >= 0);
 }
 
@@ -176,16 +185,20 @@ template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join_ro
     if (r.t >= len.count) {
         return;
     }
+    const int parts = parts_of(a, len, r);
+    if (parts <= 1) {
+        return;
+    }
     float m[kFewParts], l[kFewParts];
     f32x4 o[kFewParts];
     float top = -INFINITY;
 #pragma unroll
     for (int s = 0; s < kFewParts; ++s) {
-        const int     p  = min(s, a.nsplit - 1);
+        const int     p  = min(s, parts - 1);
         const float * ml = partial_ml(a, row, p);
         m[s]             = ml[0];
-        l[s]             = s < a.nsplit ? ml[1] : 0.0f;
-        o[s]             = s < a.nsplit ? *reinterpret_cast<const f32x4 *>(partial_o(a, row, p) + dim) : splat4(0.0f);
+        l[s]             = s < parts ? ml[1] : 0.0f;
+        o[s]             = s < parts ? *reinterpret_cast<const f32x4 *>(partial_o(a, row, p) + dim) : splat4(0.0f);
         top              = fmaxf(top, m[s]);
     }
     const float ref = top == -INFINITY ? 0.0f : top;
@@ -232,6 +245,8 @@ bool wide_takes(const shp_tensor & c) {
            (kv_blocks(kv_kind(c.type)) || kv_bytes_of_row(c) % 4 == 0);
 }
 
+constexpr int64_t kWideGroups  = 512;  // workgroups of k_attn_wide that the chip holds
+constexpr int64_t kWideSpan    = 2;    // key tiles at least: 300 positions take 20.9 us, with 3 23.4
 constexpr int64_t kWhole       = 4;
 constexpr int64_t kShortGroups = 256;
 
@@ -291,8 +306,44 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
     }
     p.wide = !p.few && wide_takes(*k_cache);
     if (p.wide) {
+        // Splits of equally many key tiles for all rows, however many a row has,
+        // as short as lets the chip hold all of them at once: 2048 positions of
+        // 16 heads take 81 us, and 99 with every row in thirds (Q4_0, 8 kv heads,
+        // MI355X). With more rows than half of that they are halved, so that a
+        // long row's half runs beside another (4096 positions of 12 heads of 64
+        // values: 131 us, 164 by the rule above), and left whole where the rows
+        // alone fill the chip.
         const int64_t tiles = (rows + kWideRows - 1) / kWideRows;
-        p.nsplit = plan_splits(tiles * kv * q->ne[3], (keys + 4 * kTileKeys - 1) / (4 * kTileKeys), 512);
+        const int64_t most  = (keys + kTileKeys - 1) / kTileKeys + (p.window > 0 ? 2 : 0);
+        const int64_t pairs = kv * q->ne[3];
+        int64_t       span  = (most + kMaxSplits - 1) / kMaxSplits;
+        span                = span > kWideSpan ? span : kWideSpan;
+        if (tiles * pairs >= kWideGroups) {
+            span = most;
+        } else if (tiles * pairs > kWideGroups / 2) {
+            span = span > (most + 1) / 2 ? span : (most + 1) / 2;
+        } else {
+            auto fits = [&](int64_t of) {
+                int64_t groups = 0;
+                for (int64_t t = 0; t < tiles && groups <= kWideGroups; ++t) {
+                    // of a whole cache, and within a window all alike
+                    const int64_t end = cap - T + ((t + 1) * kWideRows * T + rows - 1) / rows;
+                    const int64_t n   = ((end < cap ? end : cap) + kTileKeys - 1) / kTileKeys;
+                    groups += ((n < most ? n : most) + of - 1) / of * pairs;
+                }
+                return groups <= kWideGroups;
+            };
+            for (int64_t upto = most; span < upto;) {  // the shortest that fits
+                const int64_t mid = (span + upto) / 2;
+                if (fits(mid)) {
+                    upto = mid;
+                } else {
+                    span = mid + 1;
+                }
+            }
+        }
+        p.span   = static_cast<int32_t>(span < most ? span : most);
+        p.nsplit = static_cast<int32_t>((most + p.span - 1) / p.span);
     } else if (!p.few) {
         p.nsplit = plan_splits(tiles16 * kv * q->ne[3], (keys + 63) / 64, 2048);
     }
@@ -439,6 +490,17 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
     }
     if (wide_takes(*k_cache) && wide_takes(*v_cache)) {
         a.tiles = static_cast<int32_t>((static_cast<int64_t>(a.T) * a.G + kWideRows - 1) / kWideRows);
+        a.per   = p.span;
+        if (!p.wide) {  // in place of k_attn_few: splits as its workspace has room for
+            const int64_t most = (a.cap + kTileKeys - 1) / kTileKeys + 2;
+            a.per              = static_cast<int32_t>((most + a.nsplit - 1) / a.nsplit);
+        }
+        a.fper = make_fastdiv(static_cast<uint32_t>(a.per));
+        const int64_t groups = static_cast<int64_t>(a.tiles) * a.KV;
+        // with all of them on the chip, two to a CU, a long row tile's neighbour is a
+        // short one (4096 positions: 289 us with the longest first throughout, 278)
+        const bool    twos   = a.nsplit == 1 && a.N == 1 && groups > kWideGroups / 2 && groups <= kWideGroups;
+        a.half               = twos ? static_cast<int32_t>((kWideGroups / 2 + a.KV - 1) / a.KV) : a.tiles;
         st = launch_attn_wide(kind, a, s);
         return st == SHP_OK && a.nsplit > 1 ? launch_join(a, s) : st;
     }

@@ -20,6 +20,10 @@ namespace {
 //         against P in two; lo x lo, below 2^-22 of the product, is left out.
 // P is held times 2^15, so that its pieces keep their bits where it is small:
 // a weight is off by at most 2^-40 of the largest, or 2^-23 of itself.
+// Bound by LDS reads and what forms the operands, about as long as the bytes
+// take: 64 streams of 512 to 8192 rows (16 heads of 128 over 8, Q4_0) take 95
+// us, 3.4 TB/s of the cache's 5; one stream of 8191 rows 19 us, 7 of them the
+// join's launch (MI355X).
 // ---------------------------------------------------------------------------
 
 // Dwords at two-byte boundaries of LDS. A wave's read of them as they are takes
@@ -68,7 +72,7 @@ struct FewArgs {
 // few for each of a workgroup's waves; sequence after sequence, head group after head
 // group, the units of the call stand in one line, of which every workgroup
 // takes an equal stretch. So lengths may differ as they like (64 streams of 512
-// to 8192 rows, MI355X: XX us, YY with an equal number of workgroups for each
+// to 8192 rows, MI355X: 113 us, 169 with an equal number of workgroups for each
 // sequence). A stretch that ends inside a group leaves a partial result; a
 // workgroup has two at most, of the group that it begins in and did not begin
 // (0), and of the one that it began and did not end (1).
@@ -292,358 +296,358 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
     int     hg    = f.groups == 1 ? 0 : (unit - at.before) / at.units;
     int32_t begin = at.before + hg * at.units;  // the group's first unit
     for (;;) {
-    const int     u0     = unit - begin;
-    const int     u1     = min(last - begin, at.units);
-    const int     h0     = hg << f.hgs;
-    const SeqLens  len   = seq_lens(a, n);
-    if (a.work != nullptr && u0 == 0 && threadIdx.x == 0) {
-        few_span(f, n * f.groups + hg)[0] = wg;
-        few_span(f, n * f.groups + hg)[1] = few_owner(f, line.total, begin + at.units - 1);
-    }
-    const KeyTiles kt    = few_tiles(f, len);
-    const int32_t base   = len.length - len.count;
-    const int32_t p1     = len.length - 1;
-    const int     head   = (h0 + hc) * a.G + r - t * a.G;
-    const bool    live   = hc <= mask && t < len.count;
-    const int32_t p      = live ? base + t : -1;
-
-    const char * kb = a.k + n * a.kn + h0 * a.kh;
-    const char * vb = a.v + n * a.vn + h0 * a.vh;
-
-    f32x4 o[TILES];
-#pragma unroll
-    for (int u = 0; u < TILES; ++u) {
-        o[u] = splat4(0.0f);
-    }
-    float m    = -INFINITY;
-    float l    = 0.0f;
-    int   vexp = 0;  // V's d is times 2^-vexp, and o
-
-    // the chunks of these units, one a wave
-    const int end = min(kt.n, u1 * f.per);
-    int       i   = u0 * f.per + wave;
-
-    Staged<BYTES, P> ks, vs;
-    auto             fetch = [&](int32_t tile) {
-        const int32_t j0 = key_tile(kt, tile) << (5 - f.hgs);
-        const Rsrc    kr = rows_from(kb + static_cast<int64_t>(j0) * a.kt, static_cast<int64_t>(a.cap - j0 - 1) * a.kt + (rb << f.hgs));
-        const Rsrc    vr = rows_from(vb + static_cast<int64_t>(j0) * a.vt, static_cast<int64_t>(a.cap - j0 - 1) * a.vt + (rb << f.hgs));
-#pragma unroll
-        for (int x = 0; x < P; ++x) {
-            ks.load(x, kr, RUNS ? krel[x] : krel[0] + x * kWave * BYTES);
-            vs.load(x, vr, RUNS ? vrel[x] : krel[0] + x * kWave * BYTES);
+        const int     u0     = unit - begin;
+        const int     u1     = min(last - begin, at.units);
+        const int     h0     = hg << f.hgs;
+        const SeqLens  len   = seq_lens(a, n);
+        if (a.work != nullptr && u0 == 0 && threadIdx.x == 0) {
+            few_span(f, n * f.groups + hg)[0] = wg;
+            few_span(f, n * f.groups + hg)[1] = few_owner(f, line.total, begin + at.units - 1);
         }
-    };
-    if (i < end) {
-        fetch(i);
-    }
-    // The queries' operands, the same for every wave: in LDS, each wave's blocks
-    // formed by it. A query is scaled by a power of two that brings its largest
-    // value to [2^13, 2^14), so that both pieces of all that counts are normal.
-    float qscale;
-    {
-        constexpr int MINE = (NB + WAVES - 1) / WAVES;
-        const float * qr   = reinterpret_cast<const float *>(a.q + n * a.qn + t * a.qt + head * a.qh);
-        float         q[MINE][8];
-        float         top = 0.0f;
+        const KeyTiles kt    = few_tiles(f, len);
+        const int32_t base   = len.length - len.count;
+        const int32_t p1     = len.length - 1;
+        const int     head   = (h0 + hc) * a.G + r - t * a.G;
+        const bool    live   = hc <= mask && t < len.count;
+        const int32_t p      = live ? base + t : -1;
+
+        const char * kb = a.k + n * a.kn + h0 * a.kh;
+        const char * vb = a.v + n * a.vn + h0 * a.vh;
+
+        f32x4 o[TILES];
 #pragma unroll
-        for (int k = 0; k < MINE; ++k) {
-            const int   b   = wave + k * WAVES;
-            const bool  has = live && b < nb;
-            const f32x4 x0  = has ? ld4u(qr + 32 * b + C::kFirst * g) : splat4(0.0f);
-            const f32x4 x1  = has ? ld4u(qr + 32 * b + C::kFirst * g + C::kSecond) : splat4(0.0f);
+        for (int u = 0; u < TILES; ++u) {
+            o[u] = splat4(0.0f);
+        }
+        float m    = -INFINITY;
+        float l    = 0.0f;
+        int   vexp = 0;  // V's d is times 2^-vexp, and o
+
+        // the chunks of these units, one a wave
+        const int end = min(kt.n, u1 * f.per);
+        int       i   = u0 * f.per + wave;
+
+        Staged<BYTES, P> ks, vs;
+        auto             fetch = [&](int32_t tile) {
+            const int32_t j0 = key_tile(kt, tile) << (5 - f.hgs);
+            const Rsrc    kr = rows_from(kb + static_cast<int64_t>(j0) * a.kt, static_cast<int64_t>(a.cap - j0 - 1) * a.kt + (rb << f.hgs));
+            const Rsrc    vr = rows_from(vb + static_cast<int64_t>(j0) * a.vt, static_cast<int64_t>(a.cap - j0 - 1) * a.vt + (rb << f.hgs));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                q[k][e] = (e < 4 ? x0[C::order(e)] : x1[C::order(e - 4)]) * a.scale;
-                top     = fmaxf(top, fabsf(q[k][e]));
+            for (int x = 0; x < P; ++x) {
+                ks.load(x, kr, RUNS ? krel[x] : krel[0] + x * kWave * BYTES);
+                vs.load(x, vr, RUNS ? vrel[x] : krel[0] + x * kWave * BYTES);
             }
+        };
+        if (i < end) {
+            fetch(i);
         }
-        qmax[wave * kWave + lane] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            top = fmaxf(top, qmax[w * kWave + lane]);
-        }
-        top = max_quarters(top);
-        const int ex   = exponent_of(top) - 13;
-        const float to = pow2(-ex);
-        qscale         = pow2(ex);
-#pragma unroll
-        for (int k = 0; k < MINE; ++k) {
-            const int b = wave + k * WAVES;
-            f16x2     h[4], l[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                split2(q[k][2 * e] * to, q[k][2 * e + 1] * to, h[e], l[e]);
-            }
-            if (b < nb) {
-                qop[(2 * b) * kWave + lane]     = join8(h[0], h[1], h[2], h[3]);
-                qop[(2 * b + 1) * kWave + lane] = join8(l[0], l[1], l[2], l[3]);
-            }
-        }
-        __syncthreads();
-    }
-
-    for (; i < end; i += WAVES) {
-        const int32_t j0 = key_tile(kt, i) << (5 - f.hgs);
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int x = 0; x < P; ++x) {
-            const int pc = lane + x * kWave;
-            if (pc < f.pieces) {
-                ks.keep(x, kl, pc);
-                vs.keep(x, vl, pc);
-            }
-        }
-        if (i + WAVES < end) {
-            fetch(i + WAVES);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        // d of the 32 rows: K's as F32, V's as they are; a V row that no query
-        // of the call sees has d = 0
+        // The queries' operands, the same for every wave: in LDS, each wave's blocks
+        // formed by it. A query is scaled by a power of two that brings its largest
+        // value to [2^13, 2^14), so that both pieces of all that counts are normal.
+        float qscale;
         {
-            const int    row  = lane & 31;
-            const bool   isk  = lane < 32;
-            const char * from = (isk ? kl : vl) + row * rb;
-            const bool   keep = isk || seen_by(a, base, p1, j0 + (row >> f.hgs));
-            uint16_t     d[NB];
-            uint32_t     most = 0;
+            constexpr int MINE = (NB + WAVES - 1) / WAVES;
+            const float * qr   = reinterpret_cast<const float *>(a.q + n * a.qn + t * a.qt + head * a.qh);
+            float         q[MINE][8];
+            float         top = 0.0f;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                d[b] = b < nb && keep ? *reinterpret_cast<const uint16_t *>(from + b * UNIT) : 0;
-                most = max(most, d[b] & 0x7fffu);
-            }
-            // a row of V that holds an infinity or NaN counts for nothing in the products ...
-            if (__any(!isk && most >= kInfD)) {
-                uint32_t bad = static_cast<uint32_t>(__ballot(!isk && most >= kInfD) >> 32);
-                if (!isk && most >= kInfD) {
-                    most = 0;
+            for (int k = 0; k < MINE; ++k) {
+                const int   b   = wave + k * WAVES;
+                const bool  has = live && b < nb;
+                const f32x4 x0  = has ? ld4u(qr + 32 * b + C::kFirst * g) : splat4(0.0f);
+                const f32x4 x1  = has ? ld4u(qr + 32 * b + C::kFirst * g + C::kSecond) : splat4(0.0f);
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        d[b] = 0;
-                    }
-                }
-                // ... make the result of a query that sees one NaN, and no other's
-                for (; bad != 0; bad &= bad - 1) {
-                    const int x = __ffs(static_cast<int>(bad)) - 1;
-                    if ((x & mask) == hc && sees(a, p, j0 + (x >> f.hgs))) {
-                        l = NAN;
-                    }
+                for (int e = 0; e < 8; ++e) {
+                    q[k][e] = (e < 4 ? x0[C::order(e)] : x1[C::order(e - 4)]) * a.scale;
+                    top     = fmaxf(top, fabsf(q[k][e]));
                 }
             }
-            if (__any(!isk && most > kBigD)) {  // V's code * d may be out of F16's range: 2^vexp out of it
-                const int shift = shift_of_d(wave_max(isk ? 0.0f : f16_bits_to_f32(most)));
-                if (shift > vexp) {
+            qmax[wave * kWave + lane] = top;
+            __syncthreads();
 #pragma unroll
-                    for (int u = 0; u < TILES; ++u) {
-                        o[u] *= pow2(vexp - shift);
-                    }
-                    vexp = shift;
+            for (int w = 0; w < WAVES; ++w) {
+                top = fmaxf(top, qmax[w * kWave + lane]);
+            }
+            top = max_quarters(top);
+            const int ex   = exponent_of(top) - 13;
+            const float to = pow2(-ex);
+            qscale         = pow2(ex);
+#pragma unroll
+            for (int k = 0; k < MINE; ++k) {
+                const int b = wave + k * WAVES;
+                f16x2     h[4], l[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    split2(q[k][2 * e] * to, q[k][2 * e + 1] * to, h[e], l[e]);
+                }
+                if (b < nb) {
+                    qop[(2 * b) * kWave + lane]     = join8(h[0], h[1], h[2], h[3]);
+                    qop[(2 * b + 1) * kWave + lane] = join8(l[0], l[1], l[2], l[3]);
                 }
             }
-            const _Float16 by = static_cast<_Float16>(pow2(-vexp));
+            __syncthreads();
+        }
+
+        for (; i < end; i += WAVES) {
+            const int32_t j0 = key_tile(kt, i) << (5 - f.hgs);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int x = 0; x < P; ++x) {
+                const int pc = lane + x * kWave;
+                if (pc < f.pieces) {
+                    ks.keep(x, kl, pc);
+                    vs.keep(x, vl, pc);
+                }
+            }
+            if (i + WAVES < end) {
+                fetch(i + WAVES);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            // d of the 32 rows: K's as F32, V's as they are; a V row that no query
+            // of the call sees has d = 0
+            {
+                const int    row  = lane & 31;
+                const bool   isk  = lane < 32;
+                const char * from = (isk ? kl : vl) + row * rb;
+                const bool   keep = isk || seen_by(a, base, p1, j0 + (row >> f.hgs));
+                uint16_t     d[NB];
+                uint32_t     most = 0;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    d[b] = b < nb && keep ? *reinterpret_cast<const uint16_t *>(from + b * UNIT) : 0;
+                    most = max(most, d[b] & 0x7fffu);
+                }
+                // a row of V that holds an infinity or NaN counts for nothing in the products ...
+                if (__any(!isk && most >= kInfD)) {
+                    uint32_t bad = static_cast<uint32_t>(__ballot(!isk && most >= kInfD) >> 32);
+                    if (!isk && most >= kInfD) {
+                        most = 0;
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            d[b] = 0;
+                        }
+                    }
+                    // ... make the result of a query that sees one NaN, and no other's
+                    for (; bad != 0; bad &= bad - 1) {
+                        const int x = __ffs(static_cast<int>(bad)) - 1;
+                        if ((x & mask) == hc && sees(a, p, j0 + (x >> f.hgs))) {
+                            l = NAN;
+                        }
+                    }
+                }
+                if (__any(!isk && most > kBigD)) {  // V's code * d may be out of F16's range: 2^vexp out of it
+                    const int shift = shift_of_d(wave_max(isk ? 0.0f : f16_bits_to_f32(most)));
+                    if (shift > vexp) {
+#pragma unroll
+                        for (int u = 0; u < TILES; ++u) {
+                            o[u] *= pow2(vexp - shift);
+                        }
+                        vexp = shift;
+                    }
+                }
+                const _Float16 by = static_cast<_Float16>(pow2(-vexp));
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if (b < nb) {
+                        if (isk) {
+                            kd[b * kChunk + row] = f16_bits_to_f32(d[b]);
+                        } else {
+                            vd[b * kChunk + row] = __builtin_bit_cast(_Float16, d[b]) * by;
+                        }
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+
+            // scores: rows 16 mt + 4 g + e of the chunk against query c
+            f32x4 sc[2] = { splat4(0.0f), splat4(0.0f) };
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (b < nb) {
-                    if (isk) {
-                        kd[b * kChunk + row] = f16_bits_to_f32(d[b]);
-                    } else {
-                        vd[b * kChunk + row] = __builtin_bit_cast(_Float16, d[b]) * by;
+                    const f16x8 qh = qop[(2 * b) * kWave + lane];
+                    const f16x8 ql = qop[(2 * b + 1) * kWave + lane];
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt) {
+                        uint32_t w[C::kStep];
+#pragma unroll
+                        for (int i = 0; i < C::kStep; ++i) {
+                            const int off = 16 * mt * rb + b * UNIT + 4 * i;
+                            w[i]          = b % 2 == 0 ? k0.at(off) : k1.at(off - 2);
+                        }
+                        const f16x8 k = C::k_codes(magic, w);
+                        f32x4       x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh, splat4(0.0f), 0, 0, 0);
+                        x             = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql, x, 0, 0, 0);
+                        const f32x4 d = *reinterpret_cast<const f32x4 *>(kd + b * kChunk + 16 * mt + 4 * g);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            sc[mt][e] = __builtin_fmaf(d[e], x[e], sc[mt][e]);
+                        }
                     }
                 }
             }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-
-        // scores: rows 16 mt + 4 g + e of the chunk against query c
-        f32x4 sc[2] = { splat4(0.0f), splat4(0.0f) };
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (b < nb) {
-                const f16x8 qh = qop[(2 * b) * kWave + lane];
-                const f16x8 ql = qop[(2 * b + 1) * kWave + lane];
-#pragma unroll
-                for (int mt = 0; mt < 2; ++mt) {
-                    uint32_t w[C::kStep];
-#pragma unroll
-                    for (int i = 0; i < C::kStep; ++i) {
-                        const int off = 16 * mt * rb + b * UNIT + 4 * i;
-                        w[i]          = b % 2 == 0 ? k0.at(off) : k1.at(off - 2);
-                    }
-                    const f16x8 k = C::k_codes(magic, w);
-                    f32x4       x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh, splat4(0.0f), 0, 0, 0);
-                    x             = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql, x, 0, 0, 0);
-                    const f32x4 d = *reinterpret_cast<const f32x4 *>(kd + b * kChunk + 16 * mt + 4 * g);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        sc[mt][e] = __builtin_fmaf(d[e], x[e], sc[mt][e]);
-                    }
-                }
-            }
-        }
-        const bool all = j0 + keys - 1 <= base && (a.window == 0 || j0 > p1 - a.window || j0 + keys <= a.sinks);
-        float      top = m;
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                // (a NaN of its own head becomes +infinity, and the weights NaN)
-                sc[mt][e] = fminf(sc[mt][e] * qscale, own[e]);
-            }
-        }
-        if (!all) {  // keys that some queries do not see
-            int g4 = 4 * g;
-            asm volatile("" : "+v"(g4));  // (the rows' keys are not to wait in registers for this)
+            const bool all = j0 + keys - 1 <= base && (a.window == 0 || j0 > p1 - a.window || j0 + keys <= a.sinks);
+            float      top = m;
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    sc[mt][e] = sees(a, p, j0 + ((16 * mt + g4 + e) >> f.hgs)) ? sc[mt][e] : -INFINITY;
+                    // (a NaN of its own head becomes +infinity, and the weights NaN)
+                    sc[mt][e] = fminf(sc[mt][e] * qscale, own[e]);
                 }
             }
-        }
+            if (!all) {  // keys that some queries do not see
+                int g4 = 4 * g;
+                asm volatile("" : "+v"(g4));  // (the rows' keys are not to wait in registers for this)
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+                for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                top = fmaxf(top, sc[mt][e]);
+                    for (int e = 0; e < 4; ++e) {
+                        sc[mt][e] = sees(a, p, j0 + ((16 * mt + g4 + e) >> f.hgs)) ? sc[mt][e] : -INFINITY;
+                    }
+                }
             }
-        }
-        top             = max_quarters(top);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        if (__any(top > m)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - ref);
-            l *= alpha;
 #pragma unroll
-            for (int u = 0; u < TILES; ++u) {
-                o[u] *= alpha;
-            }
-        }
-        m = top;
-        f16x2 ph[4], pl[4];
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-            float w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                w[e] = __builtin_amdgcn_exp2f(sc[mt][e] - (ref - kPShift));
-                l += w[e];
-            }
-            split2(w[0], w[1], ph[2 * mt], pl[2 * mt]);
-            split2(w[2], w[3], ph[2 * mt + 1], pl[2 * mt + 1]);
-        }
-        const f16x8 bh = join8(ph[0], ph[1], ph[2], ph[3]);
-        const f16x8 bl = join8(pl[0], pl[1], pl[2], pl[3]);
-
-        // operand element e of quarter g is row 4 g + e, then 16 + 4 g + e - 4
-#pragma unroll
-        for (int s = 0; s < SLOTS; ++s) {
-            uint32_t w[8];
-            f16x2    d[4];
-            const f16x4 d0 = *reinterpret_cast<const f16x4 *>(vd + vblock[s] * kChunk + 4 * g);
-            const f16x4 d1 = *reinterpret_cast<const f16x4 *>(vd + vblock[s] * kChunk + 16 + 4 * g);
-            d[0] = f16x2{ d0[0], d0[1] }, d[1] = f16x2{ d0[2], d0[3] };
-            d[2] = f16x2{ d1[0], d1[1] }, d[3] = f16x2{ d1[2], d1[3] };
-            const LdsWords v0(vl, vword[s]);
-            const LdsWords v1(vl, vword[s] + 2);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int off = ((e < 4 ? 0 : 12) + e) * rb;
-                w[e]          = nb % 2 == 0 || e % 2 == 0 ? v0.at(off) : v1.at(off - 2);
-            }
-            auto tile = [&](auto uc) {
-                constexpr int U = decltype(uc)::value;
-                f16x2         hi[4], lo[4];
+            for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const f16x2 code = C::template v_codes<U>(magic, w[2 * e], w[2 * e + 1]);
-                    hi[e]            = code * d[e];
-                    lo[e]            = __builtin_elementwise_fma(code, d[e], -hi[e]);
+                    top = fmaxf(top, sc[mt][e]);
                 }
-                const f16x8 ah = join8(hi[0], hi[1], hi[2], hi[3]);
-                const f16x8 al = join8(lo[0], lo[1], lo[2], lo[3]);
-                f32x4 &     x  = o[s * C::kTiles + U];
-                x              = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, x, 0, 0, 0);
-                x              = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, x, 0, 0, 0);
-                x              = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, x, 0, 0, 0);
-            };
-            for_each(std::make_integer_sequence<int, C::kTiles>{}, tile);
-        }
-    }
-    l = sum_quarters(l);
+            }
+            top             = max_quarters(top);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            if (__any(top > m)) {
+                const float alpha = __builtin_amdgcn_exp2f(m - ref);
+                l *= alpha;
+#pragma unroll
+                for (int u = 0; u < TILES; ++u) {
+                    o[u] *= alpha;
+                }
+            }
+            m = top;
+            f16x2 ph[4], pl[4];
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(sc[mt][e] - (ref - kPShift));
+                    l += w[e];
+                }
+                split2(w[0], w[1], ph[2 * mt], pl[2 * mt]);
+                split2(w[2], w[3], ph[2 * mt + 1], pl[2 * mt + 1]);
+            }
+            const f16x8 bh = join8(ph[0], ph[1], ph[2], ph[3]);
+            const f16x8 bl = join8(pl[0], pl[1], pl[2], pl[3]);
 
-    // the waves' results joined in LDS: [wave][value][lane], then m and l of a column
-    __syncthreads();
-    float * of = reinterpret_cast<float *>(lds);
-    float * ml = of + WAVES * TILES * 4 * kWave;
+            // operand element e of quarter g is row 4 g + e, then 16 + 4 g + e - 4
 #pragma unroll
-    for (int u = 0; u < TILES; ++u) {
+            for (int s = 0; s < SLOTS; ++s) {
+                uint32_t w[8];
+                f16x2    d[4];
+                const f16x4 d0 = *reinterpret_cast<const f16x4 *>(vd + vblock[s] * kChunk + 4 * g);
+                const f16x4 d1 = *reinterpret_cast<const f16x4 *>(vd + vblock[s] * kChunk + 16 + 4 * g);
+                d[0] = f16x2{ d0[0], d0[1] }, d[1] = f16x2{ d0[2], d0[3] };
+                d[2] = f16x2{ d1[0], d1[1] }, d[3] = f16x2{ d1[2], d1[3] };
+                const LdsWords v0(vl, vword[s]);
+                const LdsWords v1(vl, vword[s] + 2);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            of[((wave * TILES + u) * 4 + e) * kWave + lane] = o[u][e] * pow2(vexp);
-        }
-    }
-    if (g == 0) {
-        ml[(wave * 16 + c) * 2]     = m;
-        ml[(wave * 16 + c) * 2 + 1] = l;
-    }
-    __syncthreads();
-    float top = -INFINITY;
+                for (int e = 0; e < 8; ++e) {
+                    const int off = ((e < 4 ? 0 : 12) + e) * rb;
+                    w[e]          = nb % 2 == 0 || e % 2 == 0 ? v0.at(off) : v1.at(off - 2);
+                }
+                auto tile = [&](auto uc) {
+                    constexpr int U = decltype(uc)::value;
+                    f16x2         hi[4], lo[4];
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        top = fmaxf(top, ml[(w * 16 + c) * 2]);
-    }
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float       part[WAVES];
-    l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        part[w] = __builtin_amdgcn_exp2f(ml[(w * 16 + c) * 2] - ref);
-        l += part[w] * ml[(w * 16 + c) * 2 + 1];
-    }
-    if (live) {
-    float * out;
-    float   by = 1.0f;
-    if (u0 == 0 && u1 == at.units) {
-        out = reinterpret_cast<float *>(a.y + n * a.yn + t * a.yt + head * a.yh);
-        by  = over(l, p >= 0);
-    } else {
-        const int which = u0 == 0 ? 1 : 0;
-        out             = few_o(f, wg, which, c);
-        if (wave == 0 && g == 0) {
-            float * pml = few_ml(f, wg, which, c);
-            pml[0]      = top;
-            pml[1]      = l;
-        }
-    }
-    // four values of a column a thread, so that a row is written in runs of 64 bytes
-    for (int dim = threadIdx.x / 16 * 4; dim < a.hd; dim += 16 * WAVES) {
-        f32x4 v = splat4(0.0f);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int at = C::v_place(dim + k);
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                v[k] += part[w] * of[w * TILES * 4 * kWave + at + c];
+                    for (int e = 0; e < 4; ++e) {
+                        const f16x2 code = C::template v_codes<U>(magic, w[2 * e], w[2 * e + 1]);
+                        hi[e]            = code * d[e];
+                        lo[e]            = __builtin_elementwise_fma(code, d[e], -hi[e]);
+                    }
+                    const f16x8 ah = join8(hi[0], hi[1], hi[2], hi[3]);
+                    const f16x8 al = join8(lo[0], lo[1], lo[2], lo[3]);
+                    f32x4 &     x  = o[s * C::kTiles + U];
+                    x              = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, x, 0, 0, 0);
+                    x              = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, x, 0, 0, 0);
+                    x              = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, x, 0, 0, 0);
+                };
+                for_each(std::make_integer_sequence<int, C::kTiles>{}, tile);
             }
         }
-        *reinterpret_cast<f32x4u *>(out + dim) = v * by;
-    }
-    }
-    unit = begin + u1;
-    if (unit >= last) {
-        return;
-    }
-    __syncthreads();  // the next group's chunks go where the results were
-    begin = unit;
-    if (++hg == f.groups) {
-        hg = 0;
-        do {
-            at.units = few_units(f, ++n);
-        } while (at.units == 0);
-    }
+        l = sum_quarters(l);
+
+        // the waves' results joined in LDS: [wave][value][lane], then m and l of a column
+        __syncthreads();
+        float * of = reinterpret_cast<float *>(lds);
+        float * ml = of + WAVES * TILES * 4 * kWave;
+#pragma unroll
+        for (int u = 0; u < TILES; ++u) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                of[((wave * TILES + u) * 4 + e) * kWave + lane] = o[u][e] * pow2(vexp);
+            }
+        }
+        if (g == 0) {
+            ml[(wave * 16 + c) * 2]     = m;
+            ml[(wave * 16 + c) * 2 + 1] = l;
+        }
+        __syncthreads();
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            top = fmaxf(top, ml[(w * 16 + c) * 2]);
+        }
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float       part[WAVES];
+        l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            part[w] = __builtin_amdgcn_exp2f(ml[(w * 16 + c) * 2] - ref);
+            l += part[w] * ml[(w * 16 + c) * 2 + 1];
+        }
+        if (live) {
+            float * out;
+            float   by = 1.0f;
+            if (u0 == 0 && u1 == at.units) {
+                out = reinterpret_cast<float *>(a.y + n * a.yn + t * a.yt + head * a.yh);
+                by  = over(l, p >= 0);
+            } else {
+                const int which = u0 == 0 ? 1 : 0;
+                out             = few_o(f, wg, which, c);
+                if (wave == 0 && g == 0) {
+                    float * pml = few_ml(f, wg, which, c);
+                    pml[0]      = top;
+                    pml[1]      = l;
+                }
+            }
+            // four values of a column a thread, so that a row is written in runs of 64 bytes
+            for (int dim = threadIdx.x / 16 * 4; dim < a.hd; dim += 16 * WAVES) {
+                f32x4 v = splat4(0.0f);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int at = C::v_place(dim + k);
+#pragma unroll
+                    for (int w = 0; w < WAVES; ++w) {
+                        v[k] += part[w] * of[w * TILES * 4 * kWave + at + c];
+                    }
+                }
+                *reinterpret_cast<f32x4u *>(out + dim) = v * by;
+            }
+        }
+        unit = begin + u1;
+        if (unit >= last) {
+            return;
+        }
+        __syncthreads();  // the next group's chunks go where the results were
+        begin = unit;
+        if (++hg == f.groups) {
+            hg = 0;
+            do {
+                at.units = few_units(f, ++n);
+            } while (at.units == 0);
+        }
     }
 }
 

@@ -12,6 +12,13 @@ namespace {
 // pieces as well, and each product is hi hi + hi lo + lo hi (a 16-bit cache has
 // no second piece). Matrix instructions 32x32x16: S^T = K Q^T has a query in
 // each lane, O^T = V^T P^T too.
+// Bound by the matrix units: 8192 positions of 16 heads of 128 values over 8 kv
+// heads take 730 us, three products at 1.15 PFLOP/s, which is the rate that a
+// large F16 product reaches on this chip, at the clock that such work leaves
+// it. A prompt that does not fill the chip is bound by the longest row: 1021
+// positions 40 us, 11 of them the second launch that joins its splits (Q4_0,
+// MI355X). 128 rows and 64 keys are what the registers (O^T, q, a tile under
+// way: 256) and two workgroups' LDS hold.
 // ---------------------------------------------------------------------------
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -375,7 +382,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
     const int     part0 = static_cast<int>(fastdiv(blockIdx.x, a.fKV));
     const int     h     = static_cast<int>(blockIdx.x) - part0 * a.KV;
     const int     back  = static_cast<int>(fastdiv(static_cast<uint32_t>(part0), a.fsplit));
-    const int     tile  = a.tiles - 1 - back;
+    const int     tile  = back < a.half ? a.tiles - 1 - back : back - a.half;
     const int     split = part0 - back * a.nsplit;
     const int     n     = blockIdx.y;
     const SeqLens len   = seq_lens(a, n);
@@ -400,9 +407,14 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
     const int     head = h * a.G + gq;
 
     const KeyTiles kt  = key_tiles<kTileKeys>(a, p0, p1);
-    const int      per = static_cast<int>(fastdiv(static_cast<uint32_t>(kt.n + a.nsplit - 1), a.fsplit));
-    const int      end = min(kt.n, (split + 1) * per);
-    const int      beg = split * per;
+    const int      beg = split * a.per;
+    const int      end = min(kt.n, beg + a.per);
+    if (split > 0 && beg >= kt.n) {
+        return;
+    }
+    // where the results go: y, or a split's rows (in a scalar register: held in
+    // a vector one through the loop it costs 6%)
+    const int      dest = __builtin_amdgcn_readfirstlane(kt.n <= a.per ? -1 : split);
 
     // K: row tid / NB, block tid % NB; V: item tid % items of group tid / items
     const int    items  = 8 * NB;
@@ -739,13 +751,13 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
     const int64_t row = ((static_cast<int64_t>(n) * a.KV + h) * a.T + t) * a.G + gq;
     float *       out;
     float         by = pow2(oexp);
-    if (a.nsplit == 1) {
+    if (dest < 0) {
         out = reinterpret_cast<float *>(a.y + n * a.yn + t * a.yt + head * a.yh);
         by *= over(l, p >= 0);
     } else {
-        out = partial_o(a, row, split);
+        out = partial_o(a, row, dest);
         if (g == 0) {
-            float * ml = partial_ml(a, row, split);
+            float * ml = partial_ml(a, row, dest);
             ml[0]      = m;
             ml[1]      = l;
         }

@@ -36,10 +36,13 @@ struct AttnArgs {
     int32_t         hd4;  // hd up to a multiple of 4: a partial row's length
     int32_t         cap;
     int32_t         nsplit;
+    int32_t         per;  // key tiles of a split of k_attn_wide; 0: k_attn_any, whose rows all have nsplit
     int32_t         tiles;  // of rows
+    int32_t         half;   // k_attn_wide: the row tiles that come first, longest first; the others follow shortest first
     FastDiv         fG;
     FastDiv         fsplit;
     FastDiv         fKV;
+    FastDiv         fper;
 };
 
 // The key tiles, KT rows each, that a tile of queries at positions p0..p1
@@ -63,6 +66,15 @@ template <int KT> __device__ __forceinline__ KeyTiles key_tiles(const AttnArgs &
     }
     s.n = s.first + last - s.second + 1;
     return s;
+}
+
+// Splits of the keys of a row tile of k_attn_wide. One or none: its rows are
+// written to y directly.
+__device__ __forceinline__ int32_t wide_parts(const AttnArgs & a, int32_t length, int32_t count, int32_t tile) {
+    const int32_t t0 = static_cast<int32_t>(fastdiv(static_cast<uint32_t>(tile * kWideRows), a.fG));
+    const int32_t t1 = static_cast<int32_t>(fastdiv(static_cast<uint32_t>(tile * kWideRows + kWideRows - 1), a.fG));
+    const int32_t n  = key_tiles<kTileKeys>(a, length - count + t0, length - count + min(t1, count - 1)).n;
+    return static_cast<int32_t>(fastdiv(static_cast<uint32_t>(n + a.per - 1), a.fper));
 }
 
 __device__ __forceinline__ int32_t key_tile(const KeyTiles & s, int32_t i) {
@@ -422,6 +434,7 @@ struct AttnPlan {
     int32_t window;
     int32_t sinks;
     int32_t nsplit;
+    int32_t span;  // key tiles of a split of k_attn_wide
 };
 
 // Waves of a workgroup of k_attn_few: two where a row is long; those that each
