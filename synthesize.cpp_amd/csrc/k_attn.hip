@@ -309,16 +309,15 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
         // Splits of equally many key tiles for all rows, however many a row has,
         // as short as lets the chip hold all of them at once: 2048 positions of
         // 16 heads take 81 us, and 99 with every row in thirds (Q4_0, 8 kv heads,
-        // MI355X). With more rows than half of that they are halved, so that a
-        // long row's half runs beside another (4096 positions of 12 heads of 64
-        // values: 131 us, 164 by the rule above), and left whole where the rows
-        // alone fill the chip.
+        // MI355X). Where the row tiles alone are more than half of what it holds,
+        // long rows are halved (2560 positions: 123 us, whole rows 169), and from
+        // three quarters on all are left whole (3584 positions: 234 us, halves 264).
         const int64_t tiles = (rows + kWideRows - 1) / kWideRows;
         const int64_t most  = (keys + kTileKeys - 1) / kTileKeys + (p.window > 0 ? 2 : 0);
         const int64_t pairs = kv * q->ne[3];
         int64_t       span  = (most + kMaxSplits - 1) / kMaxSplits;
         span                = span > kWideSpan ? span : kWideSpan;
-        if (tiles * pairs >= kWideGroups) {
+        if (tiles * pairs > kWideGroups * 3 / 4) {
             span = most;
         } else if (tiles * pairs > kWideGroups / 2) {
             span = span > (most + 1) / 2 ? span : (most + 1) / 2;
@@ -498,7 +497,7 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
         a.fper = make_fastdiv(static_cast<uint32_t>(a.per));
         const int64_t groups = static_cast<int64_t>(a.tiles) * a.KV;
         // with all of them on the chip, two to a CU, a long row tile's neighbour is a
-        // short one (4096 positions: 289 us with the longest first throughout, 278)
+        // short one (4096 positions: 274 us, with the longest first throughout 287)
         const bool    twos   = a.nsplit == 1 && a.N == 1 && groups > kWideGroups / 2 && groups <= kWideGroups;
         a.half               = twos ? static_cast<int32_t>((kWideGroups / 2 + a.KV - 1) / a.KV) : a.tiles;
         st = launch_attn_wide(kind, a, s);

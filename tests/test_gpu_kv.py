@@ -454,3 +454,64 @@ def test_rows_megabytes_apart(gpu, kind, t, row):
         return s
 
     check(gpu, kind, q, k, v, [cap], make=far)
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("t", [1, 3])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 5)])
+def test_long_caches_at_odd_addresses(gpu, kind, t, window, sinks):
+    """Few queries over long caches that no 4-byte read is aligned in."""
+    n, kv, g, hd, cap = 2, 8, 2, 64, 4000
+    q, k, v = rand(n, t, kv * g, kv, hd, cap, 18)
+
+    def odd(c):
+        pool = torch.empty(c.numel() + 2, dtype=torch.uint8, device="cuda")
+        s = pool[2:].view(c.shape)
+        s.copy_(c)
+        return s
+
+    check(gpu, kind, q, k, v, [cap, 1999], window=window, sinks=sinks, make=odd)
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "f16"])
+@pytest.mark.parametrize("t", [1, 33])
+def test_rows_megabytes_apart_in_parts(gpu, kind, t):
+    """As above, with enough of them that the keys of a query are split."""
+    kv, g, hd, cap, row = 8, 2, 64, 150, 40 << 20
+    q, k, v = rand(1, t, kv * g, kv, hd, cap, 19)
+    size = R.pack(k, kind).element_size()
+    width = hd if kind in R.FLOAT else hd // 32 * R.UNIT[kind]
+    pool = torch.empty(cap * row // size, dtype=R.pack(k, kind).dtype, device="cuda")
+    make = [0]
+
+    def far(c):
+        s = pool.as_strided((1, cap, kv, width), (0, row // size, width, 1), 4096 * make[0])
+        make[0] += 1
+        s.copy_(c)
+        return s
+
+    check(gpu, kind, q, k, v, [cap], make=far)
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q8_0", "f16"])
+@pytest.mark.parametrize("t", [1, 3])
+def test_more_sequences_than_a_wave_has_lanes(gpu, kind, t):
+    n, kv, g, hd, cap = 150, 4, 2, 32, 300
+    q, k, v = rand(n, t, kv * g, kv, hd, cap, 20)
+    length = [(37 * b * b + 11 * b) % (cap + 1) for b in range(n)]
+    count = [min(b % (t + 2), t, length[b]) for b in range(n)]
+    check(gpu, kind, q, k, v, length, count)
+    check(gpu, kind, q, k, v, length, [0] * (n - 1) + [min(t, length[-1])])
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "f16"])
+@pytest.mark.parametrize("n,t,kv,g,cap", [(2, 700, 4, 2, 900),      # keys split, rows of one part and of several
+                                          (1, 380, 100, 1, 380),    # rows in two
+                                          (1, 500, 100, 1, 530),    # whole rows, all at once
+                                          (1, 700, 100, 1, 700)])   # and more than that
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 70)])
+def test_prompts_of_many_tiles(gpu, kind, n, t, kv, g, cap, window, sinks):
+    hd = 32
+    q, k, v = rand(n, t, kv * g, kv, hd, cap, 21)
+    length = [cap, 400][:n]
+    check(gpu, kind, q, k, v, length, [min(t, x) - 3 * b for b, x in enumerate(length)], window, sinks)
