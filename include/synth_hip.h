@@ -1,6 +1,7 @@
 /*
  * synth_hip.h -- C ABI of libsynth_hip, the MI355X (gfx950) kernels for the
- * memory-bound non-GEMM primitives that synthesize.cpp's graph builders emit.
+ * memory-bound non-GEMM primitives that synthesize.cpp's graph builders emit,
+ * and for the decoder's KV cache and the attention over it.
  *
  * Every entry point keeps the semantics of the ggml op (or the ggml op run)
  * the reference graphs build today, so a ggml backend module can map nodes

@@ -4,7 +4,7 @@
 // loading, writes) 1 KB of F32 at a time; a block's largest magnitude is three
 // DPP steps away. Both directions are bound by the F32 side's bytes: 16
 // sequences of 8192 rows of 8 heads of 128 values load in 234 us, 5.2 TB/s (a
-// large copy: 5.0), a prompt of 8192 rows is stored in 35 us, 4.4 TB/s (MI355X).
+// large copy: 5.0), and 8192 rows are stored and read back in 35 us (MI355X).
 #include <cmath>
 
 #include "shp_kv.hpp"
