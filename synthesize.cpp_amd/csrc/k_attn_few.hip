@@ -20,10 +20,10 @@ namespace {
 //         against P in two; lo x lo, below 2^-22 of the product, is left out.
 // P is held times 2^15, so that its pieces keep their bits where it is small:
 // a weight is off by at most 2^-40 of the largest, or 2^-23 of itself.
-// Bound by LDS reads and what forms the operands, about as long as the bytes
-// take: 64 streams of 512 to 8192 rows (16 heads of 128 over 8, Q4_0) take 95
-// us, 3.4 TB/s of the cache's 5; one stream of 8191 rows 19 us, 7 of them the
-// join's launch (MI355X).
+// Bound by the vector instructions that form the operands: 470 a chunk of 4.6
+// KB (128 values, Q4_0), which is 61 us of issue on every SIMD for 64 streams of
+// 512 to 8192 rows (16 heads over 8), a call of 93 to 105 us at 3.1 to 3.5
+// TB/s; one stream of 8191 rows takes 18 us, 7 of them the join (MI355X).
 // ---------------------------------------------------------------------------
 
 // Dwords at two-byte boundaries of LDS. A wave's read of them as they are takes

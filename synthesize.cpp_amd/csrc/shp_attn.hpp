@@ -327,10 +327,12 @@ __device__ __forceinline__ void join_parts(int parts, int hd, const ML & ml, con
     const int        tid   = threadIdx.x;
     const int        dim   = tid % (HD / 4) * 4;
     const int        group = tid / (HD / 4);
-    // this thread's first two values on their way while the weights are formed
-    f32x4 first[2];
+    // this thread's first values on their way while the weights are formed (one
+    // stream of 8191 rows, 256 parts of each row: 17.8 us, two ahead 19.2)
+    constexpr int kAhead = 8;
+    f32x4         first[kAhead];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < kAhead; ++k) {
         const int s = group + k * GROUPS;
         first[k]    = dim < hd && s < parts ? *reinterpret_cast<const f32x4 *>(o(s) + dim) : splat4(0.0f);
     }
@@ -377,13 +379,13 @@ __device__ __forceinline__ void join_parts(int parts, int hd, const ML & ml, con
     };
     if (dim < hd) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < kAhead; ++k) {
             if (group + k * GROUPS < parts) {
                 add(group + k * GROUPS, first[k]);
             }
         }
 #pragma unroll 8
-        for (int s = group + 2 * GROUPS; s < parts; s += GROUPS) {
+        for (int s = group + kAhead * GROUPS; s < parts; s += GROUPS) {
             add(s, *reinterpret_cast<const f32x4 *>(o(s) + dim));
         }
     }
