@@ -515,3 +515,19 @@ def test_prompts_of_many_tiles(gpu, kind, n, t, kv, g, cap, window, sinks):
     q, k, v = rand(n, t, kv * g, kv, hd, cap, 21)
     length = [cap, 400][:n]
     check(gpu, kind, q, k, v, length, [min(t, x) - 3 * b for b, x in enumerate(length)], window, sinks)
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q8_0", "bf16", "f32"])
+@pytest.mark.parametrize("t", [1, 5, 40])
+def test_sequences_that_share_a_cache(gpu, kind, t):
+    """One cache's rows at a sequence stride of zero, several queries' continuations."""
+    n, kv, g, hd, cap = 3, 4, 2, 64, 900
+    q, k, v = rand(n, t, kv * g, kv, hd, cap, 22)
+    k, v = (x[:1].expand(n, -1, -1, -1).contiguous() for x in (k, v))
+    check(gpu, kind, q, k, v, [cap] * n, [t, 1, 0], make=lambda c: c[:1].contiguous().expand(n, -1, -1, -1))
+    c = R.pack(k[:1], kind).cuda()
+    h = R.handle(gpu, c.expand(n, -1, -1, -1), kind, hd)
+    x, y = gpu.kv_load(h, h, ints(0, 7, 300), t)
+    for b, slot in enumerate((0, 7, 300)):
+        want = R.values(c[0, slot:slot + t].cpu().contiguous(), kind)
+        assert torch.equal(x[b].cpu(), want) and torch.equal(y[b].cpu(), want)
