@@ -227,6 +227,7 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
     constexpr int    UNIT   = kv_unit_bytes(KIND);
     constexpr int    SLOTS  = (NB * C::kWords + 15) / 16;
     constexpr int    TILES  = SLOTS * C::kTiles;
+    constexpr int    kAtOnce = 2;  // tiles of V whose products take turns: no wait for the one before (a call 3% shorter; 4: 1%)
     constexpr int    P      = (kChunk * NB * UNIT / BYTES + kWave - 1) / kWave;
     extern __shared__ char lds[];
     const AttnArgs & a    = f.a;
@@ -468,6 +469,7 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
                 if (b < nb) {
                     const f16x8 qh = qop[(2 * b) * kWave + lane];
                     const f16x8 ql = qop[(2 * b + 1) * kWave + lane];
+                    f16x8 k[2];
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt) {
                         uint32_t w[C::kStep];
@@ -476,13 +478,23 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
                             const int off = 16 * mt * rb + b * UNIT + 4 * i;
                             w[i]          = b % 2 == 0 ? k0.at(off) : k1.at(off - 2);
                         }
-                        const f16x8 k = C::k_codes(magic, w);
-                        f32x4       x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh, splat4(0.0f), 0, 0, 0);
-                        x             = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql, x, 0, 0, 0);
+                        k[mt] = C::k_codes(magic, w);
+                    }
+                    f32x4 x[2];
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt) {
+                        x[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[mt], qh, splat4(0.0f), 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt) {
+                        x[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[mt], ql, x[mt], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt) {
                         const f32x4 d = *reinterpret_cast<const f32x4 *>(kd + b * kChunk + 16 * mt + 4 * g);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            sc[mt][e] = __builtin_fmaf(d[e], x[e], sc[mt][e]);
+                            sc[mt][e] = __builtin_fmaf(d[e], x[mt][e], sc[mt][e]);
                         }
                     }
                 }
@@ -557,23 +569,38 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
                     const int off = ((e < 4 ? 0 : 12) + e) * rb;
                     w[e]          = nb % 2 == 0 || e % 2 == 0 ? v0.at(off) : v1.at(off - 2);
                 }
-                auto tile = [&](auto uc) {
-                    constexpr int U = decltype(uc)::value;
-                    f16x2         hi[4], lo[4];
+                // kAtOnce tiles at a time, so that their products need not wait for each other
+                auto tiles = [&](auto uc) {
+                    constexpr int U = kAtOnce * decltype(uc)::value;
+                    f16x8         ah[kAtOnce], al[kAtOnce];
+                    auto          pieces = [&](auto vc) {
+                        constexpr int V = decltype(vc)::value;
+                        f16x2         hi[4], lo[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const f16x2 code = C::template v_codes<U>(magic, w[2 * e], w[2 * e + 1]);
-                        hi[e]            = code * d[e];
-                        lo[e]            = __builtin_elementwise_fma(code, d[e], -hi[e]);
+                        for (int e = 0; e < 4; ++e) {
+                            const f16x2 code = C::template v_codes<U + V>(magic, w[2 * e], w[2 * e + 1]);
+                            hi[e]            = code * d[e];
+                            lo[e]            = __builtin_elementwise_fma(code, d[e], -hi[e]);
+                        }
+                        ah[V] = join8(hi[0], hi[1], hi[2], hi[3]);
+                        al[V] = join8(lo[0], lo[1], lo[2], lo[3]);
+                    };
+                    for_each(std::make_integer_sequence<int, kAtOnce>{}, pieces);
+                    f32x4 * x = o + s * C::kTiles + U;
+#pragma unroll
+                    for (int v = 0; v < kAtOnce; ++v) {
+                        x[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[v], bh, x[v], 0, 0, 0);
                     }
-                    const f16x8 ah = join8(hi[0], hi[1], hi[2], hi[3]);
-                    const f16x8 al = join8(lo[0], lo[1], lo[2], lo[3]);
-                    f32x4 &     x  = o[s * C::kTiles + U];
-                    x              = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, x, 0, 0, 0);
-                    x              = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, x, 0, 0, 0);
-                    x              = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, x, 0, 0, 0);
+#pragma unroll
+                    for (int v = 0; v < kAtOnce; ++v) {
+                        x[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[v], bl, x[v], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int v = 0; v < kAtOnce; ++v) {
+                        x[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[v], bh, x[v], 0, 0, 0);
+                    }
                 };
-                for_each(std::make_integer_sequence<int, C::kTiles>{}, tile);
+                for_each(std::make_integer_sequence<int, C::kTiles / kAtOnce>{}, tiles);
             }
         }
         l = sum_quarters(l);
