@@ -247,8 +247,9 @@ bool wide_takes(const shp_tensor & c) {
 
 constexpr int64_t kWideGroups  = 512;  // workgroups of k_attn_wide that the chip holds
 constexpr int64_t kWideSpan    = 2;    // key tiles at least: 300 positions take 20.9 us, with 3 23.4
-constexpr int64_t kWhole       = 4;
-constexpr int64_t kShortGroups = 256;
+constexpr int64_t kWhole       = 4;    // chunks a wave of a group of k_attn_few that is not split
+constexpr int64_t kShortGroups = 256;  // its groups where a short cache is shared out by heads, at most
+constexpr int64_t kFewGroups   = 256;  // parts of one of its groups that have one chunk a wave
 
 shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t window, int32_t sinks, AttnPlan & p) {
     if (!well_formed(q) || !kv_well_formed(k_cache) || q->ne[0] != k_cache->ne[0] || q->ne[1] % k_cache->ne[1] != 0 ||
@@ -295,9 +296,11 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
         p.few               = units < INT32_MAX;
         p.parts             = units > groups();
         p.groups            = static_cast<int32_t>(groups());
-        // a group that is split: two chunks a wave at least (one stream of 8191
-        // rows: 20 us with the join, 24 with one chunk, 22 with four)
-        const int64_t want = p.parts ? (units + 1) / 2 : units;
+        // A chunk a wave, while a group has no more parts for its join than one of
+        // a CU; past that two chunks (4000 rows of 12 heads of 64 values: 12.9 us,
+        // 15.5 with two chunks; 8191 rows of 8 heads of 128: 17.3 us, 21.5 with one
+        // chunk, 19.2 with three).
+        const int64_t want = units > kFewGroups * groups() ? (units + 1) / 2 : units;
         const int64_t most = few_resident(kv_kind(k_cache->type), k_cache->ne[0]);
         p.wgs              = static_cast<int32_t>(want < most ? want : most);
         // where the caches' strides are not that kernel's: as many splits as its workspace holds

@@ -23,7 +23,7 @@ namespace {
 // Bound by the vector instructions that form the operands: 470 a chunk of 4.6
 // KB (128 values, Q4_0), which is 61 us of issue on every SIMD for 64 streams of
 // 512 to 8192 rows (16 heads over 8), a call of 93 to 105 us at 3.1 to 3.5
-// TB/s; one stream of 8191 rows takes 18 us, 7 of them the join (MI355X).
+// TB/s; one stream of 8191 rows takes 17 us, 7 of them the join (MI355X).
 // ---------------------------------------------------------------------------
 
 // Dwords at two-byte boundaries of LDS. A wave's read of them as they are takes

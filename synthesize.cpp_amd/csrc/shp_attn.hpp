@@ -328,7 +328,7 @@ __device__ __forceinline__ void join_parts(int parts, int hd, const ML & ml, con
     const int        dim   = tid % (HD / 4) * 4;
     const int        group = tid / (HD / 4);
     // this thread's first values on their way while the weights are formed (one
-    // stream of 8191 rows, 256 parts of each row: 17.8 us, two ahead 19.2)
+    // stream of 8191 rows, 256 parts of each row: 1.4 us less than two ahead)
     constexpr int kAhead = 8;
     f32x4         first[kAhead];
 #pragma unroll
