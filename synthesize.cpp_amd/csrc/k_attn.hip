@@ -15,8 +15,11 @@ namespace shp {
 namespace {
 
 // ---------------------------------------------------------------------------
-// Any type, stride and alignment: a wave takes 16 rows and, of its split, 16
-// keys at a time, in F32 matrix instructions (16x16x4) fed value by value.
+// Any type, stride and alignment, for what the other kernels do not take (rows
+// 16 MB and more apart, 16-bit rows of an odd length): a wave takes 16 rows and,
+// of its split, 16 keys at a time, in F32 matrix instructions (16x16x4) fed value
+// by value. Bound by those loads (2048 positions of 8 heads of 256 values over 4:
+// 1.8 to 2.8 ms, MI355X).
 // ---------------------------------------------------------------------------
 
 template <int KIND, int HD> __global__ __launch_bounds__(64) void k_attn_any(const AttnArgs a) {
@@ -237,19 +240,22 @@ int32_t plan_splits(int64_t tiles, int64_t units, int64_t want) {
 // Positions and windows are int32, and so are their sums and differences.
 constexpr int64_t kAttnMaxKeys = int64_t{ 1 } << 30;
 
-// Whether k_attn_wide takes a cache: its operands fit the registers, 64 rows
-// lie at 32-bit offsets, and a row ends with a whole dword (the last that its
-// descriptor lets through).
+// Whether k_attn_wide takes a cache: 64 rows lie at 32-bit offsets, and a row
+// ends with a whole dword (the last that its descriptor lets through).
 bool wide_takes(const shp_tensor & c) {
-    return c.ne[0] <= 4 * kKvBlock && (c.ne[2] == 1 || c.nb[2] < (size_t{ 1 } << 24)) &&
+    return (c.ne[2] == 1 || c.nb[2] < (size_t{ 1 } << 24)) &&
            (kv_blocks(kv_kind(c.type)) || kv_bytes_of_row(c) % 4 == 0);
 }
 
-constexpr int64_t kWideGroups  = 512;  // workgroups of k_attn_wide that the chip holds
 constexpr int64_t kWideSpan    = 2;    // key tiles at least: 300 positions take 20.9 us, with 3 23.4
 constexpr int64_t kWhole       = 4;    // chunks a wave of a group of k_attn_few that is not split
 constexpr int64_t kShortGroups = 256;  // its groups where a short cache is shared out by heads, at most
 constexpr int64_t kFewGroups   = 256;  // parts of one of its groups that have one chunk a wave
+
+// Workgroups of k_attn_wide that the chip holds.
+int64_t wide_groups(int64_t hd) {
+    return hd <= 4 * kKvBlock ? 512 : 256;
+}
 
 shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t window, int32_t sinks, AttnPlan & p) {
     if (!well_formed(q) || !kv_well_formed(k_cache) || q->ne[0] != k_cache->ne[0] || q->ne[1] % k_cache->ne[1] != 0 ||
@@ -315,25 +321,26 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
         // MI355X). Where the row tiles alone are more than half of what it holds,
         // long rows are halved (2560 positions: 123 us, whole rows 169), and from
         // three quarters on all are left whole (3584 positions: 234 us, halves 264).
+        const int64_t chip  = wide_groups(q->ne[0]);
         const int64_t tiles = (rows + kWideRows - 1) / kWideRows;
         const int64_t most  = (keys + kTileKeys - 1) / kTileKeys + (p.window > 0 ? 2 : 0);
         const int64_t pairs = kv * q->ne[3];
         int64_t       span  = (most + kMaxSplits - 1) / kMaxSplits;
         span                = span > kWideSpan ? span : kWideSpan;
-        if (tiles * pairs > kWideGroups * 3 / 4) {
+        if (tiles * pairs > chip * 3 / 4) {
             span = most;
-        } else if (tiles * pairs > kWideGroups / 2) {
+        } else if (tiles * pairs > chip / 2) {
             span = span > (most + 1) / 2 ? span : (most + 1) / 2;
         } else {
             auto fits = [&](int64_t of) {
                 int64_t groups = 0;
-                for (int64_t t = 0; t < tiles && groups <= kWideGroups; ++t) {
+                for (int64_t t = 0; t < tiles && groups <= chip; ++t) {
                     // of a whole cache, and within a window all alike
                     const int64_t end = cap - T + ((t + 1) * kWideRows * T + rows - 1) / rows;
                     const int64_t n   = ((end < cap ? end : cap) + kTileKeys - 1) / kTileKeys;
                     groups += ((n < most ? n : most) + of - 1) / of * pairs;
                 }
-                return groups <= kWideGroups;
+                return groups <= chip;
             };
             for (int64_t upto = most; span < upto;) {  // the shortest that fits
                 const int64_t mid = (span + upto) / 2;
@@ -498,11 +505,12 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
             a.per              = static_cast<int32_t>((most + a.nsplit - 1) / a.nsplit);
         }
         a.fper = make_fastdiv(static_cast<uint32_t>(a.per));
+        const int64_t chip   = wide_groups(a.hd);
         const int64_t groups = static_cast<int64_t>(a.tiles) * a.KV;
         // with all of them on the chip, two to a CU, a long row tile's neighbour is a
         // short one (4096 positions: 274 us, with the longest first throughout 287)
-        const bool    twos   = a.nsplit == 1 && a.N == 1 && groups > kWideGroups / 2 && groups <= kWideGroups;
-        a.half               = twos ? static_cast<int32_t>((kWideGroups / 2 + a.KV - 1) / a.KV) : a.tiles;
+        const bool    twos   = a.nsplit == 1 && a.N == 1 && groups > chip / 2 && groups <= chip;
+        a.half               = twos ? static_cast<int32_t>((chip / 2 + a.KV - 1) / a.KV) : a.tiles;
         st = launch_attn_wide(kind, a, s);
         return st == SHP_OK && a.nsplit > 1 ? launch_join(a, s) : st;
     }

@@ -18,7 +18,8 @@ namespace {
 // it. A prompt that does not fill the chip is bound by the longest row: 1021
 // positions 40 us, 11 of them the second launch that joins its splits (Q4_0,
 // MI355X). 128 rows and 64 keys are what the registers (O^T, q, a tile under
-// way: 256) and two workgroups' LDS hold.
+// way: 256) and two workgroups' LDS hold; heads of more than 128 values have one
+// workgroup a CU, with 512 (2048 positions of 8 heads of 256 over 4, Q4_0: 136 us).
 // ---------------------------------------------------------------------------
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -50,8 +51,10 @@ template <int KIND, int WORDS> struct BlockPart {
     static constexpr bool kScaled = true;
     uint32_t              k[WORDS];
     uint32_t              v[8];
-    uint16_t              kd;
-    uint16_t              vd[8];
+    // (dwords: halves are put into pairs, for which a wave waits as soon as it has
+    // asked for them; 8192 positions 780 to 736 us)
+    uint32_t              kd;
+    uint32_t              vd[8];
 
     // the block `at` bytes into the tile
     __device__ void load_k(const Rsrc & r, int at) {
@@ -110,7 +113,7 @@ template <int KIND, int WORDS> struct BlockPart {
         f16x2 h[4], l[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const f16x2 d = as_f16x2(vd[2 * e] | static_cast<uint32_t>(vd[2 * e + 1]) << 16) * splat2(by);
+            const f16x2 d = as_f16x2(vd[2 * e] | vd[2 * e + 1] << 16) * splat2(by);
             exact(Codes<KIND>::template v_codes<U>(m, v[2 * e] >> shift, v[2 * e + 1] >> shift), d, h[e], l[e]);
         }
         hi = join8(h[0], h[1], h[2], h[3]);
@@ -358,7 +361,7 @@ template <int KIND, int NB> constexpr int wide_lds() {
     return (kTileKeys * (HD * 2 + 16) + HD * kVStride) * (Part<KIND>::kTwo ? 2 : 1) + 16 * kWaves;
 }
 
-template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_attn_wide(const AttnArgs a) {
+template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2 : 1) void k_attn_wide(const AttnArgs a) {
     using PartT             = Part<KIND>;
     using C                 = KOrder<KIND>;
     constexpr int  HD       = NB * kKvBlock;
@@ -416,34 +419,45 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
     // a vector one through the loop it costs 6%)
     const int      dest = __builtin_amdgcn_readfirstlane(kt.n <= a.per ? -1 : split);
 
-    // K: row tid / NB, block tid % NB; V: item tid % items of group tid / items
-    const int    items  = 8 * NB;
-    const int    words  = PartT::words(NB);
-    const bool   mine   = tid < kTileKeys * NB;
-    const int    krow   = tid / NB;
-    const int    kblk   = tid % NB;
-    const int    vgroup = tid / items;
-    const int    vitem  = tid % items;
-    const int    vkey   = 16 * (vgroup >> 1) + 4 * (vgroup & 1);
-    const char * kb     = a.k + n * a.kn + h * a.kh;
-    const char * vb     = a.v + n * a.vn + h * a.vh;
-    const int    kstep  = static_cast<int>(a.kt);
-    const int    vstep  = static_cast<int>(a.vt);
-    const int    kat    = krow * kstep + kblk * UNIT;
-    const int    vat0   = vkey * vstep + PartT::word_at(vitem, words);
-    const int    vat1   = vkey * vstep + PartT::block_at(vitem, words);
-    const int    rb     = static_cast<int>(kv_row_bytes(KIND, a.hd));
-    PartT        part;
+    // Part z of a thread is number id = tid + 256 z. K: row id / NB, block id % NB;
+    // V: item id % items of group id / items
+    constexpr int PARTS = (kTileKeys * NB + kWideBlock - 1) / kWideBlock;
+    const int     items = 8 * NB;
+    const int     words = PartT::words(NB);
+    const int     kstep = static_cast<int>(a.kt);
+    const int     vstep = static_cast<int>(a.vt);
+    bool          mine[PARTS];
+    int           krow[PARTS], kblk[PARTS], vgroup[PARTS], vitem[PARTS], vkey[PARTS], kat[PARTS], vat0[PARTS], vat1[PARTS];
+#pragma unroll
+    for (int z = 0; z < PARTS; ++z) {
+        const int id = tid + kWideBlock * z;
+        mine[z]      = id < kTileKeys * NB;
+        krow[z]      = id / NB;
+        kblk[z]      = id % NB;
+        vgroup[z]    = id / items;
+        vitem[z]     = id % items;
+        vkey[z]      = 16 * (vgroup[z] >> 1) + 4 * (vgroup[z] & 1);
+        kat[z]       = krow[z] * kstep + kblk[z] * UNIT;
+        vat0[z]      = vkey[z] * vstep + PartT::word_at(vitem[z], words);
+        vat1[z]      = vkey[z] * vstep + PartT::block_at(vitem[z], words);
+    }
+    const char * kb = a.k + n * a.kn + h * a.kh;
+    const char * vb = a.v + n * a.vn + h * a.vh;
+    const int    rb = static_cast<int>(kv_row_bytes(KIND, a.hd));
+    PartT        part[PARTS];
     // (rows past the last that a query sees read as zero)
     auto fetch = [&](int i) {
         const int32_t j0 = key_tile(kt, i) * kTileKeys;
         const Rsrc    kr = rows_from(kb + j0 * a.kt, (p1 - j0) * a.kt + rb);
         const Rsrc    vr = rows_from(vb + j0 * a.vt, (p1 - j0) * a.vt + rb);
-        if (mine) {
-            part.load_k(kr, kat);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                part.load_v(e, vr, vat0, vat1, (e < 4 ? e : e + 4) * vstep);
+        for (int z = 0; z < PARTS; ++z) {
+            if (mine[z]) {
+                part[z].load_k(kr, kat[z]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    part[z].load_v(e, vr, vat0[z], vat1[z], (e < 4 ? e : e + 4) * vstep);
+                }
             }
         }
     };
@@ -516,43 +530,54 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
         const int32_t j0 = key_tile(kt, i) * kTileKeys;
         float kby = 1.0f, vby = 1.0f;
         int   kexp = 0;
-        if (mine) {
-            const bool edge = j0 + kTileKeys - 1 > p0 || (a.window > 0 && j0 <= p1 - a.window && j0 + kTileKeys > a.sinks);
-            if (edge) {  // rows that no query of the tile sees count for nothing, whatever they hold
-                part.keep_k(seen_by(a, p0, p1, j0 + krow));
+        const bool edge = j0 + kTileKeys - 1 > p0 || (a.window > 0 && j0 <= p1 - a.window && j0 + kTileKeys > a.sinks);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    part.keep_v(e, seen_by(a, p0, p1, j0 + vkey + (e < 4 ? e : e + 4)));
+        for (int z = 0; z < PARTS; ++z) {
+            if (mine[z]) {
+                if (edge) {  // rows that no query of the tile sees count for nothing, whatever they hold
+                    part[z].keep_k(seen_by(a, p0, p1, j0 + krow[z]));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        part[z].keep_v(e, seen_by(a, p0, p1, j0 + vkey[z] + (e < 4 ? e : e + 4)));
+                    }
                 }
-            }
-            if constexpr (!kv_blocks(KIND)) {
-                if (a.hd < HD) {
-                    part.cut(a.hd - kKvBlock * kblk, a.hd - 4 * vitem);
+                if constexpr (!kv_blocks(KIND)) {
+                    if (a.hd < HD) {
+                        part[z].cut(a.hd - kKvBlock * kblk[z], a.hd - 4 * vitem[z]);
+                    }
                 }
             }
         }
         {
             uint32_t tk = 0, tv = 0;
             uint64_t bad = 0;  // keys
-            if (mine) {
-                tk = part.top_k();
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    tv = max(tv, part.top_v(e));
+            for (int z = 0; z < PARTS; ++z) {
+                if (mine[z]) {
+                    tk = max(tk, part[z].top_k());
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        tv = max(tv, part[z].top_v(e));
+                    }
                 }
             }
             if (__any(max(tk, tv) >= PartT::kInf)) {
                 // what is not finite in K is its key's alone; a key whose V has
                 // such a value counts for nothing in the products
-                if (mine) {
-                    tk = tk >= PartT::kInf ? part.finite_k() : tk;
-                    tv = 0;
+                tk = 0;
+                tv = 0;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const bool is = part.top_v(e) >= PartT::kInf;
-                        bad |= static_cast<uint64_t>(is) << (vkey + (e < 4 ? e : e + 4));
-                        part.keep_v(e, !is);
-                        tv = max(tv, part.top_v(e));
+                for (int z = 0; z < PARTS; ++z) {
+                    if (mine[z]) {
+                        const uint32_t whole = part[z].top_k();
+                        tk                   = max(tk, whole >= PartT::kInf ? part[z].finite_k() : whole);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const bool is = part[z].top_v(e) >= PartT::kInf;
+                            bad |= static_cast<uint64_t>(is) << (vkey[z] + (e < 4 ? e : e + 4));
+                            part[z].keep_v(e, !is);
+                            tv = max(tv, part[z].top_v(e));
+                        }
                     }
                 }
 #pragma unroll
@@ -590,29 +615,32 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, 2) void k_a
             kby  = pow2(-kexp);
             vby  = pow2(-vexp);
         }
-        if (mine) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f16x8 hi, lo;
-                part.k_pieces(magic, kby, j, hi, lo);
-                const int at = krow * KSTRIDE + kblk * 64 + 16 * j;
-                *reinterpret_cast<f16x8 *>(kh + at) = hi;
-                if constexpr (TWO) {
-                    *reinterpret_cast<f16x8 *>(kl + at) = lo;
+        for (int z = 0; z < PARTS; ++z) {
+            if (mine[z]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f16x8 hi, lo;
+                    part[z].k_pieces(magic, kby, j, hi, lo);
+                    const int at = krow[z] * KSTRIDE + kblk[z] * 64 + 16 * j;
+                    *reinterpret_cast<f16x8 *>(kh + at) = hi;
+                    if constexpr (TWO) {
+                        *reinterpret_cast<f16x8 *>(kl + at) = lo;
+                    }
                 }
+                auto column = [&](auto uc) {
+                    constexpr int U = decltype(uc)::value;
+                    f16x8         hi, lo;
+                    part[z].template v_column<U>(magic, vby, vitem[z], words, hi, lo);
+                    const int dim = PartT::index(vitem[z], words, U);
+                    const int at  = dim * kVStride + (vgroup[z] ^ (dim >> PartT::kTurn & 3)) * 16;
+                    *reinterpret_cast<f16x8 *>(vh + at) = hi;
+                    if constexpr (TWO) {
+                        *reinterpret_cast<f16x8 *>(vl + at) = lo;
+                    }
+                };
+                for_each(std::make_integer_sequence<int, 4>{}, column);
             }
-            auto column = [&](auto uc) {
-                constexpr int U = decltype(uc)::value;
-                f16x8         hi, lo;
-                part.template v_column<U>(magic, vby, vitem, words, hi, lo);
-                const int dim = PartT::index(vitem, words, U);
-                const int at  = dim * kVStride + (vgroup ^ (dim >> PartT::kTurn & 3)) * 16;
-                *reinterpret_cast<f16x8 *>(vh + at) = hi;
-                if constexpr (TWO) {
-                    *reinterpret_cast<f16x8 *>(vl + at) = lo;
-                }
-            };
-            for_each(std::make_integer_sequence<int, 4>{}, column);
         }
         if (i + 1 < end) {
             fetch(i + 1);
@@ -794,8 +822,16 @@ template <int KIND> shp_status_t launch_wide(const AttnArgs & a, hipStream_t str
             return launch_wide_as<KIND, 2>(a, stream);
         case 3:
             return launch_wide_as<KIND, 3>(a, stream);
-        default:
+        case 4:
             return launch_wide_as<KIND, 4>(a, stream);
+        case 5:
+            return launch_wide_as<KIND, 5>(a, stream);
+        case 6:
+            return launch_wide_as<KIND, 6>(a, stream);
+        case 7:
+            return launch_wide_as<KIND, 7>(a, stream);
+        default:
+            return launch_wide_as<KIND, 8>(a, stream);
     }
 }
 

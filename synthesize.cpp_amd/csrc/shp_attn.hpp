@@ -459,7 +459,7 @@ constexpr int few_resident(int kind, int64_t hd) {
 int          few_piece(const shp_tensor & k, const shp_tensor & v, int hgs, int32_t & run);
 shp_status_t launch_attn_few(int kind, const AttnArgs & a, const AttnPlan & p, int piece, int32_t run, hipStream_t stream);
 
-// k_attn_wide.hip: head_dim up to 128.
+// k_attn_wide.hip.
 shp_status_t launch_attn_wide(int kind, const AttnArgs & a, hipStream_t stream);
 
 }  // namespace shp

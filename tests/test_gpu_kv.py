@@ -531,3 +531,13 @@ def test_sequences_that_share_a_cache(gpu, kind, t):
     for b, slot in enumerate((0, 7, 300)):
         want = R.values(c[0, slot:slot + t].cpu().contiguous(), kind)
         assert torch.equal(x[b].cpu(), want) and torch.equal(y[b].cpu(), want)
+
+
+@pytest.mark.parametrize("kind,hd", [(k, hd) for k in R.TYPES for hd in (160, 192, 224, 256)] +
+                         [("f32", 129), ("f16", 130), ("bf16", 250), ("f16", 131)])
+@pytest.mark.parametrize("t,cap", [(1, 300), (90, 200), (300, 700)])
+def test_long_heads(gpu, kind, hd, t, cap):
+    n, kv, g = 2, 2, 3
+    q, k, v = rand(n, t, kv * g, kv, hd, cap, 23)
+    check(gpu, kind, q, k, v, [cap, 100], [t, min(t, 60)])
+    check(gpu, kind, q, k, v, [cap, 100], [t, min(t, 60)], window=50, sinks=3)
