@@ -368,6 +368,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
     constexpr int  UNIT     = kv_unit_bytes(KIND) * (kv_blocks(KIND) ? 1 : kKvBlock);
     constexpr int  KSTRIDE  = HD * 2 + 16;
     constexpr bool TWO      = PartT::kTwo;
+    constexpr bool kPlainScaled = PartT::kScaled && !kv_blocks(KIND);
     extern __shared__ char lds[];
     char * const   kh   = lds;
     char * const   kl   = kh + kTileKeys * KSTRIDE;  // (of two pieces)
@@ -478,7 +479,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
     };
     // the query's operands; the largest of its values scaled to [2^13, 2^14)
     f16x8 qh[2 * NB], ql[2 * NB];
-    float qscale;
+    int   qexp;
     {
         const float * qr = reinterpret_cast<const float *>(a.q + n * a.qn + t * a.qt + head * a.qh);
         float         q[2 * NB][8];
@@ -496,9 +497,8 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
         }
         const Pair both = swap32(top);
         top             = fmaxf(both.a, both.b);
-        const int ex    = exponent_of(top) - 13;
-        const float to  = pow2(-ex);
-        qscale          = pow2(ex);
+        qexp            = exponent_of(top) - 13;
+        const float to  = pow2(-qexp);
 #pragma unroll
         for (int s = 0; s < 2 * NB; ++s) {
             f16x2 hi[4], lo[4];
@@ -656,7 +656,10 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                 }
             }
         }
-        const float qs = qscale * pow2(kexp);
+        // what the scores are times: of blocks (kexp >= 0) and of F16 (0) a normal
+        // number; of the others, a zero query's and zero keys' exponents add up to
+        // -226, so it is multiplied in here, ahead of the mask's infinities
+        const float qs = kPlainScaled ? 1.0f : pow2(qexp) * pow2(kexp);
         if (PartT::kScaled && vexp != oexp) {
             const float by = pow2(max(oexp - vexp, -126));
 #pragma unroll
@@ -698,6 +701,15 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
             }
         }
         __builtin_amdgcn_s_setprio(0);
+        if constexpr (kPlainScaled) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    sc[x][e] = __builtin_ldexpf(sc[x][e], qexp + kexp);
+                }
+            }
+        }
         const bool all = j0 + kTileKeys - 1 <= w0 && (a.window == 0 || j0 > w1 - a.window || j0 + kTileKeys <= a.sinks);
         if (!all) {
             int g4 = 4 * g;

@@ -94,3 +94,59 @@ def attend(q, k, v, length, count, scale, window=0, sinks=0):
                 e = (hd + 16) * EPS * float((kh.abs() @ q[b, i, h].abs()).max()) * abs(scale)
                 bound[b, i, h] = (np.expm1(2 * e) + (len(seen) + 32) * EPS) * (w @ vh.abs()) + 2.0 ** -40 * vh.abs().sum(0) + 2.0 ** -126
     return y, bound
+
+
+def attend_by_row(q, k, v, kind, length, count, scale, window=0, sinks=0):
+    """(y, bound) as attend() gives them, with a bound that lets each row of the
+    cache err by what is its own alone, so that a row whose weight is nothing, or
+    that a query does not see, cannot hide what it does to the others.
+
+    A score s_j = scale q.k_j is off by e_j: hd products summed in f32, operands,
+    lo x lo and the scale's product off by half steps each (16 more), the
+    difference s_j - max rounded (|s_j| + |max|), and, what two F16 pieces under
+    one power of two for a row leave, 2^-38 of the row's largest value for each
+    value of q and of k_j: hd 2^-37 max|q| max|k_j|. A weight then moves by
+    w_j (e^(e_j) - 1), and the sum of weights by E = sum_j w_j (e^(e_j) - 1).
+    To this come attend()'s n + 32 half steps of the sum and of the joins, and
+    2^-126 where f32 ends. A weight is held to 2^-40 of the largest, which moves a
+    result by 2^-40 |v_j| w_max; F32 and BF16 weights, held times their row's
+    largest value, to 2^-37 of the largest such product, and V's values to 2^-38
+    of their row's largest."""
+    n, t, heads, hd = q.shape
+    group = heads // k.shape[2]
+    y = torch.full(q.shape, float("nan"), dtype=torch.float64)
+    bound = torch.zeros_like(y)
+    for b in range(n):
+        ln, c = int(length[b]), int(count[b])
+        if c == 0:
+            continue
+        kk = k[b, :ln].double().repeat_interleave(group, 1).transpose(0, 1)    # (heads, ln, hd)
+        vv = v[b, :ln].double().repeat_interleave(group, 1).transpose(0, 1)
+        at = ln - c + torch.arange(c)
+        j = torch.arange(ln)
+        hidden = j > at[:, None]
+        if window:
+            hidden |= (j <= at[:, None] - window) & (j >= sinks)
+        some = ~hidden.all(1)
+        # what no query of the sequence sees may be anything at all
+        kk, vv = (torch.where(hidden.all(0)[None, :, None], 0.0, x) for x in (kk, vv))
+        x = q[b, :c].double().transpose(0, 1)                                  # (heads, c, hd)
+        s = scale * (x @ kk.transpose(1, 2))
+        s = s.masked_fill(hidden, -float("inf"))
+        top = s.amax(-1, keepdim=True).nan_to_num(neginf=0.0)
+        w = (s - top).exp()
+        w = w / w.sum(-1, keepdim=True).clamp_min(1e-300)
+        size = abs(scale) * (x.abs() @ kk.abs().transpose(1, 2))
+        kmax, vmax = kk.abs().amax(-1), vv.abs().amax(-1)                      # (heads, ln)
+        e = (hd + 16) * EPS * size + abs(scale) * hd * 2.0 ** -37 * x.abs().amax(-1)[..., None] * kmax[:, None]
+        e = e + EPS * (s.abs() + top.abs())
+        e = torch.where(hidden, 0.0, torch.expm1(e.nan_to_num(posinf=0.0).clamp_max(700.0)))
+        moved = w * (e + (w * e).sum(-1, keepdim=True))
+        far = moved @ vv.abs() + (ln + 32) * EPS * (w @ vv.abs())
+        if kind in ("f32", "bf16"):
+            far = far + (2.0 ** -38 * (w @ vmax[..., None]) + ln * 2.0 ** -37 * (w * vmax[:, None]).amax(-1, keepdim=True))
+        else:
+            far = far + 2.0 ** -40 * w.amax(-1, keepdim=True) * ((~hidden).double() @ vv.abs())
+        y[b, :c] = torch.where(some[None, :, None], w @ vv, 0.0).transpose(0, 1)
+        bound[b, :c] = (far + 2.0 ** -126).transpose(0, 1)
+    return y, bound
