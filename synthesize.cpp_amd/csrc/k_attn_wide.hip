@@ -8,10 +8,11 @@ namespace {
 // Many queries (prompts): a workgroup takes 128 rows, 32 a wave, and 64 keys at
 // a time, whose K and V it brings into LDS once, as matrix operands: K by row,
 // V by column with the keys in the order in which the scores stand in
-// registers. A block's code * d is exact as two F16 pieces; q and P are two
-// pieces as well, and each product is hi hi + hi lo + lo hi (a 16-bit cache has
-// no second piece). Matrix instructions 32x32x16: S^T = K Q^T has a query in
-// each lane, O^T = V^T P^T too.
+// registers. A block's code * d is exact as two F16 pieces, and an F32 value is two
+// as well; so are q and P, and each product is hi hi + hi lo + lo hi (an F16 cache
+// has no second piece). A BF16 cache is BF16 operands as it is, of any size, and q
+// and P are three BF16 pieces, all 24 bits of them. Matrix instructions 32x32x16:
+// S^T = K Q^T has a query in each lane, O^T = V^T P^T too.
 // Bound by the matrix units: 8192 positions of 16 heads of 128 values over 8 kv
 // heads take 730 us, three products at 1.15 PFLOP/s, which is the rate that a
 // large F16 product reaches on this chip, at the clock that such work leaves
@@ -34,15 +35,15 @@ constexpr int kVStride   = kTileKeys * 2 + 16;  // bytes of a column of V in LDS
 // `dim` of V the groups stand in the order group ^ (dim >> kTurn & 3): sixteen
 // lanes that write a group of sixteen columns then meet every bank once (four
 // times four without it: a third of the LDS unit's time).
-// The pieces are of the values times 2^-shift, where a tile's values are out of
-// F16's range or, F32 and BF16, always: their largest comes to [2^13, 2^14).
+// The pieces are of the values times 2^-shift, where a tile's blocks are out of
+// F16's range or, F32, always (see by_size): their largest comes to [2^13, 2^14).
 //   load_k, load_v  from the cache, through descriptors of the tile
 //   keep_k, keep_v  or zeros in place of K's row, of V's of key e
 //   top_k, top_v    bits that bound the magnitudes, kInf and more where one is
 //                   infinite or NaN; finite_k without those; no scale is needed
 //                   up to kLeave
 //   k_pieces        operand j of the row's four, times `by`
-//   v_pieces        value U of the eight keys
+//   v_column        value U of the eight keys, times `by`
 template <int KIND> struct Part;
 
 // Codes and d: exact products; a scale goes to d.
@@ -160,7 +161,7 @@ template <> struct Part<kKvQ8> : BlockPart<kKvQ8, 8> {
 // Plain values, four next to each other a key of V.
 template <int KIND> struct PlainPart {
     static constexpr bool  kTwo    = KIND == kKvF32;
-    static constexpr bool  kScaled = KIND != kKvF16;
+    static constexpr bool  kScaled = KIND == kKvF32;
     static constexpr int   kTurn   = 4;
     static constexpr uint32_t kLeave = 0;
     static constexpr int   kSize   = kv_unit_bytes(KIND);
@@ -231,14 +232,6 @@ template <int KIND> struct PlainPart {
         }
     }
 
-    __device__ static float value(const uint32_t * w, int i) {
-        if constexpr (KIND == kKvF32) {
-            return __uint_as_float(w[i]);
-        } else {
-            return i % 2 == 0 ? __uint_as_float(w[i / 2] << 16) : __uint_as_float(w[i / 2] & 0xffff0000u);
-        }
-    }
-
     // Magnitudes as their bits, in whose order a NaN is the largest.
     static constexpr uint32_t kInf = KIND == kKvF32 ? 0x7f800000u : KIND == kKvF16 ? 0x7c00u : 0x7f80u;
 
@@ -297,22 +290,14 @@ template <int KIND> struct PlainPart {
 
     __device__ static int index(int item, int, int u) { return 4 * item + u; }
 
-    __device__ static void pieces(float a, float b, float by, f16x2 & hi, f16x2 & lo) {
-        if constexpr (kTwo) {
-            split2(a * by, b * by, hi, lo);
-        } else {
-            hi = f16x2{ static_cast<_Float16>(a * by), static_cast<_Float16>(b * by) };
-        }
-    }
-
     __device__ void k_pieces(const Magic &, float by, int j, f16x8 & hi, f16x8 & lo) const {
         f16x2 h[4], l[4] = {};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if constexpr (KIND == kKvF16) {
-                h[e] = as_f16x2(k[4 * j + e]);
+            if constexpr (kTwo) {
+                split2(__uint_as_float(k[8 * j + 2 * e]) * by, __uint_as_float(k[8 * j + 2 * e + 1]) * by, h[e], l[e]);
             } else {
-                pieces(value(k, 8 * j + 2 * e), value(k, 8 * j + 2 * e + 1), by, h[e], l[e]);
+                h[e] = as_f16x2(k[4 * j + e]);  // (BF16's bits, of two values)
             }
         }
         hi = join8(h[0], h[1], h[2], h[3]);
@@ -323,11 +308,11 @@ template <int KIND> struct PlainPart {
         f16x2 h[4], l[4] = {};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if constexpr (KIND == kKvF16) {
+            if constexpr (kTwo) {
+                split2(__uint_as_float(v[2 * e][U]) * by, __uint_as_float(v[2 * e + 1][U]) * by, h[e], l[e]);
+            } else {
                 constexpr uint32_t kSel = U % 2 == 0 ? 0x05040100u : 0x07060302u;
                 h[e]                    = as_f16x2(__builtin_amdgcn_perm(v[2 * e + 1][U / 2], v[2 * e][U / 2], kSel));
-            } else {
-                pieces(value(v[2 * e], U), value(v[2 * e + 1], U), by, h[e], l[e]);
             }
         }
         hi = join8(h[0], h[1], h[2], h[3]);
@@ -351,14 +336,57 @@ template <int KIND> struct KOrder {
 
 template <> struct KOrder<kKvQ4> : Codes<kKvQ4> {};
 
-// The shift that brings values bounded by `top` to [2^13, 2^14), if they need one.
-template <int KIND> __device__ __forceinline__ int shift_of(float top) {
-    return kv_blocks(KIND) ? shift_of_d(top) : Part<KIND>::kScaled ? exponent_of(top) - 13 : 0;
+// F32, whose values may be of any size. One power of two for the K and one for the
+// V of a tile cost a value up to 2^-39 of the tile's largest, so they are used
+// where no row is much smaller than that: a tile is even where every 32 values of
+// K and four of V that are not all zero have one of 2^-8 of the tile's largest and
+// more. A tile that is not is taken in several passes, each over the rows of about
+// one size (2^kAlike times smaller or larger than the first that is left) as if the
+// others were hidden. So a value is off by 2^-30 of its own row's largest at most,
+// whatever the others are, and a row that a query does not see has no part in its
+// result.
+// V's sizes differ from pass to pass: weights are held times 2^(E - X + 15), 2^E
+// being that of the pass and 2^X, which is the query's own, what the largest so
+// far of weight times 2^E needs. So P loses 2^-29 of the largest weighted row at
+// most (2^-39 of the largest weight where all rows are of one size).
+constexpr bool by_size(int kind) {
+    return kind == kKvF32;
+}
+
+constexpr float kEven  = 0x1p-7f;  // of the largest that a wave holds, and waves within a factor of 2
+constexpr int   kAlike = 4;
+constexpr int   kVTop  = 13;       // the largest value of V comes to 2^13 and more
+constexpr int   kMinX  = -99;      // of values of 2^-100 and less
+
+// Three pieces of q and P. The third of q is in LDS: 2 NB operands a lane.
+constexpr bool in_three(int kind) {
+    return kind == kKvBF16;
 }
 
 template <int KIND, int NB> constexpr int wide_lds() {
     constexpr int HD = NB * kKvBlock;
-    return (kTileKeys * (HD * 2 + 16) + HD * kVStride) * (Part<KIND>::kTwo ? 2 : 1) + 16 * kWaves;
+    return (kTileKeys * (HD * 2 + 16) + HD * kVStride) * (Part<KIND>::kTwo ? 2 : 1) + 24 * kWaves +
+           (by_size(KIND) ? 2 * 4 * kTileKeys : 0) + (in_three(KIND) ? 2 * NB * kWideBlock * 16 : 0);
+}
+
+typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+
+// a and b: BF16 rounded, as a pair of bits, and what that leaves of them.
+__device__ __forceinline__ f16x2 take_b16(float & a, float & b) {
+    typedef float  f32x2 __attribute__((ext_vector_type(2)));
+    const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{ a, b }), b16x2));
+    a -= __uint_as_float(w << 16);
+    b -= __uint_as_float(w & 0xffff0000u);
+    return as_f16x2(w);
+}
+
+template <int KIND> __device__ __forceinline__ f32x16 product(const f16x8 & a, const f16x8 & b, const f32x16 & c) {
+    if constexpr (in_three(KIND)) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
 }
 
 template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2 : 1) void k_attn_wide(const AttnArgs a) {
@@ -368,14 +396,17 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
     constexpr int  UNIT     = kv_unit_bytes(KIND) * (kv_blocks(KIND) ? 1 : kKvBlock);
     constexpr int  KSTRIDE  = HD * 2 + 16;
     constexpr bool TWO      = PartT::kTwo;
-    constexpr bool kPlainScaled = PartT::kScaled && !kv_blocks(KIND);
+    constexpr bool SIZES    = by_size(KIND);
+    constexpr bool THREE    = in_three(KIND);
     extern __shared__ char lds[];
     char * const   kh   = lds;
     char * const   kl   = kh + kTileKeys * KSTRIDE;  // (of two pieces)
     char * const   vh   = kl + (TWO ? kTileKeys * KSTRIDE : 0);
     char * const   vl   = vh + HD * kVStride;
-    float * const  tops = reinterpret_cast<float *>(vl + (TWO ? HD * kVStride : 0));  // of each wave's K and V
-    uint64_t *     bads = reinterpret_cast<uint64_t *>(tops + 2 * kWaves);            // a wave's keys that are not finite in V
+    float * const  tops = reinterpret_cast<float *>(vl + (TWO ? HD * kVStride : 0));  // of each wave's K and V, then the least
+    uint64_t *     bads = reinterpret_cast<uint64_t *>(tops + 4 * kWaves);            // a wave's keys that are not finite in V
+    uint32_t *     rmax = reinterpret_cast<uint32_t *>(bads + kWaves);                // SIZES: the largest of each row of K, then V
+    f16x8 *        q3   = reinterpret_cast<f16x8 *>(bads + kWaves) + threadIdx.x;     // THREE: the third pieces of a lane's query
 
     const int     tid   = threadIdx.x;
     const int     wave  = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -421,26 +452,37 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
     const int      dest = __builtin_amdgcn_readfirstlane(kt.n <= a.per ? -1 : split);
 
     // Part z of a thread is number id = tid + 256 z. K: row id / NB, block id % NB;
-    // V: item id % items of group id / items
+    // V: item id % items of group id / items, keys key_v and on.
+    // Indexes that begin with tid_again() are not formed ahead of the loop and held
+    // through it: those of what only some tiles need, and, with tid_each(), all of
+    // them where registers are short (F32: 16 sequences of 4096 rows take 166 us, 211
+    // without; heads of 256 values: F16 91, 98; but F16 at 128: 199, 191).
+    auto tid_again = [] {
+        int id = threadIdx.x;
+        asm volatile("" : "+v"(id));
+        return id;
+    };
+    auto tid_each = [&] {
+        if constexpr (SIZES || NB > 4) {
+            return tid_again();
+        } else {
+            return tid;
+        }
+    };
+    auto row_k = [](int id, int z) { return (id + kWideBlock * z) / NB; };
+    auto key_v = [](int id, int z) {
+        const int group = (id + kWideBlock * z) / (8 * NB);
+        return 16 * (group >> 1) + 4 * (group & 1);
+    };
     constexpr int PARTS = (kTileKeys * NB + kWideBlock - 1) / kWideBlock;
     const int     items = 8 * NB;
     const int     words = PartT::words(NB);
     const int     kstep = static_cast<int>(a.kt);
     const int     vstep = static_cast<int>(a.vt);
     bool          mine[PARTS];
-    int           krow[PARTS], kblk[PARTS], vgroup[PARTS], vitem[PARTS], vkey[PARTS], kat[PARTS], vat0[PARTS], vat1[PARTS];
 #pragma unroll
     for (int z = 0; z < PARTS; ++z) {
-        const int id = tid + kWideBlock * z;
-        mine[z]      = id < kTileKeys * NB;
-        krow[z]      = id / NB;
-        kblk[z]      = id % NB;
-        vgroup[z]    = id / items;
-        vitem[z]     = id % items;
-        vkey[z]      = 16 * (vgroup[z] >> 1) + 4 * (vgroup[z] & 1);
-        kat[z]       = krow[z] * kstep + kblk[z] * UNIT;
-        vat0[z]      = vkey[z] * vstep + PartT::word_at(vitem[z], words);
-        vat1[z]      = vkey[z] * vstep + PartT::block_at(vitem[z], words);
+        mine[z] = tid + kWideBlock * z < kTileKeys * NB;
     }
     const char * kb = a.k + n * a.kn + h * a.kh;
     const char * vb = a.v + n * a.vn + h * a.vh;
@@ -451,13 +493,16 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
         const int32_t j0 = key_tile(kt, i) * kTileKeys;
         const Rsrc    kr = rows_from(kb + j0 * a.kt, (p1 - j0) * a.kt + rb);
         const Rsrc    vr = rows_from(vb + j0 * a.vt, (p1 - j0) * a.vt + rb);
+        const int     id = tid_each();
 #pragma unroll
         for (int z = 0; z < PARTS; ++z) {
             if (mine[z]) {
-                part[z].load_k(kr, kat[z]);
+                const int item = (id + kWideBlock * z) % items;
+                const int key  = key_v(id, z) * vstep;
+                part[z].load_k(kr, row_k(id, z) * kstep + (id + kWideBlock * z) % NB * UNIT);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    part[z].load_v(e, vr, vat0[z], vat1[z], (e < 4 ? e : e + 4) * vstep);
+                    part[z].load_v(e, vr, key + PartT::word_at(item, words), key + PartT::block_at(item, words), (e < 4 ? e : e + 4) * vstep);
                 }
             }
         }
@@ -495,26 +540,43 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                 top     = fmaxf(top, fabsf(q[s][e]));
             }
         }
-        const Pair both = swap32(top);
-        top             = fmaxf(both.a, both.b);
-        qexp            = exponent_of(top) - 13;
-        const float to  = pow2(-qexp);
+        if constexpr (THREE) {
+            qexp = 0;
 #pragma unroll
-        for (int s = 0; s < 2 * NB; ++s) {
-            f16x2 hi[4], lo[4];
+            for (int s = 0; s < 2 * NB; ++s) {
+                f16x2 hi[4], mid[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                split2(q[s][2 * e] * to, q[s][2 * e + 1] * to, hi[e], lo[e]);
+                for (int e = 0; e < 4; ++e) {
+                    hi[e]  = take_b16(q[s][2 * e], q[s][2 * e + 1]);
+                    mid[e] = take_b16(q[s][2 * e], q[s][2 * e + 1]);
+                    lo[e]  = take_b16(q[s][2 * e], q[s][2 * e + 1]);
+                }
+                qh[s]              = join8(hi[0], hi[1], hi[2], hi[3]);
+                ql[s]              = join8(mid[0], mid[1], mid[2], mid[3]);
+                q3[s * kWideBlock] = join8(lo[0], lo[1], lo[2], lo[3]);
             }
-            qh[s] = join8(hi[0], hi[1], hi[2], hi[3]);
-            ql[s] = join8(lo[0], lo[1], lo[2], lo[3]);
+        } else {
+            const Pair both = swap32(top);
+            top             = fmaxf(both.a, both.b);
+            qexp            = exponent_of(top) - 13;
+            const float to  = pow2(-qexp);
+#pragma unroll
+            for (int s = 0; s < 2 * NB; ++s) {
+                f16x2 hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    split2(q[s][2 * e] * to, q[s][2 * e + 1] * to, hi[e], lo[e]);
+                }
+                qh[s] = join8(hi[0], hi[1], hi[2], hi[3]);
+                ql[s] = join8(lo[0], lo[1], lo[2], lo[3]);
+            }
         }
     }
 
     // group `even` + g of column 32 u + c
-    auto vat = [&](int u, int even) {
-        const int turn = (32 * u >> PartT::kTurn & 3) ^ (PartT::kTurn == 4 ? c >> 4 : 0);
-        return (32 * u + c) * kVStride + ((even + g) ^ turn) * 16;
+    auto vat = [&](int lane_of, int u, int even) {
+        const int turn = (32 * u >> PartT::kTurn & 3) ^ (PartT::kTurn == 4 ? lane_of >> 4 & 1 : 0);
+        return (32 * u + (lane_of & 31)) * kVStride + ((even + (lane_of >> 5)) ^ turn) * 16;
     };
     f32x16 o[NB];
 #pragma unroll
@@ -523,60 +585,90 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
     }
     float m    = -INFINITY;
     float l    = 0.0f;
-    int   vexp = shift_of<KIND>(0.0f);  // V in LDS is times 2^-vexp, o times 2^-oexp
-    int   oexp = vexp;
+    int   vexp = 0;  // blocks: V in LDS is times 2^-vexp, o times 2^-oexp
+    int   oexp = 0;
+    int   X    = kMinX;  // SIZES: o is times 2^(15 + kVTop - X)
 
-    for (int i = beg; i < end; ++i) {
+    constexpr uint64_t kEvery = ~uint64_t{ 0 };
+    uint64_t           left   = kEvery;  // SIZES: the tile's keys that no pass has had,
+    uint64_t           pass   = kEvery;  // those of this one,
+    bool               alike  = false;   // and whether they are known to be of one size
+
+    for (int i = beg; i < end;) {
         const int32_t j0 = key_tile(kt, i) * kTileKeys;
         float kby = 1.0f, vby = 1.0f;
-        int   kexp = 0;
+        int      kexp   = 0;
+        int      vsize  = 0;       // SIZES: the exponent of V's largest
+        const uint64_t member = pass;
+        bool     ready  = true;
         const bool edge = j0 + kTileKeys - 1 > p0 || (a.window > 0 && j0 <= p1 - a.window && j0 + kTileKeys > a.sinks);
 #pragma unroll
         for (int z = 0; z < PARTS; ++z) {
             if (mine[z]) {
                 if (edge) {  // rows that no query of the tile sees count for nothing, whatever they hold
-                    part[z].keep_k(seen_by(a, p0, p1, j0 + krow[z]));
+                    const int id = tid_again();
+                    part[z].keep_k(seen_by(a, p0, p1, j0 + row_k(id, z)));
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        part[z].keep_v(e, seen_by(a, p0, p1, j0 + vkey[z] + (e < 4 ? e : e + 4)));
+                        part[z].keep_v(e, seen_by(a, p0, p1, j0 + key_v(id, z) + (e < 4 ? e : e + 4)));
                     }
                 }
                 if constexpr (!kv_blocks(KIND)) {
                     if (a.hd < HD) {
-                        part[z].cut(a.hd - kKvBlock * kblk[z], a.hd - 4 * vitem[z]);
+                        const int id = tid_again() + kWideBlock * z;
+                        part[z].cut(a.hd - kKvBlock * (id % NB), a.hd - 4 * (id % items));
                     }
                 }
             }
         }
         {
+            if (SIZES && pass != kEvery) {  // the others as if hidden
+                const int id = tid_again();
+#pragma unroll
+                for (int z = 0; z < PARTS; ++z) {
+                    if (mine[z]) {
+                        part[z].keep_k(pass >> row_k(id, z) & 1);
+                        const uint32_t from = static_cast<uint32_t>(pass >> key_v(id, z));
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            part[z].keep_v(e, from >> (e < 4 ? e : e + 4) & 1);
+                        }
+                    }
+                }
+            }
             uint32_t tk = 0, tv = 0;
-            uint64_t bad = 0;  // keys
+            uint32_t lk = ~0u, lv = ~0u;  // the least that is not 0, less 1
+            uint64_t bad = 0;             // keys
+            auto     note = [&](uint32_t x, uint32_t & most, uint32_t & least) {
+                most  = max(most, x);
+                least = min(least, x - 1u);
+            };
 #pragma unroll
             for (int z = 0; z < PARTS; ++z) {
                 if (mine[z]) {
-                    tk = max(tk, part[z].top_k());
+                    note(part[z].top_k(), tk, lk);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        tv = max(tv, part[z].top_v(e));
+                        note(part[z].top_v(e), tv, lv);
                     }
                 }
             }
             if (__any(max(tk, tv) >= PartT::kInf)) {
                 // what is not finite in K is its key's alone; a key whose V has
                 // such a value counts for nothing in the products
-                tk = 0;
-                tv = 0;
+                tk = tv = 0;
+                lk = lv = ~0u;
 #pragma unroll
                 for (int z = 0; z < PARTS; ++z) {
                     if (mine[z]) {
                         const uint32_t whole = part[z].top_k();
-                        tk                   = max(tk, whole >= PartT::kInf ? part[z].finite_k() : whole);
+                        note(whole >= PartT::kInf ? part[z].finite_k() : whole, tk, lk);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const bool is = part[z].top_v(e) >= PartT::kInf;
-                            bad |= static_cast<uint64_t>(is) << (vkey[z] + (e < 4 ? e : e + 4));
+                            bad |= static_cast<uint64_t>(is) << (key_v(tid_again(), z) + (e < 4 ? e : e + 4));
                             part[z].keep_v(e, !is);
-                            tv = max(tv, part[z].top_v(e));
+                            note(part[z].top_v(e), tv, lv);
                         }
                     }
                 }
@@ -585,7 +677,16 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                     bad |= __shfl_xor(static_cast<unsigned long long>(bad), off);
                 }
             }
-            if (PartT::kScaled && (!kv_blocks(KIND) || __any(max(tk, tv) > PartT::kLeave))) {  // (blocks: hardly ever)
+            if constexpr (SIZES) {
+                const float fk  = wave_max(PartT::magnitude(tk));
+                const float fv  = wave_max(PartT::magnitude(tv));
+                const bool  odd = (lk != ~0u && PartT::magnitude(lk + 1u) < fk * kEven) ||
+                                 (lv != ~0u && PartT::magnitude(lv + 1u) < fv * kEven);
+                const float none = __any(odd) ? 1.0f : 0.0f;
+                if (lane < 3) {
+                    tops[lane * kWaves + wave] = lane == 0 ? fk : lane == 1 ? fv : none;
+                }
+            } else if (PartT::kScaled && __any(max(tk, tv) > PartT::kLeave)) {  // (hardly ever)
                 const float fk = wave_max(PartT::magnitude(tk));
                 const float fv = wave_max(PartT::magnitude(tv));
                 if (lane == 0) {
@@ -604,10 +705,62 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
         const uint64_t every = bads[0] | bads[1] | bads[2] | bads[3];
         uint64_t       none  = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(every >> 32)));
         none                 = none << 32 | static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(every)));
-        if constexpr (PartT::kScaled) {
+        if constexpr (SIZES) {
+            auto waves = [&](int which) { return *reinterpret_cast<const f32x4 *>(tops + which * kWaves); };
+            auto most  = [](const f32x4 & t) { return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])); };
+            auto apart = [](const f32x4 & t, float top) {
+                bool is = false;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    is = is || (t[w] != 0.0f && t[w] < 0.5f * top);
+                }
+                return is;
+            };
+            const f32x4 k4 = waves(0), v4 = waves(1);
+            const float kt = most(k4);
+            const float vt = most(v4);
+            if (!alike && __builtin_amdgcn_readfirstlane(apart(k4, kt) || apart(v4, vt) || most(waves(2)) != 0.0f)) {
+                if (tid < 2 * kTileKeys) {
+                    rmax[tid] = 0;
+                }
+                __syncthreads();
+                auto at_least = [&](int row, uint32_t top) {
+                    __hip_atomic_fetch_max(rmax + row, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                };
+                const int id = tid_again();
+#pragma unroll
+                for (int z = 0; z < PARTS; ++z) {
+                    if (mine[z]) {
+                        at_least(row_k(id, z), part[z].finite_k());
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            at_least(kTileKeys + key_v(id, z) + (e < 4 ? e : e + 4), part[z].top_v(e));
+                        }
+                    }
+                }
+                __syncthreads();
+                // a lane a key; rows of zeros go with any
+                const float    k1   = PartT::magnitude(rmax[lane]);
+                const float    v1   = PartT::magnitude(rmax[kTileKeys + lane]);
+                const bool     zero = k1 == 0.0f && v1 == 0.0f;
+                const int      ke   = exponent_of(k1);
+                const int      ve   = exponent_of(v1);
+                const uint64_t some = __ballot((left >> lane & 1) && !zero);
+                const int      one  = some == 0 ? 0 : __ffsll(static_cast<unsigned long long>(some)) - 1;
+                const bool     in   = (left >> lane & 1) && (zero || (abs(ke - __builtin_amdgcn_readlane(ke, one)) <= kAlike &&
+                                                                   abs(ve - __builtin_amdgcn_readlane(ve, one)) <= kAlike));
+                alike               = true;
+                pass                = __ballot(in);
+                ready               = pass == left;
+            }
+            kexp  = __builtin_amdgcn_readfirstlane(exponent_of(kt)) - 13;
+            vsize = __builtin_amdgcn_readfirstlane(exponent_of(vt));
+            kby   = pow2(-kexp);
+            vby   = pow2(kVTop - vsize);
+        } else if constexpr (PartT::kScaled) {
             auto most = [&](int at) {
                 const f32x4 t = *reinterpret_cast<const f32x4 *>(tops + at);
-                return __builtin_amdgcn_readfirstlane(shift_of<KIND>(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]))));
+                return __builtin_amdgcn_readfirstlane(shift_of_d(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]))));
             };
             // K by tile; V never less than for the tiles before, which o holds
             kexp = most(0);
@@ -615,14 +768,17 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
             kby  = pow2(-kexp);
             vby  = pow2(-vexp);
         }
+        const int staged = tid_each();
 #pragma unroll
         for (int z = 0; z < PARTS; ++z) {
             if (mine[z]) {
+                const int id   = staged + kWideBlock * z;
+                const int item = id % items;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     f16x8 hi, lo;
                     part[z].k_pieces(magic, kby, j, hi, lo);
-                    const int at = krow[z] * KSTRIDE + kblk[z] * 64 + 16 * j;
+                    const int at = id / NB * KSTRIDE + id % NB * 64 + 16 * j;
                     *reinterpret_cast<f16x8 *>(kh + at) = hi;
                     if constexpr (TWO) {
                         *reinterpret_cast<f16x8 *>(kl + at) = lo;
@@ -631,9 +787,9 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                 auto column = [&](auto uc) {
                     constexpr int U = decltype(uc)::value;
                     f16x8         hi, lo;
-                    part[z].template v_column<U>(magic, vby, vitem[z], words, hi, lo);
-                    const int dim = PartT::index(vitem[z], words, U);
-                    const int at  = dim * kVStride + (vgroup[z] ^ (dim >> PartT::kTurn & 3)) * 16;
+                    part[z].template v_column<U>(magic, vby, item, words, hi, lo);
+                    const int dim = PartT::index(item, words, U);
+                    const int at  = dim * kVStride + (id / items ^ (dim >> PartT::kTurn & 3)) * 16;
                     *reinterpret_cast<f16x8 *>(vh + at) = hi;
                     if constexpr (TWO) {
                         *reinterpret_cast<f16x8 *>(vl + at) = lo;
@@ -642,12 +798,21 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                 for_each(std::make_integer_sequence<int, 4>{}, column);
             }
         }
-        if (i + 1 < end) {
-            fetch(i + 1);
+        if constexpr (SIZES) {
+            const uint64_t rest = ready ? left & ~pass : left;
+            i += rest == 0;
+            left  = rest == 0 ? kEvery : rest;
+            pass  = ready ? left : pass;
+            alike = !ready;
+        } else {
+            ++i;
+        }
+        if (i < end) {
+            fetch(i);
         }
         __syncthreads();
-        if (j0 > w1) {
-            continue;  // none of it is seen by this wave's queries
+        if (!ready || j0 > w1) {
+            continue;  // to be had again in part, or none of it is seen by this wave's queries
         }
         if (none != 0) {  // ... but it makes the result of a query that sees it NaN, and no other's
             for (; none != 0; none &= none - 1) {
@@ -656,11 +821,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                 }
             }
         }
-        // what the scores are times: of blocks (kexp >= 0) and of F16 (0) a normal
-        // number; of the others, a zero query's and zero keys' exponents add up to
-        // -226, so it is multiplied in here, ahead of the mask's infinities
-        const float qs = kPlainScaled ? 1.0f : pow2(qexp) * pow2(kexp);
-        if (PartT::kScaled && vexp != oexp) {
+        if (kv_blocks(KIND) && vexp != oexp) {
             const float by = pow2(max(oexp - vexp, -126));
 #pragma unroll
             for (int u = 0; u < NB; ++u) {
@@ -687,29 +848,30 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
             }
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[x], qh[s], sc[x], 0, 0, 0);
+                sc[x] = product<KIND>(hi[x], qh[s], sc[x]);
             }
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[x], ql[s], sc[x], 0, 0, 0);
+                sc[x] = product<KIND>(hi[x], ql[s], sc[x]);
+            }
+            if constexpr (THREE) {
+                const f16x8 third = q3[s * kWideBlock];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    sc[x] = product<KIND>(hi[x], third, sc[x]);
+                }
             }
             if constexpr (TWO) {
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo[x], qh[s], sc[x], 0, 0, 0);
+                    sc[x] = product<KIND>(lo[x], qh[s], sc[x]);
                 }
             }
         }
         __builtin_amdgcn_s_setprio(0);
-        if constexpr (kPlainScaled) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    sc[x][e] = __builtin_ldexpf(sc[x][e], qexp + kexp);
-                }
-            }
-        }
+        // (within what is a normal number: a zero query's and zero keys' exponents
+        // add up to -226, and 0 times a hidden key's -infinity is NaN)
+        const float qs = pow2(min(max(qexp + kexp, -126), 127));
         const bool all = j0 + kTileKeys - 1 <= w0 && (a.window == 0 || j0 > w1 - a.window || j0 + kTileKeys <= a.sinks);
         if (!all) {
             int g4 = 4 * g;
@@ -722,6 +884,16 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                 }
             }
         }
+        if (SIZES && member != kEvery) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t in = static_cast<uint32_t>(member >> (32 * x)) >> (4 * g);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    sc[x][e] = in >> (8 * (e / 4) + e % 4) & 1u ? sc[x][e] : -INFINITY;
+                }
+            }
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -730,54 +902,84 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                 top = fmaxf(top, sc[x][e]);
             }
         }
-        const Pair both = swap32(top);
-        top             = fmaxf(m, fmaxf(both.a, both.b) * qs);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        if (__any(top > m)) {
+        const Pair  both = swap32(top);
+        const float here = fmaxf(both.a, both.b) * qs;
+        top              = fmaxf(m, here);
+        const float ref  = top == -INFINITY ? 0.0f : top;
+        int         need = X;
+        if constexpr (SIZES) {
+            // what this pass's largest weighted row needs, or those before it, whose
+            // weights have gone down
+            const int down = static_cast<int>(fminf(floorf(ref - m), 1000.0f));
+            need           = vsize + 1 + static_cast<int>(fmaxf(floorf(here - ref), -1000.0f));
+            need           = max(max(need, X - down), kMinX);
+        }
+        if (__any(top > m || need != X)) {
             const float alpha = __builtin_amdgcn_exp2f(m - ref);
+            const float by    = SIZES ? __builtin_ldexpf(alpha, X - need) : alpha;
             l *= alpha;
 #pragma unroll
             for (int u = 0; u < NB; ++u) {
-                o[u] *= alpha;
+                o[u] *= by;
             }
         }
-        m = top;
-        const float less = kPShift - ref;
+        m                 = top;
+        X                 = need;
+        const float less  = (SIZES || THREE ? 0.0f : kPShift) - ref;
+        const int   times = vsize + 15 - X;
+        auto        held  = [&](float score) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score, qs, less));
+            l += w;
+            return SIZES ? __builtin_ldexpf(w, times) : w;
+        };
+        const int from = tid_each() % kWave;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                f16x2 hi[4], lo[4];
+                f16x2 hi[4], lo[4], third[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float a0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][8 * s + 2 * e], qs, less));
-                    const float a1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][8 * s + 2 * e + 1], qs, less));
-                    l += a0 + a1;
-                    split2(a0, a1, hi[e], lo[e]);
+                    float a0 = held(sc[x][8 * s + 2 * e]);
+                    float a1 = held(sc[x][8 * s + 2 * e + 1]);
+                    if constexpr (THREE) {
+                        hi[e]    = take_b16(a0, a1);
+                        lo[e]    = take_b16(a0, a1);
+                        third[e] = take_b16(a0, a1);
+                    } else {
+                        split2(a0, a1, hi[e], lo[e]);
+                    }
                 }
                 const f16x8 ph = join8(hi[0], hi[1], hi[2], hi[3]);
                 const f16x8 pl = join8(lo[0], lo[1], lo[2], lo[3]);
                 f16x8 vv[NB];
 #pragma unroll
                 for (int u = 0; u < NB; ++u) {
-                    vv[u] = *reinterpret_cast<const f16x8 *>(vh + vat(u, 4 * x + 2 * s));
+                    vv[u] = *reinterpret_cast<const f16x8 *>(vh + vat(from, u, 4 * x + 2 * s));
                 }
 #pragma unroll
                 for (int u = 0; u < NB; ++u) {
-                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u], ph, o[u], 0, 0, 0);
+                    o[u] = product<KIND>(vv[u], ph, o[u]);
                 }
 #pragma unroll
                 for (int u = 0; u < NB; ++u) {
-                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u], pl, o[u], 0, 0, 0);
+                    o[u] = product<KIND>(vv[u], pl, o[u]);
+                }
+                if constexpr (THREE) {
+                    const f16x8 p3 = join8(third[0], third[1], third[2], third[3]);
+#pragma unroll
+                    for (int u = 0; u < NB; ++u) {
+                        o[u] = product<KIND>(vv[u], p3, o[u]);
+                    }
                 }
                 if constexpr (TWO) {
 #pragma unroll
                     for (int u = 0; u < NB; ++u) {
-                        vv[u] = *reinterpret_cast<const f16x8 *>(vl + vat(u, 4 * x + 2 * s));
+                        vv[u] = *reinterpret_cast<const f16x8 *>(vl + vat(from, u, 4 * x + 2 * s));
                     }
 #pragma unroll
                     for (int u = 0; u < NB; ++u) {
-                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vv[u], ph, o[u], 0, 0, 0);
+                        o[u] = product<KIND>(vv[u], ph, o[u]);
                     }
                 }
             }
@@ -790,7 +992,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
     }
     const int64_t row = ((static_cast<int64_t>(n) * a.KV + h) * a.T + t) * a.G + gq;
     float *       out;
-    float         by = pow2(oexp);
+    float         by = SIZES ? 1.0f : pow2(oexp);
     if (dest < 0) {
         out = reinterpret_cast<float *>(a.y + n * a.yn + t * a.yt + head * a.yh);
         by *= over(l, p >= 0);
@@ -801,6 +1003,16 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
             ml[0]      = m;
             ml[1]      = l;
         }
+    }
+    if constexpr (SIZES) {
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                o[u][e] = __builtin_ldexpf(o[u][e] * by, X - 15 - kVTop);
+            }
+        }
+        by = 1.0f;
     }
 #pragma unroll
     for (int u = 0; u < NB; ++u) {

@@ -48,3 +48,79 @@ def test_queries_and_keys_of_zero_and_next_to_it(gpu, kind, t, hd, cap, small):
     ks[:, 64::3] *= small
     run(gpu, kind, qs, ks, v, [cap, (cap + 1) // 2])
     run(gpu, kind, q * small, k * small, v * small, [cap, (cap + 1) // 2], window=30, sinks=2)
+
+
+LARGE = {"f32": 1e12, "bf16": 1e12, "f16": 1e4}
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("t,hd,cap", [(40, 64, 200), (130, 128, 130), (3, 128, 300), (5, 160, 90), (64, 32, 64)])
+@pytest.mark.parametrize("window", [0, 20])
+def test_a_large_key_does_not_touch_the_queries_that_do_not_see_it(gpu, kind, t, hd, cap, window):
+    """Ahead of the first queries and, with the window, behind the last."""
+    q, k, v = rand(1, t, 4, 2, hd, cap, 33)
+    for row in (cap - t, cap - t // 2, cap - 1):
+        x = k.clone()
+        x[0, row] *= LARGE[kind]
+        run(gpu, kind, q, x, v, [cap], window=window, sinks=1)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("t,hd,cap", [(1, 64, 100), (1, 128, 700), (40, 64, 200), (130, 128, 130), (5, 160, 90)])
+def test_a_large_key_of_no_weight(gpu, kind, t, hd, cap):
+    """Its scores are far below the others'; it moves no other row's weight."""
+    q, k, v = rand(1, t, 4, 2, hd, cap, 34)
+    q = q.abs() + 0.5
+    for row in (0, cap - t, cap // 3):
+        x = k.clone()
+        x[0, row] = -LARGE[kind]
+        run(gpu, kind, q, x, v, [cap])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("t,hd,cap", [(40, 64, 200), (130, 128, 130), (3, 128, 300), (5, 160, 90), (300, 32, 300)])
+@pytest.mark.parametrize("window", [0, 20])
+def test_a_large_value_does_not_touch_the_queries_that_do_not_see_it(gpu, kind, t, hd, cap, window):
+    q, k, v = rand(1, t, 4, 2, hd, cap, 35)
+    for row in (cap - t, cap - t // 2, cap - 1):
+        x = v.clone()
+        x[0, row] *= LARGE[kind]
+        run(gpu, kind, q, k, x, [cap], window=window, sinks=1)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("t,hd,cap", [(1, 64, 100), (1, 128, 700), (40, 64, 200), (130, 128, 130), (5, 160, 90)])
+def test_a_large_value_of_no_weight(gpu, kind, t, hd, cap):
+    q, k, v = rand(1, t, 4, 2, hd, cap, 36)
+    q = q.abs() + 0.5
+    for row in (0, cap - t, cap // 3):
+        x, z = k.clone(), v.clone()
+        x[0, row] = -1e4
+        z[0, row] *= LARGE[kind]
+        run(gpu, kind, q, x, z, [cap])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("t,kv,g,hd", [(1, 8, 2, 128), (1, 8, 1, 64), (2, 4, 2, 64), (40, 4, 2, 64)])
+def test_heads_of_different_sizes(gpu, kind, t, kv, g, hd):
+    """A head whose values are large beside heads of ordinary and small ones."""
+    q, k, v = rand(2, t, kv * g, kv, hd, 150, 37)
+    v[:, :, 1] *= LARGE[kind] / 20
+    v[:, :, 0] *= 0.06
+    v[:, 70:, 2] *= LARGE[kind] / 20
+    run(gpu, kind, q, k, v, [150, 90])
+    k[:, :, 1], q[:, :, g:2 * g] = k[:, :, 1] * LARGE[kind] / 20, q[:, :, g:2 * g] * 1e-5
+    k[:, :, 0] *= 1e-3
+    run(gpu, kind, q, k, v, [150, 90])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("t,hd", [(1, 64), (40, 64), (130, 128), (7, 200)])
+def test_rows_of_all_sizes(gpu, kind, t, hd):
+    """Rows of V from 1e-30 to 1e30 and of K from 1e-12 to 1e3, in any order."""
+    q, k, v = rand(2, t, 4, 2, hd, 200, 39)
+    g = torch.Generator().manual_seed(40)
+    up = lambda lo, hi: 10.0 ** (lo + (hi - lo) * torch.rand((2, 200, 2, 1), generator=g))
+    run(gpu, kind, q, k, v * up(-30, 30), [200, 131])
+    run(gpu, kind, q, k * up(-12, 0), v * up(-30, 30), [200, 131], window=30, sinks=4)
+    run(gpu, kind, q, k * up(-12, 3), v * up(-3, 3), [200, 131])
