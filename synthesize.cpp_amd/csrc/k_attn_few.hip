@@ -320,7 +320,7 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
         for (int u = 0; u < TILES; ++u) {
             o[u] = splat4(0.0f);
         }
-        float m    = -INFINITY;
+        float less = INFINITY;  // weights are 2^(score + less)
         float l    = 0.0f;
         int   vexp = 0;  // V's d is times 2^-vexp, and o
 
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
                 }
             }
             const bool all = j0 + keys - 1 <= base && (a.window == 0 || j0 > p1 - a.window || j0 + keys <= a.sinks);
-            float      top = m;
+            float      top = -INFINITY;
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -528,23 +528,24 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
                 }
             }
             top             = max_quarters(top);
-            const float ref = top == -INFINITY ? 0.0f : top;
-            if (__any(top > m)) {
-                const float alpha = __builtin_amdgcn_exp2f(m - ref);
+            const float now = fminf(less, shift_for(top, kPShift));
+            if (__any(now < less)) {
+                const float alpha = shift_change(less, now);
                 l *= alpha;
 #pragma unroll
                 for (int u = 0; u < TILES; ++u) {
                     o[u] *= alpha;
                 }
             }
-            m = top;
+            less            = now;
+            const float add = shift_added(less);
             f16x2 ph[4], pl[4];
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
                 float w[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    w[e] = __builtin_amdgcn_exp2f(sc[mt][e] - (ref - kPShift));
+                    w[e] = __builtin_amdgcn_exp2f(sc[mt][e] + add);
                     l += w[e];
                 }
                 split2(w[0], w[1], ph[2 * mt], pl[2 * mt]);
@@ -605,7 +606,7 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
         }
         l = sum_quarters(l);
 
-        // the waves' results joined in LDS: [wave][value][lane], then m and l of a column
+        // the waves' results joined in LDS: [wave][value][lane], then -less and l of a column
         __syncthreads();
         float * of = reinterpret_cast<float *>(lds);
         float * ml = of + WAVES * TILES * 4 * kWave;
@@ -617,7 +618,7 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
             }
         }
         if (g == 0) {
-            ml[(wave * 16 + c) * 2]     = m;
+            ml[(wave * 16 + c) * 2]     = -less;
             ml[(wave * 16 + c) * 2 + 1] = l;
         }
         __syncthreads();

@@ -583,7 +583,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
     for (int u = 0; u < NB; ++u) {
         o[u] = f32x16{};
     }
-    float m    = -INFINITY;
+    float less = INFINITY;  // weights are 2^(score + less)
     float l    = 0.0f;
     int   vexp = 0;  // blocks: V in LDS is times 2^-vexp, o times 2^-oexp
     int   oexp = 0;
@@ -904,18 +904,17 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
         }
         const Pair  both = swap32(top);
         const float here = fmaxf(both.a, both.b) * qs;
-        top              = fmaxf(m, here);
-        const float ref  = top == -INFINITY ? 0.0f : top;
+        const float now  = fminf(less, shift_for(here, SIZES || THREE ? 0.0f : kPShift));
         int         need = X;
         if constexpr (SIZES) {
             // what this pass's largest weighted row needs, or those before it, whose
             // weights have gone down
-            const int down = static_cast<int>(fminf(floorf(ref - m), 1000.0f));
-            need           = vsize + 1 + static_cast<int>(fmaxf(floorf(here - ref), -1000.0f));
+            const int down = static_cast<int>(fminf(floorf(less - now), 1000.0f));
+            need           = vsize + 1 + static_cast<int>(fmaxf(floorf(here + now), -1000.0f));
             need           = max(max(need, X - down), kMinX);
         }
-        if (__any(top > m || need != X)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        if (__any(now < less || need != X)) {
+            const float alpha = shift_change(less, now);
             const float by    = SIZES ? __builtin_ldexpf(alpha, X - need) : alpha;
             l *= alpha;
 #pragma unroll
@@ -923,12 +922,12 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                 o[u] *= by;
             }
         }
-        m                 = top;
+        less              = now;
         X                 = need;
-        const float less  = (SIZES || THREE ? 0.0f : kPShift) - ref;
+        const float add   = shift_added(less);
         const int   times = vsize + 15 - X;
         auto        held  = [&](float score) {
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score, qs, less));
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score, qs, add));
             l += w;
             return SIZES ? __builtin_ldexpf(w, times) : w;
         };
@@ -1000,7 +999,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
         out = partial_o(a, row, dest);
         if (g == 0) {
             float * ml = partial_ml(a, row, dest);
-            ml[0]      = m;
+            ml[0]      = -less;
             ml[1]      = l;
         }
     }

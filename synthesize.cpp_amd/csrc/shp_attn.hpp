@@ -166,6 +166,25 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kPShift  = 15.0f;  // P times 2^15, at most half of F16's range
 
+// Weights are 2^(score + less), less the least of shift_for() of the scores so far:
+// 2^shift for the largest score. From 2^23 on a score holds no more than whole
+// numbers, and score + shift would be rounded up to a weight past F16's range; there
+// the largest weight is 1 (the others are 1 or next to nothing). What less was
+// rounded to is what all weights of a row have in common; it stands for -max in
+// a partial result.
+__device__ __forceinline__ float shift_for(float top, float shift) {
+    return (fabsf(top) < 0x1p23f ? shift : 0.0f) - top;
+}
+
+// What weights under `less` become under `now`, at most that; nothing seen: infinity.
+__device__ __forceinline__ float shift_change(float less, float now) {
+    return now < less ? __builtin_amdgcn_exp2f(now - less) : 1.0f;
+}
+
+__device__ __forceinline__ float shift_added(float less) {
+    return less == INFINITY ? 0.0f : less;
+}
+
 __device__ __forceinline__ f16x2 as_f16x2(uint32_t v) {
     return __builtin_bit_cast(f16x2, v);
 }

@@ -124,3 +124,28 @@ def test_rows_of_all_sizes(gpu, kind, t, hd):
     run(gpu, kind, q, k, v * up(-30, 30), [200, 131])
     run(gpu, kind, q, k * up(-12, 0), v * up(-30, 30), [200, 131], window=30, sinks=4)
     run(gpu, kind, q, k * up(-12, 3), v * up(-3, 3), [200, 131])
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("t,hd,cap", [(1, 64, 100), (1, 128, 700), (3, 160, 90), (40, 64, 150), (130, 128, 130)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 22, 2.0 ** 24, 3.0 * 2 ** 24, 2.0 ** 26, 2.0 ** 30, 2.0 ** 40])
+def test_scores_past_whole_numbers(gpu, kind, t, hd, cap, sign, size):
+    """Scores so large that f32 holds no units of them: the row of the largest has
+    all the weight. Its score is twice the others' (half, where they are below
+    zero), so that the others' weights are below e^-1000: what is left is that
+    row's own values, off by the weight's and the sum's half steps (8) and, where
+    V is two F16 pieces, by 2^-23 of themselves and 2^-30 of the row's largest."""
+    q, k, v = rand(1, t, 4, 2, hd, cap, 41)
+    k = 1.0 + k.abs().clamp(max=1.0)
+    star = cap - t // 2 - 1
+    k[0, star] = 4.0 if sign > 0 else 0.5
+    q = torch.full(q.shape, sign * size / hd ** 0.5)
+    cache = [R.pack(x, kind) for x in (k, v)]
+    h = [R.handle(gpu, c.cuda(), kind, hd) for c in cache]
+    got = gpu.attn_kv(q.cuda(), h[0], h[1], ints(cap)).cpu()
+    assert torch.isfinite(got).all()
+    want = R.values(cache[1], kind)[0, star].double().repeat_interleave(2, 0)
+    bound = (8 * R.EPS + 2.0 ** -23) * want.abs() + 2.0 ** -30 * want.abs().amax(-1, keepdim=True)
+    for i in range(star - (cap - t), t):
+        assert ((got[0, i].double() - want).abs() <= bound).all(), i
