@@ -35,21 +35,22 @@ constexpr int kVStride   = kTileKeys * 2 + 16;  // bytes of a column of V in LDS
 // `dim` of V the groups stand in the order group ^ (dim >> kTurn & 3): sixteen
 // lanes that write a group of sixteen columns then meet every bank once (four
 // times four without it: a third of the LDS unit's time).
-// The pieces are of the values times 2^-shift, where a tile's blocks are out of
-// F16's range or, F32, always (see by_size): their largest comes to [2^13, 2^14).
+// F32's pieces are of the values times a power of two (see by_size). A block's are
+// of the values themselves, but in a tile where a d is above kBigD, and values may
+// be out of F16's range: there the first piece is 2^-8 of its value, and the second
+// what 2^8 times that leaves, which is exact as well (18 bits are 11 and 7, whatever
+// the sizes: a block of small values beside one of large is as exact as alone).
 //   load_k, load_v  from the cache, through descriptors of the tile
 //   keep_k, keep_v  or zeros in place of K's row, of V's of key e
 //   top_k, top_v    bits that bound the magnitudes, kInf and more where one is
-//                   infinite or NaN; finite_k without those; no scale is needed
-//                   up to kLeave
-//   k_pieces        operand j of the row's four, times `by`
-//   v_column        value U of the eight keys, times `by`
+//                   infinite or NaN; finite_k without those
+//   k_pieces        operand j of the row's four, times `by` (F32), of a large tile
+//   v_column        value U of the eight keys, likewise
 template <int KIND> struct Part;
 
-// Codes and d: exact products; a scale goes to d.
+// Codes and d.
 template <int KIND, int WORDS> struct BlockPart {
-    static constexpr bool kTwo    = true;
-    static constexpr bool kScaled = true;
+    static constexpr bool kTwo = true;
     uint32_t              k[WORDS];
     uint32_t              v[8];
     // (dwords: halves are put into pairs, for which a wave waits as soon as it has
@@ -76,8 +77,7 @@ template <int KIND, int WORDS> struct BlockPart {
 
     __device__ void keep_v(int e, bool yes) { vd[e] = yes ? vd[e] : 0; }
 
-    static constexpr uint32_t kInf   = kInfD;
-    static constexpr uint32_t kLeave = kBigD;
+    static constexpr uint32_t kInf = kInfD;
 
     __device__ uint32_t top_k() const { return kd & 0x7fffu; }
 
@@ -87,12 +87,16 @@ template <int KIND, int WORDS> struct BlockPart {
 
     __device__ static float magnitude(uint32_t bits) { return f16_bits_to_f32(bits); }
 
-    __device__ static void exact(f16x2 code, f16x2 d, f16x2 & hi, f16x2 & lo) {
-        hi = code * d;
-        lo = __builtin_elementwise_fma(code, d, -hi);
+    template <bool LARGE> __device__ static void exact(f16x2 code, f16x2 d, f16x2 & hi, f16x2 & lo) {
+        if constexpr (LARGE) {
+            large_pieces(code, d, hi, lo);
+        } else {
+            hi = code * d;
+            lo = __builtin_elementwise_fma(code, d, -hi);
+        }
     }
 
-    __device__ void k_pieces(const Magic & m, float by, int j, f16x8 & hi, f16x8 & lo) const {
+    template <bool LARGE> __device__ void k_pieces(const Magic & m, float, int j, f16x8 & hi, f16x8 & lo) const {
         constexpr int STEP = WORDS / 4;
         uint32_t      w[STEP];
 #pragma unroll
@@ -100,22 +104,21 @@ template <int KIND, int WORDS> struct BlockPart {
             w[i] = k[STEP * j + i];
         }
         const f16x8 code = Codes<KIND>::k_codes(m, w);
-        const f16x2 d    = as_f16x2(kd * 0x10001u) * splat2(by);
         f16x2       h[4], l[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            exact(f16x2{ code[2 * e], code[2 * e + 1] }, d, h[e], l[e]);
+            exact<LARGE>(f16x2{ code[2 * e], code[2 * e + 1] }, as_f16x2(kd * 0x10001u), h[e], l[e]);
         }
         hi = join8(h[0], h[1], h[2], h[3]);
         lo = join8(l[0], l[1], l[2], l[3]);
     }
 
-    template <int U> __device__ void v_pieces(const Magic & m, float by, int shift, f16x8 & hi, f16x8 & lo) const {
+    template <int U, bool LARGE> __device__ void v_pieces(const Magic & m, int shift, f16x8 & hi, f16x8 & lo) const {
         f16x2 h[4], l[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const f16x2 d = as_f16x2(vd[2 * e] | vd[2 * e + 1] << 16) * splat2(by);
-            exact(Codes<KIND>::template v_codes<U>(m, v[2 * e] >> shift, v[2 * e + 1] >> shift), d, h[e], l[e]);
+            exact<LARGE>(Codes<KIND>::template v_codes<U>(m, v[2 * e] >> shift, v[2 * e + 1] >> shift),
+                         as_f16x2(vd[2 * e] | vd[2 * e + 1] << 16), h[e], l[e]);
         }
         hi = join8(h[0], h[1], h[2], h[3]);
         lo = join8(l[0], l[1], l[2], l[3]);
@@ -137,8 +140,9 @@ template <> struct Part<kKvQ4> : BlockPart<kKvQ4, 4> {
         return 32 * (w >> 2) + 4 * (w & 3) + u + (item >= words ? 16 : 0);
     }
 
-    template <int U> __device__ void v_column(const Magic & m, float by, int item, int words, f16x8 & hi, f16x8 & lo) const {
-        v_pieces<2 * U>(m, by, item >= words ? 4 : 0, hi, lo);
+    template <int U, bool LARGE>
+    __device__ void v_column(const Magic & m, float, int item, int words, f16x8 & hi, f16x8 & lo) const {
+        v_pieces<2 * U, LARGE>(m, item >= words ? 4 : 0, hi, lo);
     }
 };
 
@@ -153,17 +157,15 @@ template <> struct Part<kKvQ8> : BlockPart<kKvQ8, 8> {
 
     __device__ static int index(int item, int, int u) { return 4 * item + u; }
 
-    template <int U> __device__ void v_column(const Magic & m, float by, int, int, f16x8 & hi, f16x8 & lo) const {
-        v_pieces<U>(m, by, 0, hi, lo);
+    template <int U, bool LARGE> __device__ void v_column(const Magic & m, float, int, int, f16x8 & hi, f16x8 & lo) const {
+        v_pieces<U, LARGE>(m, 0, hi, lo);
     }
 };
 
 // Plain values, four next to each other a key of V.
 template <int KIND> struct PlainPart {
     static constexpr bool  kTwo    = KIND == kKvF32;
-    static constexpr bool  kScaled = KIND == kKvF32;
     static constexpr int   kTurn   = 4;
-    static constexpr uint32_t kLeave = 0;
     static constexpr int   kSize   = kv_unit_bytes(KIND);
     static constexpr int   kFour   = kSize;  // dwords of four values
     uint32_t               k[8 * kFour];
@@ -290,7 +292,7 @@ template <int KIND> struct PlainPart {
 
     __device__ static int index(int item, int, int u) { return 4 * item + u; }
 
-    __device__ void k_pieces(const Magic &, float by, int j, f16x8 & hi, f16x8 & lo) const {
+    template <bool> __device__ void k_pieces(const Magic &, float by, int j, f16x8 & hi, f16x8 & lo) const {
         f16x2 h[4], l[4] = {};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -304,7 +306,7 @@ template <int KIND> struct PlainPart {
         lo = join8(l[0], l[1], l[2], l[3]);
     }
 
-    template <int U> __device__ void v_column(const Magic &, float by, int, int, f16x8 & hi, f16x8 & lo) const {
+    template <int U, bool> __device__ void v_column(const Magic &, float by, int, int, f16x8 & hi, f16x8 & lo) const {
         f16x2 h[4], l[4] = {};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -585,21 +587,32 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
     }
     float less = INFINITY;  // weights are 2^(score + less)
     float l    = 0.0f;
-    int   vexp = 0;  // blocks: V in LDS is times 2^-vexp, o times 2^-oexp
-    int   oexp = 0;
     int   X    = kMinX;  // SIZES: o is times 2^(15 + kVTop - X)
 
     constexpr uint64_t kEvery = ~uint64_t{ 0 };
     uint64_t           left   = kEvery;  // SIZES: the tile's keys that no pass has had,
     uint64_t           pass   = kEvery;  // those of this one,
     bool               alike  = false;   // and whether they are known to be of one size
+    bool               again  = false;   // blocks: the second pass over a large tile, of V's second pieces
 
     for (int i = beg; i < end;) {
         const int32_t j0 = key_tile(kt, i) * kTileKeys;
-        float kby = 1.0f, vby = 1.0f;
+        float    kby = 1.0f, vby = 1.0f;
         int      kexp   = 0;
+        bool     large  = false;   // blocks: a d is
+        const bool second = again;
         int      vsize  = 0;       // SIZES: the exponent of V's largest
         const uint64_t member = pass;
+        // go(whether the tile is large): what that changes is apart, so that the others' code is as without it
+        auto if_large = [&](const auto & go) {
+            if constexpr (kv_blocks(KIND)) {
+                if (large) {
+                    go(std::true_type{});
+                    return;
+                }
+            }
+            go(std::false_type{});
+        };
         bool     ready  = true;
         const bool edge = j0 + kTileKeys - 1 > p0 || (a.window > 0 && j0 <= p1 - a.window && j0 + kTileKeys > a.sinks);
 #pragma unroll
@@ -686,16 +699,11 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                 if (lane < 3) {
                     tops[lane * kWaves + wave] = lane == 0 ? fk : lane == 1 ? fv : none;
                 }
-            } else if (PartT::kScaled && __any(max(tk, tv) > PartT::kLeave)) {  // (hardly ever)
-                const float fk = wave_max(PartT::magnitude(tk));
-                const float fv = wave_max(PartT::magnitude(tv));
+            } else if constexpr (kv_blocks(KIND)) {
+                const float is = __any(max(tk, tv) > kBigD) ? 1.0f : 0.0f;
                 if (lane == 0) {
-                    tops[wave]         = fk;
-                    tops[kWaves + wave] = fv;
+                    tops[wave] = is;
                 }
-            } else if (lane == 0) {
-                tops[wave]         = 0.0f;
-                tops[kWaves + wave] = 0.0f;
             }
             if (lane == 0) {
                 bads[wave] = bad;
@@ -757,53 +765,57 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
             vsize = __builtin_amdgcn_readfirstlane(exponent_of(vt));
             kby   = pow2(-kexp);
             vby   = pow2(kVTop - vsize);
-        } else if constexpr (PartT::kScaled) {
-            auto most = [&](int at) {
-                const f32x4 t = *reinterpret_cast<const f32x4 *>(tops + at);
-                return __builtin_amdgcn_readfirstlane(shift_of_d(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]))));
-            };
-            // K by tile; V never less than for the tiles before, which o holds
-            kexp = most(0);
-            vexp = max(vexp, most(4));
-            kby  = pow2(-kexp);
-            vby  = pow2(-vexp);
+        } else if constexpr (kv_blocks(KIND)) {
+            const f32x4 t = *reinterpret_cast<const f32x4 *>(tops);
+            large         = __builtin_amdgcn_readfirstlane(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) != 0.0f);
         }
-        const int staged = tid_each();
+        auto stage = [&](auto larger) {
+            constexpr bool LARGE  = decltype(larger)::value;
+            const int      staged = tid_each();
 #pragma unroll
-        for (int z = 0; z < PARTS; ++z) {
-            if (mine[z]) {
-                const int id   = staged + kWideBlock * z;
-                const int item = id % items;
+            for (int z = 0; z < PARTS; ++z) {
+                if (mine[z]) {
+                    const int id   = staged + kWideBlock * z;
+                    const int item = id % items;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    f16x8 hi, lo;
-                    part[z].k_pieces(magic, kby, j, hi, lo);
-                    const int at = id / NB * KSTRIDE + id % NB * 64 + 16 * j;
-                    *reinterpret_cast<f16x8 *>(kh + at) = hi;
-                    if constexpr (TWO) {
-                        *reinterpret_cast<f16x8 *>(kl + at) = lo;
+                    for (int j = 0; j < 4; ++j) {
+                        f16x8 hi, lo;
+                        part[z].template k_pieces<LARGE>(magic, kby, j, hi, lo);
+                        const int at = id / NB * KSTRIDE + id % NB * 64 + 16 * j;
+                        *reinterpret_cast<f16x8 *>(kh + at) = hi;
+                        if constexpr (TWO) {
+                            *reinterpret_cast<f16x8 *>(kl + at) = lo;
+                        }
                     }
+                    auto column = [&](auto uc) {
+                        constexpr int U = decltype(uc)::value;
+                        f16x8         hi, lo;
+                        part[z].template v_column<U, LARGE>(magic, vby, item, words, hi, lo);
+                        if constexpr (LARGE) {
+                            hi = second ? lo : hi;
+                            lo = f16x8{};
+                        }
+                        const int dim = PartT::index(item, words, U);
+                        const int at  = dim * kVStride + (id / items ^ (dim >> PartT::kTurn & 3)) * 16;
+                        *reinterpret_cast<f16x8 *>(vh + at) = hi;
+                        if constexpr (TWO) {
+                            *reinterpret_cast<f16x8 *>(vl + at) = lo;
+                        }
+                    };
+                    for_each(std::make_integer_sequence<int, 4>{}, column);
                 }
-                auto column = [&](auto uc) {
-                    constexpr int U = decltype(uc)::value;
-                    f16x8         hi, lo;
-                    part[z].template v_column<U>(magic, vby, item, words, hi, lo);
-                    const int dim = PartT::index(item, words, U);
-                    const int at  = dim * kVStride + (id / items ^ (dim >> PartT::kTurn & 3)) * 16;
-                    *reinterpret_cast<f16x8 *>(vh + at) = hi;
-                    if constexpr (TWO) {
-                        *reinterpret_cast<f16x8 *>(vl + at) = lo;
-                    }
-                };
-                for_each(std::make_integer_sequence<int, 4>{}, column);
             }
-        }
+        };
+        if_large(stage);
         if constexpr (SIZES) {
             const uint64_t rest = ready ? left & ~pass : left;
             i += rest == 0;
             left  = rest == 0 ? kEvery : rest;
             pass  = ready ? left : pass;
             alike = !ready;
+        } else if constexpr (kv_blocks(KIND)) {
+            again = large && !second;
+            i += !again;
         } else {
             ++i;
         }
@@ -821,53 +833,63 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                 }
             }
         }
-        if (kv_blocks(KIND) && vexp != oexp) {
-            const float by = pow2(max(oexp - vexp, -126));
-#pragma unroll
-            for (int u = 0; u < NB; ++u) {
-                o[u] *= by;
-            }
-            oexp = vexp;
-        }
-
         // scores of key 32 x + 8 (i / 4) + 4 g + i % 4
         // (ahead of the waves that are at their exponentials: 8192 positions 860
         // to 790 us)
         __builtin_amdgcn_s_setprio(1);
         f32x16 sc[2] = { f32x16{}, f32x16{} };
+        auto keys_at = [&](const char * from, int x, int s) {
+            return *reinterpret_cast<const f16x8 *>(from + (32 * x + c) * KSTRIDE + 32 * s + 16 * g);
+        };
+        auto score = [&](auto larger) {
+            constexpr bool LARGE = decltype(larger)::value;
 #pragma unroll
-        for (int s = 0; s < 2 * NB; ++s) {
-            f16x8 hi[2], lo[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int at = (32 * x + c) * KSTRIDE + 32 * s + 16 * g;
-                hi[x]        = *reinterpret_cast<const f16x8 *>(kh + at);
-                if constexpr (TWO) {
-                    lo[x] = *reinterpret_cast<const f16x8 *>(kl + at);
-                }
-            }
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                sc[x] = product<KIND>(hi[x], qh[s], sc[x]);
-            }
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                sc[x] = product<KIND>(hi[x], ql[s], sc[x]);
-            }
-            if constexpr (THREE) {
-                const f16x8 third = q3[s * kWideBlock];
+            for (int s = 0; s < 2 * NB; ++s) {
+                f16x8 hi[2], lo[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    sc[x] = product<KIND>(hi[x], third, sc[x]);
+                    hi[x] = keys_at(kh, x, s);
+                    if constexpr (TWO && !LARGE) {
+                        lo[x] = keys_at(kl, x, s);
+                    }
                 }
-            }
-            if constexpr (TWO) {
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    sc[x] = product<KIND>(lo[x], qh[s], sc[x]);
+                    sc[x] = product<KIND>(hi[x], qh[s], sc[x]);
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    sc[x] = product<KIND>(hi[x], ql[s], sc[x]);
+                }
+                if constexpr (THREE) {
+                    const f16x8 third = q3[s * kWideBlock];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        sc[x] = product<KIND>(hi[x], third, sc[x]);
+                    }
+                }
+                if constexpr (TWO && !LARGE) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        sc[x] = product<KIND>(lo[x], qh[s], sc[x]);
+                    }
                 }
             }
-        }
+            if constexpr (LARGE) {
+                sc[0] *= kLargeBy;
+                sc[1] *= kLargeBy;
+#pragma unroll
+                for (int s = 0; s < 2 * NB; ++s) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const f16x8 lo = keys_at(kl, x, s);
+                        sc[x]          = product<KIND>(lo, qh[s], sc[x]);
+                        sc[x]          = product<KIND>(lo, ql[s], sc[x]);
+                    }
+                }
+            }
+        };
+        if_large(score);
         __builtin_amdgcn_s_setprio(0);
         // (within what is a normal number: a zero query's and zero keys' exponents
         // add up to -226, and 0 times a hidden key's -infinity is NaN)
@@ -913,14 +935,17 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
             need           = vsize + 1 + static_cast<int>(fmaxf(floorf(here + now), -1000.0f));
             need           = max(max(need, X - down), kMinX);
         }
-        if (__any(now < less || need != X)) {
-            const float alpha = shift_change(less, now);
-            const float by    = SIZES ? __builtin_ldexpf(alpha, X - need) : alpha;
-            l *= alpha;
+        auto turn = [&](float by) {
 #pragma unroll
             for (int u = 0; u < NB; ++u) {
                 o[u] *= by;
             }
+        };
+        if (__any(now < less || need != X)) {
+            const float alpha = shift_change(less, now);
+            const float by    = SIZES ? __builtin_ldexpf(alpha, X - need) : alpha;
+            l *= alpha;
+            turn(by);
         }
         less              = now;
         X                 = need;
@@ -931,56 +956,72 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
             l += w;
             return SIZES ? __builtin_ldexpf(w, times) : w;
         };
-        const int from = tid_each() % kWave;
+        // a large tile: V's first pieces, 2^-8 of their values, in the first pass, what
+        // they leave in the second, which has been counted in l already
+        if (kv_blocks(KIND) && large && !second) {
+            turn(1.0f / kLargeBy);
+        }
+        const float before = l;
+        auto        weigh  = [&] {
+            const int from = tid_each() % kWave;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+            for (int x = 0; x < 2; ++x) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                f16x2 hi[4], lo[4], third[4];
+                for (int s = 0; s < 2; ++s) {
+                    f16x2 hi[4], lo[4], third[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float a0 = held(sc[x][8 * s + 2 * e]);
-                    float a1 = held(sc[x][8 * s + 2 * e + 1]);
-                    if constexpr (THREE) {
-                        hi[e]    = take_b16(a0, a1);
-                        lo[e]    = take_b16(a0, a1);
-                        third[e] = take_b16(a0, a1);
-                    } else {
-                        split2(a0, a1, hi[e], lo[e]);
+                    for (int e = 0; e < 4; ++e) {
+                        float a0 = held(sc[x][8 * s + 2 * e]);
+                        float a1 = held(sc[x][8 * s + 2 * e + 1]);
+                        if constexpr (THREE) {
+                            hi[e]    = take_b16(a0, a1);
+                            lo[e]    = take_b16(a0, a1);
+                            third[e] = take_b16(a0, a1);
+                        } else {
+                            split2(a0, a1, hi[e], lo[e]);
+                        }
                     }
-                }
-                const f16x8 ph = join8(hi[0], hi[1], hi[2], hi[3]);
-                const f16x8 pl = join8(lo[0], lo[1], lo[2], lo[3]);
-                f16x8 vv[NB];
-#pragma unroll
-                for (int u = 0; u < NB; ++u) {
-                    vv[u] = *reinterpret_cast<const f16x8 *>(vh + vat(from, u, 4 * x + 2 * s));
-                }
-#pragma unroll
-                for (int u = 0; u < NB; ++u) {
-                    o[u] = product<KIND>(vv[u], ph, o[u]);
-                }
-#pragma unroll
-                for (int u = 0; u < NB; ++u) {
-                    o[u] = product<KIND>(vv[u], pl, o[u]);
-                }
-                if constexpr (THREE) {
-                    const f16x8 p3 = join8(third[0], third[1], third[2], third[3]);
+                    const f16x8 ph = join8(hi[0], hi[1], hi[2], hi[3]);
+                    const f16x8 pl = join8(lo[0], lo[1], lo[2], lo[3]);
+                    f16x8 vv[NB];
 #pragma unroll
                     for (int u = 0; u < NB; ++u) {
-                        o[u] = product<KIND>(vv[u], p3, o[u]);
-                    }
-                }
-                if constexpr (TWO) {
-#pragma unroll
-                    for (int u = 0; u < NB; ++u) {
-                        vv[u] = *reinterpret_cast<const f16x8 *>(vl + vat(from, u, 4 * x + 2 * s));
+                        vv[u] = *reinterpret_cast<const f16x8 *>(vh + vat(from, u, 4 * x + 2 * s));
                     }
 #pragma unroll
                     for (int u = 0; u < NB; ++u) {
                         o[u] = product<KIND>(vv[u], ph, o[u]);
                     }
+#pragma unroll
+                    for (int u = 0; u < NB; ++u) {
+                        o[u] = product<KIND>(vv[u], pl, o[u]);
+                    }
+                    if constexpr (THREE) {
+                        const f16x8 p3 = join8(third[0], third[1], third[2], third[3]);
+#pragma unroll
+                        for (int u = 0; u < NB; ++u) {
+                            o[u] = product<KIND>(vv[u], p3, o[u]);
+                        }
+                    }
+                    if constexpr (TWO) {
+#pragma unroll
+                        for (int u = 0; u < NB; ++u) {
+                            vv[u] = *reinterpret_cast<const f16x8 *>(vl + vat(from, u, 4 * x + 2 * s));
+                        }
+#pragma unroll
+                        for (int u = 0; u < NB; ++u) {
+                            o[u] = product<KIND>(vv[u], ph, o[u]);
+                        }
+                    }
                 }
+            }
+        };
+        weigh();
+        if (kv_blocks(KIND) && large) {
+            if (second) {
+                l = before;
+            } else {
+                turn(kLargeBy);
             }
         }
     }
@@ -991,7 +1032,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
     }
     const int64_t row = ((static_cast<int64_t>(n) * a.KV + h) * a.T + t) * a.G + gq;
     float *       out;
-    float         by = SIZES ? 1.0f : pow2(oexp);
+    float         by = 1.0f;
     if (dest < 0) {
         out = reinterpret_cast<float *>(a.y + n * a.yn + t * a.yt + head * a.yh);
         by *= over(l, p >= 0);

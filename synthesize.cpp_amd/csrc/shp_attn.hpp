@@ -214,11 +214,22 @@ __device__ __forceinline__ int exponent_of(float top) {
     return min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 127);
 }
 
-// A block's code * d, |code| <= 128, is within F16's range for d up to 256;
-// where a larger one is about, d is divided by 2^shift, which brings it below
-// 2^6 (what that takes from the small ones is below 2^-24 of the large).
-constexpr uint32_t kBigD = 0x5c00;
-constexpr uint32_t kInfD = 0x7c00;
+// A block's code * d, |code| <= 128, is within F16's range for d up to 256. Beside
+// a larger one its values are v = 2^8 hi + lo: hi is 2^-8 v rounded, 2^15 at most,
+// and lo the rest, exact: v has 18 bits and whole multiples of 2^-24, of which hi
+// takes 11, or those down to 2^-16.
+constexpr uint32_t kBigD    = 0x5c00;
+constexpr uint32_t kInfD    = 0x7c00;
+constexpr float    kLargeBy = 256.0f;
+
+__device__ __forceinline__ void large_pieces(f16x2 code, f16x2 d, f16x2 & hi, f16x2 & lo) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float v = static_cast<float>(code[i]) * static_cast<float>(d[i]);
+        hi[i]         = static_cast<_Float16>(v * (1.0f / kLargeBy));
+        lo[i]         = static_cast<_Float16>(v - static_cast<float>(hi[i]) * kLargeBy);
+    }
+}
 
 __device__ __forceinline__ int shift_of_d(float top) {
     return top > 256.0f ? exponent_of(top) - 5 : 0;

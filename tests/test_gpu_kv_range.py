@@ -50,11 +50,15 @@ def test_queries_and_keys_of_zero_and_next_to_it(gpu, kind, t, hd, cap, small):
     run(gpu, kind, q * small, k * small, v * small, [cap, (cap + 1) // 2], window=30, sinks=2)
 
 
-LARGE = {"f32": 1e12, "bf16": 1e12, "f16": 1e4}
+def cases(*shapes, kinds=R.TYPES):
+    """Shapes (t first) for all types, blocks' prompts alone."""
+    return [(k, *x) for k in kinds for x in shapes if k in R.FLOAT or x[0] >= 40]
 
 
-@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("t,hd,cap", [(40, 64, 200), (130, 128, 130), (3, 128, 300), (5, 160, 90), (64, 32, 64)])
+LARGE = {"f32": 1e12, "bf16": 1e12, "f16": 1e4, "q8_0": 1.5e6, "q4_0": 1e5}  # (finite as the cache holds them: d up to 53000)
+
+
+@pytest.mark.parametrize("kind,t,hd,cap", cases((40, 64, 200), (130, 128, 130), (3, 128, 300), (5, 160, 90), (64, 32, 64)))
 @pytest.mark.parametrize("window", [0, 20])
 def test_a_large_key_does_not_touch_the_queries_that_do_not_see_it(gpu, kind, t, hd, cap, window):
     """Ahead of the first queries and, with the window, behind the last."""
@@ -65,8 +69,7 @@ def test_a_large_key_does_not_touch_the_queries_that_do_not_see_it(gpu, kind, t,
         run(gpu, kind, q, x, v, [cap], window=window, sinks=1)
 
 
-@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("t,hd,cap", [(1, 64, 100), (1, 128, 700), (40, 64, 200), (130, 128, 130), (5, 160, 90)])
+@pytest.mark.parametrize("kind,t,hd,cap", cases((1, 64, 100), (1, 128, 700), (40, 64, 200), (130, 128, 130), (5, 160, 90)))
 def test_a_large_key_of_no_weight(gpu, kind, t, hd, cap):
     """Its scores are far below the others'; it moves no other row's weight."""
     q, k, v = rand(1, t, 4, 2, hd, cap, 34)
@@ -77,8 +80,7 @@ def test_a_large_key_of_no_weight(gpu, kind, t, hd, cap):
         run(gpu, kind, q, x, v, [cap])
 
 
-@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("t,hd,cap", [(40, 64, 200), (130, 128, 130), (3, 128, 300), (5, 160, 90), (300, 32, 300)])
+@pytest.mark.parametrize("kind,t,hd,cap", cases((40, 64, 200), (130, 128, 130), (3, 128, 300), (5, 160, 90), (300, 32, 300)))
 @pytest.mark.parametrize("window", [0, 20])
 def test_a_large_value_does_not_touch_the_queries_that_do_not_see_it(gpu, kind, t, hd, cap, window):
     q, k, v = rand(1, t, 4, 2, hd, cap, 35)
@@ -88,8 +90,7 @@ def test_a_large_value_does_not_touch_the_queries_that_do_not_see_it(gpu, kind, 
         run(gpu, kind, q, k, x, [cap], window=window, sinks=1)
 
 
-@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("t,hd,cap", [(1, 64, 100), (1, 128, 700), (40, 64, 200), (130, 128, 130), (5, 160, 90)])
+@pytest.mark.parametrize("kind,t,hd,cap", cases((1, 64, 100), (1, 128, 700), (40, 64, 200), (130, 128, 130), (5, 160, 90)))
 def test_a_large_value_of_no_weight(gpu, kind, t, hd, cap):
     q, k, v = rand(1, t, 4, 2, hd, cap, 36)
     q = q.abs() + 0.5
@@ -100,8 +101,7 @@ def test_a_large_value_of_no_weight(gpu, kind, t, hd, cap):
         run(gpu, kind, q, x, z, [cap])
 
 
-@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("t,kv,g,hd", [(1, 8, 2, 128), (1, 8, 1, 64), (2, 4, 2, 64), (40, 4, 2, 64)])
+@pytest.mark.parametrize("kind,t,kv,g,hd", cases((1, 8, 2, 128), (1, 8, 1, 64), (2, 4, 2, 64), (40, 4, 2, 64)))
 def test_heads_of_different_sizes(gpu, kind, t, kv, g, hd):
     """A head whose values are large beside heads of ordinary and small ones."""
     q, k, v = rand(2, t, kv * g, kv, hd, 150, 37)
@@ -114,8 +114,21 @@ def test_heads_of_different_sizes(gpu, kind, t, kv, g, hd):
     run(gpu, kind, q, k, v, [150, 90])
 
 
-@pytest.mark.parametrize("kind", ["f32", "bf16"])
-@pytest.mark.parametrize("t,hd", [(1, 64), (40, 64), (130, 128), (7, 200)])
+@pytest.mark.parametrize("kind,t,hd", cases((1, 128), (1, 64), (3, 160), (40, 128), (40, 64), kinds=["q8_0", "q4_0"]))
+def test_blocks_of_different_sizes(gpu, kind, t, hd):
+    """One block of a row large, the next one small: both exact."""
+    q, k, v = rand(1, t, 4, 2, hd, 150, 38)
+    v[..., :32] *= LARGE[kind] / 10
+    v[..., 32:64] *= 0.05
+    v[:, 60:90] *= 1e-3
+    run(gpu, kind, q, k, v, [150])
+    q[..., :32] *= 1e-6
+    k[..., :32] *= LARGE[kind] / 10
+    k[..., 32:64] *= 0.05
+    run(gpu, kind, q, k, v, [150])
+
+
+@pytest.mark.parametrize("kind,t,hd", cases((1, 64), (40, 64), (130, 128), (7, 200), kinds=["f32", "bf16"]))
 def test_rows_of_all_sizes(gpu, kind, t, hd):
     """Rows of V from 1e-30 to 1e30 and of K from 1e-12 to 1e3, in any order."""
     q, k, v = rand(2, t, 4, 2, hd, 200, 39)
