@@ -322,7 +322,6 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
         }
         float less = INFINITY;  // weights are 2^(score + less)
         float l    = 0.0f;
-        int   vexp = 0;  // V's d is times 2^-vexp, and o
 
         // the chunks of these units, one a wave
         const int end = min(kt.n, u1 * f.per);
@@ -407,6 +406,7 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
             __builtin_amdgcn_wave_barrier();
             // d of the 32 rows: K's as F32, V's as they are; a V row that no query
             // of the call sees has d = 0
+            bool large;
             {
                 const int    row  = lane & 31;
                 const bool   isk  = lane < 32;
@@ -437,24 +437,26 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
                         }
                     }
                 }
-                if (__any(!isk && most > kBigD)) {  // V's code * d may be out of F16's range: 2^vexp out of it
-                    const int shift = shift_of_d(wave_max(isk ? 0.0f : f16_bits_to_f32(most)));
-                    if (shift > vexp) {
-#pragma unroll
-                        for (int u = 0; u < TILES; ++u) {
-                            o[u] *= pow2(vexp - shift);
-                        }
-                        vexp = shift;
-                    }
-                }
-                const _Float16 by = static_cast<_Float16>(pow2(-vexp));
+                large = __any(!isk && most > kBigD);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     if (b < nb) {
                         if (isk) {
                             kd[b * kChunk + row] = f16_bits_to_f32(d[b]);
                         } else {
-                            vd[b * kChunk + row] = __builtin_bit_cast(_Float16, d[b]) * by;
+                            vd[b * kChunk + row] = __builtin_bit_cast(_Float16, d[b]);
+                        }
+                    }
+                }
+                if (large && !isk) {
+                    // d = 2^8 first + rest, both exact and values of either within F16's range
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        if (b < nb) {
+                            const float    v     = f16_bits_to_f32(d[b]);
+                            const _Float16 first = static_cast<_Float16>(v * (1.0f / kLargeBy));
+                            vd[(NB + b) * kChunk + row] = first;
+                            vd[b * kChunk + row]        = static_cast<_Float16>(v - static_cast<float>(first) * kLargeBy);
                         }
                     }
                 }
@@ -555,54 +557,68 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
             const f16x8 bl = join8(pl[0], pl[1], pl[2], pl[3]);
 
             // operand element e of quarter g is row 4 g + e, then 16 + 4 g + e - 4
+            auto turn = [&](float by) {
 #pragma unroll
-            for (int s = 0; s < SLOTS; ++s) {
-                uint32_t w[8];
-                f16x2    d[4];
-                const f16x4 d0 = *reinterpret_cast<const f16x4 *>(vd + vblock[s] * kChunk + 4 * g);
-                const f16x4 d1 = *reinterpret_cast<const f16x4 *>(vd + vblock[s] * kChunk + 16 + 4 * g);
-                d[0] = f16x2{ d0[0], d0[1] }, d[1] = f16x2{ d0[2], d0[3] };
-                d[2] = f16x2{ d1[0], d1[1] }, d[3] = f16x2{ d1[2], d1[3] };
-                const LdsWords v0(vl, vword[s]);
-                const LdsWords v1(vl, vword[s] + 2);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int off = ((e < 4 ? 0 : 12) + e) * rb;
-                    w[e]          = nb % 2 == 0 || e % 2 == 0 ? v0.at(off) : v1.at(off - 2);
+                for (int u = 0; u < TILES; ++u) {
+                    o[u] *= by;
                 }
-                // kAtOnce tiles at a time, so that their products need not wait for each other
-                auto tiles = [&](auto uc) {
-                    constexpr int U = kAtOnce * decltype(uc)::value;
-                    f16x8         ah[kAtOnce], al[kAtOnce];
-                    auto          pieces = [&](auto vc) {
-                        constexpr int V = decltype(vc)::value;
-                        f16x2         hi[4], lo[4];
+            };
+            auto products = [&](const _Float16 * ds) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const f16x2 code = C::template v_codes<U + V>(magic, w[2 * e], w[2 * e + 1]);
-                            hi[e]            = code * d[e];
-                            lo[e]            = __builtin_elementwise_fma(code, d[e], -hi[e]);
+                for (int s = 0; s < SLOTS; ++s) {
+                    uint32_t w[8];
+                    f16x2    d[4];
+                    const f16x4 d0 = *reinterpret_cast<const f16x4 *>(ds + vblock[s] * kChunk + 4 * g);
+                    const f16x4 d1 = *reinterpret_cast<const f16x4 *>(ds + vblock[s] * kChunk + 16 + 4 * g);
+                    d[0] = f16x2{ d0[0], d0[1] }, d[1] = f16x2{ d0[2], d0[3] };
+                    d[2] = f16x2{ d1[0], d1[1] }, d[3] = f16x2{ d1[2], d1[3] };
+                    const LdsWords v0(vl, vword[s]);
+                    const LdsWords v1(vl, vword[s] + 2);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int off = ((e < 4 ? 0 : 12) + e) * rb;
+                        w[e]          = nb % 2 == 0 || e % 2 == 0 ? v0.at(off) : v1.at(off - 2);
+                    }
+                    // kAtOnce tiles at a time, so that their products need not wait for each other
+                    auto tiles = [&](auto uc) {
+                        constexpr int U = kAtOnce * decltype(uc)::value;
+                        f16x8         ah[kAtOnce], al[kAtOnce];
+                        auto          pieces = [&](auto vc) {
+                            constexpr int V = decltype(vc)::value;
+                            f16x2         hi[4], lo[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const f16x2 code = C::template v_codes<U + V>(magic, w[2 * e], w[2 * e + 1]);
+                                hi[e]            = code * d[e];
+                                lo[e]            = __builtin_elementwise_fma(code, d[e], -hi[e]);
+                            }
+                            ah[V] = join8(hi[0], hi[1], hi[2], hi[3]);
+                            al[V] = join8(lo[0], lo[1], lo[2], lo[3]);
+                        };
+                        for_each(std::make_integer_sequence<int, kAtOnce>{}, pieces);
+                        f32x4 * x = o + s * C::kTiles + U;
+#pragma unroll
+                        for (int v = 0; v < kAtOnce; ++v) {
+                            x[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[v], bh, x[v], 0, 0, 0);
                         }
-                        ah[V] = join8(hi[0], hi[1], hi[2], hi[3]);
-                        al[V] = join8(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+                        for (int v = 0; v < kAtOnce; ++v) {
+                            x[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[v], bl, x[v], 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int v = 0; v < kAtOnce; ++v) {
+                            x[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[v], bh, x[v], 0, 0, 0);
+                        }
                     };
-                    for_each(std::make_integer_sequence<int, kAtOnce>{}, pieces);
-                    f32x4 * x = o + s * C::kTiles + U;
-#pragma unroll
-                    for (int v = 0; v < kAtOnce; ++v) {
-                        x[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[v], bh, x[v], 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int v = 0; v < kAtOnce; ++v) {
-                        x[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[v], bl, x[v], 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int v = 0; v < kAtOnce; ++v) {
-                        x[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[v], bh, x[v], 0, 0, 0);
-                    }
-                };
-                for_each(std::make_integer_sequence<int, C::kTiles / kAtOnce>{}, tiles);
+                    for_each(std::make_integer_sequence<int, C::kTiles / kAtOnce>{}, tiles);
+                }
+            };
+            if (large) {
+                turn(1.0f / kLargeBy);
+                products(vd + NB * kChunk);
+                turn(kLargeBy);
             }
+            products(vd);
         }
         l = sum_quarters(l);
 
@@ -614,7 +630,7 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
         for (int u = 0; u < TILES; ++u) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                of[((wave * TILES + u) * 4 + e) * kWave + lane] = o[u][e] * pow2(vexp);
+                of[((wave * TILES + u) * 4 + e) * kWave + lane] = o[u][e];
             }
         }
         if (g == 0) {
@@ -721,7 +737,7 @@ template <int KIND, int NB, int BYTES, bool RUNS, int WAVES> shp_status_t launch
     using C             = Codes<KIND>;
     constexpr int TILES = (NB * C::kWords + 15) / 16 * C::kTiles;
     const int     rb    = f.nb * kv_unit_bytes(KIND);
-    f.wave_lds          = 2 * kChunk * rb + NB * kChunk * 6;
+    f.wave_lds          = 2 * kChunk * rb + NB * kChunk * 8;
     const int join      = WAVES * (TILES * 4 * kWave + 32) * 4;
     const int stage     = few_shared(NB, WAVES) + f.wave_lds * WAVES;
     const int lds       = stage > join ? stage : join;

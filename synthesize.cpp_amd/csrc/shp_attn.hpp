@@ -231,10 +231,6 @@ __device__ __forceinline__ void large_pieces(f16x2 code, f16x2 d, f16x2 & hi, f1
     }
 }
 
-__device__ __forceinline__ int shift_of_d(float top) {
-    return top > 256.0f ? exponent_of(top) - 5 : 0;
-}
-
 // Exponents that turn an integer in a mantissa's low bits into an F16. Held in
 // vector registers once a kernel, behind the compiler's back: (w & mask) | bits
 // is then one v_and_or_b32, which takes at most one scalar or literal operand.
