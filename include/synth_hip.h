@@ -756,8 +756,10 @@ shp_status_t shp_kv_load(const shp_tensor * k_cache,
  * j < sinks):
  *   y = sum_j softmax_j(scale * q.k_j) v_j over the rows it sees; 0 where p < 0.
  * Queries t >= count[n] are left as they were. A row that a query does not see
- * has no part in its result, whatever it holds; an infinity or NaN in a row of V
- * that it sees (or in its q, or through K in its scores) makes the result NaN.
+ * has no part in its result, whatever it holds; an infinity or NaN in a row of K
+ * or V that it sees, of its kv head, or in its q makes the result NaN, whatever
+ * the score would be (a block whose d is an infinity or NaN counts as such: d is
+ * infinite where kv_store met a value of 65520 times 127 in Q8_0, or 8 in Q4_0).
  * head_dim 1..256; y and work overlap nothing else of the call. Products are
  * formed to f32's precision and summed in f32; a weight is held to 2^-40 of the
  * row's largest. SHP_ERR_UNSUPPORTED past 2^28 query rows or 2^30 cache rows a

@@ -48,12 +48,15 @@ template <int KIND, int HD> __global__ __launch_bounds__(64) void k_attn_any(con
     const int     head  = h * a.G + gq;
     const int     steps = (a.hd + 3) / 4;
 
+    // An infinity in q or in a row of K is NaN to every query that sees the row,
+    // also where its score would be -infinity.
+    auto          or_nan = [](float x) { return fabsf(x) < INFINITY ? x : NAN; };
     float         qf[HD / 4];
     const float * qr = reinterpret_cast<const float *>(a.q + n * a.qn + t * a.qt + head * a.qh);
 #pragma unroll
     for (int s = 0; s < HD / 4; ++s) {
         const int dim = 4 * s + g;
-        qf[s]         = live && dim < a.hd ? qr[dim] * a.scale : 0.0f;
+        qf[s]         = live && dim < a.hd ? or_nan(qr[dim]) * a.scale : 0.0f;
     }
     f32x4 o[HD / 16];
 #pragma unroll
@@ -77,7 +80,7 @@ template <int KIND, int HD> __global__ __launch_bounds__(64) void k_attn_any(con
         for (int s = 0; s < HD / 4; ++s) {
             if (s < steps) {
                 const int   dim = 4 * s + g;
-                const float kv  = has && dim < a.hd ? kv_value<KIND>(kr, dim) : 0.0f;
+                const float kv  = has && dim < a.hd ? or_nan(kv_value<KIND>(kr, dim)) : 0.0f;
                 acc             = __builtin_amdgcn_mfma_f32_16x16x4f32(kv, qf[s], acc, 0, 0, 0);
             }
         }

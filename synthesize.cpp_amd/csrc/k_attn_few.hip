@@ -404,14 +404,14 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            // d of the 32 rows: K's as F32, V's as they are; a V row that no query
-            // of the call sees has d = 0
+            // d of the 32 rows: K's as F32, V's as they are; a row that no query of
+            // the call sees has d = 0
             bool large;
             {
                 const int    row  = lane & 31;
                 const bool   isk  = lane < 32;
                 const char * from = (isk ? kl : vl) + row * rb;
-                const bool   keep = isk || seen_by(a, base, p1, j0 + (row >> f.hgs));
+                const bool   keep = seen_by(a, base, p1, j0 + (row >> f.hgs));
                 uint16_t     d[NB];
                 uint32_t     most = 0;
 #pragma unroll
@@ -419,10 +419,11 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
                     d[b] = b < nb && keep ? *reinterpret_cast<const uint16_t *>(from + b * UNIT) : 0;
                     most = max(most, d[b] & 0x7fffu);
                 }
-                // a row of V that holds an infinity or NaN counts for nothing in the products ...
-                if (__any(!isk && most >= kInfD)) {
-                    uint32_t bad = static_cast<uint32_t>(__ballot(!isk && most >= kInfD) >> 32);
-                    if (!isk && most >= kInfD) {
+                // a row of K or V that holds an infinity or NaN counts for nothing in the products ...
+                const uint64_t not_finite = __ballot(most >= kInfD);
+                if (not_finite != 0) {
+                    uint32_t bad = static_cast<uint32_t>(not_finite | not_finite >> 32);
+                    if (most >= kInfD) {
                         most = 0;
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
@@ -507,7 +508,7 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
             for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    // (a NaN of its own head becomes +infinity, and the weights NaN)
+                    // (a NaN, of a query that is not finite, becomes +infinity, and the weights NaN)
                     sc[mt][e] = fminf(sc[mt][e] * qscale, own[e]);
                 }
             }

@@ -43,7 +43,7 @@ constexpr int kVStride   = kTileKeys * 2 + 16;  // bytes of a column of V in LDS
 //   load_k, load_v  from the cache, through descriptors of the tile
 //   keep_k, keep_v  or zeros in place of K's row, of V's of key e
 //   top_k, top_v    bits that bound the magnitudes, kInf and more where one is
-//                   infinite or NaN; finite_k without those
+//                   infinite or NaN
 //   k_pieces        operand j of the row's four, times `by` (F32), of a large tile
 //   v_column        value U of the eight keys, likewise
 template <int KIND> struct Part;
@@ -82,8 +82,6 @@ template <int KIND, int WORDS> struct BlockPart {
     __device__ uint32_t top_k() const { return kd & 0x7fffu; }
 
     __device__ uint32_t top_v(int e) const { return vd[e] & 0x7fffu; }
-
-    __device__ uint32_t finite_k() const { return 0; }
 
     __device__ static float magnitude(uint32_t bits) { return f16_bits_to_f32(bits); }
 
@@ -254,23 +252,6 @@ template <int KIND> struct PlainPart {
         return m;
     }
 
-    // ... of K's finite ones: an infinity or NaN is its own row's alone
-    __device__ uint32_t finite_k() const {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 8 * kFour; ++i) {
-            if constexpr (kSize == 4) {
-                const uint32_t x = k[i] & 0x7fffffffu;
-                m                = x < kInf ? max(m, x) : m;
-            } else {
-                const uint32_t x = k[i] & 0x7fffu, y = k[i] >> 16 & 0x7fffu;
-                m                = x < kInf ? max(m, x) : m;
-                m                = y < kInf ? max(m, y) : m;
-            }
-        }
-        return m;
-    }
-
     __device__ uint32_t top_v(int e) const {
         uint32_t m = 0;
 #pragma unroll
@@ -406,7 +387,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
     char * const   vh   = kl + (TWO ? kTileKeys * KSTRIDE : 0);
     char * const   vl   = vh + HD * kVStride;
     float * const  tops = reinterpret_cast<float *>(vl + (TWO ? HD * kVStride : 0));  // of each wave's K and V, then the least
-    uint64_t *     bads = reinterpret_cast<uint64_t *>(tops + 4 * kWaves);            // a wave's keys that are not finite in V
+    uint64_t *     bads = reinterpret_cast<uint64_t *>(tops + 4 * kWaves);            // a wave's keys that are not finite in K or V
     uint32_t *     rmax = reinterpret_cast<uint32_t *>(bads + kWaves);                // SIZES: the largest of each row of K, then V
     f16x8 *        q3   = reinterpret_cast<f16x8 *>(bads + kWaves) + threadIdx.x;     // THREE: the third pieces of a lane's query
 
@@ -667,19 +648,21 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                 }
             }
             if (__any(max(tk, tv) >= PartT::kInf)) {
-                // what is not finite in K is its key's alone; a key whose V has
-                // such a value counts for nothing in the products
+                // a value that is not finite makes its key a bad one; in V it counts
+                // for nothing in the products (in K it is its key's scores' alone)
                 tk = tv = 0;
                 lk = lv = ~0u;
 #pragma unroll
                 for (int z = 0; z < PARTS; ++z) {
                     if (mine[z]) {
-                        const uint32_t whole = part[z].top_k();
-                        note(whole >= PartT::kInf ? part[z].finite_k() : whole, tk, lk);
+                        const int  id = tid_again();
+                        const bool it = part[z].top_k() >= PartT::kInf;
+                        bad |= static_cast<uint64_t>(it) << row_k(id, z);
+                        note(it ? 0 : part[z].top_k(), tk, lk);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const bool is = part[z].top_v(e) >= PartT::kInf;
-                            bad |= static_cast<uint64_t>(is) << (key_v(tid_again(), z) + (e < 4 ? e : e + 4));
+                            bad |= static_cast<uint64_t>(is) << (key_v(id, z) + (e < 4 ? e : e + 4));
                             part[z].keep_v(e, !is);
                             note(part[z].top_v(e), tv, lv);
                         }
@@ -739,7 +722,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
 #pragma unroll
                 for (int z = 0; z < PARTS; ++z) {
                     if (mine[z]) {
-                        at_least(row_k(id, z), part[z].finite_k());
+                        at_least(row_k(id, z), part[z].top_k());
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             at_least(kTileKeys + key_v(id, z) + (e < 4 ? e : e + 4), part[z].top_v(e));

@@ -162,3 +162,55 @@ def test_scores_past_whole_numbers(gpu, kind, t, hd, cap, sign, size):
     bound = (8 * R.EPS + 2.0 ** -23) * want.abs() + 2.0 ** -30 * want.abs().amax(-1, keepdim=True)
     for i in range(star - (cap - t), t):
         assert ((got[0, i].double() - want).abs() <= bound).all(), i
+
+
+@pytest.mark.parametrize("kind,hd", [(k, 64) for k in R.TYPES] + [("f16", 75), ("bf16", 33), ("q8_0", 160), ("f32", 200)])
+@pytest.mark.parametrize("t", [1, 3, 40])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("score", [1.0, -1.0])
+def test_an_infinite_key_is_nan_for_those_that_see_it(gpu, kind, hd, t, sign, score):
+    """Whatever the sign of its score; a block's d becomes infinite where a value is
+    past what F16's d holds. Queries that do not see it, and other heads, are as ever."""
+    n, kv, g, cap = 1, 4, 2, 100
+    q, k, v = rand(n, t, kv * g, kv, hd, cap, 42)
+    row = cap - t // 2 - 1
+    cache = [R.pack(x, kind) for x in (k, v)]
+    y, bound = R.attend_by_row(q.abs() * sign * score, *(R.values(c, kind) for c in cache), kind, [cap], [t], hd ** -0.5,
+                               window=60, sinks=2)
+    k = k.clone()
+    k[0, row, 1] = sign * 1e30 if kind in ("q8_0", "q4_0") else k[0, row, 1]
+    k[0, row, 1, 5] = sign * (1e30 if kind in ("q8_0", "q4_0") else float("inf"))
+    k[0, 20, 2, 7] = sign * (1e30 if kind in ("q8_0", "q4_0") else float("inf"))  # behind the window
+    q = q.abs() * sign * score
+    h = [R.handle(gpu, R.pack(x, kind).cuda(), kind, hd) for x in (k, v)]
+    got = gpu.attn_kv(q.cuda(), h[0], h[1], ints(cap), window=60, sinks=2).cpu().double()
+    nan = torch.zeros(t, kv * g, dtype=torch.bool)
+    p = torch.arange(cap - t, cap)
+    nan[p >= row, g:2 * g] = True
+    nan[20 > p - 60, 2 * g:3 * g] = True
+    assert torch.isnan(got[0][nan]).all()
+    assert ((got - y).abs()[0][~nan] <= bound[0][~nan]).all()
+
+
+@pytest.mark.parametrize("kind,hd", [(k, 64) for k in R.TYPES] + [("f16", 75), ("q8_0", 160)])
+@pytest.mark.parametrize("t", [1, 3, 40])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_a_query_that_is_not_finite(gpu, kind, hd, t, value, zeros):
+    """NaN for that query and head, whatever the keys' signs, zero among them or not."""
+    n, kv, g, cap = 1, 4, 2, 100
+    q, k, v = rand(n, t, kv * g, kv, hd, cap, 43)
+    k = k.abs() + 0.5
+    if zeros:
+        k[0, ::3] = 0.0
+    cache = [R.pack(x, kind) for x in (k, v)]
+    y, bound = R.attend_by_row(q, *(R.values(c, kind) for c in cache), kind, [cap], [t], hd ** -0.5)
+    q = q.clone()
+    nan = torch.zeros(t, kv * g, dtype=torch.bool)
+    for i, head in ((0, 1), (t - 1, 6)):
+        q[0, i, head, 3] = value
+        nan[i, head] = True
+    h = [R.handle(gpu, c.cuda(), kind, hd) for c in cache]
+    got = gpu.attn_kv(q.cuda(), h[0], h[1], ints(cap)).cpu().double()
+    assert torch.isnan(got[0][nan]).all()
+    assert ((got - y).abs()[0][~nan] <= bound[0][~nan]).all()
