@@ -322,22 +322,27 @@ template <> struct KOrder<kKvQ4> : Codes<kKvQ4> {};
 // F32, whose values may be of any size. One power of two for the K and one for the
 // V of a tile cost a value up to 2^-39 of the tile's largest, so they are used
 // where no row is much smaller than that: a tile is even where every 32 values of
-// K and four of V that are not all zero have one of 2^-8 of the tile's largest and
-// more. A tile that is not is taken in several passes, each over the rows of about
-// one size (2^kAlike times smaller or larger than the first that is left) as if the
-// others were hidden. So a value is off by 2^-30 of its own row's largest at most,
-// whatever the others are, and a row that a query does not see has no part in its
-// result.
+// K and four of V that are not all zero have one of 2^-14 of the tile's largest and
+// more. A tile that is not is taken in several passes, each over rows of about one
+// size as if the others were hidden: those down to 2^-(2 kAlike) of the largest that
+// are left, or, where none is that in K and V, 2^kAlike times smaller and larger
+// than the first. So a value is off by 2^-25 of its own row's largest at most,
+// a half step, whatever the others are; a row that a query does not see has no
+// other part in its result.
 // V's sizes differ from pass to pass: weights are held times 2^(E - X + 15), 2^E
 // being that of the pass and 2^X, which is the query's own, what the largest so
-// far of weight times 2^E needs. So P loses 2^-29 of the largest weighted row at
-// most (2^-39 of the largest weight where all rows are of one size).
+// far of weight times 2^E needs. So P loses 2^-39 of the largest weight where one
+// size is all that the query sees, and else 2^-39 of the largest of weight times
+// 2^E, whose row may be 2^14 smaller than 2^E.
+// (4096 positions of 16 heads over 8, MI355X: 377 us, 365 with one power of two in
+// any case. A channel thirty times the others leaves all tiles even, one of V a
+// thousand times them takes 1.25 times as long, rows from 1e-8 to 1e8 5.7 times.)
 constexpr bool by_size(int kind) {
     return kind == kKvF32;
 }
 
-constexpr float kEven  = 0x1p-7f;  // of the largest that a wave holds, and waves within a factor of 2
-constexpr int   kAlike = 4;
+constexpr float kEven  = 0x1p-13f;  // of the largest that a wave holds, and waves within a factor of 2
+constexpr int   kAlike = 6;
 constexpr int   kVTop  = 13;       // the largest value of V comes to 2^13 and more
 constexpr int   kMinX  = -99;      // of values of 2^-100 and less
 
@@ -730,19 +735,25 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
                     }
                 }
                 __syncthreads();
-                // a lane a key; rows of zeros go with any
+                // a lane a key; zeros are of any size
                 const float    k1   = PartT::magnitude(rmax[lane]);
                 const float    v1   = PartT::magnitude(rmax[kTileKeys + lane]);
-                const bool     zero = k1 == 0.0f && v1 == 0.0f;
+                const bool     here = left >> lane & 1;
                 const int      ke   = exponent_of(k1);
                 const int      ve   = exponent_of(v1);
-                const uint64_t some = __ballot((left >> lane & 1) && !zero);
-                const int      one  = some == 0 ? 0 : __ffsll(static_cast<unsigned long long>(some)) - 1;
-                const bool     in   = (left >> lane & 1) && (zero || (abs(ke - __builtin_amdgcn_readlane(ke, one)) <= kAlike &&
-                                                                   abs(ve - __builtin_amdgcn_readlane(ve, one)) <= kAlike));
-                alike               = true;
-                pass                = __ballot(in);
-                ready               = pass == left;
+                const uint64_t some = __ballot(here && (k1 != 0.0f || v1 != 0.0f));
+                auto           rows = [&](int k0, int k2, int v0, int v2) {
+                    return __ballot(here && (k1 == 0.0f || (ke >= k0 && ke <= k2)) && (v1 == 0.0f || (ve >= v0 && ve <= v2)));
+                };
+                pass = rows(exponent_of(wave_max(here ? k1 : 0.0f)) - 2 * kAlike, INT_MAX,
+                            exponent_of(wave_max(here ? v1 : 0.0f)) - 2 * kAlike, INT_MAX);
+                if (some != 0 && (pass & some) == 0) {  // no row is of the largest in K and V
+                    const int one = __ffsll(static_cast<unsigned long long>(some)) - 1;
+                    const int k0  = __builtin_amdgcn_readlane(ke, one), v0 = __builtin_amdgcn_readlane(ve, one);
+                    pass          = rows(k0 - kAlike, k0 + kAlike, v0 - kAlike, v0 + kAlike);
+                }
+                alike = true;
+                ready = pass == left;
             }
             kexp  = __builtin_amdgcn_readfirstlane(exponent_of(kt)) - 13;
             vsize = __builtin_amdgcn_readfirstlane(exponent_of(vt));

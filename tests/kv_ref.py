@@ -104,14 +104,14 @@ def attend_by_row(q, k, v, kind, length, count, scale, window=0, sinks=0):
     A score s_j = scale q.k_j is off by e_j: hd products summed in f32, operands,
     lo x lo and the scale's product off by half steps each (16 more), the
     difference s_j - max rounded (|s_j| + |max|), and, where operands are two F16
-    pieces, 2^-38 of q's largest value for each of q and, f32, 2^-30 of its largest
-    for each value of the row k_j: 2^-30 and 2^-38 of hd max|q| max|k_j|. A weight
+    pieces, 2^-38 of q's largest value for each of q and, f32, 2^-25 of its largest
+    for each value of the row k_j: 2^-25 and 2^-38 of hd max|q| max|k_j|. A weight
     then moves by w_j (e^(e_j) - 1), and the sum of weights by E = sum_j w_j (e^(e_j)
     - 1).
     To this come attend()'s n + 32 half steps of the sum and of the joins, and
     2^-126 where f32 ends. Pieces hold a weight to 2^-40 of the largest, which moves a
     result by 2^-40 |v_j| w_max; over f32, times its row's largest value, to 2^-39
-    of 2^10 times the largest such product, and V to 2^-30 of its row's largest.
+    of 2^15 times the largest such product, and V to 2^-25 of its row's largest.
     bf16 has neither: its pieces hold all 24 bits."""
     n, t, heads, hd = q.shape
     group = heads // k.shape[2]
@@ -139,7 +139,7 @@ def attend_by_row(q, k, v, kind, length, count, scale, window=0, sinks=0):
         w = w / w.sum(-1, keepdim=True).clamp_min(1e-300)
         size = abs(scale) * (x.abs() @ kk.abs().transpose(1, 2))
         kmax, vmax = kk.abs().amax(-1), vv.abs().amax(-1)                      # (heads, ln)
-        rows = 2.0 ** -30 if kind == "f32" else 0.0
+        rows = 2.0 ** -25 if kind == "f32" else 0.0
         e = (hd + 16) * EPS * size + abs(scale) * hd * (rows + 2.0 ** -38) * x.abs().amax(-1)[..., None] * kmax[:, None]
         e = e + EPS * (s.abs() + top.abs())
         e = torch.where(hidden, 0.0, torch.expm1(e.nan_to_num(posinf=0.0).clamp_max(700.0)))
@@ -147,7 +147,7 @@ def attend_by_row(q, k, v, kind, length, count, scale, window=0, sinks=0):
         far = moved @ vv.abs() + (ln + 32) * EPS * (w @ vv.abs())
         far = far + rows * (w @ vmax[..., None])
         if kind == "f32":
-            far = far + ln * 2.0 ** -29 * (w * vmax[:, None]).amax(-1, keepdim=True)
+            far = far + ln * 2.0 ** -24 * (w * vmax[:, None]).amax(-1, keepdim=True)
         elif kind != "bf16":
             far = far + 2.0 ** -40 * w.amax(-1, keepdim=True) * ((~hidden).double() @ vv.abs())
         y[b, :c] = torch.where(some[None, :, None], w @ vv, 0.0).transpose(0, 1)

@@ -214,3 +214,36 @@ def test_a_query_that_is_not_finite(gpu, kind, hd, t, value, zeros):
     got = gpu.attn_kv(q.cuda(), h[0], h[1], ints(cap)).cpu().double()
     assert torch.isnan(got[0][nan]).all()
     assert ((got - y).abs()[0][~nan] <= bound[0][~nan]).all()
+
+
+@pytest.mark.parametrize("kind,t,hd", cases((1, 64), (40, 64), (130, 128), (3, 160)))
+@pytest.mark.parametrize("window", [0, 70])
+def test_rows_of_all_sizes_beside_what_is_not_finite(gpu, kind, t, hd, window):
+    """Rows of many sizes, among them some with a NaN that no query, or only the
+    later ones, see, and a channel far above the others."""
+    q, k, v = rand(2, t, 4, 2, hd, 200, 44)
+    q[..., 7] *= 1e-3
+    g = torch.Generator().manual_seed(45)
+    wide = {"f32": 6.0, "bf16": 6.0, "f16": 2.0, "q8_0": 2.0, "q4_0": 2.0}[kind]
+    up = lambda: 10.0 ** (wide * (2 * torch.rand((2, 200, 2, 1), generator=g) - 1))
+    v = v * up()
+    v[..., 5] *= 50.0
+    k = k * up().clamp(max=3.0)
+    k[..., 7] *= 50.0
+    length = [200, 131]
+    cache = [R.pack(x, kind) for x in (k, v)]
+    y, bound = R.attend_by_row(q, *(R.values(c, kind) for c in cache), kind, length, [t, t], hd ** -0.5, window, 2)
+    nan = torch.zeros(2, t, 4, dtype=torch.bool)
+    for b in range(2):
+        p = torch.arange(length[b] - t, length[b])
+        for row, head, which in ((length[b] - 1, 0, 0), (length[b] - 1 - t // 2, 1, 1), (40, 0, 1)):
+            (k, v)[which][b, row, head, 3] = float("nan")
+            seen = (row <= p) & ((row > p - window) if window else (row >= 0))
+            nan[b, seen, 2 * head:2 * head + 2] = True
+    h = [R.handle(gpu, R.pack(x, kind).cuda(), kind, hd) for x in (k, v)]
+    got = gpu.attn_kv(q.cuda(), h[0], h[1], ints(*length), window=window, sinks=2).cpu().double()
+    real = ~torch.isnan(y).any(-1)
+    assert torch.isnan(got[nan & real]).all()
+    fine = real & ~nan
+    err = (got - y).abs()[fine]
+    assert (err <= bound[fine]).all(), float((err / bound[fine].clamp_min(1e-300)).max())
