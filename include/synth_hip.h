@@ -760,10 +760,22 @@ shp_status_t shp_kv_load(const shp_tensor * k_cache,
  * or V that it sees, of its kv head, or in its q makes the result NaN, whatever
  * the score would be (a block whose d is an infinity or NaN counts as such: d is
  * infinite where kv_store met a value of 65520 times 127 in Q8_0, or 8 in Q4_0).
- * head_dim 1..256; y and work overlap nothing else of the call. Products are
- * formed to f32's precision and summed in f32; a weight is held to 2^-40 of the
- * row's largest. SHP_ERR_UNSUPPORTED past 2^28 query rows or 2^30 cache rows a
- * sequence, and past 65535 heads or sequences.
+ * head_dim 1..256; y and work overlap nothing else of the call.
+ *
+ * Precision: products are summed in f32, of operands held as follows. K and V in
+ * F16, BF16 and blocks exactly, whatever the sizes of the values beside each
+ * other; F32 values to 2^-23 of themselves or 2^-25 of the largest of their own row
+ * (one position of one kv head; of 2^-100, where that is smaller), whichever is
+ * more. q to 2^-22 of itself or 2^-38 of the largest value of its head (BF16 caches:
+ * f32's 24 bits). A weight to 2^-22 of itself or 2^-39 of the largest that the query
+ * has (BF16: 24 bits; F32, where rows of V are of very different sizes: of the
+ * largest of weight times its row's size, which is known to a factor of 2^14). A
+ * weight below 2^-126 of the largest may count as 0. What a row holds has no other
+ * part in what the others come to. The sum of weight times value over the rows,
+ * with the largest weight as 1, has to be within f32's range.
+ *
+ * SHP_ERR_UNSUPPORTED past 2^28 query rows or 2^30 cache rows a sequence, and past
+ * 65535 heads or sequences.
  *
  * work: F32, contiguous, at least the number of floats that
  * shp_attn_kv_work gives for the same q, k_cache, window and sinks (partial

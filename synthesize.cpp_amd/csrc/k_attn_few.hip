@@ -18,12 +18,16 @@ namespace {
 //         more: q = 2^e (hi + lo)), each block's sum times its d in F32;
 //   O^T = V^T P^T: code * d as two F16 pieces, exact (at most 8 + 11 bits),
 //         against P in two; lo x lo, below 2^-22 of the product, is left out.
+//         Where a d of V is above 256, d is two parts (see kBigD), one after
+//         the other.
 // P is held times 2^15, so that its pieces keep their bits where it is small:
-// a weight is off by at most 2^-40 of the largest, or 2^-23 of itself.
-// Bound by the vector instructions that form the operands: 470 a chunk of 4.6
-// KB (128 values, Q4_0), which is 61 us of issue on every SIMD for 64 streams of
-// 512 to 8192 rows (16 heads over 8), a call of 93 to 105 us at 3.1 to 3.5
-// TB/s; one stream of 8191 rows takes 17 us, 7 of them the join (MI355X).
+// a weight is off by at most 2^-40 of the largest, or 2^-22 of itself.
+// 64 streams of 512 to 8192 rows (Q4_0, 16 heads of 128 values over 8, MI355X)
+// take 93 to 106 us, 3.0 to 3.5 TB/s. Vector instructions, most of them forming
+// operands, are 480 a chunk of 4.6 KB: 62 us of issue on every SIMD. Matrix
+// instructions are 20 % of the time and LDS 35 %; what overlaps of these, and what
+// the rest waits for, has not been measured. One stream of 8191 rows takes 17 us,
+// 7 of them the join.
 // ---------------------------------------------------------------------------
 
 // Dwords at two-byte boundaries of LDS. A wave's read of them as they are takes

@@ -14,13 +14,15 @@ namespace {
 // and P are three BF16 pieces, all 24 bits of them. Matrix instructions 32x32x16:
 // S^T = K Q^T has a query in each lane, O^T = V^T P^T too.
 // Bound by the matrix units: 8192 positions of 16 heads of 128 values over 8 kv
-// heads take 730 us, three products at 1.15 PFLOP/s, which is the rate that a
-// large F16 product reaches on this chip, at the clock that such work leaves
-// it. A prompt that does not fill the chip is bound by the longest row: 1021
-// positions 40 us, 11 of them the second launch that joins its splits (Q4_0,
-// MI355X). 128 rows and 64 keys are what the registers (O^T, q, a tile under
+// heads take 700 to 745 us (Q4_0, MI355X), three products at 1.11 to 1.18 PFLOP/s,
+// where a large F16 product reaches 1.12, at the clock that such work leaves the
+// chip. (K's codes could do with one piece and d by key, as in k_attn_few: two
+// products and a half in all.) A prompt that does not fill the chip is bound by the longest row: 1021
+// positions 40 us, 10 of them the second launch that joins its splits. 4096
+// positions: F16 180 us, BF16 226, Q4_0 250, Q8_0 282, F32 380 to 400, whose
+// registers spill. 128 rows and 64 keys are what the registers (O^T, q, a tile under
 // way: 256) and two workgroups' LDS hold; heads of more than 128 values have one
-// workgroup a CU, with 512 (2048 positions of 8 heads of 256 over 4, Q4_0: 136 us).
+// workgroup a CU, with 512 (2048 positions of 8 heads of 256 over 4, Q4_0: 118 us).
 // ---------------------------------------------------------------------------
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
