@@ -393,7 +393,7 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
     char * const   kl   = kh + kTileKeys * KSTRIDE;  // (of two pieces)
     char * const   vh   = kl + (TWO ? kTileKeys * KSTRIDE : 0);
     char * const   vl   = vh + HD * kVStride;
-    float * const  tops = reinterpret_cast<float *>(vl + (TWO ? HD * kVStride : 0));  // of each wave's K and V, then the least
+    float * const  tops = reinterpret_cast<float *>(vl + (TWO ? HD * kVStride : 0));  // SIZES: each wave's largest of K, of V, and whether some are far below; blocks: whether a d is large
     uint64_t *     bads = reinterpret_cast<uint64_t *>(tops + 4 * kWaves);            // a wave's keys that are not finite in K or V
     uint32_t *     rmax = reinterpret_cast<uint32_t *>(bads + kWaves);                // SIZES: the largest of each row of K, then V
     f16x8 *        q3   = reinterpret_cast<f16x8 *>(bads + kWaves) + threadIdx.x;     // THREE: the third pieces of a lane's query

@@ -247,3 +247,42 @@ def test_rows_of_all_sizes_beside_what_is_not_finite(gpu, kind, t, hd, window):
     fine = real & ~nan
     err = (got - y).abs()[fine]
     assert (err <= bound[fine]).all(), float((err / bound[fine].clamp_min(1e-300)).max())
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("t,cap", [(1, 700), (70, 300)])
+def test_captured_over_zeros_and_replayed(gpu, kind, t, cap):
+    """A call captured while its inputs are zeros, replayed over ordinary values,
+    over rows of very different sizes and over zeros again: the eager call's
+    results each time, and the definition's."""
+    n, heads, kv, hd = 2, 4, 2, 64
+    q, k, v = rand(n, t, heads, kv, hd, cap, 46)
+    g = torch.Generator().manual_seed(47)
+    up = 10.0 ** (8 * torch.rand((n, cap, kv, 1), generator=g) - 4) if kind in ("f32", "bf16") else torch.ones(n, cap, kv, 1)
+    up[:, ::9] *= 1.0 if kind == "f16" else 1e5
+    zero = [R.pack(torch.zeros_like(x), kind).cuda() for x in (k, v)]
+    cache = [x.clone() for x in zero]
+    h = [R.handle(gpu, c, kind, hd) for c in cache]
+    length, qd = ints(cap, cap - 33), torch.zeros(q.shape, device="cuda")
+    out = torch.zeros(q.shape, device="cuda")
+    call = lambda: gpu.attn_kv(qd, h[0], h[1], length, out=out)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.current_stream().wait_stream(s)
+    assert (out == 0).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for a, b, c in ((q, k, v), (q, k * up.clamp(max=10.0), v * up), (0 * q, 0 * k, v), (q, k, v * up), (0 * q, 0 * k, 0 * v)):
+        qd.copy_(a)
+        host = [R.pack(x, kind) for x in (b, c)]
+        for x, y in zip(cache, host):
+            x.copy_(y)
+        graph.replay()
+        eager = gpu.attn_kv(qd, h[0], h[1], length)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        y, bound = R.attend_by_row(a, *(R.values(x, kind) for x in host), kind, [cap, cap - 33], [t, t], hd ** -0.5)
+        assert ((out.cpu().double() - y).abs() <= bound).all()
