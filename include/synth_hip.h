@@ -760,7 +760,8 @@ shp_status_t shp_kv_load(const shp_tensor * k_cache,
  * or V that it sees, of its kv head, or in its q makes the result NaN, whatever
  * the score would be (a block whose d is an infinity or NaN counts as such: d is
  * infinite where kv_store met a value of 65520 times 127 in Q8_0, or 8 in Q4_0).
- * head_dim 1..256; y and work overlap nothing else of the call.
+ * head_dim 1..256, scale log2(e) finite; y and work overlap nothing else of the
+ * call.
  *
  * Precision: products are summed in f32, of operands held as follows. K and V in
  * F16, BF16 and blocks exactly, whatever the sizes of the values beside each

@@ -443,8 +443,10 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
     if (st != SHP_OK) {
         return st;
     }
+    // exp(x) = exp2(x log2 e)
+    const float scale2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
     if (!well_formed(y) || !same_shape(*q, *y) || (length != nullptr && !kv_numbers(length, q->ne[3])) ||
-        (count != nullptr && !kv_numbers(count, q->ne[3])) || !(fabsf(scale) < INFINITY)) {
+        (count != nullptr && !kv_numbers(count, q->ne[3])) || !(fabsf(scale2) < INFINITY)) {
         return SHP_ERR_INVALID_ARG;
     }
     const int64_t floats = plan_floats(p, *q);
@@ -478,7 +480,7 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
     a.kh = nb(*k_cache, 1), a.kt = nb(*k_cache, 2), a.kn = nb(*k_cache, 3);
     a.vh = nb(*v_cache, 1), a.vt = nb(*v_cache, 2), a.vn = nb(*v_cache, 3);
     a.yh = nb(*y, 1), a.yt = nb(*y, 2), a.yn = nb(*y, 3);
-    a.scale  = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);  // exp(x) = exp2(x log2 e)
+    a.scale  = scale2;
     a.window = p.window;
     a.sinks  = p.sinks;
     a.T      = static_cast<int32_t>(q->ne[2]);

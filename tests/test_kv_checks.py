@@ -194,3 +194,10 @@ def test_binding_raises(monkeypatch):
         assert e.value.status == status
     with pytest.raises(AssertionError):
         S.Q4Tensor(torch.zeros(9, 35, dtype=torch.uint8), 64)
+
+
+def test_a_scale_past_what_f32_holds_in_powers_of_two():
+    """scale log2(e) has to be finite: the kernels' exponentials are of two."""
+    for scale in (3e38, -2.5e38):
+        assert attend(scale=scale) == BAD
+    assert attend(scale=2e38, work=None) == BAD                           # (the workspace; nothing is run)
