@@ -119,7 +119,9 @@ def attend_by_row(q, k, v, kind, length, count, scale, window=0, sinks=0):
     bound = torch.zeros_like(y)
     for b in range(n):
         ln, c = int(length[b]), int(count[b])
-        if c == 0:
+        if ln == 0:
+            y[b, :c], bound[b, :c] = 0.0, 2.0 ** -126
+        if c == 0 or ln == 0:
             continue
         kk = k[b, :ln].double().repeat_interleave(group, 1).transpose(0, 1)    # (heads, ln, hd)
         vv = v[b, :ln].double().repeat_interleave(group, 1).transpose(0, 1)

@@ -48,6 +48,7 @@ def test_queries_and_keys_of_zero_and_next_to_it(gpu, kind, t, hd, cap, small):
     ks[:, 64::3] *= small
     run(gpu, kind, qs, ks, v, [cap, (cap + 1) // 2])
     run(gpu, kind, q * small, k * small, v * small, [cap, (cap + 1) // 2], window=30, sinks=2)
+    run(gpu, kind, q * small, k * small, v, [0, cap])
 
 
 def cases(*shapes, kinds=R.TYPES):
