@@ -50,6 +50,7 @@ typedef int32_t shp_status_t;
 #define SHP_TYPE_Q4_0 2 /* the KV cache's entry points only (shp_kv_store, shp_kv_load, shp_attn_kv) */
 #define SHP_TYPE_Q8_0 8
 #define SHP_TYPE_Q5_K 13
+#define SHP_TYPE_I8   24 /* codes of a paged KV cache only (shp_kv_store_pages and what follows it) */
 #define SHP_TYPE_I32  26
 #define SHP_TYPE_BF16 30
 
@@ -800,6 +801,106 @@ shp_status_t shp_attn_kv(const shp_tensor * q,
                          shp_tensor *       work,
                          shp_tensor *       y,
                          shp_stream_t       stream);
+
+/*
+ * The paged KV cache, in 8 bits.
+ *
+ * Sequences share a pool of pages. A page holds `page` positions (16, 32, 64,
+ * 128 or 256) of every kv head, as int8 codes under one F32 scale for each
+ * (page, head), a block; a value is code * scale. The pool is four tensors:
+ *   k_pages  I8 [head_dim, page, kv_heads, pages]   a block's rows one after the other
+ *   v_pages  I8 [page, head_dim, kv_heads, pages]   a block's columns one after the other
+ *   k_scale, v_scale  F32 [kv_heads, pages]
+ * so that both are operands of matrix instructions as they lie. head_dim is a
+ * multiple of 16 up to 256; blocks are contiguous, and heads and pages at any
+ * strides that are multiples of 16 bytes (else SHP_ERR_UNSUPPORTED).
+ * Scales are finite and not negative; a block whose scale is anything else reads
+ * as NaN.
+ *
+ * table, I32 [max_pages, N]: row r of sequence n is row r % page of the page
+ * table[n][r / page]. length[n] counts a sequence's rows, the count[n] newest
+ * of a call among them (I32 [N] each; count NULL: as many as the call's tensors
+ * have). All of them are in device memory and read when the kernel runs. What a
+ * table holds past a sequence's rows does not matter to any call but
+ * shp_kv_pages. max_pages * page may be up to 2^30, pages * page below 2^31.
+ *
+ * shp_kv_pages makes the tables fit new lengths: sequence n needs ceil(length[n]
+ * / page) pages and has held[n]. First the pages past a sequence's need go on the
+ * stack of free ones (free_pages[0..left), I32 [pages] and I32 [1]), the last page of
+ * the last sequence first, and their entries become -1; then missing ones are
+ * taken from its top, the first page of the first sequence first. held and left
+ * are updated. So going back to the lengths before gives back tables and stack
+ * as they were. Where a length is negative or past the table, held is outside
+ * [0, max_pages], the stack would hold more than `pages` or has too few,
+ * nothing is changed at all and *status (I32 [1], or NULL) is set to 1; the
+ * library never clears it. To begin with: held 0, free_pages a permutation of
+ * the pages, left their number. work: I32, contiguous, at least
+ * what shp_kv_pages_work gives for the table; NULL where that is 0; calls that
+ * may run at the same time need one each, and tables and stacks of their own.
+ *
+ * shp_kv_slots: where the new rows lie, slots[n][t] = table[n][p / page] * page +
+ * p % page with p = length[n] - count[n] + t, and -1 for t >= count[n] and where
+ * the table has no page >= 0 for p. slots I32 [T, N].
+ */
+shp_status_t shp_kv_pages_work(const shp_tensor * table, int64_t * ints);
+shp_status_t shp_kv_pages(const shp_tensor * length,
+                          int32_t            page,
+                          shp_tensor *       held,
+                          shp_tensor *       free_pages,
+                          shp_tensor *       left,
+                          shp_tensor *       table,
+                          shp_tensor *       work,
+                          shp_tensor *       status,
+                          shp_stream_t       stream);
+shp_status_t shp_kv_slots(const shp_tensor * table,
+                          const shp_tensor * length,
+                          const shp_tensor * count,
+                          int32_t            page,
+                          shp_tensor *       slots,
+                          shp_stream_t       stream);
+
+/*
+ * shp_kv_store_pages writes new rows: row t < count[n] of k and v, F32 [head_dim,
+ * kv_heads, T, N], becomes row length[n] - count[n] + t of sequence n. For a block
+ * whose new rows' largest magnitude is m:
+ *   d = m / 127, and, where the sequence has rows in front of the new ones in this
+ *       block, the larger of that and the block's scale;
+ *   if that is more than the scale was, the codes c of the rows in front become
+ *       rint(c * (scale / d)): at most half a step of the larger scale for each
+ *       time that it grows;
+ *   the new rows' codes are rint(x / d), at most 127 in magnitude, 0 where d is 0;
+ * each quotient and product rounded in f32, rint to even. Rows behind the new ones are
+ * left as they were. A block that gets an infinity or NaN, or has such a scale
+ * and rows in front, has NaN for its scale, until its first row is
+ * written again. A sequence whose rows do not fit (count[n] outside [0, T] or past length[n], a
+ * length past the table, a page outside the pool among those to be written) is
+ * not written at all, and *status (I32 [1], or NULL) is set to 1.
+ * No page that is written may stand in the tables of the call twice.
+ *
+ * shp_kv_load_pages reads rows back by slot, in any order: row t of k and v, F32
+ * [head_dim, kv_heads, T, N], is the one at slots[n][t] (as shp_kv_slots gives
+ * them; I32 [T, N]): code * scale, one f32 product. It is left as it was for a slot of
+ * -1, and NaN for any other outside the pool.
+ */
+shp_status_t shp_kv_store_pages(const shp_tensor * k,
+                                const shp_tensor * v,
+                                const shp_tensor * table,
+                                const shp_tensor * length,
+                                const shp_tensor * count,
+                                shp_tensor *       k_pages,
+                                shp_tensor *       v_pages,
+                                shp_tensor *       k_scale,
+                                shp_tensor *       v_scale,
+                                shp_tensor *       status,
+                                shp_stream_t       stream);
+shp_status_t shp_kv_load_pages(const shp_tensor * k_pages,
+                               const shp_tensor * v_pages,
+                               const shp_tensor * k_scale,
+                               const shp_tensor * v_scale,
+                               const shp_tensor * slots,
+                               shp_tensor *       k,
+                               shp_tensor *       v,
+                               shp_stream_t       stream);
 
 /*
  * ggml_exp: y = expf(x) per element, F32 of one shape

@@ -79,8 +79,10 @@ bool from_tensor(PyObject * o, shp_tensor & d) {
         case at::kInt:
             d.type = SHP_TYPE_I32;
             break;
-        case at::kByte:
         case at::kChar:
+            d.type = SHP_TYPE_I8;
+            break;
+        case at::kByte:
             d.type = -1;  // raw blocks: the caller names the type
             break;
         default: {
@@ -377,24 +379,33 @@ PyObject * run_layer(void * fn, PyObject * const * args, Py_ssize_t n) {
     return PyLong_FromLong(st);
 }
 
-// The workspace of shp_attn_kv: q, k_cache, window and sinks to its floats, or
-// to minus the status.
-PyObject * run_attn_work(void * fn, PyObject * const * args, Py_ssize_t n) {
-    if (!counted(n, 4)) {
-        return nullptr;
+// A workspace's size: an entry point whose last parameter takes it, without that
+// parameter; its value, or minus the status.
+template <class F> struct Work;
+
+template <class... A> struct Work<shp_status_t (*)(A...)> {
+    template <size_t... I>
+    static bool convert(PyObject * const * args, std::array<Slot, sizeof...(A)> & slots, std::tuple<A...> & vals,
+                        std::index_sequence<I...>) {
+        return (Arg<std::tuple_element_t<I, std::tuple<A...>>>::get(args[I], slots[I], std::get<I>(vals)) && ...);
     }
-    Slot               s[4];
-    const shp_tensor * q      = nullptr;
-    const shp_tensor * k      = nullptr;
-    int32_t            window = 0, sinks = 0;
-    int64_t            floats = 0;
-    if (!Arg<const shp_tensor *>::get(args[0], s[0], q) || !Arg<const shp_tensor *>::get(args[1], s[1], k) ||
-        !Arg<int32_t>::get(args[2], s[2], window) || !Arg<int32_t>::get(args[3], s[3], sinks)) {
-        return nullptr;
+
+    static PyObject * run(void * fn, PyObject * const * args, Py_ssize_t n) {
+        constexpr size_t kTaken = sizeof...(A) - 1;
+        if (!counted(n, kTaken)) {
+            return nullptr;
+        }
+        std::array<Slot, sizeof...(A)> slots;
+        std::tuple<A...>               vals{};
+        int64_t                        size = 0;
+        if (!convert(args, slots, vals, std::make_index_sequence<kTaken>{})) {
+            return nullptr;
+        }
+        std::get<kTaken>(vals) = &size;
+        const shp_status_t st  = std::apply(reinterpret_cast<shp_status_t (*)(A...)>(fn), vals);
+        return PyLong_FromLongLong(st == SHP_OK ? size : -static_cast<int64_t>(st));
     }
-    const shp_status_t st = reinterpret_cast<decltype(&shp_attn_kv_work)>(fn)(q, k, window, sinks, &floats);
-    return PyLong_FromLongLong(st == SHP_OK ? floats : -static_cast<int64_t>(st));
-}
+};
 
 using Runner = PyObject * (*) (void *, PyObject * const *, Py_ssize_t);
 
@@ -405,6 +416,7 @@ struct Entry {
 
 #define SHP_ENTRY_FIRST(f, first) { #f, &Call<decltype(&f), first>::run }
 #define SHP_ENTRY(f) SHP_ENTRY_FIRST(f, kTensor)
+#define SHP_WORK(f) { #f, &Work<decltype(&f)>::run }
 
 const Entry kEntries[] = {
     SHP_ENTRY(shp_get_rows), SHP_ENTRY_FIRST(shp_get_rows_sum, kArray), SHP_ENTRY(shp_rms_norm_mul), SHP_ENTRY(shp_add_rms_norm_mul),
@@ -420,7 +432,9 @@ const Entry kEntries[] = {
     SHP_ENTRY(shp_acc), SHP_ENTRY_FIRST(shp_im2col, kShape), SHP_ENTRY(shp_cont_add_leaky_relu), SHP_ENTRY(shp_soft_max_ext),
     SHP_ENTRY(shp_diag_mask_inf), SHP_ENTRY(shp_soft_max_causal), SHP_ENTRY(shp_exp), SHP_ENTRY(shp_scale_bias),
     SHP_ENTRY_FIRST(shp_sum_scale_leaky_relu, kArray), { "shp_layer_nongemm_step", &run_layer },
-    SHP_ENTRY(shp_kv_store), SHP_ENTRY(shp_kv_load), SHP_ENTRY(shp_attn_kv), { "shp_attn_kv_work", &run_attn_work },
+    SHP_ENTRY(shp_kv_store), SHP_ENTRY(shp_kv_load), SHP_ENTRY(shp_attn_kv), SHP_WORK(shp_attn_kv_work),
+    SHP_WORK(shp_kv_pages_work), SHP_ENTRY(shp_kv_pages), SHP_ENTRY(shp_kv_slots), SHP_ENTRY(shp_kv_store_pages),
+    SHP_ENTRY(shp_kv_load_pages),
 };
 
 struct Bound {

@@ -24,7 +24,7 @@ LIB_PATH = os.environ.get("SHP_LIB") or os.path.join(HERE, "libsynth_hip.so")
 BIND_PATH = os.path.join(HERE, "shp_bind.so")
 
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_BACKEND = 0, 1, 2, 17
-TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q5_K, TYPE_I32, TYPE_BF16 = 0, 1, 2, 8, 13, 26, 30
+TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q5_K, TYPE_I8, TYPE_I32, TYPE_BF16 = 0, 1, 2, 8, 13, 24, 26, 30
 ROPE_TYPE_NEOX = 2
 Q8_0_BLOCK_BYTES, Q8_0_BLOCK_ELEMS = 34, 32
 Q5_K_BLOCK_BYTES, Q5_K_BLOCK_ELEMS = 176, 256
@@ -128,6 +128,11 @@ def load(path=None):
         "shp_kv_load": [_PT, _PT, _PT, _PT, _PT, _PT, vp],
         "shp_attn_kv": [_PT, _PT, _PT, _PT, _PT, f, i32, i32, _PT, _PT, vp],
         "shp_attn_kv_work": [_PT, _PT, i32, i32, ctypes.POINTER(i64)],
+        "shp_kv_pages_work": [_PT, ctypes.POINTER(i64)],
+        "shp_kv_pages": [_PT, i32, _PT, _PT, _PT, _PT, _PT, _PT, vp],
+        "shp_kv_slots": [_PT, _PT, _PT, i32, _PT, vp],
+        "shp_kv_store_pages": [_PT, _PT, _PT, _PT, _PT, _PT, _PT, _PT, _PT, _PT, vp],
+        "shp_kv_load_pages": [_PT, _PT, _PT, _PT, _PT, _PT, _PT, vp],
         "shp_graph_compute": [ctypes.POINTER(ShpNode), i32, vp],
         "shp_graph_plan": [ctypes.POINTER(ShpNode), i32, ctypes.POINTER(ShpGraphRun), i32, ctypes.POINTER(i32)],
     }
@@ -205,6 +210,28 @@ class Q5KTensor(BlockTensor):
 class Q4Tensor(BlockTensor):
     """Q4_0: 32-element blocks {f16 d; uint8 qs[16]}; a KV cache (kv_store, kv_load, attn_kv)."""
     TYPE, ELEMS, BYTES = TYPE_Q4_0, Q4_0_BLOCK_ELEMS, Q4_0_BLOCK_BYTES
+
+
+class PagedCache:
+    """The pool of a paged KV cache (kv_store_pages, kv_load_pages, attn_pages):
+    int8 codes under one F32 scale for each page and head. k (pages, kv_heads, page,
+    head_dim) and v (pages, kv_heads, head_dim, page) int8; k_scale and v_scale
+    (pages, kv_heads) F32."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+
+    @classmethod
+    def empty(cls, pages, page, kv_heads, head_dim, device="cuda"):
+        """A pool of `pages` pages of `page` positions, all of its values zero."""
+        import torch
+        return cls(torch.zeros(pages, kv_heads, page, head_dim, dtype=torch.int8, device=device),
+                   torch.zeros(pages, kv_heads, head_dim, page, dtype=torch.int8, device=device),
+                   torch.zeros(pages, kv_heads, device=device), torch.zeros(pages, kv_heads, device=device))
+
+    @property
+    def page(self):
+        return self.k.shape[-2]
 
 
 _bind = None
@@ -445,6 +472,61 @@ def attn_kv(q, k_cache, v_cache, length=None, count=None, scale=None, window=0, 
                               float(q.shape[-1] ** -0.5 if scale is None else scale), int(window), int(sinks), work,
                               out, _stream()), "attn_kv")
     return out
+
+
+def kv_pages_work(table):
+    """The int32 elements of workspace that kv_pages needs for a table (0: none)."""
+    n = _fn("shp_kv_pages_work")(table)
+    if n < 0:
+        raise ShpError(-n, "kv_pages_work")
+    return n
+
+
+def kv_pages(length, page, held, free, left, table, status=None, work=None):
+    """Makes the tables of a paged KV cache fit new lengths, in place: sequence n
+    is to have pages for length[n] rows and has held[n] (int32 (N,)). Pages past
+    that go back on the stack free[:left] (int32 (pages,), (1,)), missing ones are
+    taken from it; table is int32 (N, max_pages), -1 where there is no page. Where
+    the stack has too few, or a length does not fit the table, nothing is changed
+    and `status` (int32, one element) is set to 1. work: int32 of
+    kv_pages_work()'s elements, allocated here unless given."""
+    if work is None:
+        n = kv_pages_work(table)
+        work = table.new_empty(n) if n else None
+    _check(_fn("shp_kv_pages")(length, int(page), held, free, left, table, work, status, _stream()), "kv_pages")
+
+
+def kv_slots(table, length, page, t, count=None, out=None):
+    """Where the t newest rows of each sequence lie in a paged KV cache, count[n]
+    of them: int32 (N, t), page number * page + row in the page, and -1 past
+    count[n] and where the table has no page."""
+    out = table.new_empty((table.shape[0], int(t))) if out is None else out
+    _check(_fn("shp_kv_slots")(table, length, count, int(page), out, _stream()), "kv_slots")
+    return out
+
+
+def kv_store_pages(k, v, cache, table, length, count=None, status=None):
+    """New rows into a paged KV cache: k, v (N, T, kv_heads, head_dim) F32; row t <
+    count[n] (all T without count) of sequence n becomes its row length[n] -
+    count[n] + t, in the page that table[n] (int32 (N, max_pages)) names. A block's
+    scale grows with what it gets, and the codes of its rows in front with it. A
+    sequence whose rows do not fit is not written, and `status` (int32, one element)
+    is then set to 1."""
+    _check(_fn("shp_kv_store_pages")(k, v, table, length, count, cache.k, cache.v, cache.k_scale, cache.v_scale, status,
+                                     _stream()), "kv_store_pages")
+
+
+def kv_load_pages(cache, slots, k_out=None, v_out=None):
+    """Rows of a paged KV cache as F32 by their slots (int32 (N, T), as kv_slots
+    gives them): (k, v), each (N, T, kv_heads, head_dim), or k_out and v_out. A row
+    of slot -1 is not written, one outside the pool is NaN."""
+    if k_out is None or v_out is None:
+        shape = tuple(slots.shape) + (cache.k.shape[-3], cache.k.shape[-1])
+        k_out = _empty_like_f32(shape, cache.k.device) if k_out is None else k_out
+        v_out = _empty_like_f32(shape, cache.k.device) if v_out is None else v_out
+    _check(_fn("shp_kv_load_pages")(cache.k, cache.v, cache.k_scale, cache.v_scale, slots, k_out, v_out, _stream()),
+           "kv_load_pages")
+    return k_out, v_out
 
 
 def exp(x, out=None):
