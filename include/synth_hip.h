@@ -903,6 +903,41 @@ shp_status_t shp_kv_load_pages(const shp_tensor * k_pages,
                                shp_stream_t       stream);
 
 /*
+ * shp_attn_kv over a paged cache: the same queries, positions, window, first rows
+ * and results, with length and table in place of the caches' rows (a length is
+ * clamped to what the table holds). Rows of a page outside the pool are NaN, to
+ * the queries that see them. A block is NaN as a whole, so it makes
+ * every query NaN that sees a row of it.
+ *
+ * Precision: codes are exact; q and products as in shp_attn_kv. Of weight times V's
+ * scale 2^-22 of itself or 2^-38 of the query's largest is lost. Scales may be up
+ * to 2^120, so that values are within f32's range.
+ *
+ * work as in shp_attn_kv, of shp_attn_pages_work's size for the same q, k_pages, table,
+ * window and sinks.
+ */
+shp_status_t shp_attn_pages_work(const shp_tensor * q,
+                                 const shp_tensor * k_pages,
+                                 const shp_tensor * table,
+                                 int32_t            window,
+                                 int32_t            sinks,
+                                 int64_t *          floats);
+shp_status_t shp_attn_pages(const shp_tensor * q,
+                            const shp_tensor * k_pages,
+                            const shp_tensor * v_pages,
+                            const shp_tensor * k_scale,
+                            const shp_tensor * v_scale,
+                            const shp_tensor * table,
+                            const shp_tensor * length,
+                            const shp_tensor * count,
+                            float              scale,
+                            int32_t            window,
+                            int32_t            sinks,
+                            shp_tensor *       work,
+                            shp_tensor *       y,
+                            shp_stream_t       stream);
+
+/*
  * ggml_exp: y = expf(x) per element, F32 of one shape
  * (src/arch/qwen3-tts/codec.cpp:193-194, vits/latent-sampling.cpp:30).
  */

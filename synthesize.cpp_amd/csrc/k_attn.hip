@@ -260,6 +260,51 @@ int64_t wide_groups(int64_t hd) {
     return hd <= 4 * kKvBlock ? 512 : 256;
 }
 
+}  // namespace
+
+// `rows` query rows of each of `pairs` (kv head, sequence), of T positions, over
+// `keys` of `cap` rows, for a chip that holds `chip` workgroups.
+void plan_spans(int64_t rows, int64_t T, int64_t cap, int64_t keys, int64_t pairs, int64_t chip, AttnPlan & p) {
+    // Splits of equally many key tiles for all rows, however many a row has,
+    // as short as lets the chip hold all of them at once: 2048 positions of
+    // 16 heads take 81 us, and 99 with every row in thirds (Q4_0, 8 kv heads,
+    // MI355X). Where the row tiles alone are more than half of what it holds,
+    // long rows are halved (2560 positions: 123 us, whole rows 169), and from
+    // three quarters on all are left whole (3584 positions: 234 us, halves 264).
+    const int64_t tiles = (rows + kWideRows - 1) / kWideRows;
+    const int64_t most  = (keys + kTileKeys - 1) / kTileKeys + (p.window > 0 ? 2 : 0);
+    int64_t       span  = (most + kMaxSplits - 1) / kMaxSplits;
+    span                = span > kWideSpan ? span : kWideSpan;
+    if (tiles * pairs > chip * 3 / 4) {
+        span = most;
+    } else if (tiles * pairs > chip / 2) {
+        span = span > (most + 1) / 2 ? span : (most + 1) / 2;
+    } else {
+        auto fits = [&](int64_t of) {
+            int64_t groups = 0;
+            for (int64_t t = 0; t < tiles && groups <= chip; ++t) {
+                // of a whole cache, and within a window all alike
+                const int64_t end = cap - T + ((t + 1) * kWideRows * T + rows - 1) / rows;
+                const int64_t n   = ((end < cap ? end : cap) + kTileKeys - 1) / kTileKeys;
+                groups += ((n < most ? n : most) + of - 1) / of * pairs;
+            }
+            return groups <= chip;
+        };
+        for (int64_t upto = most; span < upto;) {  // the shortest that fits
+            const int64_t mid = (span + upto) / 2;
+            if (fits(mid)) {
+                upto = mid;
+            } else {
+                span = mid + 1;
+            }
+        }
+    }
+    p.span   = static_cast<int32_t>(span < most ? span : most);
+    p.nsplit = static_cast<int32_t>((most + p.span - 1) / p.span);
+}
+
+namespace {
+
 shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t window, int32_t sinks, AttnPlan & p) {
     if (!well_formed(q) || !kv_well_formed(k_cache) || q->ne[0] != k_cache->ne[0] || q->ne[1] % k_cache->ne[1] != 0 ||
         q->ne[3] != k_cache->ne[3] || window < 0 || sinks < 0) {
@@ -318,49 +363,14 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
     }
     p.wide = !p.few && wide_takes(*k_cache);
     if (p.wide) {
-        // Splits of equally many key tiles for all rows, however many a row has,
-        // as short as lets the chip hold all of them at once: 2048 positions of
-        // 16 heads take 81 us, and 99 with every row in thirds (Q4_0, 8 kv heads,
-        // MI355X). Where the row tiles alone are more than half of what it holds,
-        // long rows are halved (2560 positions: 123 us, whole rows 169), and from
-        // three quarters on all are left whole (3584 positions: 234 us, halves 264).
-        const int64_t chip  = wide_groups(q->ne[0]);
-        const int64_t tiles = (rows + kWideRows - 1) / kWideRows;
-        const int64_t most  = (keys + kTileKeys - 1) / kTileKeys + (p.window > 0 ? 2 : 0);
-        const int64_t pairs = kv * q->ne[3];
-        int64_t       span  = (most + kMaxSplits - 1) / kMaxSplits;
-        span                = span > kWideSpan ? span : kWideSpan;
-        if (tiles * pairs > chip * 3 / 4) {
-            span = most;
-        } else if (tiles * pairs > chip / 2) {
-            span = span > (most + 1) / 2 ? span : (most + 1) / 2;
-        } else {
-            auto fits = [&](int64_t of) {
-                int64_t groups = 0;
-                for (int64_t t = 0; t < tiles && groups <= chip; ++t) {
-                    // of a whole cache, and within a window all alike
-                    const int64_t end = cap - T + ((t + 1) * kWideRows * T + rows - 1) / rows;
-                    const int64_t n   = ((end < cap ? end : cap) + kTileKeys - 1) / kTileKeys;
-                    groups += ((n < most ? n : most) + of - 1) / of * pairs;
-                }
-                return groups <= chip;
-            };
-            for (int64_t upto = most; span < upto;) {  // the shortest that fits
-                const int64_t mid = (span + upto) / 2;
-                if (fits(mid)) {
-                    upto = mid;
-                } else {
-                    span = mid + 1;
-                }
-            }
-        }
-        p.span   = static_cast<int32_t>(span < most ? span : most);
-        p.nsplit = static_cast<int32_t>((most + p.span - 1) / p.span);
+        plan_spans(rows, T, cap, keys, kv * q->ne[3], wide_groups(q->ne[0]), p);
     } else if (!p.few) {
         p.nsplit = plan_splits(tiles16 * kv * q->ne[3], (keys + 63) / 64, 2048);
     }
     return SHP_OK;
 }
+
+}  // namespace
 
 int64_t plan_floats(const AttnPlan & p, const shp_tensor & q) {
     const int64_t row = (q.ne[0] + 3) / 4 * 4 + 2;
@@ -369,6 +379,8 @@ int64_t plan_floats(const AttnPlan & p, const shp_tensor & q) {
     }
     return p.nsplit == 1 ? 0 : q.ne[1] * q.ne[2] * q.ne[3] * p.nsplit * row;
 }
+
+namespace {
 
 template <int KIND> shp_status_t launch_any(const AttnArgs & a, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(a.tiles) * static_cast<unsigned>(a.nsplit), static_cast<unsigned>(a.KV),
@@ -382,6 +394,8 @@ template <int KIND> shp_status_t launch_any(const AttnArgs & a, hipStream_t stre
     }
     return launch_status();
 }
+
+}  // namespace
 
 shp_status_t launch_join(const AttnArgs & a, hipStream_t stream) {
     const int64_t rows = static_cast<int64_t>(a.N) * a.KV * a.T * a.G;
@@ -403,7 +417,71 @@ shp_status_t launch_join(const AttnArgs & a, hipStream_t stream) {
     return a.hd <= 64 ? go(k_attn_join<64>) : a.hd <= 128 ? go(k_attn_join<128>) : go(k_attn_join<256>);
 }
 
-}  // namespace
+// The checks that shp_attn_kv and shp_attn_pages share once a call is planned, and
+// the arguments but for the cache's; `read`: what y and work may not overlap, beside q.
+shp_status_t attn_args(const shp_tensor *         q,
+                       const shp_tensor *         length,
+                       const shp_tensor *         count,
+                       float                      scale,
+                       const AttnPlan &           p,
+                       const shp_tensor * const * read,
+                       int                        n_read,
+                       const shp_tensor *         work,
+                       const shp_tensor *         y,
+                       AttnArgs &                 a) {
+    // exp(x) = exp2(x log2 e)
+    const float scale2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+    if (!well_formed(y) || !same_shape(*q, *y) || (length != nullptr && !kv_numbers(length, q->ne[3])) ||
+        (count != nullptr && !kv_numbers(count, q->ne[3])) || !(fabsf(scale2) < INFINITY)) {
+        return SHP_ERR_INVALID_ARG;
+    }
+    const int64_t floats = plan_floats(p, *q);
+    if (floats > 0 && (!well_formed(work) || work->type != SHP_TYPE_F32 || !contiguous(*work) || nelements(*work) < floats)) {
+        return SHP_ERR_INVALID_ARG;
+    }
+    if (y->type != SHP_TYPE_F32 || !kv_aligned(*q) || !kv_aligned(*y) || !kv_addressable(*y) || !kv_rows_apart(*y) ||
+        (length != nullptr && !i32_aligned(*length)) || (count != nullptr && !i32_aligned(*count)) ||
+        (floats > 0 && !rows_aligned(*work, 16))) {
+        return SHP_ERR_UNSUPPORTED;
+    }
+    for (int i = -2; i < n_read; ++i) {
+        const shp_tensor * t = i == -2 ? q : i == -1 ? (floats > 0 ? work : nullptr) : read[i];
+        if (t != nullptr && (kv_overlap(*y, *t) || (floats > 0 && t != work && kv_overlap(*work, *t)))) {
+            return SHP_ERR_UNSUPPORTED;
+        }
+    }
+    auto nb  = [](const shp_tensor & t, int d) { return static_cast<int64_t>(t.ne[d] > 1 ? t.nb[d] : 0); };
+    a.q      = static_cast<const char *>(q->data);
+    a.y      = static_cast<char *>(y->data);
+    a.length = length != nullptr ? static_cast<const int32_t *>(length->data) : nullptr;
+    a.count  = count != nullptr ? static_cast<const int32_t *>(count->data) : nullptr;
+    a.work   = floats > 0 ? static_cast<float *>(work->data) : nullptr;
+    a.qh = nb(*q, 1), a.qt = nb(*q, 2), a.qn = nb(*q, 3);
+    a.yh = nb(*y, 1), a.yt = nb(*y, 2), a.yn = nb(*y, 3);
+    a.scale  = scale2;
+    a.window = p.window;
+    a.sinks  = p.sinks;
+    a.T      = static_cast<int32_t>(q->ne[2]);
+    a.N      = static_cast<int32_t>(q->ne[3]);
+    a.hd     = static_cast<int32_t>(q->ne[0]);
+    a.hd4    = (a.hd + 3) / 4 * 4;
+    a.nsplit = p.nsplit;
+    a.fsplit = make_fastdiv(static_cast<uint32_t>(a.nsplit > 0 ? a.nsplit : 1));
+    return SHP_OK;
+}
+
+// Row tiles of kWideRows for a chip that holds `chip` workgroups, `per` key tiles a split.
+void wide_args(int32_t per, int64_t chip, AttnArgs & a) {
+    a.tiles              = static_cast<int32_t>((static_cast<int64_t>(a.T) * a.G + kWideRows - 1) / kWideRows);
+    a.per                = per;
+    a.fper               = make_fastdiv(static_cast<uint32_t>(a.per));
+    const int64_t groups = static_cast<int64_t>(a.tiles) * a.KV;
+    // with all of them on the chip, two to a CU, a long row tile's neighbour is a
+    // short one (4096 positions: 274 us, with the longest first throughout 287)
+    const bool twos = a.nsplit == 1 && a.N == 1 && groups > chip / 2 && groups <= chip;
+    a.half          = twos ? static_cast<int32_t>((chip / 2 + a.KV - 1) / a.KV) : a.tiles;
+}
+
 }  // namespace shp
 
 using namespace shp;
@@ -443,58 +521,23 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
     if (st != SHP_OK) {
         return st;
     }
-    // exp(x) = exp2(x log2 e)
-    const float scale2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
-    if (!well_formed(y) || !same_shape(*q, *y) || (length != nullptr && !kv_numbers(length, q->ne[3])) ||
-        (count != nullptr && !kv_numbers(count, q->ne[3])) || !(fabsf(scale2) < INFINITY)) {
-        return SHP_ERR_INVALID_ARG;
-    }
-    const int64_t floats = plan_floats(p, *q);
-    if (floats > 0 && (!well_formed(work) || work->type != SHP_TYPE_F32 || !contiguous(*work) || nelements(*work) < floats)) {
-        return SHP_ERR_INVALID_ARG;
-    }
-    if (y->type != SHP_TYPE_F32 || !kv_aligned(*q) || !kv_aligned(*y) || !kv_addressable(*y) || !kv_rows_apart(*y) ||
-        (length != nullptr && !i32_aligned(*length)) || (count != nullptr && !i32_aligned(*count)) ||
-        (floats > 0 && !rows_aligned(*work, 16))) {
-        return SHP_ERR_UNSUPPORTED;
-    }
-    const shp_tensor * others[6] = { q, k_cache, v_cache, length, count, floats > 0 ? work : nullptr };
-    for (const shp_tensor * t : others) {
-        if (t != nullptr && (kv_overlap(*y, *t) || (floats > 0 && t != work && kv_overlap(*work, *t)))) {
-            return SHP_ERR_UNSUPPORTED;
-        }
-    }
-    if (dry_run()) {
-        return SHP_OK;
+    AttnArgs           a{};
+    const shp_tensor * read[4] = { k_cache, v_cache, length, count };
+    st                         = attn_args(q, length, count, scale, p, read, 4, work, y, a);
+    if (st != SHP_OK || dry_run()) {
+        return st;
     }
     auto nb = [](const shp_tensor & t, int d) { return static_cast<int64_t>(t.ne[d] > 1 ? t.nb[d] : 0); };
-    AttnArgs a{};
-    a.q      = static_cast<const char *>(q->data);
-    a.k      = static_cast<const char *>(k_cache->data);
-    a.v      = static_cast<const char *>(v_cache->data);
-    a.y      = static_cast<char *>(y->data);
-    a.length = length != nullptr ? static_cast<const int32_t *>(length->data) : nullptr;
-    a.count  = count != nullptr ? static_cast<const int32_t *>(count->data) : nullptr;
-    a.work   = floats > 0 ? static_cast<float *>(work->data) : nullptr;
-    a.qh = nb(*q, 1), a.qt = nb(*q, 2), a.qn = nb(*q, 3);
+    a.k     = static_cast<const char *>(k_cache->data);
+    a.v     = static_cast<const char *>(v_cache->data);
     a.kh = nb(*k_cache, 1), a.kt = nb(*k_cache, 2), a.kn = nb(*k_cache, 3);
     a.vh = nb(*v_cache, 1), a.vt = nb(*v_cache, 2), a.vn = nb(*v_cache, 3);
-    a.yh = nb(*y, 1), a.yt = nb(*y, 2), a.yn = nb(*y, 3);
-    a.scale  = scale2;
-    a.window = p.window;
-    a.sinks  = p.sinks;
-    a.T      = static_cast<int32_t>(q->ne[2]);
-    a.KV     = static_cast<int32_t>(k_cache->ne[1]);
-    a.G      = static_cast<int32_t>(q->ne[1] / k_cache->ne[1]);
-    a.N      = static_cast<int32_t>(q->ne[3]);
-    a.hd     = static_cast<int32_t>(q->ne[0]);
-    a.hd4    = (a.hd + 3) / 4 * 4;
-    a.cap    = static_cast<int32_t>(k_cache->ne[2]);
-    a.nsplit = p.nsplit;  // (as the workspace has them, whichever kernel it is)
-    a.tiles  = static_cast<int32_t>((static_cast<int64_t>(a.T) * a.G + 15) / 16);
-    a.fG     = make_fastdiv(static_cast<uint32_t>(a.G));
-    a.fsplit = make_fastdiv(static_cast<uint32_t>(a.nsplit));
-    a.fKV    = make_fastdiv(static_cast<uint32_t>(a.KV));
+    a.KV    = static_cast<int32_t>(k_cache->ne[1]);
+    a.G     = static_cast<int32_t>(q->ne[1] / k_cache->ne[1]);
+    a.cap   = static_cast<int32_t>(k_cache->ne[2]);
+    a.tiles = static_cast<int32_t>((static_cast<int64_t>(a.T) * a.G + 15) / 16);
+    a.fG    = make_fastdiv(static_cast<uint32_t>(a.G));
+    a.fKV   = make_fastdiv(static_cast<uint32_t>(a.KV));
     const hipStream_t s     = as_stream(stream);
     const int         kind  = kv_kind(k_cache->type);
     int32_t           run   = 0;
@@ -503,19 +546,12 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
         return launch_attn_few(kind, a, p, piece, run, s);
     }
     if (wide_takes(*k_cache) && wide_takes(*v_cache)) {
-        a.tiles = static_cast<int32_t>((static_cast<int64_t>(a.T) * a.G + kWideRows - 1) / kWideRows);
-        a.per   = p.span;
+        int32_t per = p.span;
         if (!p.wide) {  // in place of k_attn_few: splits as its workspace has room for
             const int64_t most = (a.cap + kTileKeys - 1) / kTileKeys + 2;
-            a.per              = static_cast<int32_t>((most + a.nsplit - 1) / a.nsplit);
+            per                = static_cast<int32_t>((most + a.nsplit - 1) / a.nsplit);
         }
-        a.fper = make_fastdiv(static_cast<uint32_t>(a.per));
-        const int64_t chip   = wide_groups(a.hd);
-        const int64_t groups = static_cast<int64_t>(a.tiles) * a.KV;
-        // with all of them on the chip, two to a CU, a long row tile's neighbour is a
-        // short one (4096 positions: 274 us, with the longest first throughout 287)
-        const bool    twos   = a.nsplit == 1 && a.N == 1 && groups > chip / 2 && groups <= chip;
-        a.half               = twos ? static_cast<int32_t>((chip / 2 + a.KV - 1) / a.KV) : a.tiles;
+        wide_args(per, wide_groups(a.hd), a);
         st = launch_attn_wide(kind, a, s);
         return st == SHP_OK && a.nsplit > 1 ? launch_join(a, s) : st;
     }

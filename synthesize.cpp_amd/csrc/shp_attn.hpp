@@ -448,6 +448,174 @@ __device__ __forceinline__ float * out_of(const AttnArgs & a, const RowOf & r) {
 }
 
 // ---------------------------------------------------------------------------
+// Few queries: what k_attn_few.hip and k_attn_pages.hip share.
+// ---------------------------------------------------------------------------
+
+struct FewArgs {
+    AttnArgs a;
+    int32_t  hgs;      // log2 of HG
+    int32_t  shift;    // log2 of the keys of a chunk
+    int32_t  cols;     // queries of a kv head: T x G
+    int32_t  nb;       // 32-value blocks of a row
+    int32_t  pieces;   // of a chunk
+    int32_t  run;      // pieces of a key's HG rows where keys are apart, 0 where a chunk is one run
+    FastDiv  frun;
+    FastDiv  fcols;
+    int32_t  wave_lds;
+    int32_t  groups;   // of HG heads
+    int32_t  wgs;      // workgroups that share the work
+    FastDiv  fwgs;
+    int32_t  per;      // chunks of a unit
+    FastDiv  fper;
+};
+
+// How the work is dealt out. A sequence's chunks make units of one chunk or a
+// few for each of a workgroup's waves; sequence after sequence, head group after head
+// group, the units of the call stand in one line, of which every workgroup
+// takes an equal stretch. So lengths may differ as they like (64 streams of 512
+// to 8192 rows, MI355X: 113 us, 169 with an equal number of workgroups for each
+// sequence). A stretch that ends inside a group leaves a partial result; a
+// workgroup has two at most, of the group that it begins in and did not begin
+// (0), and of the one that it began and did not end (1).
+__device__ __forceinline__ float * few_o(const FewArgs & f, int wg, int which, int col) {
+    return f.a.work + (static_cast<int64_t>(wg * 2 + which) * kCols + col) * f.a.hd4;
+}
+
+__device__ __forceinline__ float * few_ml(const FewArgs & f, int wg, int which, int col) {
+    return f.a.work + static_cast<int64_t>(f.wgs) * 2 * kCols * f.a.hd4 + ((wg * 2 + which) * kCols + col) * 2;
+}
+
+// The first and last workgroup of a head group.
+__device__ __forceinline__ int32_t * few_span(const FewArgs & f, int64_t group) {
+    return reinterpret_cast<int32_t *>(few_ml(f, f.wgs, 0, 0)) + 2 * group;
+}
+
+// A sequence's key chunks; `len` as seq_lens gives it.
+__device__ __forceinline__ KeyTiles few_tiles(const FewArgs & f, const SeqLens & len) {
+    const AttnArgs & a     = f.a;
+    const int        shift = f.shift;
+    const int32_t    base  = len.length - len.count;
+    const int32_t    p1    = len.length - 1;
+    KeyTiles         kt{ 0, 0, 0 };
+    if (p1 >= 0) {
+        if (a.window > 0) {
+            kt.second = max(base - a.window + 1, 0) >> shift;
+            kt.first  = min((min(a.sinks, p1 + 1) + (1 << shift) - 1) >> shift, kt.second);
+        }
+        kt.n = kt.first + (p1 >> shift) - kt.second + 1;
+    }
+    return kt;
+}
+
+// Units of sequence n and head group: at least one where it has a query, which
+// then writes its zeros.
+__device__ __forceinline__ int few_units(const FewArgs & f, int n) {
+    const SeqLens len = seq_lens(f.a, n);
+    return len.count == 0 ? 0 : max(static_cast<int>(fastdiv(static_cast<uint32_t>(few_tiles(f, len).n + f.per - 1), f.fper)), 1);
+}
+
+// The sum of a wave's lanes up to and with this one.
+__device__ __forceinline__ int32_t sum_up_to(int32_t v) {
+    auto below = [](int32_t x, auto ctrl, auto rows) {
+        return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+    };
+    using All = std::integral_constant<int, 0xF>;
+    v += below(v, std::integral_constant<int, 0x111>{}, All{});  // row_shr:1, 2, 4, 8
+    v += below(v, std::integral_constant<int, 0x112>{}, All{});
+    v += below(v, std::integral_constant<int, 0x114>{}, All{});
+    v += below(v, std::integral_constant<int, 0x118>{}, All{});
+    v += below(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15
+    v += below(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31
+    return v;
+}
+
+// The sequence that a unit of the line falls in.
+struct Place {
+    int32_t n;
+    int32_t units;   // of one head group of it
+    int32_t before;  // of all head groups of the sequences before it
+};
+
+// The line's units of all head groups, and where workgroup wg's stretch begins
+// in it, for a whole wave: 64 sequences at a time, a sum over lanes.
+struct Line {
+    int32_t total;
+    int32_t begin;
+    int32_t end;
+    Place   at;  // of begin, if the stretch is not empty
+};
+
+__device__ __forceinline__ int32_t few_start(const FewArgs & f, int32_t total, int32_t wg);
+
+__device__ __forceinline__ Line few_line(const FewArgs & f, int wg, int lane) {
+    Line s{};
+    if (f.a.N == 1) {
+        const int units = few_units(f, 0);
+        s.total         = units * f.groups;
+        s.at            = Place{ 0, units, 0 };
+    } else {
+        auto units_of = [&](int first) { return first + lane < f.a.N ? few_units(f, first + lane) : 0; };
+        int  units    = units_of(0);
+        int  sum      = sum_up_to(units);
+        s.total       = __builtin_amdgcn_readlane(sum, kWave - 1);
+        for (int first = kWave; first < f.a.N; first += kWave) {
+            s.total += __builtin_amdgcn_readlane(sum_up_to(units_of(first)), kWave - 1);
+        }
+        s.total *= f.groups;
+        const int32_t unit   = few_start(f, s.total, wg);
+        int32_t       before = 0;
+        for (int first = 0; first < f.a.N; first += kWave) {
+            if (first > 0) {
+                units = units_of(first);
+                sum   = sum_up_to(units);
+            }
+            const uint64_t past = __ballot(before + sum * f.groups > unit);
+            if (past != 0) {
+                const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+                const int k = __builtin_amdgcn_readlane(units, l);
+                s.at        = Place{ first + l, k, before + (__builtin_amdgcn_readlane(sum, l) - k) * f.groups };
+                break;
+            }
+            before += __builtin_amdgcn_readlane(sum, kWave - 1) * f.groups;
+        }
+    }
+    s.begin = few_start(f, s.total, wg);
+    s.end   = few_start(f, s.total, wg + 1);
+    return s;
+}
+
+// Where workgroup wg's stretch of `total` units begins, and whose unit u is.
+__device__ __forceinline__ int32_t few_start(const FewArgs & f, int32_t total, int32_t wg) {
+    const int32_t each = static_cast<int32_t>(fastdiv(static_cast<uint32_t>(total), f.fwgs));
+    return each * wg + min(wg, total - each * f.wgs);
+}
+
+__device__ __forceinline__ int32_t few_owner(const FewArgs & f, int32_t total, int32_t u) {
+    const int32_t each = static_cast<int32_t>(fastdiv(static_cast<uint32_t>(total), f.fwgs));
+    const int32_t more = total - each * f.wgs;  // workgroups with one more
+    return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each;
+}
+
+// One row's parts, by a workgroup.
+template <int HD> __device__ __forceinline__ void join_few(const FewArgs & f, int64_t row) {
+    const AttnArgs & a   = f.a;
+    const RowOf      r   = row_of(a, row);
+    const SeqLens    len = seq_lens(a, r.n);
+    if (r.t >= len.count) {
+        return;
+    }
+    const int32_t * span = few_span(f, static_cast<int64_t>(r.n) * f.groups + (r.h >> f.hgs));
+    const int32_t   w0   = span[0];
+    const int32_t   w1   = span[1];
+    if (w0 == w1) {
+        return;  // whole already
+    }
+    const int col = (r.h & ((1 << f.hgs) - 1)) * f.cols + r.t * a.G + r.gq;
+    join_parts<HD>(w1 - w0 + 1, a.hd, [&](int s) { return few_ml(f, w0 + s, s == 0, col); },
+                   [&](int s) { return few_o(f, w0 + s, s == 0, col); }, out_of(a, r), len.length - len.count + r.t >= 0);
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 
@@ -484,6 +652,15 @@ constexpr int few_resident(int kind, int64_t hd) {
 // size in which it can read both caches, or 0; and its launches, join included.
 int          few_piece(const shp_tensor & k, const shp_tensor & v, int hgs, int32_t & run);
 shp_status_t launch_attn_few(int kind, const AttnArgs & a, const AttnPlan & p, int piece, int32_t run, hipStream_t stream);
+
+// k_attn.hip: splits of a prompt's keys, the workspace of a plan, what all calls check
+// and pass on, and the launch that joins the splits of k_attn_wide and k_attn_pages_wide.
+void         plan_spans(int64_t rows, int64_t T, int64_t cap, int64_t keys, int64_t pairs, int64_t chip, AttnPlan & p);
+int64_t      plan_floats(const AttnPlan & p, const shp_tensor & q);
+shp_status_t attn_args(const shp_tensor * q, const shp_tensor * length, const shp_tensor * count, float scale, const AttnPlan & p,
+                       const shp_tensor * const * read, int n_read, const shp_tensor * work, const shp_tensor * y, AttnArgs & a);
+void         wide_args(int32_t per, int64_t chip, AttnArgs & a);
+shp_status_t launch_join(const AttnArgs & a, hipStream_t stream);
 
 // k_attn_wide.hip.
 shp_status_t launch_attn_wide(int kind, const AttnArgs & a, hipStream_t stream);

@@ -434,7 +434,7 @@ const Entry kEntries[] = {
     SHP_ENTRY_FIRST(shp_sum_scale_leaky_relu, kArray), { "shp_layer_nongemm_step", &run_layer },
     SHP_ENTRY(shp_kv_store), SHP_ENTRY(shp_kv_load), SHP_ENTRY(shp_attn_kv), SHP_WORK(shp_attn_kv_work),
     SHP_WORK(shp_kv_pages_work), SHP_ENTRY(shp_kv_pages), SHP_ENTRY(shp_kv_slots), SHP_ENTRY(shp_kv_store_pages),
-    SHP_ENTRY(shp_kv_load_pages),
+    SHP_ENTRY(shp_kv_load_pages), SHP_WORK(shp_attn_pages_work), SHP_ENTRY(shp_attn_pages),
 };
 
 struct Bound {

@@ -36,9 +36,9 @@ __device__ __forceinline__ const int32_t * table_of(const Tables & t, int n) {
     return reinterpret_cast<const int32_t *>(t.data + n * t.tn);
 }
 
-// A block's scale as it counts: not finite or negative is NaN.
+// A block's scale as it counts: not finite or negative is NaN (and -0 is 0).
 __device__ __forceinline__ float block_scale(float d) {
-    return d >= 0.0f && d < INFINITY ? d : NAN;
+    return d >= 0.0f && d < INFINITY ? fabsf(d) : NAN;
 }
 
 // ---------------------------------------------------------------------------
@@ -135,7 +135,7 @@ inline bool numbers2_usable(const shp_tensor & t) {
     return i32_aligned(t) && kv_addressable(t);
 }
 
-// Tables of n sequences (any number for n 0) for pages of `page` rows.
+// Tables of n sequences, for pages of `page` rows.
 inline shp_status_t check_table(const shp_tensor * t, int64_t n, int64_t page, Tables & out) {
     if (!numbers2(t, n)) {
         return SHP_ERR_INVALID_ARG;

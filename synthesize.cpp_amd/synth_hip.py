@@ -133,6 +133,8 @@ def load(path=None):
         "shp_kv_slots": [_PT, _PT, _PT, i32, _PT, vp],
         "shp_kv_store_pages": [_PT, _PT, _PT, _PT, _PT, _PT, _PT, _PT, _PT, _PT, vp],
         "shp_kv_load_pages": [_PT, _PT, _PT, _PT, _PT, _PT, _PT, vp],
+        "shp_attn_pages": [_PT, _PT, _PT, _PT, _PT, _PT, _PT, _PT, f, i32, i32, _PT, _PT, vp],
+        "shp_attn_pages_work": [_PT, _PT, _PT, i32, i32, ctypes.POINTER(i64)],
         "shp_graph_compute": [ctypes.POINTER(ShpNode), i32, vp],
         "shp_graph_plan": [ctypes.POINTER(ShpNode), i32, ctypes.POINTER(ShpGraphRun), i32, ctypes.POINTER(i32)],
     }
@@ -527,6 +529,28 @@ def kv_load_pages(cache, slots, k_out=None, v_out=None):
     _check(_fn("shp_kv_load_pages")(cache.k, cache.v, cache.k_scale, cache.v_scale, slots, k_out, v_out, _stream()),
            "kv_load_pages")
     return k_out, v_out
+
+
+def attn_pages_work(q, cache, table, window=0, sinks=0):
+    """The floats of workspace that attn_pages needs for these shapes (0: none)."""
+    n = _fn("shp_attn_pages_work")(q, cache.k, table, int(window), int(sinks))
+    if n < 0:
+        raise ShpError(-n, "attn_pages_work")
+    return n
+
+
+def attn_pages(q, cache, table, length, count=None, scale=None, window=0, sinks=0, out=None, work=None):
+    """attn_kv over a paged cache: q (N, T, heads, head_dim) F32, a PagedCache, table
+    int32 (N, max_pages), length and count int32 (N,); the other arguments and the
+    result as attn_kv's."""
+    out = q.new_empty(q.shape) if out is None else out
+    if work is None:
+        n = attn_pages_work(q, cache, table, window, sinks)
+        work = q.new_empty(n) if n else None
+    _check(_fn("shp_attn_pages")(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, length, count,
+                                 float(q.shape[-1] ** -0.5 if scale is None else scale), int(window), int(sinks), work, out,
+                                 _stream()), "attn_pages")
+    return out
 
 
 def exp(x, out=None):

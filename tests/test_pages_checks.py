@@ -189,3 +189,66 @@ def test_binding_raises(monkeypatch):
         assert e.value.status == status
     with pytest.raises(KeyError):
         S.desc(torch.zeros(3, dtype=torch.uint8))
+
+
+def attend(**over):
+    a = dict(q=mk(F, 64, 8, 1, 3), kp=mk(C, 64, 32, 2, 7), vp=mk(C, 32, 64, 2, 7), ks=mk(F, 2, 7), vs=mk(F, 2, 7), table=mk(I, 90, 3),
+             length=mk(I, 3), count=mk(I, 3), scale=0.125, window=0, sinks=0, work=mk(F, 1 << 22), y=mk(F, 64, 8, 1, 3))
+    a.update(over)
+    return S.load().shp_attn_pages(R(a["q"]), R(a["kp"]), R(a["vp"]), R(a["ks"]), R(a["vs"]), R(a["table"]), R(a["length"]),
+                                   R(a["count"]), a["scale"], a["window"], a["sinks"], R(a["work"]), R(a["y"]), None)
+
+
+def floats(q, kp, table, window=0, sinks=0):
+    n = ctypes.c_int64(-7)
+    st = S.load().shp_attn_pages_work(R(q), R(kp), R(table), window, sinks, ctypes.byref(n))
+    return n.value if st == S.OK else -st
+
+
+def test_attention_refuses():
+    for name in ("q", "kp", "vp", "ks", "vs", "table", "length", "y"):
+        assert attend(**{name: None}) == BAD, name
+    for over in POOLS:
+        assert attend(**over) == BAD, over
+    for over in FAR:
+        assert attend(**over) == NOT_HERE or over.get("kp", mk(C, 64, 32, 2, 7)).ne[0] != 64, over
+    for hd in (72, 272):
+        q = mk(F, hd, 8, 1, 3)
+        assert attend(q=q, y=mk(F, hd, 8, 1, 3), kp=mk(C, hd, 32, 2, 7), vp=mk(C, 32, hd, 2, 7)) == NOT_HERE
+    for shape in ((64, 7, 1, 3), (96, 8, 1, 3)):
+        assert attend(q=mk(F, *shape), y=mk(F, *shape)) == BAD
+    assert attend(q=mk(F, 64, 8, 1, 2), y=mk(F, 64, 8, 1, 2)) == BAD                        # tables of another number of sequences
+    assert attend(y=mk(F, 64, 8, 2, 3)) == BAD and attend(y=mk(S.TYPE_F16, 64, 8, 1, 3)) == NOT_HERE
+    assert attend(q=mk(S.TYPE_BF16, 64, 8, 1, 3)) == NOT_HERE and attend(q=mk(F, 64, 8, 1, 3, at=(1 << 43) + 2)) == NOT_HERE
+    assert attend(window=-1) == BAD and attend(sinks=-1) == BAD
+    for scale in (float("nan"), float("inf"), 3e38):
+        assert attend(scale=scale) == BAD
+    for name, shape in (("table", (90, 2)), ("table", (90, 3, 2)), ("length", (2,)), ("count", (2,))):
+        assert attend(**{name: mk(I, *shape)}) == BAD, name
+    for name, shape in (("table", (90, 3)), ("length", (3,)), ("count", (3,))):
+        assert attend(**{name: mk(F, *shape)}) == BAD, name
+        assert attend(**{name: mk(I, *shape, at=(1 << 43) + 2)}) == NOT_HERE, name
+    assert attend(table=mk(I, (1 << 25) + 1, 3)) == NOT_HERE
+    for name, shape in (("q", (F, 64, 8, 1, 3)), ("kp", (C, 64, 32, 2, 7)), ("vp", (C, 32, 64, 2, 7)), ("ks", (F, 2, 7)), ("vs", (F, 2, 7)),
+                        ("table", (I, 90, 3)), ("length", (I, 3)), ("count", (I, 3))):
+        first = mk(*shape)
+        assert attend(**{name: first, "y": mk(F, 64, 8, 1, 3, at=first.data)}) == NOT_HERE, name
+        assert attend(**{name: first, "work": mk(F, 1 << 22, at=first.data)}) == NOT_HERE, name
+    y = mk(F, 64, 8, 1, 3)
+    assert attend(work=mk(F, 1 << 22, at=y.data), y=y) == NOT_HERE
+    flat = mk(F, 64, 8, 1, 3)
+    flat.nb[1] = 0
+    assert attend(y=flat) == NOT_HERE
+
+
+def test_workspace_of_the_attention():
+    q, kp, table = mk(F, 64, 8, 1, 3), mk(C, 64, 32, 2, 7), mk(I, 90, 3)
+    need = floats(q, kp, table)
+    assert need > 0
+    assert attend(work=None) == BAD and attend(work=mk(F, need - 1)) == BAD and attend(work=mk(S.TYPE_F16, need)) == BAD
+    assert attend(work=mk(F, need, at=(1 << 43) + 4)) == NOT_HERE
+    assert floats(q, kp, mk(I, 2, 3)) == 0 and floats(q, kp, table, window=30, sinks=4) == 0
+    assert floats(mk(F, 64, 8, 9000, 3), kp, mk(I, 290, 3)) == 0                            # enough queries
+    assert floats(mk(F, 64, 7, 1, 3), kp, table) == -BAD and floats(q, kp, mk(I, 90, 2)) == -BAD
+    assert floats(q, kp, table, window=-1) == -BAD and floats(mk(S.TYPE_F16, 64, 8, 1, 3), kp, table) == -NOT_HERE
+    assert S.load().shp_attn_pages_work(R(q), R(kp), R(table), 0, 0, None) == BAD
