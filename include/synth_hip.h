@@ -803,6 +803,31 @@ shp_status_t shp_attn_kv(const shp_tensor * q,
                          shp_stream_t       stream);
 
 /*
+ * Attention of every query to every row of another sequence: a decoder's cross
+ * attention to the states of an encoder, and, with q, k and v of one sequence, the
+ * attention of an encoder that looks both ways. k, v [head_dim, kv_heads,
+ * rows, N] as a KV cache of shp_attn_kv, in any of its types and layouts (N may be repeated
+ * by a stride of 0: one text for all sequences); q, y F32 [head_dim, heads, T, N].
+ * length[n] (all rows without a length; clamped to [0, rows]) counts the rows
+ * that sequence n has, count[n] (T without a count; clamped to [0, T]) its queries:
+ *   y = sum_j softmax_j(scale * q.k_j) v_j over j < length[n]; 0 where that is 0
+ * for t < count[n]; queries t >= count[n] are left as they were. The ggml node run
+ * of src/arch/qwen3-tts/operations.cpp:123-140 without a mask. Everything
+ * else, precision and workspace among it, is as shp_attn_kv's; work is of
+ * shp_attn_cross_work's size for the same q and k.
+ */
+shp_status_t shp_attn_cross_work(const shp_tensor * q, const shp_tensor * k, int64_t * floats);
+shp_status_t shp_attn_cross(const shp_tensor * q,
+                            const shp_tensor * k,
+                            const shp_tensor * v,
+                            const shp_tensor * length,
+                            const shp_tensor * count,
+                            float              scale,
+                            shp_tensor *       work,
+                            shp_tensor *       y,
+                            shp_stream_t       stream);
+
+/*
  * The paged KV cache, in 8 bits.
  *
  * Sequences share a pool of pages. A page holds `page` positions (16, 32, 64,

@@ -40,11 +40,11 @@ template <int KIND, int HD> __global__ __launch_bounds__(64) void k_attn_any(con
         return;
     }
     const int     t1    = min(static_cast<int>(fastdiv(static_cast<uint32_t>(tile * 16 + 15), a.fG)), len.count - 1);
-    const int32_t base  = len.length - len.count;
-    const int32_t p0    = base + t0;
-    const int32_t p1    = base + t1;
+    const int32_t base  = first_position(a, len);
+    const int32_t p0    = position(a, base, t0);
+    const int32_t p1    = position(a, base, t1);
     const bool    live  = t < len.count;
-    const int32_t p     = live ? base + t : -1;
+    const int32_t p     = live ? position(a, base, t) : -1;
     const int     head  = h * a.G + gq;
     const int     steps = (a.hd + 3) / 4;
 
@@ -157,7 +157,7 @@ template <int KIND, int HD> __global__ __launch_bounds__(64) void k_attn_any(con
 
 // Parts of a row's result; one has been written to y.
 __device__ __forceinline__ int parts_of(const AttnArgs & a, const SeqLens & len, const RowOf & r) {
-    return a.per == 0 ? a.nsplit : wide_parts(a, len.length, len.count, (r.t * a.G + r.gq) / kWideRows);
+    return a.per == 0 ? a.nsplit : wide_parts(a, len, (r.t * a.G + r.gq) / kWideRows);
 }
 
 template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join(const AttnArgs a, int64_t row0) {
@@ -172,7 +172,7 @@ template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join(co
         return;
     }
     join_parts<HD>(parts, a.hd, [&](int s) { return partial_ml(a, row, s); }, [&](int s) { return partial_o(a, row, s); },
-                   out_of(a, r), len.length - len.count + r.t >= 0);
+                   out_of(a, r), position(a, first_position(a, len), r.t) >= 0);
 }
 
 // Many rows of a few parts: HD/4 lanes a row, each the row's weights for itself
@@ -218,7 +218,7 @@ template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join_ro
             v += o[s] * w;
         }
     }
-    const float by  = over(sum, len.length - len.count + r.t >= 0);
+    const float by  = over(sum, position(a, first_position(a, len), r.t) >= 0);
     float *     out = out_of(a, r) + dim;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -264,7 +264,7 @@ int64_t wide_groups(int64_t hd) {
 
 // `rows` query rows of each of `pairs` (kv head, sequence), of T positions, over
 // `keys` of `cap` rows, for a chip that holds `chip` workgroups.
-void plan_spans(int64_t rows, int64_t T, int64_t cap, int64_t keys, int64_t pairs, int64_t chip, AttnPlan & p) {
+void plan_spans(int64_t rows, int64_t T, int64_t cap, int64_t keys, int64_t pairs, int64_t chip, bool causal, AttnPlan & p) {
     // Splits of equally many key tiles for all rows, however many a row has,
     // as short as lets the chip hold all of them at once: 2048 positions of
     // 16 heads take 81 us, and 99 with every row in thirds (Q4_0, 8 kv heads,
@@ -284,7 +284,7 @@ void plan_spans(int64_t rows, int64_t T, int64_t cap, int64_t keys, int64_t pair
             int64_t groups = 0;
             for (int64_t t = 0; t < tiles && groups <= chip; ++t) {
                 // of a whole cache, and within a window all alike
-                const int64_t end = cap - T + ((t + 1) * kWideRows * T + rows - 1) / rows;
+                const int64_t end = causal ? cap - T + ((t + 1) * kWideRows * T + rows - 1) / rows : cap;
                 const int64_t n   = ((end < cap ? end : cap) + kTileKeys - 1) / kTileKeys;
                 groups += ((n < most ? n : most) + of - 1) / of * pairs;
             }
@@ -305,7 +305,7 @@ void plan_spans(int64_t rows, int64_t T, int64_t cap, int64_t keys, int64_t pair
 
 namespace {
 
-shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t window, int32_t sinks, AttnPlan & p) {
+shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t window, int32_t sinks, bool causal, AttnPlan & p) {
     if (!well_formed(q) || !kv_well_formed(k_cache) || q->ne[0] != k_cache->ne[0] || q->ne[1] % k_cache->ne[1] != 0 ||
         q->ne[3] != k_cache->ne[3] || window < 0 || sinks < 0) {
         return SHP_ERR_INVALID_ARG;
@@ -363,7 +363,7 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
     }
     p.wide = !p.few && wide_takes(*k_cache);
     if (p.wide) {
-        plan_spans(rows, T, cap, keys, kv * q->ne[3], wide_groups(q->ne[0]), p);
+        plan_spans(rows, T, cap, keys, kv * q->ne[3], wide_groups(q->ne[0]), causal, p);
     } else if (!p.few) {
         p.nsplit = plan_splits(tiles16 * kv * q->ne[3], (keys + 63) / 64, 2048);
     }
@@ -461,6 +461,7 @@ shp_status_t attn_args(const shp_tensor *         q,
     a.scale  = scale2;
     a.window = p.window;
     a.sinks  = p.sinks;
+    a.apart  = -1;
     a.T      = static_cast<int32_t>(q->ne[2]);
     a.N      = static_cast<int32_t>(q->ne[3]);
     a.hd     = static_cast<int32_t>(q->ne[0]);
@@ -482,41 +483,36 @@ void wide_args(int32_t per, int64_t chip, AttnArgs & a) {
     a.half          = twos ? static_cast<int32_t>((chip / 2 + a.KV - 1) / a.KV) : a.tiles;
 }
 
-}  // namespace shp
+namespace {
 
-using namespace shp;
-
-extern "C" shp_status_t shp_attn_kv_work(const shp_tensor * q,
-                                         const shp_tensor * k_cache,
-                                         int32_t            window,
-                                         int32_t            sinks,
-                                         int64_t *          floats) {
+shp_status_t attn_work(const shp_tensor * q, const shp_tensor * k_cache, int32_t window, int32_t sinks, bool causal, int64_t * floats) {
     AttnPlan p{};
     if (floats == nullptr) {
         return SHP_ERR_INVALID_ARG;
     }
-    const shp_status_t st = plan_attn(q, k_cache, window, sinks, p);
+    const shp_status_t st = plan_attn(q, k_cache, window, sinks, causal, p);
     if (st == SHP_OK) {
         *floats = plan_floats(p, *q);
     }
     return st;
 }
 
-extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
-                                    const shp_tensor * k_cache,
-                                    const shp_tensor * v_cache,
-                                    const shp_tensor * length,
-                                    const shp_tensor * count,
-                                    float              scale,
-                                    int32_t            window,
-                                    int32_t            sinks,
-                                    shp_tensor *       work,
-                                    shp_tensor *       y,
-                                    shp_stream_t       stream) {
+shp_status_t attn(const shp_tensor * q,
+                  const shp_tensor * k_cache,
+                  const shp_tensor * v_cache,
+                  const shp_tensor * length,
+                  const shp_tensor * count,
+                  float              scale,
+                  int32_t            window,
+                  int32_t            sinks,
+                  bool               causal,
+                  shp_tensor *       work,
+                  shp_tensor *       y,
+                  shp_stream_t       stream) {
     AttnPlan     p{};
     shp_status_t st = kv_check_caches(k_cache, v_cache);
     if (st == SHP_OK) {
-        st = plan_attn(q, k_cache, window, sinks, p);
+        st = plan_attn(q, k_cache, window, sinks, causal, p);
     }
     if (st != SHP_OK) {
         return st;
@@ -527,6 +523,7 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
     if (st != SHP_OK || dry_run()) {
         return st;
     }
+    a.apart = causal ? -1 : 0;
     auto nb = [](const shp_tensor & t, int d) { return static_cast<int64_t>(t.ne[d] > 1 ? t.nb[d] : 0); };
     a.k     = static_cast<const char *>(k_cache->data);
     a.v     = static_cast<const char *>(v_cache->data);
@@ -573,4 +570,47 @@ extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
             break;
     }
     return st == SHP_OK && a.nsplit > 1 ? launch_join(a, s) : st;
+}
+
+}  // namespace
+}  // namespace shp
+
+using namespace shp;
+
+extern "C" shp_status_t shp_attn_kv_work(const shp_tensor * q,
+                                         const shp_tensor * k_cache,
+                                         int32_t            window,
+                                         int32_t            sinks,
+                                         int64_t *          floats) {
+    return attn_work(q, k_cache, window, sinks, true, floats);
+}
+
+extern "C" shp_status_t shp_attn_kv(const shp_tensor * q,
+                                    const shp_tensor * k_cache,
+                                    const shp_tensor * v_cache,
+                                    const shp_tensor * length,
+                                    const shp_tensor * count,
+                                    float              scale,
+                                    int32_t            window,
+                                    int32_t            sinks,
+                                    shp_tensor *       work,
+                                    shp_tensor *       y,
+                                    shp_stream_t       stream) {
+    return attn(q, k_cache, v_cache, length, count, scale, window, sinks, true, work, y, stream);
+}
+
+extern "C" shp_status_t shp_attn_cross_work(const shp_tensor * q, const shp_tensor * k, int64_t * floats) {
+    return attn_work(q, k, 0, 0, false, floats);
+}
+
+extern "C" shp_status_t shp_attn_cross(const shp_tensor * q,
+                                       const shp_tensor * k,
+                                       const shp_tensor * v,
+                                       const shp_tensor * length,
+                                       const shp_tensor * count,
+                                       float              scale,
+                                       shp_tensor *       work,
+                                       shp_tensor *       y,
+                                       shp_stream_t       stream) {
+    return attn(q, k, v, length, count, scale, 0, 0, false, work, y, stream);
 }

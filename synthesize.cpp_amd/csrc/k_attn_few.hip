@@ -166,11 +166,11 @@ __global__ __launch_bounds__(64 * WAVES, few_occupancy(KIND, NB * kKvBlock)) voi
             few_span(f, n * f.groups + hg)[1] = few_owner(f, line.total, begin + at.units - 1);
         }
         const KeyTiles kt    = few_tiles(f, len);
-        const int32_t base   = len.length - len.count;
+        const int32_t base   = first_position(a, len);
         const int32_t p1     = len.length - 1;
         const int     head   = (h0 + hc) * a.G + r - t * a.G;
         const bool    live   = hc <= mask && t < len.count;
-        const int32_t p      = live ? base + t : -1;
+        const int32_t p      = live ? position(a, base, t) : -1;
 
         const char * kb = a.k + n * a.kn + h0 * a.kh;
         const char * vb = a.v + n * a.vn + h0 * a.vh;

@@ -838,7 +838,7 @@ shp_status_t plan_pages(const shp_tensor * q, const shp_tensor * k, const shp_te
         const int64_t want = units > kMostParts * p.groups ? (units + 1) / 2 : units;
         p.wgs              = static_cast<int32_t>(want < chip ? want : chip);
     } else {
-        plan_spans(rows, T, cap, keys, kv * q->ne[3], chip, p);
+        plan_spans(rows, T, cap, keys, kv * q->ne[3], chip, true, p);
     }
     return SHP_OK;
 }

@@ -417,18 +417,18 @@ template <int KIND, int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2
         return;
     }
     const Magic   magic;
-    const int32_t base = len.length - len.count;
-    const int32_t p0   = base + t0;
-    const int32_t p1   = base + min(t_of(tile * kWideRows + kWideRows - 1), len.count - 1);
+    const int32_t base = first_position(a, len);
+    const int32_t p0   = position(a, base, t0);
+    const int32_t p1   = position(a, base, min(t_of(tile * kWideRows + kWideRows - 1), len.count - 1));
     // this wave's positions, and this lane's query
     const int     r0   = tile * kWideRows + wave * 32;
-    const int32_t w0   = base + t_of(r0);
-    const int32_t w1   = t_of(r0) < len.count ? base + min(t_of(r0 + 31), len.count - 1) : -1;
+    const int32_t w0   = position(a, base, t_of(r0));
+    const int32_t w1   = t_of(r0) < len.count ? position(a, base, min(t_of(r0 + 31), len.count - 1)) : -1;
     const int     r    = r0 + c;
     const int     t    = t_of(r);
     const int     gq   = r - t * a.G;
     const bool    live = t < len.count;
-    const int32_t p    = live ? base + t : -1;
+    const int32_t p    = live ? position(a, base, t) : -1;
     const int     head = h * a.G + gq;
 
     const KeyTiles kt  = key_tiles<kTileKeys>(a, p0, p1);

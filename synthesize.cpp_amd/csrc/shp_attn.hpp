@@ -28,6 +28,7 @@ struct AttnArgs {
     float           scale;  // times log2 e
     int32_t         window;  // 0: none
     int32_t         sinks;
+    int32_t         apart;  // -1: queries stand one row apart; 0: all at the last row, so that all see every row
     int32_t         T;
     int32_t         G;  // query heads of a kv head
     int32_t         KV;
@@ -68,12 +69,28 @@ template <int KT> __device__ __forceinline__ KeyTiles key_tiles(const AttnArgs &
     return s;
 }
 
+// A sequence's filled rows and new positions.
+struct SeqLens {
+    int32_t length;
+    int32_t count;
+};
+
+// The row at which query 0 of a sequence stands, and query t for that.
+__device__ __forceinline__ int32_t first_position(const AttnArgs & a, const SeqLens & len) {
+    return len.length - 1 - ((len.count - 1) & a.apart);
+}
+
+__device__ __forceinline__ int32_t position(const AttnArgs & a, int32_t first, int32_t t) {
+    return first + (t & a.apart);
+}
+
 // Splits of the keys of a row tile of k_attn_wide. One or none: its rows are
 // written to y directly.
-__device__ __forceinline__ int32_t wide_parts(const AttnArgs & a, int32_t length, int32_t count, int32_t tile) {
+__device__ __forceinline__ int32_t wide_parts(const AttnArgs & a, const SeqLens & len, int32_t tile) {
     const int32_t t0 = static_cast<int32_t>(fastdiv(static_cast<uint32_t>(tile * kWideRows), a.fG));
     const int32_t t1 = static_cast<int32_t>(fastdiv(static_cast<uint32_t>(tile * kWideRows + kWideRows - 1), a.fG));
-    const int32_t n  = key_tiles<kTileKeys>(a, length - count + t0, length - count + min(t1, count - 1)).n;
+    const int32_t p  = first_position(a, len);
+    const int32_t n  = key_tiles<kTileKeys>(a, position(a, p, t0), position(a, p, min(t1, len.count - 1))).n;
     return static_cast<int32_t>(fastdiv(static_cast<uint32_t>(n + a.per - 1), a.fper));
 }
 
@@ -90,12 +107,6 @@ __device__ __forceinline__ bool sees(const AttnArgs & a, int32_t p, int32_t j) {
 __device__ __forceinline__ bool seen_by(const AttnArgs & a, int32_t p0, int32_t p1, int32_t j) {
     return j <= p1 && (a.window == 0 || j > p0 - a.window || j < a.sinks);
 }
-
-// A sequence's filled rows and new positions.
-struct SeqLens {
-    int32_t length;
-    int32_t count;
-};
 
 __device__ __forceinline__ SeqLens seq_lens(const AttnArgs & a, int n) {
     SeqLens s{ a.cap, a.T };
@@ -494,7 +505,7 @@ __device__ __forceinline__ int32_t * few_span(const FewArgs & f, int64_t group) 
 __device__ __forceinline__ KeyTiles few_tiles(const FewArgs & f, const SeqLens & len) {
     const AttnArgs & a     = f.a;
     const int        shift = f.shift;
-    const int32_t    base  = len.length - len.count;
+    const int32_t    base  = first_position(a, len);
     const int32_t    p1    = len.length - 1;
     KeyTiles         kt{ 0, 0, 0 };
     if (p1 >= 0) {
@@ -612,7 +623,7 @@ template <int HD> __device__ __forceinline__ void join_few(const FewArgs & f, in
     }
     const int col = (r.h & ((1 << f.hgs) - 1)) * f.cols + r.t * a.G + r.gq;
     join_parts<HD>(w1 - w0 + 1, a.hd, [&](int s) { return few_ml(f, w0 + s, s == 0, col); },
-                   [&](int s) { return few_o(f, w0 + s, s == 0, col); }, out_of(a, r), len.length - len.count + r.t >= 0);
+                   [&](int s) { return few_o(f, w0 + s, s == 0, col); }, out_of(a, r), position(a, first_position(a, len), r.t) >= 0);
 }
 
 // ---------------------------------------------------------------------------
@@ -655,7 +666,8 @@ shp_status_t launch_attn_few(int kind, const AttnArgs & a, const AttnPlan & p, i
 
 // k_attn.hip: splits of a prompt's keys, the workspace of a plan, what all calls check
 // and pass on, and the launch that joins the splits of k_attn_wide and k_attn_pages_wide.
-void         plan_spans(int64_t rows, int64_t T, int64_t cap, int64_t keys, int64_t pairs, int64_t chip, AttnPlan & p);
+void         plan_spans(int64_t rows, int64_t T, int64_t cap, int64_t keys, int64_t pairs, int64_t chip, bool causal,
+                        AttnPlan & p);
 int64_t      plan_floats(const AttnPlan & p, const shp_tensor & q);
 shp_status_t attn_args(const shp_tensor * q, const shp_tensor * length, const shp_tensor * count, float scale, const AttnPlan & p,
                        const shp_tensor * const * read, int n_read, const shp_tensor * work, const shp_tensor * y, AttnArgs & a);

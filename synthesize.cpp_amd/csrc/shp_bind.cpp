@@ -432,7 +432,7 @@ const Entry kEntries[] = {
     SHP_ENTRY(shp_acc), SHP_ENTRY_FIRST(shp_im2col, kShape), SHP_ENTRY(shp_cont_add_leaky_relu), SHP_ENTRY(shp_soft_max_ext),
     SHP_ENTRY(shp_diag_mask_inf), SHP_ENTRY(shp_soft_max_causal), SHP_ENTRY(shp_exp), SHP_ENTRY(shp_scale_bias),
     SHP_ENTRY_FIRST(shp_sum_scale_leaky_relu, kArray), { "shp_layer_nongemm_step", &run_layer },
-    SHP_ENTRY(shp_kv_store), SHP_ENTRY(shp_kv_load), SHP_ENTRY(shp_attn_kv), SHP_WORK(shp_attn_kv_work),
+    SHP_ENTRY(shp_kv_store), SHP_ENTRY(shp_kv_load), SHP_ENTRY(shp_attn_kv), SHP_WORK(shp_attn_kv_work), SHP_WORK(shp_attn_cross_work), SHP_ENTRY(shp_attn_cross),
     SHP_WORK(shp_kv_pages_work), SHP_ENTRY(shp_kv_pages), SHP_ENTRY(shp_kv_slots), SHP_ENTRY(shp_kv_store_pages),
     SHP_ENTRY(shp_kv_load_pages), SHP_WORK(shp_attn_pages_work), SHP_ENTRY(shp_attn_pages),
 };

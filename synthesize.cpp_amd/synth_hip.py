@@ -128,6 +128,8 @@ def load(path=None):
         "shp_kv_load": [_PT, _PT, _PT, _PT, _PT, _PT, vp],
         "shp_attn_kv": [_PT, _PT, _PT, _PT, _PT, f, i32, i32, _PT, _PT, vp],
         "shp_attn_kv_work": [_PT, _PT, i32, i32, ctypes.POINTER(i64)],
+        "shp_attn_cross": [_PT, _PT, _PT, _PT, _PT, f, _PT, _PT, vp],
+        "shp_attn_cross_work": [_PT, _PT, ctypes.POINTER(i64)],
         "shp_kv_pages_work": [_PT, ctypes.POINTER(i64)],
         "shp_kv_pages": [_PT, i32, _PT, _PT, _PT, _PT, _PT, _PT, vp],
         "shp_kv_slots": [_PT, _PT, _PT, i32, _PT, vp],
@@ -473,6 +475,30 @@ def attn_kv(q, k_cache, v_cache, length=None, count=None, scale=None, window=0, 
     _check(_fn("shp_attn_kv")(q, k_cache, v_cache, length, count,
                               float(q.shape[-1] ** -0.5 if scale is None else scale), int(window), int(sinks), work,
                               out, _stream()), "attn_kv")
+    return out
+
+
+def attn_cross_work(q, k):
+    """The floats of workspace that attn_cross needs for these shapes (0: none)."""
+    n = _fn("shp_attn_cross_work")(q, k)
+    if n < 0:
+        raise ShpError(-n, "attn_cross_work")
+    return n
+
+
+def attn_cross(q, k, v, length=None, count=None, scale=None, out=None, work=None):
+    """Attention of every query to every row of another sequence, an encoder's
+    states say: q (N, T, heads, head_dim) F32, k and v (N, rows, kv_heads, head_dim) as
+    attn_kv's caches. length (int32 (N,); all rows without one) counts a sequence's rows,
+    count its queries. scale: head_dim ** -0.5 unless given. work: F32 of
+    attn_cross_work()'s floats, allocated here unless given. Returns (N, T, heads,
+    head_dim); without rows zeros, and queries past count[n] are not written."""
+    out = q.new_empty(q.shape) if out is None else out
+    if work is None:
+        n = attn_cross_work(q, k)
+        work = q.new_empty(n) if n else None
+    _check(_fn("shp_attn_cross")(q, k, v, length, count, float(q.shape[-1] ** -0.5 if scale is None else scale), work, out,
+                                 _stream()), "attn_cross")
     return out
 
 

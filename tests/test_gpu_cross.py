@@ -1,0 +1,177 @@
+"""attn_cross on the GPU against its definition, within the bound of
+kv_ref.attend_by_row: a query that sees all rows is the newest position over a
+cache of them."""
+import pytest
+import torch
+
+import kv_ref as R
+
+pytestmark = pytest.mark.gpu
+I32 = torch.int32
+
+
+def ints(*v):
+    return torch.tensor(v, dtype=I32, device="cuda")
+
+
+def attend(q, k, v, kind, length, count, scale):
+    """(y, bound): the positions of a kv head as so many heads of one position."""
+    n, t, heads, hd = q.shape
+    kv = k.shape[2]
+    many = q.reshape(n, t, kv, heads // kv, hd).transpose(1, 2).reshape(n, 1, -1, hd)
+    back = [x.reshape(n, kv, t, heads // kv, hd).transpose(1, 2).reshape(n, t, heads, hd)
+            for x in R.attend_by_row(many, k, v, kind, length, [1] * n, scale)]
+    for b in range(n):
+        back[0][b, count[b]:] = float("nan")
+    return back
+
+
+def states(kind, n, rows, kv, hd, seed):
+    """K and V as a cache holds them, and their values."""
+    g = torch.Generator().manual_seed(seed)
+    packed = [R.pack(torch.randn(n, rows, kv, hd, generator=g) * by, kind) for by in (1.0, 0.5)]
+    return packed, [R.values(c, kind) for c in packed]
+
+
+def junk(c, kind, length):
+    """The cache with every row past a sequence's length reading as NaN."""
+    c = c.clone()
+    for b, ln in enumerate(length):
+        c[b, max(ln, 0):] = float("nan") if kind in R.FLOAT else 0x7e
+    return c
+
+
+def check(gpu, kind, heads, kv, hd, t, rows, length, count=None, scale=None, make=lambda x: x, lengths_given=True, q=None):
+    n = len(length)
+    q = torch.randn(n, t, heads, hd, generator=torch.Generator().manual_seed(t)) * 1.5 if q is None else q
+    packed, values = states(kind, n, rows, kv, hd, rows)
+    clamped = [min(max(x, 0), rows) for x in length]
+    cnt = [t] * n if count is None else [min(max(x, 0), t) for x in count]
+    y, bound = attend(q, *values, kind, clamped, cnt, hd ** -0.5 if scale is None else scale)
+    k, v = (R.handle(gpu, make(junk(c, kind, clamped).cuda()), kind, hd) for c in packed)
+    out = torch.full(q.shape, 9.25, device="cuda")
+    gpu.attn_cross(q.cuda(), k, v, ints(*length) if lengths_given else None, None if count is None else ints(*count),
+                   scale=scale, out=out)
+    got = out.cpu().double()
+    none = torch.isnan(y)
+    assert (got[none] == 9.25).all()
+    err = (got - y)[~none].abs()
+    assert (err <= bound[~none]).all(), (float((err / bound[~none].clamp_min(1e-300)).max()), float(err.max()))
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+@pytest.mark.parametrize("heads,kv,hd,t,rows", [(16, 16, 64, 1, 300), (12, 12, 64, 130, 130), (16, 8, 128, 1, 1000), (4, 2, 128, 200, 77),
+                                                (7, 1, 96, 5, 260), (3, 3, 32, 17, 1), (2, 1, 256, 33, 150), (8, 2, 160, 2, 65)])
+def test_all_queries_see_all_rows(gpu, kind, heads, kv, hd, t, rows):
+    length = [rows, rows - 1, 1, 0, max(1, rows // 2), -4, rows + 7]
+    check(gpu, kind, heads, kv, hd, t, rows, length)
+    check(gpu, kind, heads, kv, hd, t, rows, length, [t, 1, t, t, t - 1, 0, t + 3])
+    check(gpu, kind, heads, kv, hd, t, rows, [rows] * 2, lengths_given=False, scale=-0.3)
+
+
+@pytest.mark.parametrize("kind", sorted(R.FLOAT))
+@pytest.mark.parametrize("hd", [1, 7, 40, 80, 91])
+def test_heads_of_odd_length(gpu, kind, hd):
+    check(gpu, kind, 6, 3, hd, 1, 90, [90, 33])
+    check(gpu, kind, 6, 3, hd, 70, 90, [90, 33])
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
+def test_long_states(gpu, kind):
+    """Queries whose parts are joined."""
+    check(gpu, kind, 2, 1, 64, 1, 9000, [9000, 4500])
+    check(gpu, kind, 2, 1, 64, 40, 5000, [5000])
+    check(gpu, kind, 4, 4, 64, 600, 700, [700, 650])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "q8_0"])
+@pytest.mark.parametrize("t", [1, 60])
+def test_what_is_not_finite(gpu, kind, t):
+    """An infinity or NaN in a row of K or V, or a query: NaN, to its own head only."""
+    n, rows, heads, kv, hd = 2, 100, 4, 2, 64
+    packed, _ = states(kind, n, rows, kv, hd, 3)
+    q = torch.randn(n, t, heads, hd)
+    want = torch.zeros(n, t, heads, dtype=torch.bool)
+    for side, (b, row, h) in zip(packed, ((0, 17, 1), (1, 99, 0))):
+        if kind in R.FLOAT:
+            side[b, row, h, 5] = float("inf")
+        else:
+            side[b, row, h, :2] = torch.tensor([0, 0x7e], dtype=torch.uint8)
+        want[b, :, h * 2:h * 2 + 2] = True
+    q[0, t - 1, 0, 3], q[1, 0, 3, 0] = float("nan"), float("-inf")
+    want[0, t - 1, 0] = want[1, 0, 3] = True
+    k, v = (R.handle(gpu, c.cuda(), kind, hd) for c in packed)
+    got = gpu.attn_cross(q.cuda(), k, v).cpu()
+    assert torch.equal(torch.isnan(got).all(-1), want) and torch.equal(torch.isnan(got).any(-1), want)
+    got = gpu.attn_cross(q.cuda(), k, v, ints(17, 99)).cpu()      # (they are past the rows now)
+    own = torch.zeros_like(want)
+    own[0, t - 1, 0] = own[1, 0, 3] = True
+    assert torch.equal(torch.isnan(got).any(-1), own)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16", "q4_0"])
+def test_layouts(gpu, kind):
+    """Head-major states, queries cut from a fused projection, and one sequence of
+    states for all queries by a stride of 0."""
+    heads, kv, hd, rows = 6, 2, 64, 70
+    for t in (1, 50):
+        check(gpu, kind, heads, kv, hd, t, rows, [70, 30], make=lambda x: x.transpose(1, 2).contiguous().transpose(1, 2))
+        fused = torch.randn(2, t, 3, heads, hd)
+        check(gpu, kind, heads, kv, hd, t, rows, [70, 30], q=fused[:, :, 1])
+        packed, values = states(kind, 1, rows, kv, hd, 9)
+        k, v = (R.handle(gpu, c.cuda().expand(5, -1, -1, -1), kind, hd) for c in packed)
+        q = torch.randn(5, t, heads, hd)
+        y, bound = attend(q, *(x.expand(5, -1, -1, -1) for x in values), kind, [70, 1, 69, 0, 33], [t] * 5, hd ** -0.5)
+        got = gpu.attn_cross(q.cuda(), k, v, ints(70, 1, 69, 0, 33)).cpu().double()
+        assert ((got - y).abs() <= bound).all()
+
+
+def test_a_decoder_layer_and_its_encoder_together(gpu):
+    """An encoder's layer that looks both ways over its own q, k and v, the states
+    stored in a cache by kv_store, and a decoder's tokens against them, beside the
+    decoder's own attention; eagerly, and as one captured graph over new inputs."""
+    n, rows, t, heads, hd, cap = 3, 50, 1, 4, 64, 20
+    z = lambda *s: torch.zeros(*s, device="cuda")
+    s = dict(q=z(n, rows, heads, hd), k=z(n, rows, heads, hd), v=z(n, rows, heads, hd), enc=z(n, rows, heads, hd), y=z(n, t, heads, hd),
+             x=z(n, t, heads, hd), own=z(n, t, heads, hd), length=ints(*[0] * n), at=ints(*[0] * n), filled=ints(*[1] * n), zero=ints(*[0] * n))
+    states_ = [z(n, rows, heads, hd).half() for _ in range(2)]
+    cache = [z(n, cap, heads, hd).half() for _ in range(2)]
+    work = [torch.empty(max(1, w), device="cuda") for w in (gpu.attn_cross_work(s["q"], s["k"]), gpu.attn_cross_work(s["x"], states_[0]),
+                                                           gpu.attn_kv_work(s["x"], cache[0]))]
+
+    def step():
+        gpu.attn_cross(s["q"], s["k"], s["v"], s["length"], s["length"], out=s["enc"], work=work[0])
+        gpu.kv_store(s["enc"], s["enc"], states_[0], states_[1], s["zero"], s["length"])
+        gpu.kv_store(s["x"], s["x"], cache[0], cache[1], s["at"])
+        gpu.attn_kv(s["x"], cache[0], cache[1], s["filled"], out=s["own"], work=work[2])
+        gpu.attn_cross(s["own"], states_[0], states_[1], s["length"], out=s["y"], work=work[1])
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    g = torch.Generator().manual_seed(4)
+    for i in range(6):
+        length = [[50, 3, 17], [1, 0, 49], [33, 33, 33]][i % 3]
+        for name in ("q", "k", "v", "x"):
+            s[name].copy_(torch.randn(s[name].shape, generator=g))
+        s["length"].copy_(ints(*length)), s["at"].copy_(ints(i, i, i)), s["filled"].copy_(ints(i + 1, i + 1, i + 1))
+        results = []
+        for run in (step, graph.replay):
+            s["enc"].fill_(9.25)
+            run()
+            results.append([s[name].cpu() for name in ("enc", "own", "y")])
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+        enc, own, y = results[0]
+        q, k, v = (s[name].cpu() for name in ("q", "k", "v"))
+        want, bound = attend(q, k, v, "f32", length, length, hd ** -0.5)
+        live = ~torch.isnan(want)
+        assert (enc[~live] == 9.25).all() and ((enc.double() - want)[live].abs() <= bound[live]).all()
+        held = [enc.half().float(), enc.half().float()]
+        want, bound = attend(own, *held, "f16", length, [t] * n, hd ** -0.5)
+        assert ((y.double() - want).abs() <= bound).all()
