@@ -328,7 +328,24 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
     const int64_t tiles16 = (rows + 15) / 16;
     p.few            = rows <= 16 && kv_blocks(kv_kind(k_cache->type));
     p.hgs            = 0;
-    if (p.few) {
+    p.cross          = !causal && rows <= 16 && cross_few_takes(*k_cache);
+    if (p.cross) {
+        const int64_t chunk  = cross_few_rows(kv_kind(k_cache->type), q->ne[0]);
+        const int64_t chunks = (cap + chunk - 1) / chunk;
+        const int64_t groups = kv * q->ne[3];
+        const int64_t deep   = chunks <= kWhole * 4 ? (chunks + 3) / 4 : 1;
+        const int64_t units  = (chunks + 4 * deep - 1) / (4 * deep) * groups;
+        const int64_t want   = units > kFewGroups * groups ? (units + 1) / 2 : units;
+        const int64_t most   = wide_groups(q->ne[0]);
+        p.cross              = units < INT32_MAX;
+        p.few                = p.cross;
+        p.per                = static_cast<int32_t>(4 * deep);
+        p.groups             = static_cast<int32_t>(groups);
+        p.parts              = units > groups;
+        p.wgs                = static_cast<int32_t>(want < most ? want : most);
+        const int64_t fit    = p.wgs * 2 * kCols / (q->ne[1] * q->ne[2] * q->ne[3]);
+        p.nsplit             = p.parts ? plan_splits(tiles16 * kv * q->ne[3], fit, 2048) : 1;
+    } else if (p.few) {
         while ((rows << (p.hgs + 1)) <= 16 && kv % (int64_t{ 2 } << p.hgs) == 0 &&
                k_cache->nb[1] == kv_bytes_of_row(*k_cache)) {
             ++p.hgs;
@@ -538,7 +555,10 @@ shp_status_t attn(const shp_tensor * q,
     const hipStream_t s     = as_stream(stream);
     const int         kind  = kv_kind(k_cache->type);
     int32_t           run   = 0;
-    const int         piece = p.few ? few_piece(*k_cache, *v_cache, p.hgs, run) : 0;
+    if (p.cross && cross_few_takes(*v_cache)) {
+        return launch_cross_few(kind, a, p, s);
+    }
+    const int piece = p.few && !p.cross ? few_piece(*k_cache, *v_cache, p.hgs, run) : 0;
     if (piece > 0) {
         return launch_attn_few(kind, a, p, piece, run, s);
     }

@@ -632,6 +632,7 @@ template <int HD> __device__ __forceinline__ void join_few(const FewArgs & f, in
 
 struct AttnPlan {
     bool    few;
+    bool    cross;  // by k_cross_few
     bool    wide;
     int32_t hgs;
     int32_t groups;  // of heads, all sequences'
@@ -673,6 +674,16 @@ shp_status_t attn_args(const shp_tensor * q, const shp_tensor * length, const sh
                        const shp_tensor * const * read, int n_read, const shp_tensor * work, const shp_tensor * y, AttnArgs & a);
 void         wide_args(int32_t per, int64_t chip, AttnArgs & a);
 shp_status_t launch_join(const AttnArgs & a, hipStream_t stream);
+
+// k_cross.hip: plain states of any length, and at most 16 queries of a kv head. The
+// head lengths that it is built for, the rows of its chunks, and whether it reads c.
+constexpr int64_t cross_few_dims(int64_t hd) {
+    return hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+}
+
+int          cross_few_rows(int kind, int64_t hd);
+bool         cross_few_takes(const shp_tensor & c);
+shp_status_t launch_cross_few(int kind, const AttnArgs & a, const AttnPlan & p, hipStream_t stream);
 
 // k_attn_wide.hip.
 shp_status_t launch_attn_wide(int kind, const AttnArgs & a, hipStream_t stream);
