@@ -330,21 +330,10 @@ shp_status_t plan_attn(const shp_tensor * q, const shp_tensor * k_cache, int32_t
     p.hgs            = 0;
     p.cross          = !causal && rows <= 16 && cross_few_takes(*k_cache);
     if (p.cross) {
-        const int64_t chunk  = cross_few_rows(kv_kind(k_cache->type), q->ne[0]);
-        const int64_t chunks = (cap + chunk - 1) / chunk;
-        const int64_t groups = kv * q->ne[3];
-        const int64_t deep   = chunks <= kWhole * 4 ? (chunks + 3) / 4 : 1;
-        const int64_t units  = (chunks + 4 * deep - 1) / (4 * deep) * groups;
-        const int64_t want   = units > kFewGroups * groups ? (units + 1) / 2 : units;
-        const int64_t most   = wide_groups(q->ne[0]);
-        p.cross              = units < INT32_MAX;
-        p.few                = p.cross;
-        p.per                = static_cast<int32_t>(4 * deep);
-        p.groups             = static_cast<int32_t>(groups);
-        p.parts              = units > groups;
-        p.wgs                = static_cast<int32_t>(want < most ? want : most);
-        const int64_t fit    = p.wgs * 2 * kCols / (q->ne[1] * q->ne[2] * q->ne[3]);
-        p.nsplit             = p.parts ? plan_splits(tiles16 * kv * q->ne[3], fit, 2048) : 1;
+        plan_cross_few(kv_kind(k_cache->type), q->ne[0], cap, kv * q->ne[3], p);
+        p.few             = p.cross;
+        const int64_t fit = p.wgs * 2 * kCols / (q->ne[1] * q->ne[2] * q->ne[3]);
+        p.nsplit          = p.parts ? plan_splits(tiles16 * kv * q->ne[3], fit, 2048) : 1;
     } else if (p.few) {
         while ((rows << (p.hgs + 1)) <= 16 && kv % (int64_t{ 2 } << p.hgs) == 0 &&
                k_cache->nb[1] == kv_bytes_of_row(*k_cache)) {

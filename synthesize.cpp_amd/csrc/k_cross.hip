@@ -17,12 +17,17 @@
 namespace shp {
 namespace {
 
-constexpr int kCrossWaves = 4;
+constexpr int kSplitWaves = 4;  // of a workgroup whose heads are split
 
-// Rows of a chunk: 64, or as many as keep K's in 32 registers of a lane, but 16 at least.
+// Rows of a chunk: 32, or as many as keep K's in 32 registers of a lane, but 16 at least.
 constexpr int cross_rows(int kind, int hd) {
     const int rows = 8192 / (hd * kv_unit_bytes(kind));
-    return rows > 64 ? 64 : rows < 16 ? 16 : rows;
+    return rows > 32 ? 32 : rows < 16 ? 16 : rows;
+}
+
+// Waves that a SIMD holds by their registers.
+constexpr int cross_occupancy(int kind, int hd) {
+    return hd == 64 && kind != kKvF32 ? 4 : hd == 64 ? 3 : hd == 128 ? 2 : 1;
 }
 
 constexpr int cross_shift(int kind, int hd) {
@@ -39,6 +44,11 @@ __device__ __forceinline__ f16x2 take_b16(float & a, float & b) {
     a -= __uint_as_float(w << 16);
     b -= __uint_as_float(w & 0xffff0000u);
     return as_f16x2(w);
+}
+
+// Waves of a workgroup that has a whole head: as many as a CU holds, within 16.
+constexpr int cross_waves(int kind, int hd) {
+    return cross_occupancy(kind, hd) == 4 ? 16 : hd <= 128 ? 8 : 4;
 }
 
 // 16 bytes at any 4-byte boundary.
@@ -65,8 +75,8 @@ template <int KIND> __device__ __forceinline__ uint32_t larger(uint32_t most, ui
 // hd is HD, or (FULL false) less, a multiple of HD/16 and of 16 bytes: then what lies
 // past it is read from the row's start, against zeros in q and into results that
 // are not written.
-template <int KIND, int HD, bool FULL>
-__global__ __launch_bounds__(64 * kCrossWaves, HD <= 128 ? 2 : 1) void k_cross_few(const FewArgs f) {
+template <int KIND, int HD, bool FULL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, cross_occupancy(KIND, HD)) void k_cross_few(const FewArgs f) {
     constexpr int  SIZE  = kv_unit_bytes(KIND);
     constexpr int  PER   = 16 / SIZE;          // values of 16 bytes
     constexpr int  ROWS  = cross_rows(KIND, HD);
@@ -293,7 +303,7 @@ __global__ __launch_bounds__(64 * kCrossWaves, HD <= 128 ? 2 : 1) void k_cross_f
                 }
             }
             if constexpr (MORE) {
-                fetch_k(i + kCrossWaves);
+                fetch_k(i + WAVES);
             } else if (j0 + ROWS > rows) {
 #pragma unroll
                 for (int y = 0; y < TT; ++y) {
@@ -340,10 +350,10 @@ __global__ __launch_bounds__(64 * kCrossWaves, HD <= 128 ? 2 : 1) void k_cross_f
                 }
             }
             if constexpr (MORE) {
-                fetch_v(i + kCrossWaves);
+                fetch_v(i + WAVES);
             }
         };
-        for (; i + kCrossWaves < end; i += kCrossWaves) {
+        for (; i + WAVES < end; i += WAVES) {
             chunk(std::true_type{});
         }
         if (i < end) {
@@ -362,7 +372,7 @@ __global__ __launch_bounds__(64 * kCrossWaves, HD <= 128 ? 2 : 1) void k_cross_f
 
         // the waves' results joined in LDS: [wave][tile][lane], then m and l of a column
         f32x4 * of = reinterpret_cast<f32x4 *>(lds);
-        float * ml = reinterpret_cast<float *>(of + kCrossWaves * TILES * kWave);
+        float * ml = reinterpret_cast<float *>(of + WAVES * TILES * kWave);
 #pragma unroll
         for (int u = 0; u < TILES; ++u) {
             of[(wave * TILES + u) * kWave + lane] = o[u];
@@ -374,14 +384,14 @@ __global__ __launch_bounds__(64 * kCrossWaves, HD <= 128 ? 2 : 1) void k_cross_f
         __syncthreads();
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kCrossWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             top = fmaxf(top, ml[(w * 16 + c) * 2]);
         }
         const float ref = top == -INFINITY ? 0.0f : top;
-        float       part[kCrossWaves];
+        float       part[WAVES];
         l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kCrossWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float wl = ml[(w * 16 + c) * 2 + 1];
             part[w]        = wl == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml[(w * 16 + c) * 2] - ref);
             l += part[w] * wl;
@@ -401,23 +411,21 @@ __global__ __launch_bounds__(64 * kCrossWaves, HD <= 128 ? 2 : 1) void k_cross_f
                     pml[1]      = l;
                 }
             }
-            // element e of tile u in quarter g is value TILES (4 g + e) + u; wave w has
-            // the rows' elements e = w
-            f32x4 v[(TILES + 3) / 4];
+            // element e of tile u in quarter g is value TILES (4 g + e) + u: the first
+            // waves take an e and four tiles each
+            for (int from = wave; from < TILES; from += WAVES) {
+                const int e = from % 4, u0 = from / 4 * 4;
+                f32x4     v = splat4(0.0f);
 #pragma unroll
-            for (int u = 0; u < TILES; ++u) {
-                float x = 0.0f;
+                for (int w = 0; w < WAVES; ++w) {
 #pragma unroll
-                for (int w = 0; w < kCrossWaves; ++w) {
-                    x += reinterpret_cast<const float *>(of + (w * TILES + u) * kWave + lane)[wave] * part[w];
+                    for (int u = 0; u < 4; ++u) {
+                        v[u] += reinterpret_cast<const float *>(of + (w * TILES + u0 + u) * kWave + lane)[e] * part[w];
+                    }
                 }
-                v[u / 4][u % 4] = x * by;
-            }
-            const int dim = TILES * (4 * g + wave);
-            if (FULL || dim < hd) {
-#pragma unroll
-                for (int u = 0; u < TILES; u += 4) {
-                    *reinterpret_cast<f32x4u *>(out + dim + u) = v[u / 4];
+                const int dim = TILES * (4 * g + e) + u0;
+                if (FULL || dim < hd) {
+                    *reinterpret_cast<f32x4u *>(out + dim) = v * by;
                 }
             }
         }
@@ -440,10 +448,16 @@ template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_cross_join(c
     join_few<HD>(f, row0 + blockIdx.x);
 }
 
-template <int KIND, int HD, bool FULL> shp_status_t launch_as(FewArgs & f, hipStream_t stream) {
-    constexpr int lds = kCrossWaves * (HD / 16 * kWave * 16 + 16 * 2 * 4);
-    hipLaunchKernelGGL((k_cross_few<KIND, HD, FULL>), dim3(static_cast<unsigned>(f.wgs)), dim3(64 * kCrossWaves), lds, stream, f);
-    const shp_status_t st = launch_status();
+template <int KIND, int HD, bool FULL> shp_status_t launch_as(FewArgs & f, int waves, hipStream_t stream) {
+    const int lds = waves * (HD / 16 * kWave * 16 + 16 * 2 * 4);
+    auto      go  = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(f.wgs)), dim3(static_cast<unsigned>(64 * waves)), lds, stream, f);
+        return launch_status();
+    };
+    if (f.a.work == nullptr && waves > kSplitWaves) {
+        return go(k_cross_few<KIND, HD, FULL, cross_waves(KIND, HD)>);
+    }
+    const shp_status_t st = go(k_cross_few<KIND, HD, FULL, kSplitWaves>);
     if (st != SHP_OK || f.a.work == nullptr) {
         return st;  // no head was split
     }
@@ -453,21 +467,37 @@ template <int KIND, int HD, bool FULL> shp_status_t launch_as(FewArgs & f, hipSt
     });
 }
 
-template <int KIND> shp_status_t launch(FewArgs & f, hipStream_t stream) {
+template <int KIND> shp_status_t launch(FewArgs & f, int waves, hipStream_t stream) {
     switch (cross_few_dims(f.a.hd)) {
         case 64:
-            return f.a.hd == 64 ? launch_as<KIND, 64, true>(f, stream) : launch_as<KIND, 64, false>(f, stream);
+            return f.a.hd == 64 ? launch_as<KIND, 64, true>(f, waves, stream) : launch_as<KIND, 64, false>(f, waves, stream);
         case 128:
-            return f.a.hd == 128 ? launch_as<KIND, 128, true>(f, stream) : launch_as<KIND, 128, false>(f, stream);
+            return f.a.hd == 128 ? launch_as<KIND, 128, true>(f, waves, stream) : launch_as<KIND, 128, false>(f, waves, stream);
         default:
-            return f.a.hd == 256 ? launch_as<KIND, 256, true>(f, stream) : launch_as<KIND, 256, false>(f, stream);
+            return f.a.hd == 256 ? launch_as<KIND, 256, true>(f, waves, stream) : launch_as<KIND, 256, false>(f, waves, stream);
     }
 }
 
 }  // namespace
 
-int cross_few_rows(int kind, int64_t hd) {
-    return cross_rows(kind, static_cast<int>(cross_few_dims(hd)));
+// A head is whole while its chunks are at most kDeep a wave: what more of them would take
+// is less than a second launch.
+constexpr int64_t kDeep = 6;
+
+void plan_cross_few(int kind, int64_t hd, int64_t rows, int64_t groups, AttnPlan & p) {
+    const int     dims   = static_cast<int>(cross_few_dims(hd));
+    const int     most   = cross_waves(kind, dims);
+    const int64_t chunk  = cross_rows(kind, dims);
+    const int64_t chunks = (rows + chunk - 1) / chunk;
+    p.parts              = chunks > kDeep * most;
+    p.waves              = !p.parts && chunks > kSplitWaves ? most : kSplitWaves;
+    const int64_t deep   = p.parts ? 1 : (chunks + p.waves - 1) / p.waves;
+    const int64_t units  = (chunks + p.waves * deep - 1) / (p.waves * deep) * groups;
+    const int64_t held   = int64_t{ 256 } * 4 * cross_occupancy(kind, dims) / p.waves;
+    p.cross              = units < INT32_MAX;
+    p.per                = static_cast<int32_t>(p.waves * deep);
+    p.groups             = static_cast<int32_t>(groups);
+    p.wgs                = static_cast<int32_t>(units < held ? units : held);
 }
 
 bool cross_few_takes(const shp_tensor & c) {
@@ -487,11 +517,11 @@ shp_status_t launch_cross_few(int kind, const AttnArgs & a, const AttnPlan & p, 
     f.cols   = a.T * a.G;
     switch (kind) {
         case kKvF32:
-            return launch<kKvF32>(f, stream);
+            return launch<kKvF32>(f, p.waves, stream);
         case kKvF16:
-            return launch<kKvF16>(f, stream);
+            return launch<kKvF16>(f, p.waves, stream);
         default:
-            return launch<kKvBF16>(f, stream);
+            return launch<kKvBF16>(f, p.waves, stream);
     }
 }
 

@@ -638,6 +638,7 @@ struct AttnPlan {
     int32_t groups;  // of heads, all sequences'
     int32_t wgs;
     int32_t per;
+    int32_t waves;  // of a workgroup of k_cross_few
     bool    parts;
     int32_t window;
     int32_t sinks;
@@ -676,12 +677,12 @@ void         wide_args(int32_t per, int64_t chip, AttnArgs & a);
 shp_status_t launch_join(const AttnArgs & a, hipStream_t stream);
 
 // k_cross.hip: plain states of any length, and at most 16 queries of a kv head. The
-// head lengths that it is built for, the rows of its chunks, and whether it reads c.
+// head lengths that it is built for, its plan for `rows` rows, whether it reads c.
 constexpr int64_t cross_few_dims(int64_t hd) {
     return hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
 }
 
-int          cross_few_rows(int kind, int64_t hd);
+void         plan_cross_few(int kind, int64_t hd, int64_t rows, int64_t groups, AttnPlan & p);
 bool         cross_few_takes(const shp_tensor & c);
 shp_status_t launch_cross_few(int kind, const AttnArgs & a, const AttnPlan & p, hipStream_t stream);
 
