@@ -14,12 +14,13 @@ namespace {
 //   the page of number i goes to  free[left + R - 1 - i],
 //   the page of number k is       free[left + R - 1 - k],
 // which is a stack's push of every i from the last down and pop of every k from the
-// first up. So only the sums before each sequence follow each other; a page finds its
-// sequence among them by bisection.
+// first up: the page taken as number j is the one given back as number j, and past R, or
+// left over past A, one of the stack. So every j is moved by itself, and only the
+// sums before each sequence follow each other; a page finds its sequence among them
+// by bisection.
 // ---------------------------------------------------------------------------
 
-constexpr int kStepThreads = 1024;
-constexpr int kStepWaves   = kStepThreads / kWave;
+constexpr int kStepEach = 4;  // sequences of a thread at a time
 
 struct StepArgs {
     const int32_t * length;
@@ -38,68 +39,119 @@ __device__ __forceinline__ int32_t pages_of(const StepArgs & a, int32_t length) 
     return (length >> a.shift) + ((length & ((1 << a.shift) - 1)) != 0 ? 1 : 0);
 }
 
+// The sum of a wave's lanes up to and with this one, of numbers below 2^48.
 __device__ __forceinline__ int64_t wave_sum_up_to(int64_t v) {
-    const int lane = threadIdx.x % kWave;
-#pragma unroll
-    for (int off = 1; off < kWave; off *= 2) {
-        const int64_t below = __shfl_up(static_cast<long long>(v), off);
-        v += lane >= off ? below : 0;
-    }
-    return v;
+    const int32_t low  = sum_up_to(static_cast<int32_t>(v & 0xffff));
+    const int32_t mid  = sum_up_to(static_cast<int32_t>(v >> 16 & 0xffff));
+    const int32_t high = sum_up_to(static_cast<int32_t>(v >> 32));
+    return low + (static_cast<int64_t>(mid) << 16) + (static_cast<int64_t>(high) << 32);
 }
 
-// One workgroup: back[n] and take[n], the pages of the sequences before n, and
-// in [N] all of them. False where the step cannot be made. `left` is the stack's.
-__device__ __forceinline__ bool step_sums(const StepArgs & a, int32_t * back, int32_t * take, int32_t left) {
-    __shared__ int64_t sums[2][kStepWaves];
+// What kStepEach sequences from n0 on give back, take and need.
+struct StepPart {
+    int32_t back[kStepEach], take[kStepEach], need[kStepEach];
+    int64_t all_back, all_take;
+    bool    bad;
+};
+
+__device__ __forceinline__ StepPart step_part(const StepArgs & a, int n0) {
+    StepPart p{};
+    int32_t  lengths[kStepEach], helds[kStepEach];
+#pragma unroll
+    for (int k = 0; k < kStepEach; ++k) {  // (no branch around the loads: all of them are on their way at once)
+        lengths[k] = a.length[min(n0 + k, a.N - 1)];
+        helds[k]   = a.held[min(n0 + k, a.N - 1)];
+    }
+#pragma unroll
+    for (int k = 0; k < kStepEach; ++k) {
+        const int32_t length = n0 + k < a.N ? lengths[k] : 0;
+        const int32_t held   = n0 + k < a.N ? helds[k] : 0;
+        const int32_t need   = pages_of(a, max(length, 0));
+        p.bad                = p.bad || length < 0 || need > a.tables.most || held < 0 || held > a.tables.most;
+        p.back[k]            = max(held, need) - need;  // (of any held and need within the table)
+        p.take[k]            = max(held, need) - held;
+        p.need[k]            = need;
+        p.all_back += p.back[k];
+        p.all_take += p.take[k];
+    }
+    return p;
+}
+
+// back and take of the sequences from n0 on, with b and t pages before them (past
+// int32 only in a step that is refused).
+__device__ __forceinline__ void keep_part(const StepArgs & a, const StepPart & p, int n0, int64_t b, int64_t t, int32_t * back,
+                                          int32_t * take, int32_t * need) {
+#pragma unroll
+    for (int k = 0; k < kStepEach; ++k) {
+        if (n0 + k < a.N) {
+            back[n0 + k] = static_cast<int32_t>(b);
+            take[n0 + k] = static_cast<int32_t>(t);
+            if (need != nullptr) {
+                need[n0 + k] = p.need[k];
+            }
+        }
+        b += p.back[k];
+        t += p.take[k];
+    }
+}
+
+// One workgroup of THREADS: back[n] and take[n], the pages of the sequences before n, and
+// in [N] all of them; need[n], where that is not null, those that n is to have. False where
+// the step cannot be made. `left` is the stack's.
+template <int THREADS>
+__device__ __forceinline__ bool step_sums(const StepArgs & a, int32_t * back, int32_t * take, int32_t * need, int32_t left) {
+    constexpr int      WAVES = THREADS / kWave;
+    __shared__ int64_t sums[2][WAVES];
+    __shared__ int32_t fits;
     const int tid  = threadIdx.x;
     const int wave = tid / kWave;
-    const int per  = (a.N + kStepThreads - 1) / kStepThreads;
-    const int n0   = min(tid * per, a.N);
-    const int n1   = min(n0 + per, a.N);
-    int64_t   b = 0, t = 0;
-    bool      bad = false;
-    for (int n = n0; n < n1; ++n) {
-        const int32_t length = a.length[n];
-        const int32_t held   = a.held[n];
-        const int32_t need   = pages_of(a, max(length, 0));
-        bad                  = bad || length < 0 || need > a.tables.most || held < 0 || held > a.tables.most;
-        b += max(static_cast<int64_t>(held) - need, int64_t{ 0 });
-        t += max(static_cast<int64_t>(need) - held, int64_t{ 0 });
+    auto      can  = [&](int64_t b, int64_t t) { return left >= 0 && left + b <= a.pages && t <= left + b; };
+    if (a.N <= kWave * kStepEach) {  // one wave has all of them
+        if (wave == 0) {
+            const int      n0  = tid * kStepEach;
+            const StepPart p   = step_part(a, n0);
+            const int64_t  b   = wave_sum_up_to(p.all_back), t = wave_sum_up_to(p.all_take);
+            const bool     bad = __any(p.bad);
+            keep_part(a, p, n0, b - p.all_back, t - p.all_take, back, take, need);
+            if (tid == kWave - 1) {
+                back[a.N] = static_cast<int32_t>(b);
+                take[a.N] = static_cast<int32_t>(t);
+                fits      = !bad && can(b, t);
+            }
+        }
+        __syncthreads();
+        return fits != 0;
     }
-    int64_t bs = wave_sum_up_to(b), ts = wave_sum_up_to(t);
-    if (tid % kWave == kWave - 1) {
-        sums[0][wave] = bs;
-        sums[1][wave] = ts;
-    }
-    bad = __syncthreads_or(bad);
     int64_t all_b = 0, all_t = 0;
+    for (int first = 0; first < a.N; first += THREADS * kStepEach) {
+        const int      n0 = first + tid * kStepEach;
+        const StepPart p  = step_part(a, n0);
+        if (__syncthreads_or(p.bad)) {
+            return false;
+        }
+        int64_t b = wave_sum_up_to(p.all_back), t = wave_sum_up_to(p.all_take);
+        if (tid % kWave == kWave - 1) {
+            sums[0][wave] = b;
+            sums[1][wave] = t;
+        }
+        __syncthreads();
+        b += all_b - p.all_back;
+        t += all_t - p.all_take;
 #pragma unroll
-    for (int w = 0; w < kStepWaves; ++w) {
-        bs += w < wave ? sums[0][w] : 0;
-        ts += w < wave ? sums[1][w] : 0;
-        all_b += sums[0][w];
-        all_t += sums[1][w];
-    }
-    if (bad || left < 0 || left + all_b > a.pages || all_t > left + all_b) {
-        return false;
-    }
-    b = bs - b;
-    t = ts - t;
-    for (int n = n0; n < n1; ++n) {
-        const int32_t held = a.held[n];
-        const int32_t need = pages_of(a, a.length[n]);
-        back[n]            = static_cast<int32_t>(b);
-        take[n]            = static_cast<int32_t>(t);
-        b += max(held - need, 0);
-        t += max(need - held, 0);
+        for (int w = 0; w < WAVES; ++w) {
+            b += w < wave ? sums[0][w] : 0;
+            t += w < wave ? sums[1][w] : 0;
+            all_b += sums[0][w];
+            all_t += sums[1][w];
+        }
+        keep_part(a, p, n0, b, t, back, take, need);
     }
     if (tid == 0) {
         back[a.N] = static_cast<int32_t>(all_b);
         take[a.N] = static_cast<int32_t>(all_t);
     }
     __syncthreads();
-    return true;
+    return can(all_b, all_t);
 }
 
 // The sequence that page `i` is of.
@@ -120,17 +172,22 @@ __device__ __forceinline__ int32_t * table_to(const StepArgs & a, int n) {
     return const_cast<int32_t *>(table_of(a.tables, n));
 }
 
-__device__ __forceinline__ void give_back(const StepArgs & a, const int32_t * back, int32_t left, int32_t i) {
-    const int n     = sequence_of(back, a.N, i);
-    int32_t * entry = table_to(a, n) + pages_of(a, a.length[n]) + (i - back[n]);
-    a.free[left + back[a.N] - 1 - i] = *entry;
-    *entry                           = -1;
-}
-
-__device__ __forceinline__ void take_page(const StepArgs & a, const int32_t * back, const int32_t * take, int32_t left, int32_t k) {
-    const int n    = sequence_of(take, a.N, k);
-    const int held = pages_of(a, a.length[n]) - (take[n + 1] - take[n]);
-    table_to(a, n)[held + (k - take[n])] = a.free[left + back[a.N] - 1 - k];
+// Page number j of those given back, of those taken, or both.
+__device__ __forceinline__ void move_page(const StepArgs & a, const int32_t * back, const int32_t * take, const int32_t * need,
+                                          int32_t left, int32_t j) {
+    const int32_t all   = back[a.N];
+    const bool    from  = j < all;
+    const bool    to    = j < take[a.N];
+    const int     nb    = from ? sequence_of(back, a.N, j) : 0;
+    const int     nt    = to ? sequence_of(take, a.N, j) : 0;
+    int32_t *     stack = a.free + (left + all - 1 - j);
+    int32_t *     old   = table_to(a, nb) + need[nb] + (j - back[nb]);
+    int32_t *     now   = table_to(a, nt) + need[nt] - (take[nt + 1] - j);
+    const int32_t page  = *(from ? old : stack);
+    *(to ? now : stack) = page;
+    if (from) {
+        *old = -1;
+    }
 }
 
 __device__ __forceinline__ void refuse_step(const StepArgs & a) {
@@ -139,42 +196,38 @@ __device__ __forceinline__ void refuse_step(const StepArgs & a) {
     }
 }
 
-// After the sums, and before the tables of another workgroup are read.
-__device__ __forceinline__ void new_counts(const StepArgs & a, const int32_t * back, const int32_t * take, int32_t left) {
-    for (int n = threadIdx.x; n < a.N; n += kStepThreads) {
-        a.held[n] = pages_of(a, a.length[n]);
+// The whole step by one workgroup.
+template <int THREADS> __global__ __launch_bounds__(THREADS) void k_pages_step(const StepArgs a) {
+    extern __shared__ int32_t offsets[];
+    int32_t *     back = offsets;
+    int32_t *     take = offsets + a.N + 1;
+    int32_t *     need = take + a.N + 1;
+    const int32_t left = *a.left;
+    if (!step_sums<THREADS>(a, back, take, need, left)) {
+        refuse_step(a);
+        return;
+    }
+    const int32_t n = max(back[a.N], take[a.N]);
+    for (int32_t j = threadIdx.x; j < n; j += THREADS) {
+        move_page(a, back, take, need, left, j);
+    }
+    for (int i = threadIdx.x; i < a.N; i += THREADS) {
+        a.held[i] = need[i];
     }
     if (threadIdx.x == 0) {
         *a.left = left + back[a.N] - take[a.N];
     }
 }
 
-// The whole step by one workgroup.
-__global__ __launch_bounds__(kStepThreads) void k_pages_step(const StepArgs a) {
-    extern __shared__ int32_t offsets[];
-    int32_t *     back = offsets;
-    int32_t *     take = offsets + a.N + 1;
-    const int32_t left = *a.left;
-    if (!step_sums(a, back, take, left)) {
-        refuse_step(a);
-        return;
-    }
-    for (int32_t i = threadIdx.x; i < back[a.N]; i += kStepThreads) {
-        give_back(a, back, left, i);
-    }
-    __syncthreads();
-    for (int32_t k = threadIdx.x; k < take[a.N]; k += kStepThreads) {
-        take_page(a, back, take, left, k);
-    }
-    new_counts(a, back, take, left);
-}
+constexpr int kSumsThreads = 1024;
+constexpr int kMoveThreads = 256;
 
-__global__ __launch_bounds__(kStepThreads) void k_pages_sums(const StepArgs a) {
+__global__ __launch_bounds__(kSumsThreads) void k_pages_sums(const StepArgs a) {
     int32_t *     back  = a.work;
     int32_t *     take  = a.work + a.N + 1;
     int32_t *     state = take + a.N + 1;
     const int32_t left  = *a.left;
-    const bool    ok    = step_sums(a, back, take, left);
+    const bool    ok    = step_sums<kSumsThreads>(a, back, take, nullptr, left);
     if (threadIdx.x == 0) {
         state[0] = ok;
         state[1] = left;
@@ -183,23 +236,50 @@ __global__ __launch_bounds__(kStepThreads) void k_pages_sums(const StepArgs a) {
         refuse_step(a);
         return;
     }
-    new_counts(a, back, take, left);
+    // (every thread has read them)
+    for (int n = threadIdx.x; n < a.N; n += kSumsThreads) {
+        a.held[n] = pages_of(a, a.length[n]);
+    }
+    if (threadIdx.x == 0) {
+        *a.left = left + back[a.N] - take[a.N];
+    }
 }
 
-template <bool TAKE> __global__ __launch_bounds__(256) void k_pages_move(const StepArgs a) {
+// The pages after k_pages_sums; IN_LDS: what a page's place is found by is read once.
+template <bool IN_LDS> __global__ __launch_bounds__(kMoveThreads) void k_pages_move(const StepArgs a) {
+    extern __shared__ int32_t offsets[];
     const int32_t * back  = a.work;
     const int32_t * take  = a.work + a.N + 1;
+    const int32_t * need  = a.held;
     const int32_t * state = take + a.N + 1;
-    if (state[0] == 0) {
-        return;
+    const int32_t   left  = state[1];
+    const int32_t   n     = state[0] == 0 ? 0 : max(back[a.N], take[a.N]);
+    if constexpr (IN_LDS) {
+        auto keep = [&](int32_t * to, const int32_t * from, int count) {
+            constexpr int kAtOnce = 8;
+            for (int i = threadIdx.x; i < count; i += kAtOnce * kMoveThreads) {
+                int32_t x[kAtOnce];
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    x[k] = from[min(i + k * kMoveThreads, count - 1)];
+                }
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    if (i + k * kMoveThreads < count) {
+                        to[i + k * kMoveThreads] = x[k];
+                    }
+                }
+            }
+        };
+        keep(offsets, back, 2 * (a.N + 1));
+        keep(offsets + 2 * (a.N + 1), need, a.N);
+        back = offsets;
+        take = offsets + a.N + 1;
+        need = take + a.N + 1;
+        __syncthreads();
     }
-    const int32_t n = TAKE ? take[a.N] : back[a.N];
-    for (int32_t i = static_cast<int32_t>(blockIdx.x * blockDim.x + threadIdx.x); i < n; i += static_cast<int32_t>(gridDim.x * blockDim.x)) {
-        if constexpr (TAKE) {
-            take_page(a, back, take, state[1], i);
-        } else {
-            give_back(a, back, state[1], i);
-        }
+    for (int32_t j = static_cast<int32_t>(blockIdx.x * kMoveThreads + threadIdx.x); j < n; j += static_cast<int32_t>(gridDim.x * kMoveThreads)) {
+        move_page(a, back, take, need, left, j);
     }
 }
 
@@ -508,6 +588,8 @@ __global__ __launch_bounds__(kRowThreads) void k_kv_load_pages(const RowArgs a) 
 // One workgroup makes the step where its sums fit LDS and few table entries can change.
 constexpr int64_t kStepSeqs    = 4096;
 constexpr int64_t kStepEntries = int64_t{ 1 } << 16;
+constexpr int64_t kSmallEntries = 4096;
+constexpr int     kMoveGroups  = 256;
 
 bool one_group(const shp_tensor & table) {
     return table.ne[1] <= kStepSeqs && table.ne[0] * table.ne[1] <= kStepEntries;
@@ -636,22 +718,27 @@ extern "C" shp_status_t shp_kv_pages(const shp_tensor * length,
     a.N      = static_cast<int32_t>(n);
     a.pages  = static_cast<int32_t>(free_pages->ne[0]);
     a.shift  = page_shift(page);
-    const hipStream_t s = as_stream(stream);
+    const hipStream_t s   = as_stream(stream);
+    const size_t      lds = static_cast<size_t>(3 * n + 2) * 4;
     if (ints == 0) {
-        hipLaunchKernelGGL(k_pages_step, dim3(1), dim3(kStepThreads), 2 * (n + 1) * 4, s, a);
+        if (table->ne[0] * n <= kSmallEntries) {
+            hipLaunchKernelGGL(k_pages_step<256>, dim3(1), dim3(256), lds, s, a);
+        } else {
+            hipLaunchKernelGGL(k_pages_step<1024>, dim3(1), dim3(1024), lds, s, a);
+        }
         return launch_status();
     }
-    hipLaunchKernelGGL(k_pages_sums, dim3(1), dim3(kStepThreads), 0, s, a);
+    hipLaunchKernelGGL(k_pages_sums, dim3(1), dim3(kSumsThreads), 0, s, a);
     st = launch_status();
-    if (st == SHP_OK) {
-        hipLaunchKernelGGL(k_pages_move<false>, dim3(256), dim3(256), 0, s, a);
-        st = launch_status();
+    if (st != SHP_OK) {
+        return st;
     }
-    if (st == SHP_OK) {
-        hipLaunchKernelGGL(k_pages_move<true>, dim3(256), dim3(256), 0, s, a);
-        st = launch_status();
+    if (n <= kStepSeqs) {
+        hipLaunchKernelGGL(k_pages_move<true>, dim3(kMoveGroups), dim3(kMoveThreads), lds, s, a);
+    } else {
+        hipLaunchKernelGGL(k_pages_move<false>, dim3(kMoveGroups), dim3(kMoveThreads), 0, s, a);
     }
-    return st;
+    return launch_status();
 }
 
 extern "C" shp_status_t shp_kv_slots(const shp_tensor * table,

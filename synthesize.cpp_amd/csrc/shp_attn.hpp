@@ -525,21 +525,6 @@ __device__ __forceinline__ int few_units(const FewArgs & f, int n) {
     return len.count == 0 ? 0 : max(static_cast<int>(fastdiv(static_cast<uint32_t>(few_tiles(f, len).n + f.per - 1), f.fper)), 1);
 }
 
-// The sum of a wave's lanes up to and with this one.
-__device__ __forceinline__ int32_t sum_up_to(int32_t v) {
-    auto below = [](int32_t x, auto ctrl, auto rows) {
-        return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
-    };
-    using All = std::integral_constant<int, 0xF>;
-    v += below(v, std::integral_constant<int, 0x111>{}, All{});  // row_shr:1, 2, 4, 8
-    v += below(v, std::integral_constant<int, 0x112>{}, All{});
-    v += below(v, std::integral_constant<int, 0x114>{}, All{});
-    v += below(v, std::integral_constant<int, 0x118>{}, All{});
-    v += below(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15
-    v += below(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31
-    return v;
-}
-
 // The sequence that a unit of the line falls in.
 struct Place {
     int32_t n;

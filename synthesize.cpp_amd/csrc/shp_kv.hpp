@@ -2,6 +2,8 @@
 // their rows, and the checks of a cache's descriptor.
 #pragma once
 
+#include <type_traits>
+
 #include "shp_internal.hpp"
 
 namespace shp {
@@ -72,6 +74,21 @@ template <int KIND> __device__ __forceinline__ float kv_value(const char * row, 
             return static_cast<float>((j < 16 ? byte & 15 : byte >> 4) - 8) * d;
         }
     }
+}
+
+// The sum of a wave's lanes up to and with this one.
+__device__ __forceinline__ int32_t sum_up_to(int32_t v) {
+    auto below = [](int32_t x, auto ctrl, auto rows) {
+        return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+    };
+    using All = std::integral_constant<int, 0xF>;
+    v += below(v, std::integral_constant<int, 0x111>{}, All{});  // row_shr:1, 2, 4, 8
+    v += below(v, std::integral_constant<int, 0x112>{}, All{});
+    v += below(v, std::integral_constant<int, 0x114>{}, All{});
+    v += below(v, std::integral_constant<int, 0x118>{}, All{});
+    v += below(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15
+    v += below(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31
+    return v;
 }
 
 // ---------------------------------------------------------------------------
