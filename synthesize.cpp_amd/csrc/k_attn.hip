@@ -477,9 +477,9 @@ shp_status_t attn_args(const shp_tensor *         q,
     return SHP_OK;
 }
 
-// Row tiles of kWideRows for a chip that holds `chip` workgroups, `per` key tiles a split.
-void wide_args(int32_t per, int64_t chip, AttnArgs & a) {
-    a.tiles              = static_cast<int32_t>((static_cast<int64_t>(a.T) * a.G + kWideRows - 1) / kWideRows);
+// Tiles of `rows` rows for a chip that holds `chip` workgroups, `per` key tiles a split.
+void wide_args(int32_t per, int32_t rows, int64_t chip, AttnArgs & a) {
+    a.tiles              = static_cast<int32_t>((static_cast<int64_t>(a.T) * a.G + rows - 1) / rows);
     a.per                = per;
     a.fper               = make_fastdiv(static_cast<uint32_t>(a.per));
     const int64_t groups = static_cast<int64_t>(a.tiles) * a.KV;
@@ -557,7 +557,7 @@ shp_status_t attn(const shp_tensor * q,
             const int64_t most = (a.cap + kTileKeys - 1) / kTileKeys + 2;
             per                = static_cast<int32_t>((most + a.nsplit - 1) / a.nsplit);
         }
-        wide_args(per, wide_groups(a.hd), a);
+        wide_args(per, kWideRows, wide_groups(a.hd), a);
         st = launch_attn_wide(kind, a, s);
         return st == SHP_OK && a.nsplit > 1 ? launch_join(a, s) : st;
     }

@@ -29,10 +29,21 @@ struct PagesArgs {
     Tables  tables;
 };
 
-// Sixteen codes as two operands.
+// Eight codes as an operand: with their top bits turned they are code + 128, which
+// under the exponent bytes of 1024 is 1152 + code.
 __device__ __forceinline__ f16x8 operand(const Magic & m, uint32_t w0, uint32_t w1) {
-    const uint32_t w[2] = { w0, w1 };
-    return Codes<kKvQ8>::k_codes(m, w);
+    constexpr uint32_t kLow = 0x05010500u, kHigh = 0x05030502u;  // bytes 0 and 1, or 2 and 3, each below the exponent's
+    auto               two  = [&](uint32_t w, uint32_t which) { return as_f16x2(__builtin_amdgcn_perm(m.e1024, w, which)) - splat2(1152.0f); };
+    const uint32_t     a    = w0 ^ 0x80808080u;
+    const uint32_t     b    = w1 ^ 0x80808080u;
+    return join8(two(a, kLow), two(a, kHigh), two(b, kLow), two(b, kHigh));
+}
+
+// split2() in fewer instructions: the rest by a mixed multiply-add, which is exact as well.
+__device__ __forceinline__ void split_weights(float a, float b, f16x2 & hi, f16x2 & lo) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    hi = __builtin_convertvector((f32x2{ a, b }), f16x2);
+    lo = __builtin_convertvector((f32x2{ __builtin_fmaf(static_cast<float>(hi[0]), -1.0f, a), __builtin_fmaf(static_cast<float>(hi[1]), -1.0f, b) }), f16x2);
 }
 
 // A page's number, or what it is to be read as: 0 for one outside the pool.
@@ -50,9 +61,14 @@ __device__ __forceinline__ int32_t entry_of(const PagesArgs & p, const int32_t *
     return table[min(row >> p.pool.shift, p.tables.most - 1)];
 }
 
+// A block's scale as it is read. (What it counts as is formed where it is used: that waits
+// for the load.)
 __device__ __forceinline__ float scale_at(const PoolSide & s, const PageId & page, int h) {
-    const float d = s.scale[page.id * s.sp + h];
-    return page.in ? block_scale(d) : NAN;
+    return s.scale[page.id * s.sp + h];
+}
+
+__device__ __forceinline__ float scale_of(float read, bool in) {
+    return in ? block_scale(read) : NAN;
 }
 
 // d_k times what brings q back, within what is a normal number: with sums of
@@ -160,6 +176,7 @@ __global__ __launch_bounds__(64 * kPageWaves, HD <= 128 ? 2 : 1) void k_attn_pag
         u32x4   kr[4][KS];
         u32x4   vr[TILES];
         float   dk = 0.0f, dv = 0.0f;
+        bool    in = true;  // (of K's and V's scales: one block)
         auto    first_of = [&](int32_t tile) { return key_tile(kt, tile) * kPageChunk; };
         auto    entries  = [&](int32_t tile) {
             const int32_t j0 = first_of(tile);
@@ -170,7 +187,9 @@ __global__ __launch_bounds__(64 * kPageWaves, HD <= 128 ? 2 : 1) void k_attn_pag
             const int32_t j0   = first_of(tile);
             const PageId  id   = page_id(p, ke);
             const char *  from = kb + id.id * ks.cp + (((j0 + krow) & (page - 1)) + (c & 3)) * hd;
-            dk                 = scale_at(ks, page_id(p, ve), h);
+            const PageId  own  = page_id(p, ve);
+            dk                 = scale_at(ks, own, h);
+            in                 = own.in;
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
 #pragma unroll
@@ -257,8 +276,8 @@ __global__ __launch_bounds__(64 * kPageWaves, HD <= 128 ? 2 : 1) void k_attn_pag
                     sc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[x], ql[s], sc[x], 0, 0, 0);
                 }
             }
-            const float by = score_scale(dk, qscale);
-            const float d  = dv;
+            const float by = score_scale(scale_of(dk, in), qscale);
+            const float d  = scale_of(dv, in);
             if constexpr (MORE) {
                 fetch_k(i + kPageWaves);
             }
@@ -313,8 +332,8 @@ __global__ __launch_bounds__(64 * kPageWaves, HD <= 128 ? 2 : 1) void k_attn_pag
                     l += w[e];
                     w[e] *= wf;
                 }
-                split2(w[0], w[1], ph[2 * y], pl[2 * y]);
-                split2(w[2], w[3], ph[2 * y + 1], pl[2 * y + 1]);
+                split_weights(w[0], w[1], ph[2 * y], pl[2 * y]);
+                split_weights(w[2], w[3], ph[2 * y + 1], pl[2 * y + 1]);
             }
             constexpr int kAtOnce = 4;  // tiles of V whose products take turns
 #pragma unroll
@@ -436,35 +455,61 @@ template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join_pa
 }
 
 // ---------------------------------------------------------------------------
-// Many queries (prompts): 128 rows a workgroup, 32 a wave, 64 tokens at a time,
-// which it brings into LDS as F16 operands, K by row and V by column, both as the
-// pool has them. Matrix instructions 32x32x16.
+// Many queries (prompts): a workgroup of four waves, in KG groups side by side. A wave
+// has 32 rows, and a group 64 tokens at a time, every KG-th tile of them, which it brings
+// into LDS as F16 operands, K by row and V by column, both as the pool has them: the next
+// tile while this one's scores are formed, so that a tile takes one barrier, and the one
+// after that is on its way in registers. Matrix instructions 32x32x16. With KG 1 a
+// workgroup has 128 rows, which share a tile; with 2 it has 64, and its groups' results are
+// joined in LDS.
+// 8192 positions of 16 heads of 128 over 8 take 520 to 535 us (MI355X): two products at
+// 1.03 to 1.06 PFLOP/s, where a large F16 product reaches 1.14, at the clock that such work
+// leaves the chip. Two barriers a tile, with the tile brought into LDS between them: 575;
+// scales made ready as they are read, which waits for them: 15 us of 526. A lone
+// workgroup's tile takes 2.0 us, of which the matrix units work 0.9: 1021 positions 33 us.
 // ---------------------------------------------------------------------------
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWideBlock = 256;
+constexpr int kWaves     = kWideBlock / kWave;
 constexpr int kVStride   = kTileKeys * 2 + 16;  // bytes of a column of V in LDS, off the banks' period
 
 constexpr int key_stride(int nb) {
     return nb * kKvBlock * 2 + 16;
 }
 
-constexpr int wide_lds(int nb) {
+// LDS of a group's tile; of two tiles of each, or of the results of all groups but the first.
+constexpr int tile_lds(int nb) {
     return kTileKeys * key_stride(nb) + nb * kKvBlock * kVStride;
 }
 
-template <int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2 : 1) void k_attn_pages_wide(const PagesArgs p) {
+constexpr int wide_lds(int nb, int kg) {
+    const int tiles = kg * 2 * tile_lds(nb);
+    const int join  = (kWaves - kWaves / kg) * kWave * (nb * 64 + 16);
+    return tiles > join ? tiles : join;
+}
+
+// The value that lane K of each four has.
+template <int K> __device__ __forceinline__ int32_t quad(int32_t v) {
+    return static_cast<int32_t>(dpp_u32<K * 0x55>(static_cast<uint32_t>(v)));
+}
+
+// hd is 32 NB, or (FULL false) 16 less.
+template <int NB, int KG, bool FULL>
+__global__ __launch_bounds__(kWideBlock, NB <= 4 && KG == 1 ? 2 : 1) void k_attn_pages_wide(const PagesArgs p) {
     constexpr int HD      = NB * kKvBlock;
     constexpr int KSTRIDE = key_stride(NB);
+    constexpr int ROWS    = 32 * kWaves / KG;     // of the workgroup
+    constexpr int GROUP   = kWideBlock / KG;      // threads of a group
     extern __shared__ __align__(16) char lds[];
-    const AttnArgs & a  = p.f.a;
-    char * const     kl = lds;
-    char * const     vl = lds + kTileKeys * KSTRIDE;
+    const AttnArgs & a = p.f.a;
 
-    const int     tid   = threadIdx.x;
+    const int     tid   = threadIdx.x % GROUP;
+    const int     kg    = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / GROUP);
     const int     wave  = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int     lane  = tid % kWave;
+    char * const  mem   = lds + kg * 2 * tile_lds(NB);  // of the group: two tiles in turn
     const int     c     = lane & 31;
     const int     g     = lane >> 5;
     const int     part0 = static_cast<int>(fastdiv(blockIdx.x, a.fKV));
@@ -475,16 +520,16 @@ template <int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2 : 1) void
     const int     n     = blockIdx.y;
     const SeqLens len   = seq_lens(a, n);
     auto          t_of  = [&](int r) { return static_cast<int>(fastdiv(static_cast<uint32_t>(r), a.fG)); };
-    const int     t0    = t_of(tile * kWideRows);
+    const int     t0    = t_of(tile * ROWS);
     if (t0 >= len.count) {
         return;
     }
     const Magic   magic;
     const int32_t base = len.length - len.count;
     const int32_t p0   = base + t0;
-    const int32_t p1   = base + min(t_of(tile * kWideRows + kWideRows - 1), len.count - 1);
+    const int32_t p1   = base + min(t_of(tile * ROWS + ROWS - 1), len.count - 1);
     // this wave's positions, and this lane's query
-    const int     r0   = tile * kWideRows + wave * 32;
+    const int     r0   = tile * ROWS + wave * 32;
     const int32_t w0   = base + t_of(r0);
     const int32_t w1   = t_of(r0) < len.count ? base + min(t_of(r0 + 31), len.count - 1) : -1;
     const int     r    = r0 + c;
@@ -496,74 +541,92 @@ template <int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2 : 1) void
 
     const KeyTiles kt  = key_tiles<kTileKeys>(a, p0, p1);
     const int      beg = split * a.per;
-    const int      end = min(kt.n, beg + a.per);
+    const int      end = __builtin_amdgcn_readfirstlane(min(kt.n, beg + a.per));
     if (split > 0 && beg >= kt.n) {
         return;
     }
     const int dest = __builtin_amdgcn_readfirstlane(kt.n <= a.per ? -1 : split);
 
-    // Of a tile, thread id takes 16 bytes of K's row id / (HD/16), z times 256 threads
-    // on, and of V's column id / 4 the sixteen tokens id % 4.
+    // Of a tile, thread id of its group takes 16 bytes of K's row id / (HD/16), z times
+    // GROUP threads on, and of V's column id / 4 the sixteen tokens id % 4.
     constexpr int    ALL    = kTileKeys * (HD / 16);
-    constexpr int    CHUNKS = (ALL + kWideBlock - 1) / kWideBlock;  // of each, a thread
-    auto             mine   = [&](int z) { return ALL % kWideBlock == 0 || tid + kWideBlock * z < ALL; };
-    const int        hd    = a.hd;
-    const int        page  = 1 << p.pool.shift;
-    const PoolSide & ks    = p.pool.side[0];
-    const PoolSide & vs    = p.pool.side[1];
-    const char *     kb    = ks.codes + h * ks.ch;
-    const char *     vb    = vs.codes + h * vs.ch;
-    const int32_t *  table = table_of(p.tables, n);
-    auto             row_k  = [&](int z) { return (tid + kWideBlock * z) / (HD / 16); };
-    auto             dim_of = [&](int z) { return (tid + kWideBlock * z) % (HD / 16) * 16; };
+    constexpr int    CHUNKS = (ALL + GROUP - 1) / GROUP;  // of each, a thread
+    auto             mine   = [&](int z) { return ALL % GROUP == 0 || tid + GROUP * z < ALL; };
+    const int        hd     = FULL ? HD : a.hd;
+    const int        page   = 1 << p.pool.shift;
+    const PoolSide & ks     = p.pool.side[0];
+    const PoolSide & vs     = p.pool.side[1];
+    const char *     kb     = ks.codes + h * ks.ch;
+    const char *     vb     = vs.codes + h * vs.ch;
+    const int32_t *  table  = table_of(p.tables, n);
+    auto             row_k  = [&](int z) { return (tid + GROUP * z) / (HD / 16); };
+    auto             dim_of = [&](int z) { return (tid + GROUP * z) % (HD / 16) * 16; };
 
-    int32_t ke[CHUNKS], ve, se[2];
+    // The table's entries for a tile's four times sixteen rows, in the lanes k and k + 4 j,
+    // which read the scales too.
+    int32_t entry = 0;
     u32x4   kr[CHUNKS], vr[CHUNKS];
-    float   dk[2], dv[2];
-    auto    entries = [&](int i) {
-        const int32_t j0 = key_tile(kt, i) * kTileKeys;
+    float   dk = 0.0f, dv = 0.0f;
+    bool    in = true;
+    auto    at      = [&](int i) { return __builtin_amdgcn_readfirstlane(key_tile(kt, min(i, end - 1)) * kTileKeys); };
+    auto    entries = [&](int i) { entry = entry_of(p, table, at(i) + lane % 4 * 16); };
+    auto    fetch   = [&](int i) {
+        const int32_t j0    = at(i);
+        const PageId  id    = page_id(p, entry);
+        const int32_t of[4] = { quad<0>(id.id), quad<1>(id.id), quad<2>(id.id), quad<3>(id.id) };
 #pragma unroll
         for (int z = 0; z < CHUNKS; ++z) {
-            ke[z] = entry_of(p, table, j0 + row_k(z));
-        }
-        ve = entry_of(p, table, j0 + tid % 4 * 16);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            se[x] = entry_of(p, table, j0 + 32 * x + 16 * g);
-        }
-    };
-    auto fetch = [&](int i) {
-        const int32_t j0 = key_tile(kt, i) * kTileKeys;
-#pragma unroll
-        for (int z = 0; z < CHUNKS; ++z) {
-            const int dim = dim_of(z);
-            kr[z]         = u32x4{};
-            if (mine(z) && dim < hd) {
-                kr[z] = *reinterpret_cast<const u32x4 *>(kb + page_id(p, ke[z]).id * ks.cp + ((j0 + row_k(z)) & (page - 1)) * hd + dim);
+            const int     row  = row_k(z);
+            const int32_t low  = row & 16 ? of[1] : of[0];
+            const int32_t high = row & 16 ? of[3] : of[2];
+            const char *  from = kb + (row & 32 ? high : low) * ks.cp + ((j0 + row) & (page - 1)) * hd + dim_of(z);
+            if (FULL && ALL % GROUP == 0) {
+                kr[z] = *reinterpret_cast<const u32x4 *>(from);
+            } else {
+                kr[z] = u32x4{};
+                if (mine(z) && dim_of(z) < hd) {
+                    kr[z] = *reinterpret_cast<const u32x4 *>(from);
+                }
             }
         }
-        const char * from = vb + page_id(p, ve).id * vs.cp + ((j0 + tid % 4 * 16) & (page - 1));
+        const char * from = vb + id.id * vs.cp + ((j0 + tid % 4 * 16) & (page - 1));
 #pragma unroll
         for (int z = 0; z < CHUNKS; ++z) {
-            const int dim = tid / 4 + kWideBlock / 4 * z;
-            vr[z]         = u32x4{};
-            if (mine(z) && dim < hd) {
+            const int dim = tid / 4 + GROUP / 4 * z;
+            if (FULL && ALL % GROUP == 0) {
                 vr[z] = *reinterpret_cast<const u32x4 *>(from + dim * page);
+            } else {
+                vr[z] = u32x4{};
+                if (mine(z) && dim < hd) {
+                    vr[z] = *reinterpret_cast<const u32x4 *>(from + dim * page);
+                }
             }
         }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const PageId id = page_id(p, se[x]);
-            dk[x]           = scale_at(ks, id, h);
-            dv[x]           = scale_at(vs, id, h);
+        dk = scale_at(ks, id, h);
+        dv = scale_at(vs, id, h);
+        in = id.in;
+    };
+    // part of a tile's 4 CHUNKS into LDS: half an id's sixteen codes of K, then of V
+    auto stage_part = [&](char * kl, int part) {
+        const int z = part / 2 % CHUNKS, half = part % 2;
+        if (!mine(z)) {
+            return;
+        }
+        if (part < 2 * CHUNKS) {
+            const int row = row_k(z);
+            const int in  = (row & 32) + 8 * (row >> 2 & 3) + 4 * (row >> 4 & 1) + (row & 3);
+            reinterpret_cast<f16x8 *>(kl + in * KSTRIDE + 2 * dim_of(z))[half] = operand(magic, kr[z][2 * half], kr[z][2 * half + 1]);
+        } else {
+            char * vl = kl + kTileKeys * KSTRIDE;
+            reinterpret_cast<f16x8 *>(vl + (tid / 4 + GROUP / 4 * z) * kVStride + tid % 4 * 32)[half] =
+                operand(magic, vr[z][2 * half], vr[z][2 * half + 1]);
         }
     };
+    // (past its last tile a group reads that again, and nothing of it counts)
     if (beg < end) {
-        entries(beg);
-        fetch(beg);
-        if (beg + 1 < end) {
-            entries(beg + 1);
-        }
+        entries(beg + kg);
+        fetch(beg + kg);
+        entries(beg + kg + KG);
     }
 
     // the query's operands; the largest of its values scaled to [2^13, 2^14)
@@ -615,48 +678,37 @@ template <int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2 : 1) void
         return fmaxf(both.a, both.b);
     };
 
-    for (int i = beg; i < end; ++i) {
-        const int32_t j0 = key_tile(kt, i) * kTileKeys;
-        __syncthreads();  // the tile before is used up
+    // (group 2 y + g of a tile)
+    auto of_group = [&](float v, int y) {
+        const float one   = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 2 * y));
+        const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 2 * y + 1));
+        return g == 0 ? one : other;
+    };
+    float kscale[2], vscale[2];
+    if (beg < end) {
 #pragma unroll
-        for (int z = 0; z < CHUNKS; ++z) {
-            if (!mine(z)) {
-                continue;
-            }
-            const int row = row_k(z);
-            const int in  = (row & 32) + 8 * (row >> 2 & 3) + 4 * (row >> 4 & 1) + (row & 3);
-            f16x8 *   to  = reinterpret_cast<f16x8 *>(kl + in * KSTRIDE + 2 * dim_of(z));
-            to[0]         = operand(magic, kr[z][0], kr[z][1]);
-            to[1]         = operand(magic, kr[z][2], kr[z][3]);
+        for (int part = 0; part < 4 * CHUNKS; ++part) {
+            stage_part(mem, part);
         }
-#pragma unroll
-        for (int z = 0; z < CHUNKS; ++z) {
-            if (!mine(z)) {
-                continue;
-            }
-            f16x8 * to = reinterpret_cast<f16x8 *>(vl + (tid / 4 + kWideBlock / 4 * z) * kVStride + tid % 4 * 32);
-            to[0]      = operand(magic, vr[z][0], vr[z][1]);
-            to[1]      = operand(magic, vr[z][2], vr[z][3]);
-        }
-        float by[2], d[2];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-            by[y] = score_scale(dk[y], qscale);
-            d[y]  = dv[y];
+            kscale[y] = score_scale(of_group(scale_of(dk, in), y), qscale);
+            vscale[y] = of_group(scale_of(dv, in), y);
         }
-        if (i + 1 < end) {
-            fetch(i + 1);
-            if (i + 2 < end) {
-                entries(i + 2);
-            }
-        }
-        __syncthreads();
-        if (j0 > w1) {
-            continue;  // none of it is seen by this wave's queries
-        }
-        // scores of token 32 y + 16 g + e
+        fetch(beg + kg + KG);
+        entries(beg + kg + 2 * KG);
+    }
+    char * kl = mem;
+    for (int first = beg; first < end; first += KG) {
+        const int     i  = first + kg;
+        const int32_t j0 = at(i);
+        char * const  vl = kl + kTileKeys * KSTRIDE;
+        __syncthreads();  // this tile is in LDS, and the one before is used up
+        // scores of token 32 y + 16 g + e, and under their products the next tile on its
+        // way into LDS and the one after that into registers
         __builtin_amdgcn_s_setprio(1);
-        f32x16 sc[2] = { f32x16{}, f32x16{} };
+        char * const other = kl == mem ? mem + tile_lds(NB) : mem;
+        f32x16       sc[2] = { f32x16{}, f32x16{} };
 #pragma unroll
         for (int s = 0; s < 2 * NB; ++s) {
             f16x8 k[2];
@@ -672,10 +724,24 @@ template <int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2 : 1) void
             for (int y = 0; y < 2; ++y) {
                 sc[y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[y], ql[s], sc[y], 0, 0, 0);
             }
+#pragma unroll
+            for (int part = 4 * CHUNKS * s / (2 * NB); part < 4 * CHUNKS * (s + 1) / (2 * NB); ++part) {
+                stage_part(other, part);
+            }
         }
+        kl = other;
+        const float by_now[2] = { kscale[0], kscale[1] }, d_now[2] = { vscale[0], vscale[1] };
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            kscale[y] = score_scale(of_group(scale_of(dk, in), y), qscale);
+            vscale[y] = of_group(scale_of(dv, in), y);
+        }
+        fetch(i + 2 * KG);
+        entries(i + 3 * KG);
         __builtin_amdgcn_s_setprio(0);
-        sc[0] *= by[0];
-        sc[1] *= by[1];
+        if (i >= end || j0 > w1) {
+            continue;  // none of it is seen by this wave's queries
+        }
         const bool all = j0 + kTileKeys - 1 <= w0 && (a.window == 0 || j0 > w1 - a.window || j0 + kTileKeys <= a.sinks);
         if (!all) {
             int g16 = 16 * g;
@@ -688,7 +754,7 @@ template <int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2 : 1) void
                 }
             }
         }
-        float top[2];
+        float top[2], times[2];
         bool  any[2];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
@@ -697,13 +763,25 @@ template <int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2 : 1) void
             for (int e = 0; e < 16; ++e) {
                 top[y] = fmaxf(top[y], sc[y][e]);
             }
-            any[y] = top[y] != -INFINITY;
+            any[y]   = top[y] != -INFINITY;
+            times[y] = any[y] ? by_now[y] : 1.0f;  // (a scale of tokens that are not seen may be NaN)
+            top[y] *= times[y];
         }
         const float most = fmaxf(m, max_halves(fmaxf(top[0], top[1])));
         const float ref  = most == -INFINITY ? 0.0f : most;
         const float down = m - ref;
-        const float need = max_halves(fmaxf(top[0] - ref + static_cast<float>(exponent_of(d[0])),
-                                            top[1] - ref + static_cast<float>(exponent_of(d[1]))));
+        // A score is rounded with the difference from the largest, which leaves it above 0
+        // by half a step of the largest score at most: 1/16 here. From there on it is
+        // rounded before.
+        if (__any(fabsf(ref) >= 0x1p20f)) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                sc[y] *= times[y];
+                times[y] = 1.0f;
+            }
+        }
+        const float need = max_halves(fmaxf(top[0] - ref + static_cast<float>(exponent_of(d_now[0])),
+                                            top[1] - ref + static_cast<float>(exponent_of(d_now[1]))));
         const float now  = fmaxf(fmaxf(x + down, need), kLeastX);
         if (__any(down != 0.0f || now != x)) {
             l *= __builtin_amdgcn_exp2f(down);
@@ -715,43 +793,94 @@ template <int NB> __global__ __launch_bounds__(kWideBlock, NB <= 4 ? 2 : 1) void
         }
         m = most;
         x = now;
+        const float wf[2] = { weight_scale(d_now[0], x, any[0]), weight_scale(d_now[1], x, any[1]) };
+        // weights of the sixteen tokens 32 y + 16 s + 8 g + .. (part 2 y + s of four)
+        f16x8 ph[2], pl[2];
+        auto  weigh = [&](int part) {
+            const int y = part / 2, s = part % 2;
+            f16x2     hi[4], lo[4];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            const float wf = weight_scale(d[y], x, any[y]);
+            for (int e = 0; e < 4; ++e) {
+                float w[2];
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                f16x2 hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float w[2];
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        w[k] = __builtin_amdgcn_exp2f(sc[y][8 * s + 2 * e + k] - ref);
-                        l += w[k];
-                        w[k] *= wf;
-                    }
-                    split2(w[0], w[1], hi[e], lo[e]);
+                for (int k = 0; k < 2; ++k) {
+                    w[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[y][8 * s + 2 * e + k], times[y], -ref));
+                    l += w[k];
+                    w[k] *= wf[y];
                 }
-                const f16x8 ph = join8(hi[0], hi[1], hi[2], hi[3]);
-                const f16x8 pl = join8(lo[0], lo[1], lo[2], lo[3]);
-                f16x8       v[NB];
+                split_weights(w[0], w[1], hi[e], lo[e]);
+            }
+            ph[part % 2] = join8(hi[0], hi[1], hi[2], hi[3]);
+            pl[part % 2] = join8(lo[0], lo[1], lo[2], lo[3]);
+        };
+        weigh(0);
 #pragma unroll
-                for (int u = 0; u < NB; ++u) {
-                    v[u] = *reinterpret_cast<const f16x8 *>(vl + (32 * u + c) * kVStride + 64 * y + 32 * g + 16 * s);
-                }
+        for (int part = 0; part < 4; ++part) {
+            f16x8 v[NB];
 #pragma unroll
-                for (int u = 0; u < NB; ++u) {
-                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[u], ph, o[u], 0, 0, 0);
-                }
+            for (int u = 0; u < NB; ++u) {
+                v[u] = *reinterpret_cast<const f16x8 *>(vl + (32 * u + c) * kVStride + 64 * (part / 2) + 32 * g + 16 * (part % 2));
+            }
 #pragma unroll
-                for (int u = 0; u < NB; ++u) {
-                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[u], pl, o[u], 0, 0, 0);
-                }
+            for (int u = 0; u < NB; ++u) {
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[u], ph[part % 2], o[u], 0, 0, 0);
+            }
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[u], pl[part % 2], o[u], 0, 0, 0);
+            }
+            if (part < 3) {
+                weigh(part + 1);
             }
         }
     }
     const Pair sum = swap32(l);
     l              = sum.a + sum.b;
+    if constexpr (KG > 1) {
+        // the first group takes the others' results from LDS: [group and wave][tile, four
+        // elements][lane], and m, l and x of a lane
+        constexpr int WAVES = kWaves / KG;
+        f32x4 *       of    = reinterpret_cast<f32x4 *>(lds);
+        f32x4 *       mlx   = of + (kWaves - WAVES) * NB * 4 * kWave;
+        auto          slot  = [&](int group) { return (group - 1) * WAVES + wave; };
+        __syncthreads();
+        if (kg > 0) {
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    of[((slot(kg) * NB + u) * 4 + e) * kWave + lane] = f32x4{ o[u][4 * e], o[u][4 * e + 1], o[u][4 * e + 2], o[u][4 * e + 3] };
+                }
+            }
+            mlx[slot(kg) * kWave + lane] = f32x4{ m, l, x, 0.0f };
+        }
+        __syncthreads();
+        if (kg > 0) {
+            return;
+        }
+#pragma unroll
+        for (int group = 1; group < KG; ++group) {
+            const f32x4 its  = mlx[slot(group) * kWave + lane];
+            const float most = fmaxf(m, its[0]);
+            const float ref  = most == -INFINITY ? 0.0f : most;
+            const float xa = m - ref + x, xb = its[0] - ref + its[2];
+            l   = l * __builtin_amdgcn_exp2f(m - ref) + its[1] * __builtin_amdgcn_exp2f(its[0] - ref);
+            m   = most;
+            x   = fmaxf(fmaxf(xa, xb), kLeastX);
+            const float ta = __builtin_amdgcn_exp2f(xa - x), tb = __builtin_amdgcn_exp2f(xb - x);
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f32x4 v = of[((slot(group) * NB + u) * 4 + e) * kWave + lane];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        o[u][4 * e + k] = o[u][4 * e + k] * ta + v[k] * tb;
+                    }
+                }
+            }
+        }
+    }
     if (!live) {
         return;
     }
@@ -839,6 +968,19 @@ shp_status_t plan_pages(const shp_tensor * q, const shp_tensor * k, const shp_te
         p.wgs              = static_cast<int32_t>(want < chip ? want : chip);
     } else {
         plan_spans(rows, T, cap, keys, kv * q->ne[3], chip, true, p);
+        // Two groups of a workgroup rather than splits, whose results go through memory
+        // and a second launch, while a head has few tiles for the rows that there are:
+        // 512 positions take 20.2 us, 22.2 in splits (16 heads of 128 over 8, MI355X), 1021
+        // 32.8, 37.1; but 128 over 768 rows 24.8, 19.9, and 20 over 512 19.0, 14.6. One
+        // workgroup of this kind fits a CU.
+        const int64_t most   = (keys + kTileKeys - 1) / kTileKeys + (p.window > 0 ? 2 : 0);
+        const int64_t groups = (rows + kWideRows / 2 - 1) / (kWideRows / 2) * kv * q->ne[3];
+        p.groups             = 1;
+        if (q->ne[0] % kKvBlock == 0 && q->ne[0] <= 4 * kKvBlock && groups <= 256 && most > 1 && most <= 5 + groups / 20) {
+            p.groups = 2;
+            p.span   = static_cast<int32_t>(most);
+            p.nsplit = 1;
+        }
     }
     return SHP_OK;
 }
@@ -861,12 +1003,24 @@ template <int HD> shp_status_t launch_few(const PagesArgs & p, hipStream_t strea
     return p.f.a.hd == HD ? launch_few_as<HD, true>(p, stream) : launch_few_as<HD, false>(p, stream);
 }
 
-template <int NB> shp_status_t launch_wide(const PagesArgs & p, hipStream_t stream) {
+template <int NB, int KG, bool FULL> shp_status_t launch_wide_as(const PagesArgs & p, hipStream_t stream) {
     const AttnArgs & a = p.f.a;
     const dim3       grid(static_cast<unsigned>(a.KV) * static_cast<unsigned>(a.tiles) * static_cast<unsigned>(a.nsplit),
                           static_cast<unsigned>(a.N));
-    hipLaunchKernelGGL(k_attn_pages_wide<NB>, grid, dim3(kWideBlock), wide_lds(NB), stream, p);
+    hipLaunchKernelGGL((k_attn_pages_wide<NB, KG, FULL>), grid, dim3(kWideBlock), wide_lds(NB, KG), stream, p);
     return launch_status();
+}
+
+template <int NB> shp_status_t launch_wide(const PagesArgs & p, int kg, hipStream_t stream) {
+    if (p.f.a.hd < NB * kKvBlock) {
+        return launch_wide_as<NB, 1, false>(p, stream);
+    }
+    if constexpr (NB <= 4) {
+        if (kg == 2) {
+            return launch_wide_as<NB, 2, true>(p, stream);
+        }
+    }
+    return launch_wide_as<NB, 1, true>(p, stream);
 }
 
 }  // namespace
@@ -946,31 +1100,31 @@ extern "C" shp_status_t shp_attn_pages(const shp_tensor * q,
                a.hd <= 192 ? launch_few<192>(p, s) :
                              launch_few<256>(p, s);
     }
-    wide_args(plan.span, resident(a.hd), a);
+    wide_args(plan.span, kWideRows / plan.groups, resident(a.hd), a);
     switch ((a.hd + kKvBlock - 1) / kKvBlock) {
         case 1:
-            st = launch_wide<1>(p, s);
+            st = launch_wide<1>(p, plan.groups, s);
             break;
         case 2:
-            st = launch_wide<2>(p, s);
+            st = launch_wide<2>(p, plan.groups, s);
             break;
         case 3:
-            st = launch_wide<3>(p, s);
+            st = launch_wide<3>(p, plan.groups, s);
             break;
         case 4:
-            st = launch_wide<4>(p, s);
+            st = launch_wide<4>(p, plan.groups, s);
             break;
         case 5:
-            st = launch_wide<5>(p, s);
+            st = launch_wide<5>(p, plan.groups, s);
             break;
         case 6:
-            st = launch_wide<6>(p, s);
+            st = launch_wide<6>(p, plan.groups, s);
             break;
         case 7:
-            st = launch_wide<7>(p, s);
+            st = launch_wide<7>(p, plan.groups, s);
             break;
         default:
-            st = launch_wide<8>(p, s);
+            st = launch_wide<8>(p, plan.groups, s);
             break;
     }
     return st == SHP_OK && a.nsplit > 1 ? launch_join(a, s) : st;

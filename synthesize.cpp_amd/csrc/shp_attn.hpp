@@ -658,7 +658,7 @@ void         plan_spans(int64_t rows, int64_t T, int64_t cap, int64_t keys, int6
 int64_t      plan_floats(const AttnPlan & p, const shp_tensor & q);
 shp_status_t attn_args(const shp_tensor * q, const shp_tensor * length, const shp_tensor * count, float scale, const AttnPlan & p,
                        const shp_tensor * const * read, int n_read, const shp_tensor * work, const shp_tensor * y, AttnArgs & a);
-void         wide_args(int32_t per, int64_t chip, AttnArgs & a);
+void         wide_args(int32_t per, int32_t rows, int64_t chip, AttnArgs & a);
 shp_status_t launch_join(const AttnArgs & a, hipStream_t stream);
 
 // k_cross.hip: plain states of any length, and at most 16 queries of a kv head. The
