@@ -888,7 +888,7 @@ shp_status_t shp_kv_slots(const shp_tensor * table,
  * shp_kv_store_pages writes new rows: row t < count[n] of k and v, F32 [head_dim,
  * kv_heads, T, N], becomes row length[n] - count[n] + t of sequence n. For a block
  * whose new rows' largest magnitude is m:
- *   d = m / 127, and, where the sequence has rows in front of the new ones in this
+ *   d = m * (1/127), 1/127 in f32, and, where the sequence has rows in front of the new ones in this
  *       block, the larger of that and the block's scale;
  *   if that is more than the scale was, the codes c of the rows in front become
  *       rint(c * (scale / d)): at most half a step of the larger scale for each

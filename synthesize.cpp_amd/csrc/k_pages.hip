@@ -439,7 +439,7 @@ __global__ __launch_bounds__(kRowThreads) void k_kv_store_pages(const RowArgs a)
     }
     const bool  had  = r0 > 0;
     const bool  nan  = top >= 0x7f800000u || (had && !(d_old >= 0.0f));
-    const float mine = __uint_as_float(top) / 127.0f;
+    const float mine = __uint_as_float(top) * (1.0f / 127.0f);
     const float d    = nan ? NAN : had ? fmaxf(d_old, mine) : mine;
     const bool  grew = !nan && had && d > d_old;
     const float by   = grew ? d_old / d : 1.0f;

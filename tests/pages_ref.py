@@ -64,7 +64,7 @@ class Pool:
                     self.scale[at, h] = F(np.nan)
                     self.codes[at, h, r0:r1] = 0
                     continue
-                d = np.abs(new).max() / F(127)
+                d = np.abs(new).max() * (F(1) / F(127))
                 if r0 > 0 and not d > was:
                     d = was
                 elif r0 > 0:
