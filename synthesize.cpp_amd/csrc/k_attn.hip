@@ -275,20 +275,28 @@ void plan_spans(int64_t rows, int64_t T, int64_t cap, int64_t keys, int64_t pair
     const int64_t most  = (keys + kTileKeys - 1) / kTileKeys + (p.window > 0 ? 2 : 0);
     int64_t       span  = (most + kMaxSplits - 1) / kMaxSplits;
     span                = span > kWideSpan ? span : kWideSpan;
-    if (tiles * pairs > chip * 3 / 4) {
+    // Where all rows have all keys, whole rows from 3/8 of the chip on, or halves of long
+    // ones while both are on it (4 x 510 queries over as many rows, 12 heads of 64, F16:
+    // 22.5 us, halves 31.0; 2 x 1000 over 1500, 16 heads of 128 over 8, F32: halves 120, whole
+    // 147, F16 78 and 75), and below that a workgroup for each CU (2 x 100 over 1500, F16:
+    // 27.7 in sixths, 33 in twelfths).
+    const int64_t held = causal ? chip : chip / 2;
+    if (!causal && tiles * pairs >= chip * 3 / 8) {
+        span = tiles * pairs * 2 <= chip && most > 16 ? (most + 1) / 2 : most;
+    } else if (tiles * pairs > chip * 3 / 4) {
         span = most;
     } else if (tiles * pairs > chip / 2) {
         span = span > (most + 1) / 2 ? span : (most + 1) / 2;
     } else {
         auto fits = [&](int64_t of) {
             int64_t groups = 0;
-            for (int64_t t = 0; t < tiles && groups <= chip; ++t) {
+            for (int64_t t = 0; t < tiles && groups <= held; ++t) {
                 // of a whole cache, and within a window all alike
                 const int64_t end = causal ? cap - T + ((t + 1) * kWideRows * T + rows - 1) / rows : cap;
                 const int64_t n   = ((end < cap ? end : cap) + kTileKeys - 1) / kTileKeys;
                 groups += ((n < most ? n : most) + of - 1) / of * pairs;
             }
-            return groups <= chip;
+            return groups <= held;
         };
         for (int64_t upto = most; span < upto;) {  // the shortest that fits
             const int64_t mid = (span + upto) / 2;
