@@ -126,6 +126,25 @@ def test_layouts(gpu, kind):
         assert ((got - y).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows", [40, 3000])
+def test_v_of_another_layout_than_k(gpu, kind, rows):
+    """V's rows start where the kernel for few queries does not read them (an odd
+    element of 16 bits; f32: heads of another length in the row), K's where it does."""
+    heads, kv, hd = 4, 2, 64
+    packed, values = states(kind, 2, rows, kv, hd, 9)
+    k = packed[0].cuda()
+    wide = torch.zeros(2, rows, kv, hd + 3, dtype=R.FLOAT[kind], device="cuda")
+    v = wide[..., 1:hd + 1]
+    v.copy_(packed[1])
+    for t in (1, 3):
+        q = torch.randn(2, t, heads, hd, generator=torch.Generator().manual_seed(t))
+        y, bound = attend(q, *values, kind, [rows, rows // 2], [t, t], hd ** -0.5)
+        for a, b in ((k, v), (k, packed[1].cuda())):
+            got = gpu.attn_cross(q.cuda(), a, b, ints(rows, rows // 2)).cpu().double()
+            assert ((got - y).abs() <= bound).all()
+
+
 def test_a_decoder_layer_and_its_encoder_together(gpu):
     """An encoder's layer that looks both ways over its own q, k and v, the states
     stored in a cache by kv_store, and a decoder's tokens against them, beside the
