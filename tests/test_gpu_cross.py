@@ -109,6 +109,25 @@ def test_what_is_not_finite(gpu, kind, t):
     assert torch.equal(torch.isnan(got).any(-1), own)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("t", [1, 40])
+def test_states_of_all_sizes(gpu, kind, t):
+    """Rows of very different sizes beside each other, zeros, and queries of all
+    sizes: a row errs by its own values alone."""
+    n, rows, heads, kv, hd = 2, 90, 4, 2, 64
+    g = torch.Generator().manual_seed(t)
+    big = 1e4 if kind == "f16" else 1e30
+    for sizes, of_q in (([1.0, 1e-6, 0.0], 1.0), ([1e-3, 10.0], 100.0), ([1.0], 1e-20), ([1.0], 0.0)):
+        k = torch.randn(n, rows, kv, hd, generator=g) * torch.tensor(sizes).repeat(rows)[:rows, None, None]
+        v = torch.randn(n, rows, kv, hd, generator=g) * torch.tensor([1.0, 1.0 / big, big, 0.0]).repeat(rows)[:rows, None, None]
+        packed = [R.pack(x, kind) for x in (k, v)]
+        q = torch.randn(n, t, heads, hd, generator=g) * of_q
+        y, bound = attend(q, *(R.values(c, kind) for c in packed), kind, [rows, 33], [t] * n, hd ** -0.5)
+        got = gpu.attn_cross(q.cuda(), *(c.cuda() for c in packed), ints(rows, 33)).cpu().double()
+        err = (got - y).abs()
+        assert (err <= bound).all(), (sizes, of_q, float((err / bound.clamp_min(1e-300)).max()))
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16", "q4_0"])
 def test_layouts(gpu, kind):
     """Head-major states, queries cut from a fused projection, and one sequence of
