@@ -113,25 +113,30 @@ def rows(load=False, **over):
                                 R(a["ks"]), R(a["vs"]), R(a["status"]), None)
 
 
-POOLS = (dict(kp=mk(C, 64, 32, 2, 7), vp=mk(C, 64, 32, 2, 7)),                               # V not turned
-         dict(kp=mk(C, 64, 32, 2, 6)), dict(vp=mk(C, 32, 64, 3, 7)), dict(ks=mk(F, 3, 7)), dict(vs=mk(F, 2, 6)),
-         dict(ks=mk(F, 2, 7, 2)), dict(kp=mk(F, 64, 32, 2, 7)), dict(kp=mk(C, 64, 32, 2, 7, nb=[2, 128, 4096, 8192])))
-FAR = (dict(kp=mk(C, 64, 32, 2, 7, at=(1 << 43) + 8)), dict(vp=mk(C, 32, 64, 2, 7, nb=[1, 48, 4096, 8192])),
-       dict(kp=mk(C, 64, 32, 2, 7, nb=[1, 64, 2056, 8192])), dict(vp=mk(C, 32, 64, 2, 7, nb=[1, 32, 2048, 4104])),
-       dict(ks=mk(F, 2, 7, at=(1 << 43) + 2)), dict(vs=mk(S.TYPE_F16, 2, 7)),
-       dict(kp=mk(C, 64, 48, 2, 7), vp=mk(C, 48, 64, 2, 7)), dict(kp=mk(C, 64, 8, 2, 7), vp=mk(C, 8, 64, 2, 7)),
-       dict(kp=mk(C, 64, 512, 2, 7), vp=mk(C, 512, 64, 2, 7)), dict(kp=mk(C, 272, 32, 2, 7), vp=mk(C, 32, 272, 2, 7)),
-       dict(kp=mk(C, 72, 32, 2, 7), vp=mk(C, 32, 72, 2, 7)),
-       dict(kp=mk(C, 64, 32, 2, 1 << 26), vp=mk(C, 32, 64, 2, 1 << 26), ks=mk(F, 2, 1 << 26), vs=mk(F, 2, 1 << 26)))
+# (made anew for each test: the module of the binding may have been loaded again meanwhile)
+def pools():
+    return (dict(kp=mk(C, 64, 32, 2, 7), vp=mk(C, 64, 32, 2, 7)),                               # V not turned
+            dict(kp=mk(C, 64, 32, 2, 6)), dict(vp=mk(C, 32, 64, 3, 7)), dict(ks=mk(F, 3, 7)), dict(vs=mk(F, 2, 6)),
+            dict(ks=mk(F, 2, 7, 2)), dict(kp=mk(F, 64, 32, 2, 7)), dict(kp=mk(C, 64, 32, 2, 7, nb=[2, 128, 4096, 8192])))
+
+
+def far():
+    return (dict(kp=mk(C, 64, 32, 2, 7, at=(1 << 43) + 8)), dict(vp=mk(C, 32, 64, 2, 7, nb=[1, 48, 4096, 8192])),
+            dict(kp=mk(C, 64, 32, 2, 7, nb=[1, 64, 2056, 8192])), dict(vp=mk(C, 32, 64, 2, 7, nb=[1, 32, 2048, 4104])),
+            dict(ks=mk(F, 2, 7, at=(1 << 43) + 2)), dict(vs=mk(S.TYPE_F16, 2, 7)),
+            dict(kp=mk(C, 64, 48, 2, 7), vp=mk(C, 48, 64, 2, 7)), dict(kp=mk(C, 64, 8, 2, 7), vp=mk(C, 8, 64, 2, 7)),
+            dict(kp=mk(C, 64, 512, 2, 7), vp=mk(C, 512, 64, 2, 7)), dict(kp=mk(C, 272, 32, 2, 7), vp=mk(C, 32, 272, 2, 7)),
+            dict(kp=mk(C, 72, 32, 2, 7), vp=mk(C, 32, 72, 2, 7)),
+            dict(kp=mk(C, 64, 32, 2, 1 << 26), vp=mk(C, 32, 64, 2, 1 << 26), ks=mk(F, 2, 1 << 26), vs=mk(F, 2, 1 << 26)))
 
 
 @pytest.mark.parametrize("load", [False, True])
 def test_store_and_load_refuse(load):
     for name in ("k", "v", "kp", "vp", "ks", "vs") + (("slots",) if load else ("table", "length")):
         assert rows(load, **{name: None}) == BAD, name
-    for over in POOLS:
+    for over in pools():
         assert rows(load, **over) == BAD, over
-    for over in FAR:
+    for over in far():
         assert rows(load, **over) == NOT_HERE, over
     for name in ("k", "v"):
         assert rows(load, **{name: mk(F, 64, 2, 4, 3)}) == BAD
@@ -208,9 +213,9 @@ def floats(q, kp, table, window=0, sinks=0):
 def test_attention_refuses():
     for name in ("q", "kp", "vp", "ks", "vs", "table", "length", "y"):
         assert attend(**{name: None}) == BAD, name
-    for over in POOLS:
+    for over in pools():
         assert attend(**over) == BAD, over
-    for over in FAR:
+    for over in far():
         assert attend(**over) == NOT_HERE or over.get("kp", mk(C, 64, 32, 2, 7)).ne[0] != 64, over
     for hd in (72, 272):
         q = mk(F, hd, 8, 1, 3)
