@@ -920,9 +920,10 @@ __global__ __launch_bounds__(kWideBlock, NB <= 4 && KG == 1 ? 2 : 1) void k_attn
 // ---------------------------------------------------------------------------
 
 // Workgroups that the chip's 256 CUs hold.
-int64_t resident(int64_t hd) {
+constexpr int64_t resident(int64_t hd) {
     return hd <= 128 ? 512 : 256;
 }
+static_assert(resident(0) <= kMaxParts && resident(kKvMaxDim) <= kMaxParts);  // one head may have all of them
 
 constexpr int64_t kWhole     = 4;    // chunks a wave of a head that is not split
 constexpr int64_t kMostParts = 256;  // parts of a head that have one chunk a wave

@@ -487,6 +487,15 @@ template <int KIND> shp_status_t launch(FewArgs & f, int waves, hipStream_t stre
 // is less than a second launch.
 constexpr int64_t kDeep = 6;
 
+// Workgroups of `waves` that the chip's 256 CUs hold. A head that is split may have all of
+// those of kSplitWaves.
+constexpr int cross_resident(int kind, int hd, int waves) {
+    return 256 * 4 * cross_occupancy(kind, hd) / waves;
+}
+
+static_assert(cross_resident(kKvF16, 64, kSplitWaves) <= kMaxParts && cross_resident(kKvF32, 64, kSplitWaves) <= kMaxParts &&
+              cross_resident(kKvF16, 128, kSplitWaves) <= kMaxParts && cross_resident(kKvF16, 256, kSplitWaves) <= kMaxParts);
+
 void plan_cross_few(int kind, int64_t hd, int64_t rows, int64_t groups, AttnPlan & p) {
     const int     dims   = static_cast<int>(cross_few_dims(hd));
     const int     most   = cross_waves(kind, dims);
@@ -496,7 +505,7 @@ void plan_cross_few(int kind, int64_t hd, int64_t rows, int64_t groups, AttnPlan
     p.waves              = !p.parts && chunks > kSplitWaves ? most : kSplitWaves;
     const int64_t deep   = p.parts ? 1 : (chunks + p.waves - 1) / p.waves;
     const int64_t units  = (chunks + p.waves * deep - 1) / (p.waves * deep) * groups;
-    const int64_t held   = int64_t{ 256 } * 4 * cross_occupancy(kind, dims) / p.waves;
+    const int64_t held   = cross_resident(kind, dims, p.waves);
     p.cross              = units < INT32_MAX;
     p.per                = static_cast<int32_t>(p.waves * deep);
     p.groups             = static_cast<int32_t>(groups);

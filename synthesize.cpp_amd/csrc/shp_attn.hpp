@@ -351,14 +351,16 @@ __device__ __forceinline__ Rsrc rows_from(const char * at, int64_t bytes) {
 // The parts of a row joined: a workgroup a row, whose threads take four values
 // of every 1024/HD-th part each.
 constexpr int kJoinThreads = 256;
-constexpr int kMaxSplits   = 768;
+constexpr int kMaxSplits   = 768;   // splits of a row tile's keys
+constexpr int kMaxParts    = 1024;  // of one row: those splits, or the workgroups that share a line of units
+static_assert(kMaxSplits <= kMaxParts);
 
-// `parts` partial results of a row into out: ml(s) points to part s's m and l,
-// o(s) to its values. Left alone where the row has fewer than two parts.
+// `parts` partial results of a row, kMaxParts at most, into out: ml(s) points to part
+// s's m and l, o(s) to its values. Left alone where the row has fewer than two parts.
 template <int HD, class ML, class O>
 __device__ __forceinline__ void join_parts(int parts, int hd, const ML & ml, const O & o, float * out, bool sees_any) {
     constexpr int    GROUPS = kJoinThreads * 4 / HD;
-    __shared__ float weight[kMaxSplits];
+    __shared__ float weight[kMaxParts];
     __shared__ float lane_max[kJoinThreads / kWave], lane_sum[kJoinThreads / kWave];
     __shared__ f32x4 sums[kJoinThreads];
     const int        tid   = threadIdx.x;
@@ -645,6 +647,10 @@ constexpr int few_occupancy(int kind, int64_t hd) {
 constexpr int few_resident(int kind, int64_t hd) {
     return 256 * 4 * few_occupancy(kind, hd) / few_waves(hd);
 }
+
+// (one head group may have all of them)
+static_assert(few_resident(kKvQ4, 2 * kKvBlock) <= kMaxParts && few_resident(kKvQ4, 4 * kKvBlock) <= kMaxParts &&
+              few_resident(kKvQ4, 8 * kKvBlock) <= kMaxParts);
 
 // k_attn_few.hip: block caches and at most 16 queries of a kv head. The piece
 // size in which it can read both caches, or 0; and its launches, join included.

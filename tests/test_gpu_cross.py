@@ -84,6 +84,25 @@ def test_long_states(gpu, kind):
     check(gpu, kind, 4, 4, 64, 600, 700, [700, 650])
 
 
+@pytest.mark.parametrize("kind,hd,length", [("f16", 64, [131072 + 37]), ("bf16", 64, [200000, 5]), ("f16", 40, [140000, 0, 1]),
+                                            ("f32", 64, [120000]), ("bf16", 128, [70000, 64]), ("f16", 256, [50000, 16])])
+def test_one_head_for_every_workgroup(gpu, kind, hd, length):
+    """One kv head whose rows are shared out over all workgroups that the chip holds,
+    up to 1024 parts of one result. Scores are all 0 and values whole numbers, so that
+    weights are 1 and sums exact, whatever their order: what is left is 1/l and its
+    product, half a step each."""
+    n, rows = len(length), max(length)
+    v = ((torch.arange(rows)[:, None] * 7 + torch.arange(hd) * 3) % 13 - 5).float()
+    v[rows - rows // 4:] += 3.0                                            # (no part is like another)
+    k = torch.zeros(n, rows, 1, hd, dtype=R.FLOAT[kind], device="cuda")
+    vs = v[None, :, None].expand(n, -1, -1, -1).to(R.FLOAT[kind]).cuda()
+    q = torch.randn(n, 1, 2, hd, generator=torch.Generator().manual_seed(1)).cuda()
+    want = torch.stack([v[:ln].double().mean(0) if ln else torch.zeros(hd).double() for ln in length])[:, None, None]
+    for _ in range(2):
+        got = gpu.attn_cross(q, k, vs, ints(*length)).cpu().double()
+        assert ((got - want).abs() <= 2 * 2.0 ** -24 * 1.001 * want.abs()).all(), float((got - want).abs().max())
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16", "q8_0"])
 @pytest.mark.parametrize("t", [1, 60])
 def test_what_is_not_finite(gpu, kind, t):
