@@ -91,7 +91,9 @@ __device__ __forceinline__ float weight_scale(float d, float x, bool any) {
 
 // A partial result's weights are times 2^-k, so that with values up to f32's largest
 // neither it nor the sum over all parts passes that: its largest score is m + k
-// then, which is exact enough while m is below 2^22 (from there on k is 0).
+// then, which is exact enough while m is below 2^22 (from there on k is 0). A sum is
+// brought back by 2^(x - 14) after that, or after 1/l: their product, of two numbers far
+// below 1, may itself be next to nothing or 0 where the result is neither.
 __device__ __forceinline__ float part_shift(float m, float l) {
     return fabsf(m) < 0x1p22f ? static_cast<float>(exponent_of(l) + 12) : 0.0f;
 }
@@ -409,20 +411,21 @@ __global__ __launch_bounds__(64 * kPageWaves, HD <= 128 ? 2 : 1) void k_attn_pag
             part[w] = __builtin_amdgcn_exp2f(part[w] - x);
         }
         if (live) {
-            float * out;
-            float   by;
+            float *     out;
+            float       by;
+            const float by_x = __builtin_amdgcn_exp2f(x - kTopWeight);
             if (u0 == 0 && u1 == at.units) {
                 out = reinterpret_cast<float *>(a.y + n * a.yn + t * a.yt + head * a.yh);
-                by  = __builtin_amdgcn_exp2f(x - kTopWeight) * over(l, pos >= 0);
+                by  = over(l, pos >= 0);
             } else {
                 const int   which = u0 == 0 ? 1 : 0;
                 const float k     = part_shift(ref, l);
                 out               = few_o(f, wg, which, c);
-                by                = __builtin_amdgcn_exp2f(x - kTopWeight - k);
+                by                = __builtin_amdgcn_exp2f(-k);
                 if (wave == 0 && g == 0) {
                     float * pml = few_ml(f, wg, which, c);
                     pml[0]      = top + k;
-                    pml[1]      = l * __builtin_amdgcn_exp2f(-k);
+                    pml[1]      = l * by;
                 }
             }
 #pragma unroll
@@ -433,7 +436,7 @@ __global__ __launch_bounds__(64 * kPageWaves, HD <= 128 ? 2 : 1) void k_attn_pag
                     for (int w = 0; w < kPageWaves; ++w) {
                         v += of[(w * TILES + u) * kWave + lane] * part[w];
                     }
-                    *reinterpret_cast<f32x4u *>(out + 16 * u + 4 * g) = v * by;
+                    *reinterpret_cast<f32x4u *>(out + 16 * u + 4 * g) = v * by * by_x;
                 }
             }
         }
@@ -886,20 +889,21 @@ __global__ __launch_bounds__(kWideBlock, NB <= 4 && KG == 1 ? 2 : 1) void k_attn
     if (!live) {
         return;
     }
-    const int64_t row = ((static_cast<int64_t>(n) * a.KV + h) * a.T + t) * a.G + gq;
+    const int64_t row  = ((static_cast<int64_t>(n) * a.KV + h) * a.T + t) * a.G + gq;
+    const float   by_x = __builtin_amdgcn_exp2f(x - kTopWeight);
     float *       out;
     float         by;
     if (dest < 0) {
         out = reinterpret_cast<float *>(a.y + n * a.yn + t * a.yt + head * a.yh);
-        by  = __builtin_amdgcn_exp2f(x - kTopWeight) * over(l, pos >= 0);
+        by  = over(l, pos >= 0);
     } else {
         const float k = part_shift(m, l);
         out           = partial_o(a, row, dest);
-        by            = __builtin_amdgcn_exp2f(x - kTopWeight - k);
+        by            = __builtin_amdgcn_exp2f(-k);
         if (g == 0) {
             float * ml = partial_ml(a, row, dest);
             ml[0]      = m + k;
-            ml[1]      = l * __builtin_amdgcn_exp2f(-k);
+            ml[1]      = l * by;
         }
     }
 #pragma unroll
@@ -909,7 +913,7 @@ __global__ __launch_bounds__(kWideBlock, NB <= 4 && KG == 1 ? 2 : 1) void k_attn
             const int dim = 32 * u + 2 * e + 4 * g;
             if (dim < hd) {
                 *reinterpret_cast<f32x4u *>(out + dim) =
-                    f32x4{ o[u][e] * by, o[u][e + 1] * by, o[u][e + 2] * by, o[u][e + 3] * by };
+                    f32x4{ o[u][e] * by * by_x, o[u][e + 1] * by * by_x, o[u][e + 2] * by * by_x, o[u][e + 3] * by * by_x };
             }
         }
     }

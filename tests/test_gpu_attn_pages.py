@@ -176,6 +176,22 @@ def test_blocks_of_all_sizes(gpu, t):
 
 
 @pytest.mark.parametrize("t", [1, 40])
+@pytest.mark.parametrize("of", [0.0, 1.0])
+def test_small_values_of_split_heads(gpu, t, of):
+    """V's scales far below 1 over rows of like scores, whose weights' sum is large: the
+    result is an ordinary number, also where parts of the rows are joined."""
+    page, heads, kv, hd = 32, 4, 2, 64
+    ref = pool(300, page, kv, hd, 5)
+    table = tables(3, 282, 300, 2)
+    q = of * torch.randn(3, t, heads, hd, generator=torch.Generator().manual_seed(8))
+    keep = ref[1].scale.copy()
+    for by in (1e-20, 1e-26, 1e-28, 1e-30, 1e-33):
+        ref[1].scale[:] = keep * np.float32(by)
+        check(gpu, ref, q, table, [9000, 700, 4100])
+        check(gpu, ref, q[:1], table[:1], [9000], window=3000, sinks=70)
+
+
+@pytest.mark.parametrize("t", [1, 40])
 def test_queries_of_all_sizes(gpu, t):
     """Zero queries, tiny ones, ones with a value far above the others, and scores past 2^23."""
     page, heads, kv, hd = 32, 4, 2, 128
