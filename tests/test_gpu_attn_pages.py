@@ -1,6 +1,7 @@
 """attn_pages on the GPU against its definition (pages_ref.attend), within a bound
 derived from its sums, and the paged cache's operators together as a server uses
 them."""
+import math
 import random
 
 import numpy as np
@@ -207,6 +208,44 @@ def test_queries_of_all_sizes(gpu, t):
         ref[side].codes[..., 7] = 0
     check(gpu, ref, q, table, [256, 100])
     check(gpu, ref, q, table, [256, 100], scale=-0.3)
+
+
+@pytest.mark.parametrize("t", [1, 40])
+@pytest.mark.parametrize("length,window", [(300, 0), (9000, 0), (9000, 2500)])
+@pytest.mark.parametrize("power", [5, 13, 14, 15, 16])
+def test_large_scores_are_exact(gpu, t, length, window, power):
+    """Scores of 2^12 to 2^23 whose softmax is known: with a scale of ln 2 they are q.k
+    in powers of two, here whole numbers below 2^24 and so exact in f32, weights powers
+    of two. What is left: the pieces of weight times scale (2^-22 of itself, 2^-38 of the
+    largest), the sum over the rows, and 32 half steps of factors and joins. Some rows
+    have the largest code, a few steps apart by a second value; the others are at least
+    2^power below."""
+    page, heads, kv, hd, sinks = 32, 4, 2, 64, 40
+    g = torch.Generator().manual_seed(power)
+    ref = pool(300, page, kv, hd, 5)
+    codes = torch.zeros(300, kv, page, hd, dtype=torch.int8)
+    codes[..., 0] = torch.where(torch.rand(300, kv, page, generator=g) < 0.02, 127, torch.randint(-127, 127, (300, kv, page), generator=g)).to(torch.int8)
+    codes[..., 1] = torch.randint(0, 6, (300, kv, page), generator=g)
+    codes[..., 2:] = torch.randint(-127, 128, (300, kv, page, hd - 2), generator=g)     # (against zeros in q)
+    ref[0].codes[:], ref[0].scale[:] = codes.numpy(), 1.0
+    table = tables(1, 282, 300, 2)
+    q = torch.zeros(1, t, heads, hd)
+    q[..., 0], q[..., 1] = 2.0 ** power, 1.0
+    got = gpu.attn_pages(q.cuda(), cache_of(gpu, ref), table.cuda(), ints(length), scale=math.log(2), window=window, sinks=sinks).cpu().double()
+    k, v = (half.rows(table[0], length).double().transpose(0, 1) for half in ref)       # (kv, rows, hd)
+    d = torch.from_numpy(ref[1].scale)[table[0].long()].double().repeat_interleave(page, 0)[:length].T
+    s = k[..., 0] * 2.0 ** power + k[..., 1]
+    j = torch.arange(length)
+    for i in range(t):
+        at = length - t + i
+        seen = (j <= at) & ((j > at - window) | (j < sinks)) if window else j <= at
+        w = torch.exp2((s - s[:, seen].max(1, keepdim=True).values).masked_fill(~seen, -math.inf))
+        w = w / w.sum(1, keepdim=True)
+        y, size = (torch.bmm(w[:, None], x)[:, 0].repeat_interleave(heads // kv, 0) for x in (v, v.abs()))
+        lost = 2.0 ** -38 * (w * d).amax(1) * 127 * length
+        bound = (2.0 ** -22 + (length + 32) * P.EPS) * size + lost.repeat_interleave(heads // kv)[:, None]
+        err = (got[0, i] - y).abs()
+        assert (err <= bound).all(), (i, float((err / bound).max()))
 
 
 def test_one_large_weight_beside_many_small_ones(gpu):

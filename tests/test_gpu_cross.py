@@ -1,6 +1,8 @@
 """attn_cross on the GPU against its definition, within the bound of
 kv_ref.attend_by_row: a query that sees all rows is the newest position over a
 cache of them."""
+import math
+
 import pytest
 import torch
 
@@ -145,6 +147,38 @@ def test_states_of_all_sizes(gpu, kind, t):
         got = gpu.attn_cross(q.cuda(), *(c.cuda() for c in packed), ints(rows, 33)).cpu().double()
         err = (got - y).abs()
         assert (err <= bound).all(), (sizes, of_q, float((err / bound.clamp_min(1e-300)).max()))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("t,rows", [(1, 300), (1, 9000), (40, 300), (40, 9000)])
+@pytest.mark.parametrize("power", [5, 13, 16])
+def test_large_scores_are_exact(gpu, kind, t, rows, power):
+    """Scores of 2^12 to 2^23 whose softmax is known: with a scale of ln 2 they are q.k
+    in powers of two, here whole numbers below 2^24 and so exact in f32, weights powers
+    of two. What is left: the pieces of weights and, f32, of V (2^-22 of themselves, or
+    2^-39 of the largest, f32's of the largest times its row's size), the sum over the
+    rows, and 32 half steps of factors and joins."""
+    heads, kv, hd = 4, 2, 64
+    g = torch.Generator().manual_seed(power)
+    k = torch.zeros(1, rows, kv, hd)
+    k[..., 0] = torch.where(torch.rand(1, rows, kv, generator=g) < 0.02, 127, torch.randint(-127, 127, (1, rows, kv), generator=g))
+    k[..., 1] = torch.randint(0, 6, (1, rows, kv), generator=g)
+    v = R.pack(torch.randn(1, rows, kv, hd, generator=g), kind)
+    q = torch.zeros(1, t, heads, hd)
+    q[..., 0], q[..., 1] = 2.0 ** power, 1.0
+    got = gpu.attn_cross(q.cuda(), R.pack(k, kind).cuda(), v.cuda(), scale=math.log(2)).cpu().double()
+    s = (k[0, :, :, 0].double() * 2.0 ** power + k[0, :, :, 1].double()).T                  # (kv, rows)
+    x = R.values(v, kind)[0].double().transpose(0, 1)
+    w = torch.exp2(s - s.amax(1, keepdim=True))
+    w = w / w.sum(1, keepdim=True)
+    y, size, sums = (torch.bmm(a[:, None], b)[:, 0] for a, b in ((w, x), (w, x.abs()), (torch.ones_like(w), x.abs())))
+    top = x.abs().amax(2)
+    bound = (2.0 ** -22 + (rows + 32) * R.EPS) * size + 2.0 ** -39 * w.amax(1)[:, None] * sums
+    if kind == "f32":
+        bound = bound + (2.0 ** -25 * (w * top).sum(1) + rows * 2.0 ** -24 * (w * top).amax(1))[:, None]
+    y, bound = (a.repeat_interleave(heads // kv, 0) for a in (y, bound))
+    err = (got[0] - y).abs()
+    assert (err <= bound).all(), float((err / bound).max())
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16", "q4_0"])
