@@ -123,6 +123,17 @@ def test_prompts(gpu, page, t, heads, kv, hd):
     check(gpu, ref, q, table, length, count, window=50, sinks=3)
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(40, 2, 64), (33, 1, 128), (64, 2, 80), (17, 1, 256)])
+def test_one_position_of_many_query_heads(gpu, heads, kv, hd):
+    """More than sixteen query heads of a kv head: decoding by the kernel for prompts."""
+    page, length = 32, [1, 0, 700, 64, 333]
+    ref = pool(60, page, kv, hd, hd)
+    table = tables(5, 22, 60, 2)
+    q = torch.randn(5, 1, heads, hd, generator=torch.Generator().manual_seed(1)) * 1.5
+    check(gpu, ref, q, table, length)
+    check(gpu, ref, q, table, length, window=50, sinks=3)
+
+
 def test_long_caches(gpu):
     """Streams whose parts are joined: more than a chunk a wave, and parts of heads
     that begin and end inside a workgroup's stretch."""
@@ -398,6 +409,43 @@ def test_serving(gpu, captured):
         agree(dev["y"].cpu().double(), *P.attend(q, *side, table, lengths, counts, S["hd"] ** -0.5))
 
     serve(gpu, S, n, 25, 11, act)
+
+
+@pytest.mark.parametrize("t", [1, 40])
+def test_a_captured_call_of_split_heads_serves_all_lengths(gpu, t):
+    """Lengths, counts and tables change between replays: heads that were whole are split
+    and the other way round, over the workspace that the last replay left."""
+    page, heads, kv, hd, n = 32, 4, 2, 64, 3
+    ref = pool(300, page, kv, hd, 5)
+    cache = cache_of(gpu, ref)
+    table = tables(n, 282, 300, 2)
+    q = torch.zeros(n, t, heads, hd, device="cuda")
+    dev, length, count = table.cuda(), ints(*[0] * n), ints(*[0] * n)
+    out = torch.zeros(q.shape, device="cuda")
+    work = torch.full((gpu.attn_pages_work(q, cache, dev),), float("nan"), device="cuda")
+    assert work.numel() > 0
+
+    def call():
+        gpu.attn_pages(q, cache, dev, length, count, out=out, work=work)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        call()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for i, (ln, c) in enumerate([([9000, 1, 300], [t, 1, t]), ([64, 5000, 64], [t, 0, t]), ([0, 0, 9024], [1, 0, 1]), ([9000, 9000, 9000], [t, t, t])]):
+        x = torch.randn(q.shape, generator=torch.Generator().manual_seed(i))
+        q.copy_(x), length.copy_(ints(*ln)), count.copy_(ints(*c)), dev.copy_(table.roll(i, 1))
+        out.fill_(9.25)
+        graph.replay()
+        got = out.cpu()
+        agree(got.double(), *P.attend(x, *ref, table.roll(i, 1), ln, c, hd ** -0.5))
+        out.fill_(9.25)
+        call()
+        assert torch.equal(out.cpu(), got)
 
 
 def test_another_stream_than_the_current_tensors_were_made_on(gpu):

@@ -79,6 +79,49 @@ def test_heads_of_odd_length(gpu, kind, hd):
 
 
 @pytest.mark.parametrize("kind", R.TYPES)
+def test_one_position_of_many_query_heads(gpu, kind):
+    check(gpu, kind, 40, 2, 64, 1, 700, [700, 0, 1, 65])
+    check(gpu, kind, 17, 1, 256, 1, 90, [90, 33])
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32", "q8_0"])
+@pytest.mark.parametrize("t", [1, 30])
+def test_a_captured_call_of_split_heads_serves_all_lengths(gpu, kind, t):
+    """Lengths and counts change between replays, over the workspace that the last left."""
+    n, rows, heads, kv, hd = 3, 9000, 4, 2, 64
+    packed, values = states(kind, n, rows, kv, hd, 5)
+    k, v = (R.handle(gpu, c.cuda(), kind, hd) for c in packed)
+    q, out = (torch.zeros(n, t, heads, hd, device="cuda") for _ in range(2))
+    length, count = ints(*[0] * n), ints(*[0] * n)
+    work = torch.full((gpu.attn_cross_work(q, k),), float("nan"), device="cuda")
+    assert work.numel() > 0
+
+    def call():
+        gpu.attn_cross(q, k, v, length, count, out=out, work=work)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        call()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for i, (ln, c) in enumerate([([9000, 1, 300], [t, 1, t]), ([64, 5000, 64], [t, 0, t]), ([0, 0, 9000], [1, 0, 1])]):
+        x = torch.randn(q.shape, generator=torch.Generator().manual_seed(i))
+        q.copy_(x), length.copy_(ints(*ln)), count.copy_(ints(*c))
+        out.fill_(9.25)
+        graph.replay()
+        got = out.cpu()
+        y, bound = attend(x, *values, kind, ln, c, hd ** -0.5)
+        live = ~torch.isnan(y)
+        assert (got[~live] == 9.25).all() and ((got.double() - y)[live].abs() <= bound[live]).all()
+        out.fill_(9.25)
+        call()
+        assert torch.equal(out.cpu(), got)
+
+
+@pytest.mark.parametrize("kind", R.TYPES)
 def test_long_states(gpu, kind):
     """Queries whose parts are joined."""
     check(gpu, kind, 2, 1, 64, 1, 9000, [9000, 4500])
