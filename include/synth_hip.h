@@ -768,13 +768,15 @@ shp_status_t shp_kv_load(const shp_tensor * k_cache,
  * F16, BF16 and blocks exactly, whatever the sizes of the values beside each
  * other; F32 values to 2^-23 of themselves or 2^-25 of the largest of their own row
  * (one position of one kv head; of 2^-100, where that is smaller), whichever is
- * more. q to 2^-22 of itself or 2^-38 of the largest value of its head (BF16 caches:
- * f32's 24 bits). A weight to 2^-22 of itself or 2^-39 of the largest that the query
+ * more. q to 2^-22 of itself or 2^-38 of the largest value of its head (of 2^-100, where
+ * that is smaller, and scale log2(e) times q is meant; BF16 caches: f32's 24 bits). A weight to 2^-22 of itself or 2^-39 of the largest that the query
  * has (BF16: 24 bits; F32, where rows of V are of very different sizes: of the
  * largest of weight times its row's size, which is known to a factor of 2^14). A
  * weight below 2^-126 of the largest may count as 0. What a row holds has no other
- * part in what the others come to. The sum of weight times value over the rows,
- * with the largest weight as 1, has to be within f32's range.
+ * part in what the others come to. The sum of weight times value over any of the rows
+ * that a query sees, with the largest weight among those as 1, has to be within f32's
+ * range, as it is where rows times the largest value of V is: rows are taken
+ * in parts, each under its own largest weight. Past it the result is not finite.
  *
  * SHP_ERR_UNSUPPORTED past 2^28 query rows or 2^30 cache rows a sequence, and past
  * 65535 heads or sequences.
@@ -935,8 +937,8 @@ shp_status_t shp_kv_load_pages(const shp_tensor * k_pages,
  * every query NaN that sees a row of it.
  *
  * Precision: codes are exact; q and products as in shp_attn_kv. Of weight times V's
- * scale 2^-22 of itself or 2^-38 of the query's largest is lost. Scales may be up
- * to 2^120, so that values are within f32's range.
+ * scale 2^-22 of itself or 2^-38 of the query's largest (of 2^-100, where that is smaller)
+ * is lost. Scales may be up to 2^120, so that values are within f32's range.
  *
  * work as in shp_attn_kv, of shp_attn_pages_work's size for the same q, k_pages, table,
  * window and sinks.

@@ -277,9 +277,10 @@ void plan_spans(int64_t rows, int64_t T, int64_t cap, int64_t keys, int64_t pair
     span                = span > kWideSpan ? span : kWideSpan;
     // Where all rows have all keys, whole rows from 3/8 of the chip on, or halves of long
     // ones while both are on it (4 x 510 queries over as many rows, 12 heads of 64, F16:
-    // 22.5 us, halves 31.0; 2 x 1000 over 1500, 16 heads of 128 over 8, F32: halves 120, whole
+    // 22.0 us, halves 31.0; 2 x 1000 over 1500, 16 heads of 128 over 8, F32: halves 117, whole
     // 147, F16 78 and 75), and below that a workgroup for each CU (2 x 100 over 1500, F16:
-    // 27.7 in sixths, 33 in twelfths).
+    // 27.7 in sixths, 33 in twelfths). These three shapes are all that both sides were
+    // measured at.
     const int64_t held = causal ? chip : chip / 2;
     if (!causal && tiles * pairs >= chip * 3 / 8) {
         span = tiles * pairs * 2 <= chip && most > 16 ? (most + 1) / 2 : most;
@@ -431,7 +432,7 @@ shp_status_t launch_join(const AttnArgs & a, hipStream_t stream) {
     return a.hd <= 64 ? go(k_attn_join<64>) : a.hd <= 128 ? go(k_attn_join<128>) : go(k_attn_join<256>);
 }
 
-// The checks that shp_attn_kv and shp_attn_pages share once a call is planned, and
+// The checks that shp_attn_kv, shp_attn_cross and shp_attn_pages share once a call is planned, and
 // the arguments but for the cache's; `read`: what y and work may not overlap, beside q.
 shp_status_t attn_args(const shp_tensor *         q,
                        const shp_tensor *         length,

@@ -103,7 +103,7 @@ __device__ __forceinline__ float part_shift(float m, float l) {
 // takes 64 tokens at a time and reads them from the pool straight into the operands'
 // registers, 16 bytes a lane, K's of the next 64 ahead of the exponentials and V's
 // ahead of the next scores. 64 streams of 512 to 8192 rows (16 heads of 128 values over 8,
-// MI355X) take 115 us, 5.0 TB/s, as a large copy; 38 rows 8.0 us, in which the length, the
+// MI355X) take 115 us, 5.0 TB/s; 38 rows 8.0 us, in which the length, the
 // table, the codes, two products and the waves' join follow each other.
 // ---------------------------------------------------------------------------
 
@@ -467,11 +467,10 @@ template <int HD> __global__ __launch_bounds__(kJoinThreads) void k_attn_join_pa
 // after that is on its way in registers. Matrix instructions 32x32x16. With KG 1 a
 // workgroup has 128 rows, which share a tile; with 2 it has 64, and its groups' results are
 // joined in LDS.
-// 8192 positions of 16 heads of 128 over 8 take 520 to 535 us (MI355X): two products at
-// 1.03 to 1.06 PFLOP/s, where a large F16 product reaches 1.14, at the clock that such work
-// leaves the chip. Two barriers a tile, with the tile brought into LDS between them: 575;
+// 8192 positions of 16 heads of 128 over 8 take 528 to 541 us (MI355X): two products at
+// 1.02 to 1.04 PFLOP/s, where a large F16 product reaches 1.32. Two barriers a tile, with the tile brought into LDS between them: 575;
 // scales made ready as they are read, which waits for them: 15 us of 526. A lone
-// workgroup's tile takes 2.0 us, of which the matrix units work 0.9: 1021 positions 33 us.
+// workgroup's tile takes 2.0 us, of which the matrix units work 0.9: 1021 positions 31.4 us.
 // ---------------------------------------------------------------------------
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -978,8 +977,11 @@ shp_status_t plan_pages(const shp_tensor * q, const shp_tensor * k, const shp_te
         // Two groups of a workgroup rather than splits, whose results go through memory
         // and a second launch, while a head has few tiles for the rows that there are:
         // 512 positions take 20.2 us, 22.2 in splits (16 heads of 128 over 8, MI355X), 1021
-        // 32.8, 37.1; but 128 over 768 rows 24.8, 19.9, and 20 over 512 19.0, 14.6. One
-        // workgroup of this kind fits a CU.
+        // 32.8, 37.1; but 128 over 768 rows 24.8, 19.9, and 20 over 512 19.0, 14.6. The rule
+        // comes from these four. 256 are those that the chip holds at once, one a CU, with
+        // heads of 96 and 128 values; of shorter ones it holds 512, which was not measured.
+        // Heads of an odd multiple of 16 have no form of this kind, and are split (1000
+        // positions of 80: 30.7 us, of 96: 26.8).
         const int64_t most   = (keys + kTileKeys - 1) / kTileKeys + (p.window > 0 ? 2 : 0);
         const int64_t groups = (rows + kWideRows / 2 - 1) / (kWideRows / 2) * kv * q->ne[3];
         p.groups             = 1;

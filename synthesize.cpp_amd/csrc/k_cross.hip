@@ -1,6 +1,6 @@
 // shp_attn_cross for few queries over plain states (a decoder's token).
 //
-// At most 16 columns, the queries of one kv head, against chunks of 16 to 64 rows
+// At most 16 columns, the queries of one kv head, against chunks of 16 or 32 rows
 // that a wave reads straight into the operands' registers, 16 bytes a lane, the next
 // K ahead of the exponentials and the next V ahead of the next scores:
 //   S^T = K Q^T  F16 and BF16 as they lie, q in two F16 or three BF16 pieces; F32
@@ -10,9 +10,10 @@
 //                of holds the element of VE tiles, so V needs no turning, and
 //                weights and values are exact. 4096 cycles of a SIMD for 64 rows of 128
 //                values, 32 KB of F16: the chip could take 19 TB/s.
-// Bound by the bytes of long states and by latency: 16 sequences of 300 to 1500 F16 rows (16
-// heads of 64, MI355X) take 18 us, 3.2 TB/s, in one launch; in stretches, as longer ones
-// are, 22, of which 4 are the join.
+// Bound by the bytes of long states and by latency: 16 sequences of 300 to 1500 rows (16
+// heads of 64, MI355X) take 18 to 19.5 us over F16, 3.1 TB/s, 19 over BF16 and 30 over F32
+// (3.9 TB/s), in one launch; in stretches, as longer ones are, F16 takes 22, of which 4 are
+// the join. Heads of 40 F16 or BF16 values take 26: their form spills registers.
 // Every query sees every row, so rows past a sequence's are read as its last one, and
 // count for nothing.
 #include "shp_attn.hpp"
@@ -22,10 +23,9 @@ namespace {
 
 constexpr int kSplitWaves = 4;  // of a workgroup whose heads are split
 
-// Rows of a chunk: 32, or as many as keep K's in 32 registers of a lane, but 16 at least.
+// Rows of a chunk: 32, or 16 where that many would take more than 32 registers of a lane for K.
 constexpr int cross_rows(int kind, int hd) {
-    const int rows = 8192 / (hd * kv_unit_bytes(kind));
-    return rows > 32 ? 32 : rows < 16 ? 16 : rows;
+    return 8192 / (hd * kv_unit_bytes(kind)) >= 32 ? 32 : 16;
 }
 
 // Waves that a SIMD holds by their registers.
@@ -34,7 +34,7 @@ constexpr int cross_occupancy(int kind, int hd) {
 }
 
 constexpr int cross_shift(int kind, int hd) {
-    return cross_rows(kind, hd) == 64 ? 6 : cross_rows(kind, hd) == 32 ? 5 : 4;
+    return cross_rows(kind, hd) == 32 ? 5 : 4;
 }
 
 typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
